@@ -45,13 +45,19 @@ int decode_tokens_dispatch(const Geom& g, const int32_t* list, int n_ent, int32_
 int decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                     void* o, float* lse, const int32_t* tok, int n_tokens, float* ws, int n_splits,
                     hipStream_t stream);
-void ring_stream(int length, int n_q, int sink, int window, int ring, int* n_sink, int* w_lo, int* base,
-                 int* n_tokens);
 int decode_ring_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k,
                          const void* v, void* o, float* lse, int ring, float* ws, int n_splits,
                          hipStream_t stream);
 int append_dispatch(int dtype, int head_dim, void* kc, void* vc, const void* kn, const void* vn, int BH,
                     int n_new, int start, int sink, int ring, hipStream_t stream);
+int append8_dispatch(int dtype, int head_dim, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn,
+                     const void* vn, int BH, int n_new, int start, int sink, int ring, hipStream_t stream);
+int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const uint8_t* ks, const uint8_t* vs,
+                  void* ko, void* vo, int64_t* positions, int BH, int length, int sink, int ring,
+                  hipStream_t stream);
+int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                     const uint8_t* ks, const uint8_t* vs, void* o, float* lse, int ring, float* ws, int n_splits,
+                     hipStream_t stream);
 int64_t read_probe_words(int BH);
 int read_probe_dispatch(const void* k, const void* v, int BH, int64_t n_kv, int row_bytes, int n_sink,
                         int64_t w_lo, uint32_t* out, hipStream_t stream);
@@ -194,11 +200,9 @@ int rolling_decode_args(int dtype, int B, int H, int H_kv, int n_q, int head_dim
   return 0;
 }
 
-int rolling_decode_checked(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
-                           int dtype, int B, int H, int H_kv, int n_q, int head_dim, int sink_size,
-                           int window_size, int ring_size, int64_t length, float softmax_scale,
-                           float* workspace, int n_splits, void* stream) {
-  GKI_REQUIRE(n_splits == 1 || workspace, 1, "gki_rolling_decode: null workspace");
+// Geometry of a decode over a rolling cache of positions 0 .. length - 1.
+Geom rolling_geom(int B, int H, int H_kv, int n_q, int sink_size, int window_size, int64_t length,
+                  float softmax_scale) {
   Geom g{};
   g.B = B;
   g.H = H;
@@ -213,8 +217,30 @@ int rolling_decode_checked(const void* q, const void* k_cache, const void* v_cac
   g.window = window_size;
   g.mask = nullptr;                     // no stream entry carries the partial flag
   g.n_qb = g.n_kb = g.bm = g.bn = 1;
+  return g;
+}
+
+int rolling_decode_checked(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
+                           int dtype, int B, int H, int H_kv, int n_q, int head_dim, int sink_size,
+                           int window_size, int ring_size, int64_t length, float softmax_scale,
+                           float* workspace, int n_splits, void* stream) {
+  GKI_REQUIRE(n_splits == 1 || workspace, 1, "gki_rolling_decode: null workspace");
+  const Geom g = rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale);
   return decode_ring_dispatch(dtype, head_dim, g, q, k_cache, v_cache, o, lse, ring_size, workspace,
                               n_splits, (hipStream_t)stream);
+}
+
+// Checks that the 8-bit cache's entry points (and the reading of either kind) share.
+int rolling8_args(const char* what, int dtype, int B, int H, int head_dim, int sink_size, int ring_size) {
+  const std::string w = std::string(what) + ": ";
+  GKI_REQUIRE(dtype == kF32 || dtype == kF16 || dtype == kBF16, 2,
+              "unsupported dtype code " + std::to_string(dtype) + " (0=fp32, 1=fp16, 2=bf16)");
+  GKI_REQUIRE(head_dim == 64 || head_dim == 128, 2, w + "head_dim must be 64 or 128, got " + std::to_string(head_dim));
+  GKI_REQUIRE(B > 0 && H > 0 && (int64_t)B * H < (1ll << 31) / 4096, 1,
+              w + "B and H must be positive and B * H not too large");
+  GKI_REQUIRE(sink_size >= 0 && ring_size >= 1 && (int64_t)sink_size + ring_size < (1ll << kPartialBit), 1,
+              w + "sink_size must be >= 0, ring_size >= 1 and their sum below 2^30");
+  return 0;
 }
 
 }  // namespace
@@ -504,6 +530,65 @@ int gki_rolling_decode_noalloc(const void* q, const void* k_cache, const void* v
   }
   return rolling_decode_checked(q, k_cache, v_cache, o, lse, dtype, B, H, H_kv, n_q, head_dim, sink_size,
                                 window_size, ring_size, length, softmax_scale, ws, n_splits, stream);
+}
+
+int gki_stream_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
+                          int64_t n_tokens) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_tokens < 0) return 1;
+  const int rows = H / H_kv * n_q, tile = stream_rows_tile(dtype == kF32, rows);
+  return stream_splits(head_dim, (int64_t)B * H_kv * ((rows + tile - 1) / tile), n_tokens);
+}
+
+int64_t gki_stream_workspace_floats(int32_t B, int32_t H, int32_t n_q, int32_t head_dim, int32_t n_parts) {
+  return n_parts > 1 ? (int64_t)B * H * n_q * n_parts * (head_dim + 2) : 0;
+}
+
+int gki_rolling8_append(void* k_codes, void* v_codes, void* k_scale, void* v_scale, const void* k_new,
+                        const void* v_new, int32_t dtype, int32_t B, int32_t H, int32_t head_dim,
+                        int32_t sink_size, int32_t ring_size, int64_t start_pos, int32_t n_new, void* stream) {
+  const char* what = "gki_rolling8_append";
+  if (int rc = rolling8_args(what, dtype, B, H, head_dim, sink_size, ring_size)) return rc;
+  GKI_REQUIRE(start_pos >= 0 && n_new >= 0 && start_pos + n_new < (1ll << kPartialBit), 1,
+              "gki_rolling8_append: positions must lie in [0, 2^30)");
+  if (n_new == 0) return 0;
+  GKI_REQUIRE(k_codes && v_codes && k_scale && v_scale && k_new && v_new, 1, "gki_rolling8_append: null pointer");
+  GKI_REQUIRE(all_aligned16(k_codes, v_codes, k_new, v_new), 1,
+              "gki_rolling8_append: codes and new rows must be 16-byte aligned");
+  return append8_dispatch(dtype, head_dim, (uint8_t*)k_codes, (uint8_t*)v_codes, (uint8_t*)k_scale,
+                          (uint8_t*)v_scale, k_new, v_new, B * H, n_new, (int)start_pos, sink_size, ring_size,
+                          (hipStream_t)stream);
+}
+
+int gki_rolling_read(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale, void* k_out,
+                     void* v_out, int64_t* positions, int32_t dtype, int32_t B, int32_t H, int32_t head_dim,
+                     int32_t sink_size, int32_t ring_size, int64_t length, void* stream) {
+  const char* what = "gki_rolling_read";
+  if (int rc = rolling8_args(what, dtype, B, H, head_dim, sink_size, ring_size)) return rc;
+  GKI_REQUIRE(length >= 0 && length < (1ll << kPartialBit), 1, "gki_rolling_read: length must be in [0, 2^30)");
+  if (length == 0) return 0;
+  GKI_REQUIRE(k_cache && v_cache && k_out && v_out && positions && !k_scale == !v_scale, 1,
+              "gki_rolling_read: null pointer");
+  GKI_REQUIRE(all_aligned16(k_cache, v_cache, k_out, v_out), 1,
+              "gki_rolling_read: caches and outputs must be 16-byte aligned");
+  return read_dispatch(dtype, head_dim, k_cache, v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale, k_out,
+                       v_out, positions, B * H, (int)length, sink_size, ring_size, (hipStream_t)stream);
+}
+
+int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes, const void* k_scale,
+                        const void* v_scale, void* o, float* lse, int32_t dtype, int32_t B, int32_t H, int32_t H_kv,
+                        int32_t n_q, int32_t head_dim, int32_t sink_size, int32_t window_size, int32_t ring_size,
+                        int64_t length, float softmax_scale, float* workspace, int32_t n_splits, void* stream) {
+  if (int rc = rolling_decode_args(dtype, B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, length,
+                                   softmax_scale, q, k_codes, v_codes, o, lse, n_splits))
+    return rc;
+  GKI_REQUIRE(k_scale && v_scale, 1, "gki_rolling8_decode: null scale");
+  GKI_REQUIRE((((uintptr_t)o | (uintptr_t)workspace) & 15) == 0, 1,
+              "gki_rolling8_decode: o and the workspace must be 16-byte aligned");
+  GKI_REQUIRE(n_splits == 1 || workspace, 1, "gki_rolling8_decode: null workspace");
+  return attend8_dispatch(dtype, head_dim,
+                          rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale), q, k_codes,
+                          v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, o, lse, ring_size, workspace,
+                          n_splits, (hipStream_t)stream);
 }
 
 int64_t gki_read_probe_words(int32_t bh) { return bh > 0 ? read_probe_words(bh) : 0; }

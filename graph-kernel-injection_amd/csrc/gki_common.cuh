@@ -11,6 +11,7 @@
 #include <cmath>
 
 #include <string>
+#include <type_traits>
 
 namespace gki {
 
@@ -380,6 +381,48 @@ struct DmaTile {
     }
   }
 };
+
+// One ds_read_b64_tr_b16: lane (g, c) gets tile[k0 + 4g + e][n0 + c], e = 0..3,
+// the K-operand layout of v_mfma_f32_16x16x16_{bf16,f16} for a K-major matrix.
+template <int D>
+__device__ inline uint2 lds_tr4(const uint16_t* tile, int k0, int n0, int lane) {
+  const int g = lane >> 4, l = lane & 15;
+  const uint16_t* p = tile + lds_off<D>(k0 + 4 * g + (l >> 2), n0 + 4 * (l & 3));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)p));
+}
+
+template <typename T>
+__device__ inline floatx4 mfma16k(const uint2& a, const uint2& b, floatx4 c) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
+  if constexpr (std::is_same<T, BF16>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
+                                                     __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h16x4, a),
+                                                 __builtin_bit_cast(h16x4, b), c, 0, 0, 0);
+}
+
+// s_waitcnt vmcnt(N), other counters untouched (N < 64: the field's low four
+// bits at 3:0, its high two at 15:14).
+template <int N>
+__device__ inline void vm_wait() {
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// Wait until at most k chunks (of 2 * NP LDS-DMA instructions per wave each,
+// k <= NBUF) are still in flight: every memory operation issued before them
+// has completed.
+template <int NP, int NBUF>
+__device__ inline void wait_chunks(int k) {
+  static_assert(NBUF <= 4 && 8 * NP < 64, "wait_chunks covers up to four chunks in flight");
+  if (k <= 0) vm_wait<0>();
+  else if (k == 1) vm_wait<2 * NP>();
+  else if (k == 2) vm_wait<4 * NP>();
+  else if (k == 3) vm_wait<6 * NP>();
+  else vm_wait<8 * NP>();
+}
 
 // ---------------------------------------------------------------------------
 // fp32 tiles: row-major in LDS, 16-byte chunks XOR-swizzled per row, staged by
@@ -778,6 +821,30 @@ inline int f32_kv_blocks(int head_dim, int items) {
   return items <= (head_dim == 64 ? 64 : 128) ? 1 : items <= (head_dim == 64 ? 256 : 384) ? 2 : 4;
 }
 
+// Of n_new positions appended at start to a rolling cache, those that no later one of
+// the same call overwrites: the first n_a (sinks), and n_b from the i_b-th on (ring).
+inline void surviving_rows(int start, int n_new, int sink, int ring, int* n_a, int* i_b, int* n_b) {
+  const int end = start + n_new;
+  *n_a = start < sink ? (end < sink ? end : sink) - start : 0;
+  const int keep_lo = end - ring > sink ? end - ring : sink;       // first surviving ring position
+  const int b_lo = keep_lo > start ? keep_lo : start;
+  *i_b = b_lo - start;
+  *n_b = end > b_lo ? end - b_lo : 0;
+}
+
+// Query rows per workgroup of the stream kernels: one block of 16, or two where a
+// stream has more (fp32: its three pieces of each operand leave registers for one).
+inline int stream_rows_tile(bool f32, int n_rows) { return f32 || n_rows <= 16 ? 16 : 32; }
+
+// Slices of each stream: enough workgroups for two rounds of what the card holds at
+// once (two per CU at head_dim 128, four at 64, by their 64 KB and 32 KB of LDS), of
+// at least 128 tokens each.
+inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
+  const int64_t target = head_dim >= 128 ? 512 : 1024;
+  const int64_t want = (target + n_workgroups - 1) / n_workgroups;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, n_tokens / 128));
+}
+
 // XCD-aware remap: hardware dispatches workgroup b to XCD b % 8. Give each XCD
 // one contiguous range of logical ids so neighbouring q tiles of one head (which
 // share most K/V tiles) run on the same XCD and hit in its L2.
@@ -953,6 +1020,9 @@ __device__ inline float lse_base2(float lse) { return (float)((double)lse * 1.44
 // ---------------------------------------------------------------------------
 namespace gki {
 void set_error(const std::string& msg);
+// Visible-token stream of a rolling cache's last n_q positions (gki_decode.hip).
+void ring_stream(int length, int n_q, int sink, int window, int ring, int* n_sink, int* w_lo, int* base,
+                 int* n_tokens);
 int fail(int code, const std::string& msg);
 int check_launch(const char* what);
 }  // namespace gki

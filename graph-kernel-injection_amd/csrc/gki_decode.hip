@@ -535,35 +535,6 @@ int launch_decode(int dtype, int head_dim, const Geom& g, const void* q, const v
 // transposed LDS read); the row sums add the fp32 P. The four waves' states
 // merge through LDS into the same partials / output as decode_kernel.
 // ---------------------------------------------------------------------------
-// One ds_read_b64_tr_b16: lane (g, c) gets tile[k0 + 4g + e][n0 + c], e = 0..3,
-// the K-operand layout of v_mfma_f32_16x16x16_{bf16,f16} for a K-major matrix.
-template <int D>
-__device__ inline uint2 lds_tr4(const uint16_t* tile, int k0, int n0, int lane) {
-  const int g = lane >> 4, l = lane & 15;
-  const uint16_t* p = tile + lds_off<D>(k0 + 4 * g + (l >> 2), n0 + 4 * (l & 3));
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)p));
-}
-
-template <typename T>
-__device__ inline floatx4 mfma16k(const uint2& a, const uint2& b, floatx4 c) {
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
-  if constexpr (std::is_same<T, BF16>::value)
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
-                                                     __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h16x4, a),
-                                                 __builtin_bit_cast(h16x4, b), c, 0, 0, 0);
-}
-
-// s_waitcnt vmcnt(N), other counters untouched (N < 64: the field's low four
-// bits at 3:0, its high two at 15:14).
-template <int N>
-__device__ inline void vm_wait() {
-  static_assert(N >= 0 && N < 64, "vmcnt field");
-  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
-}
-
 // Chunks in flight per workgroup (LDS ring of K and V tiles): three or four
 // measured no faster than two on the grouped-query and four-position steps.
 template <int D>
@@ -573,19 +544,6 @@ constexpr int decode_mfma_bufs() { return 2; }
 template <int D, bool QLDS>
 constexpr int decode_mfma_lds() {
   return 2 * decode_mfma_bufs<D>() * kTileN * D * 2 + (QLDS ? 2 * kDecodeTileM * D * 2 : 0);
-}
-
-// Wait until at most k chunks (of 2 * NP LDS-DMA instructions per wave each,
-// k <= NBUF) are still in flight: every memory operation issued before them
-// has completed.
-template <int NP, int NBUF>
-__device__ inline void wait_chunks(int k) {
-  static_assert(NBUF <= 4 && 8 * NP < 64, "wait_chunks covers up to four chunks in flight");
-  if (k <= 0) vm_wait<0>();
-  else if (k == 1) vm_wait<2 * NP>();
-  else if (k == 2) vm_wait<4 * NP>();
-  else if (k == 3) vm_wait<6 * NP>();
-  else vm_wait<8 * NP>();
 }
 
 template <typename T, int D, bool EXACT, int NB, bool QLDS>
@@ -959,12 +917,8 @@ int decode_ring_dispatch(int dtype, int head_dim, const Geom& g, const void* q, 
 
 int append_dispatch(int dtype, int head_dim, void* kc, void* vc, const void* kn, const void* vn, int BH,
                     int n_new, int start, int sink, int ring, hipStream_t stream) {
-  const int end = start + n_new;
-  const int n_a = start < sink ? (end < sink ? end : sink) - start : 0;
-  const int keep_lo = end - ring > sink ? end - ring : sink;       // first surviving ring position
-  const int b_lo = keep_lo > start ? keep_lo : start;
-  const int i_b = b_lo - start;
-  const int n_b = end > b_lo ? end - b_lo : 0;
+  int n_a, i_b, n_b;
+  surviving_rows(start, n_new, sink, ring, &n_a, &i_b, &n_b);
   if (dtype == kF32)
     return launch_append_t<F32>(head_dim, kc, vc, kn, vn, BH, n_new, n_a, i_b, n_b, start, sink, ring, stream);
   if (dtype == kF16)

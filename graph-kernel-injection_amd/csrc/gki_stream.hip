@@ -1,0 +1,576 @@
+// Attention of few query rows over long streams of keys and values: the rolling
+// cache held in 8 bits, for gfx950.
+//
+// A stream is the K / V rows of one (b, kv head); the rows that read it are the
+// group * n_q query rows of that head's group. For each of them
+//   S_t = scale * q . k_t,  O = sum_t exp(S_t - m) v_t / sum_t exp(S_t - m),
+//   LSE = m + ln(sum),  m the largest S_t,
+// over the stream's visible tokens t; a row that sees none has O = 0, LSE = 0.
+// The work is bound by reading K and V once (HBM): a workgroup takes an equal
+// slice of a stream's tokens for up to 32 of its rows, and the slices' states
+// (max, sum, accumulator, all fp32) are joined by join_kernel when there are
+// several.
+//
+// 8-bit rows. A row x of D values is stored as D e4m3 codes and one byte e + 127:
+// e is the smallest integer (at least -117) with max |x_i| <= 448 * 2^e, code i the
+// e4m3 number nearest to x_i * 2^-e (ties to even). The scale is a power of two
+// so that the division is exact and the codes do not depend on how it is carried
+// out, and so that a stored value, code * 2^e, is a bfloat16: it enters the matrix
+// cores as it is, whatever the type of the queries. An e4m3 number has 4 significant
+// bits whatever its exponent, so a scale closer to the row's maximum would gain
+// nothing above the subnormal codes (below 2^-14.8 of the maximum). Infinities and
+// NaN are stored as NaN; the scale is that of the finite values.
+#include <algorithm>
+#include <string>
+
+#include "gki_common.cuh"
+
+namespace gki {
+namespace {
+
+constexpr int kMinExponent = -117;           // 2^-9 (the smallest code) * 2^-117 is a normal float
+constexpr float kStreamSlack = 8.f;          // log2 units the lazy reference max may lag (p <= 2^8)
+
+// ---------------------------------------------------------------------------
+// Writing and reading back.
+// ---------------------------------------------------------------------------
+// Eight consecutive elements as floats, and back.
+template <typename T>
+__device__ inline void load8(const typename T::storage* p, float (&f)[8]) {
+  if constexpr (T::is_f32) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+    const uint4 w = *(const uint4*)p;
+    const uint16_t* h = (const uint16_t*)&w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = T::to_float(h[i]);
+  }
+}
+
+// Slot of new row r of the launch (rows_of_append): its source row and cache slot.
+struct AppendRows {
+  int n_new, n_a, i_b, n_b, start, sink, ring;
+  __device__ inline int source(int r) const { return r < n_a ? r : i_b + (r - n_a); }
+  __device__ inline int slot(int i) const {
+    const int p = start + i;
+    return p < sink ? p : sink + (p - sink) % ring;
+  }
+};
+
+// One row of K or V per D / 8 lanes (16 or 8): the largest finite magnitude across
+// them, the exponent from its bits, eight codes per lane. Bound by HBM: reads the
+// rows once, writes D + 1 bytes each.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void append8_kernel(
+    uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, uint8_t* __restrict__ ks, uint8_t* __restrict__ vs,
+    const typename T::storage* __restrict__ kn, const typename T::storage* __restrict__ vn, int BH,
+    AppendRows a) {
+  constexpr int LPR = D / 8;                   // lanes per row
+  const int rows = a.n_a + a.n_b;
+  const int ch = threadIdx.x % LPR;
+  const int64_t n = (int64_t)BH * rows;
+  // whole rows: the lanes of a row leave together
+  for (int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR; row < 2 * n;
+       row += (int64_t)gridDim.x * (256 / LPR)) {
+    const bool is_v = row >= n;
+    const int64_t rr = is_v ? row - n : row;
+    const int bh = (int)(rr / rows), i = a.source((int)(rr % rows));
+    float f[8];
+    load8<T>((is_v ? vn : kn) + ((size_t)bh * a.n_new + i) * D + 8 * ch, f);
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = fabsf(f[j]);
+      top = fmaxf(top, x < __builtin_huge_valf() ? x : 0.f);     // false for NaN too
+    }
+#pragma unroll
+    for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+    // top = (1 + m / 2^23) 2^k <= 448 * 2^e = 1.75 * 2^(8 + e)
+    const uint32_t bits = __float_as_uint(top);
+    const int e = max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0), kMinExponent);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      y[j] = fabsf(f[j]) < __builtin_huge_valf() ? f[j] * inv : __builtin_nanf("");
+    int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w0, true);
+    int w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w1, true);
+    const size_t dst = (size_t)bh * (a.sink + a.ring) + a.slot(i);
+    *(uint2*)((is_v ? vc : kc) + dst * D + 8 * ch) = make_uint2((uint32_t)w0, (uint32_t)w1);
+    if (ch == 0) (is_v ? vs : ks)[dst] = (uint8_t)(e + 127);
+  }
+}
+
+// Two e4m3 codes of a word (its low or high half) times 2^e: exact in fp32.
+__device__ inline f32x2 codes2(uint32_t w, bool high, float scale) {
+  const auto x = high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  return f32x2{x[0] * scale, x[1] * scale};
+}
+__device__ inline float scale_of(uint8_t e) { return __uint_as_float((uint32_t)e << 23); }
+
+// The held rows in ascending order of position, as values of the cache's type, and
+// the positions. Row r < n_sink is position r, any other lo + r - n_sink. Eight
+// values per lane; bound by HBM.
+struct HeldRows {
+  int n, n_sink, lo, sink, ring;
+  __device__ inline int position(int r) const { return r < n_sink ? r : lo + (r - n_sink); }
+  __device__ inline int slot(int r) const {
+    const int p = position(r);
+    return p < sink ? p : sink + (p - sink) % ring;
+  }
+};
+template <typename T, int D, bool EIGHT>
+__global__ __launch_bounds__(256) void held_rows_kernel(
+    const void* __restrict__ kc, const void* __restrict__ vc, const uint8_t* __restrict__ ks,
+    const uint8_t* __restrict__ vs, typename T::storage* __restrict__ ko, typename T::storage* __restrict__ vo,
+    int64_t* __restrict__ positions, int BH, HeldRows a) {
+  using S = typename T::storage;
+  constexpr int LPR = D / 8;
+  const int ch = threadIdx.x % LPR;
+  const int64_t n = (int64_t)BH * a.n;
+  for (int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR; row < 2 * n;
+       row += (int64_t)gridDim.x * (256 / LPR)) {
+    const bool is_v = row >= n;
+    const int64_t rr = is_v ? row - n : row;
+    const int bh = (int)(rr / a.n), r = (int)(rr % a.n);
+    if (row < a.n && ch == 0) positions[r] = a.position(r);
+    const size_t src = (size_t)bh * (a.sink + a.ring) + a.slot(r);
+    S* dst = (is_v ? vo : ko) + (size_t)rr * D + 8 * ch;
+    if constexpr (EIGHT) {
+      const float s = scale_of((is_v ? vs : ks)[src]);
+      const uint2 w = *(const uint2*)((const uint8_t*)(is_v ? vc : kc) + src * D + 8 * ch);
+      const f32x2 x[4] = {codes2(w.x, false, s), codes2(w.x, true, s), codes2(w.y, false, s), codes2(w.y, true, s)};
+      if constexpr (T::is_f32) {
+        *(float4*)dst = make_float4(x[0][0], x[0][1], x[1][0], x[1][1]);
+        *(float4*)(dst + 4) = make_float4(x[2][0], x[2][1], x[3][0], x[3][1]);
+      } else {
+        *(uint4*)dst = make_uint4(pack2<T>(x[0][0], x[0][1]), pack2<T>(x[1][0], x[1][1]), pack2<T>(x[2][0], x[2][1]),
+                                  pack2<T>(x[3][0], x[3][1]));
+      }
+    } else {
+      const S* from = (const S*)(is_v ? vc : kc) + src * D + 8 * ch;
+      *(uint4*)dst = *(const uint4*)from;
+      if constexpr (T::is_f32) *(uint4*)(dst + 4) = *(const uint4*)(from + 4);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention.
+// ---------------------------------------------------------------------------
+// The tokens of a rolling cache that some of its n_q last positions see: sinks
+// 0 .. n_sink - 1, then positions w_lo .. length - 1.
+struct RingStream {
+  int n_tokens, n_sink, w_lo, sink, ring, base, q_off, window;   // base: (w_lo - sink) mod ring
+  __device__ inline int count(int) const { return n_tokens; }
+  __device__ inline int row(int t) const {
+    if (t < n_sink) return t;
+    const int j = base + (t - n_sink);
+    return sink + (j >= ring ? j - ring : j);
+  }
+  // token rule of query position i
+  __device__ inline bool visible(int i, int t) const {
+    const int p = t < n_sink ? t : w_lo + (t - n_sink), qa = q_off + i;
+    return (p <= qa) & ((p < sink) | (p > qa - window));
+  }
+};
+
+struct StreamArgs {
+  const void *q, *k, *v;
+  const uint8_t *ks, *vs;      // exponents of the 8-bit rows
+  void* o;
+  float* lse;
+  float *acc, *ml;             // states of the slices: [rows][n_parts][D] and [rows][n_parts][2]
+  int H_kv, rb;                // rb = group * n_q: rows of Q that one (b, kv head) has, one after another
+  int n_q, q_stride;           // q_stride = H * n_q rows of Q between batch entries
+  int kv_rows;                 // rows that K and V hold per stream
+  int n_rows, row_tiles;       // query rows of a stream, and tiles of them
+  int n_splits, n_parts;       // slices here; states per row in the workspace (1: O and LSE are written here)
+  float scale_log2;            // |scale| log2 e (log2 e for scale 0), the sign in q_sign
+  float q_sign;                // 1, -1, or 0: the scores are those of q_sign * q
+};
+
+// Queries as 1, 2 or 3 bfloat16 pieces whose sum they are (8, 11 and 24 significant
+// bits), so that products with the stored values are those of the queries themselves.
+template <typename T> constexpr int kPieces = std::is_same<T, BF16>::value ? 1 : std::is_same<T, F16>::value ? 2 : 3;
+
+template <int NPC>
+__device__ inline void split8(float (&f)[8], uint4 (&piece)[NPC]) {
+#pragma unroll
+  for (int n = 0; n < NPC; ++n) {
+    piece[n] = make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]),
+                          pack2<BF16>(f[6], f[7]));
+    if (n + 1 < NPC) {
+      const uint16_t* h = (const uint16_t*)&piece[n];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] -= BF16::to_float(h[i]);
+    }
+  }
+}
+
+// A workgroup of four waves: 16 NB query rows (columns of S^T = K Q^T on
+// v_mfma_f32_16x16x32_bf16) against a slice of the stream, 64 tokens at a time, 16
+// per wave. The tokens' codes come by 16-byte loads into registers, two steps ahead,
+// and are written to LDS as bfloat16 (v_cvt_scalef32_pk_bf16_fp8 applies the scale);
+// V^T operands by one transposed LDS read each. Each wave keeps a softmax state of
+// its own tokens; they meet in LDS at the end. fp16 and fp32 queries, and their
+// probabilities, are 2 and 3 bfloat16 pieces: 2 and 3 times the products, of which
+// the memory-bound stream leaves room for. bf16: P is rounded to bfloat16 for P V, as
+// in the 16-bit decode (half a unit of 2^-8 of each weight, averaged over the keys);
+// the row sums add the fp32 P.
+template <typename T, int D, int NB, bool RULE, class Src>
+__global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
+  constexpr int NPC = kPieces<T>;
+  constexpr int KS = D / 32, DT = D / 16;
+  constexpr int UPR = D / 16;                  // 16-byte units per row
+  constexpr int NU = kTileN * UPR / 256;       // units per thread and tile
+  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
+  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = lane >> 4, col = lane & 15;
+  int lb = xcd_remap(blockIdx.x, gridDim.x);
+  const int rt = lb % a.row_tiles;
+  lb /= a.row_tiles;
+  const int split = lb % a.n_splits, s_id = lb / a.n_splits;
+  const int row0 = rt * 16 * NB;
+  const size_t q_row0 = (size_t)(s_id / a.H_kv) * a.q_stride + (size_t)(s_id % a.H_kv) * a.rb;
+  const size_t kb = (size_t)s_id * a.kv_rows;
+  const int n_tok = src.count(s_id);
+  const int g0 = (int)(((int64_t)n_tok * split) / a.n_splits);
+  const int g1 = (int)(((int64_t)n_tok * (split + 1)) / a.n_splits);
+  const int n_chunks = (g1 - g0 + kTileN - 1) / kTileN;
+  const uint8_t *K = (const uint8_t*)a.k, *V = (const uint8_t*)a.v;
+
+  struct Raw {
+    uint4 k[NU], v[NU];
+    uint8_t ks[NU], vs[NU];
+  };
+  // tokens past the slice repeat its last one and are masked when consumed
+  auto fetch = [&](int c, Raw& r) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int unit = u * 256 + tid;
+      const size_t at = kb + src.row(min(g0 + c * kTileN + unit / UPR, g1 - 1));
+      r.k[u] = ld_nt16(K + at * D + 16 * (unit % UPR));
+      r.ks[u] = a.ks[at];
+      r.v[u] = ld_nt16(V + at * D + 16 * (unit % UPR));
+      r.vs[u] = a.vs[at];
+    }
+  };
+  auto put16 = [&](uint16_t* tile, int row, int c16, const uint4& w, float scale) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t out[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], scale, false));
+      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], scale, true));
+    }
+    *(uint4*)(tile + lds_off<D>(row, 16 * c16)) = make_uint4(out[0], out[1], out[2], out[3]);
+    *(uint4*)(tile + lds_off<D>(row, 16 * c16 + 8)) = make_uint4(out[4], out[5], out[6], out[7]);
+  };
+  auto put = [&](const Raw& r, int b) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int unit = u * 256 + tid;
+      put16(sk[b], unit / UPR, unit % UPR, r.k[u], scale_of(r.ks[u]));
+      put16(sv[b], unit / UPR, unit % UPR, r.v[u], scale_of(r.vs[u]));
+    }
+  };
+
+  Raw ra, rc;
+  if (n_chunks > 0) fetch(0, ra);
+  if (n_chunks > 1) fetch(1, rc);
+
+  // Q^T operand of column block h: lane (grp, col) holds elements 32 ks + 8 grp .. +7
+  // of row row0 + 16 h + col
+  uint4 qf[NB][KS][NPC];
+  int my_q[NB];
+#pragma unroll
+  for (int h = 0; h < NB; ++h) {
+    const int r = row0 + 16 * h + col;
+    my_q[h] = r % a.n_q;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float f[8];
+      load8<T>((const typename T::storage*)a.q + (q_row0 + (r < a.n_rows ? r : 0)) * D + 32 * ks + 8 * grp, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = r < a.n_rows && a.q_sign != 0.f ? f[i] * a.q_sign : 0.f;
+      split8<NPC>(f, qf[h][ks]);
+    }
+  }
+
+  floatx4 o[NB][DT];
+  float lsum[NB], m[NB];
+#pragma unroll
+  for (int h = 0; h < NB; ++h) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[h][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+    lsum[h] = 0.f;
+    m[h] = kNegInf;
+  }
+
+  auto consume = [&](int c, int b) {
+    const uint16_t *ck = sk[b], *cv = sv[b];
+    floatx4 s[NB];
+#pragma unroll
+    for (int h = 0; h < NB; ++h) s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint4 x = lds_row8<D>(ck, 16 * wave + col, 32 * ks + 8 * grp);
+#pragma unroll
+      for (int h = 0; h < NB; ++h)
+#pragma unroll
+        for (int n = 0; n < NPC; ++n) s[h] = BF16::mfma(x, qf[h][ks][n], s[h]);
+    }
+    // lane (grp, col): s[h][i] = score of token t0 + i for row row0 + 16 h + col
+    const int t0 = g0 + c * kTileN + 16 * wave + 4 * grp;
+    uint2 pb[NB][NPC];
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bool ok = t0 + i < g1;
+        if constexpr (RULE) ok = ok && src.visible(my_q[h], t0 + i);
+        s[h][i] = ok ? s[h][i] : kNegInf;
+      }
+      float mx = fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3]));
+      if (__any(mx * a.scale_log2 > m[h] + kStreamSlack)) {
+        mx = wave_max16x4(mx) * a.scale_log2;
+        const bool grow = mx > m[h] + kStreamSlack;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m[h] - mx) : 1.f;
+        m[h] = grow ? mx : m[h];
+        lsum[h] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[h][dt] *= alpha;
+      }
+      const float m_use = m[h] == kNegInf ? 0.f : m[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        s[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], a.scale_log2, -m_use));
+      lsum[h] += (s[h][0] + s[h][1]) + (s[h][2] + s[h][3]);
+#pragma unroll
+      for (int n = 0; n < NPC; ++n) {
+        pb[h][n] = make_uint2(pack2<BF16>(s[h][0], s[h][1]), pack2<BF16>(s[h][2], s[h][3]));
+        if (n + 1 < NPC) {
+          const uint16_t* p = (const uint16_t*)&pb[h][n];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][i] -= BF16::to_float(p[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const uint2 x = lds_tr4<D>(cv, 16 * wave, 16 * dt, lane);
+#pragma unroll
+      for (int h = 0; h < NB; ++h)
+#pragma unroll
+        for (int n = 0; n < NPC; ++n) o[h][dt] = mfma16k<BF16>(x, pb[h][n], o[h][dt]);
+    }
+  };
+  // One barrier per step: a buffer is rewritten two steps on, when every wave has
+  // passed the barrier of the step between.
+  auto step = [&](int c, int b, Raw& r) {
+    put(r, b);
+    if (c + 2 < n_chunks) fetch(c + 2, r);
+    __syncthreads();
+    consume(c, b);
+  };
+  int c = 0;
+  for (; c + 1 < n_chunks; c += 2) {
+    step(c, 0, ra);
+    step(c + 1, 1, rc);
+  }
+  if (c < n_chunks) step(c, 0, ra);
+
+  // The four waves' states meet, one column block at a time: lane (grp, col) holds
+  // O^T rows 16 dt + 4 grp + i of row row0 + 16 h + col.
+  float* wacc = (float*)&sk[0][0];             // [4][16][D]: both K buffers
+  float* wml = (float*)&sv[0][0];              // [4][16][2]
+#pragma unroll
+  for (int h = 0; h < NB; ++h) {
+    const float lw = wave_sum16x4(lsum[h]);
+    __syncthreads();                           // the buffers' (or the previous block's) readers are done
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      *(floatx4*)(wacc + (wave * 16 + col) * D + 16 * dt + 4 * grp) = o[h][dt];
+    if (grp == 0) {
+      wml[(wave * 16 + col) * 2] = m[h];
+      wml[(wave * 16 + col) * 2 + 1] = lw;
+    }
+    __syncthreads();
+    const int rows_h = min(16, a.n_rows - row0 - 16 * h);
+    for (int idx = tid; idx < rows_h * (D / 4); idx += 256) {
+      const int rl = idx / (D / 4), d = 4 * (idx % (D / 4));
+      const size_t row = q_row0 + row0 + 16 * h + rl;
+      float M = kNegInf;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, wml[(w * 16 + rl) * 2]);
+      const float Mu = M == kNegInf ? 0.f : M;
+      float L = 0.f;
+      floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(wml[(w * 16 + rl) * 2] - Mu);
+        L += wml[(w * 16 + rl) * 2 + 1] * f;
+        x += *(const floatx4*)(wacc + (w * 16 + rl) * D + d) * f;
+      }
+      if (a.n_parts == 1) {
+        const float den = L == 0.f ? 1.f : L;  // no visible token: 0; NaN stays NaN
+        x = x / den;
+        typename T::storage* dst = (typename T::storage*)a.o + row * D + d;
+        if constexpr (T::is_f32) *(floatx4*)dst = x;
+        else *(uint2*)dst = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+        if (d == 0) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
+      } else {
+        *(floatx4*)(a.acc + (row * a.n_parts + split) * D + d) = x;
+        if (d == 0) *(float2*)(a.ml + (row * a.n_parts + split) * 2) = make_float2(M, L);
+      }
+    }
+  }
+}
+
+// The states of a row's n_parts slices joined: a wave per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc, const float* __restrict__ ml,
+                                                   typename T::storage* __restrict__ O, float* __restrict__ LSE,
+                                                   int64_t n_rows, int n_parts) {
+  constexpr int E = D / 64;                    // elements per lane
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= n_rows) return;
+  const float2* st = (const float2*)ml + row * n_parts;
+  const float* x = acc + row * n_parts * D + E * lane;
+  float M = kNegInf;
+#pragma unroll 4
+  for (int p = 0; p < n_parts; ++p) M = fmaxf(M, st[p].x);
+  const float Mu = M == kNegInf ? 0.f : M;
+  float L = 0.f, a[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) a[e] = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < n_parts; ++p) {
+    const float f = __builtin_amdgcn_exp2f(st[p].x - Mu);
+    L += st[p].y * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) a[e] += x[(size_t)p * D + e] * f;
+  }
+  typename T::storage* dst = O + row * D + E * lane;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = T::from_float(a[e] / (L == 0.f ? 1.f : L));
+  if (lane == 0) LSE[row] = L == 0.f ? 0.f : lse_natural(M, L);
+}
+
+template <typename T, int D>
+void launch_join(const StreamArgs& a, int64_t n_rows, hipStream_t stream) {
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, stream, a.acc, a.ml,
+                     (typename T::storage*)a.o, a.lse, n_rows, a.n_parts);
+}
+
+template <typename T, int D, int NB>
+void launch_stream8(const StreamArgs& a, const RingStream& src, int n_streams, hipStream_t stream) {
+  const dim3 grid(n_streams * a.n_splits * a.row_tiles);
+  if (a.n_q == 1) hipLaunchKernelGGL((stream8_kernel<T, D, NB, false, RingStream>), grid, dim3(256), 0, stream, a, src);
+  else hipLaunchKernelGGL((stream8_kernel<T, D, NB, true, RingStream>), grid, dim3(256), 0, stream, a, src);
+}
+
+template <typename T, int D>
+int attend8(StreamArgs a, const RingStream& src, int n_streams, hipStream_t stream) {
+  const int tile = stream_rows_tile(T::is_f32, a.n_rows);
+  a.row_tiles = (a.n_rows + tile - 1) / tile;
+  if constexpr (!T::is_f32) {
+    if (tile == 32) launch_stream8<T, D, 2>(a, src, n_streams, stream);
+    else launch_stream8<T, D, 1>(a, src, n_streams, stream);
+  } else {
+    launch_stream8<T, D, 1>(a, src, n_streams, stream);
+  }
+  if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
+  return check_launch("gki_rolling8_decode");
+}
+
+// A workgroup per 256 lanes of work, up to a grid whose lanes a launch can count.
+inline dim3 row_grid(int64_t lanes) { return dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)); }
+
+template <typename T, int D>
+int append8(uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn, const void* vn, int BH,
+            const AppendRows& a, hipStream_t stream) {
+  const int64_t lanes = 2 * (int64_t)BH * (a.n_a + a.n_b) * (D / 8);
+  if (lanes == 0) return 0;
+  using S = typename T::storage;
+  hipLaunchKernelGGL((append8_kernel<T, D>), row_grid(lanes), dim3(256), 0, stream, kc, vc, ks,
+                     vs, (const S*)kn, (const S*)vn, BH, a);
+  return check_launch("gki_rolling8_append");
+}
+
+template <typename T, int D>
+int held_rows(const void* kc, const void* vc, const uint8_t* ks, const uint8_t* vs, void* ko, void* vo,
+              int64_t* positions, int BH, const HeldRows& a, hipStream_t stream) {
+  using S = typename T::storage;
+  const int64_t lanes = 2 * (int64_t)BH * a.n * (D / 8);
+  const dim3 grid = row_grid(lanes);
+  if (ks) hipLaunchKernelGGL((held_rows_kernel<T, D, true>), grid, dim3(256), 0, stream, kc, vc, ks, vs, (S*)ko, (S*)vo, positions, BH, a);
+  else hipLaunchKernelGGL((held_rows_kernel<T, D, false>), grid, dim3(256), 0, stream, kc, vc, ks, vs, (S*)ko, (S*)vo, positions, BH, a);
+  return check_launch("gki_rolling_read");
+}
+
+}  // namespace
+
+#define GKI_BY_TYPE(FN, ...)                                                        \
+  if (head_dim == 64) {                                                             \
+    if (dtype == kF32) return FN<F32, 64>(__VA_ARGS__);                             \
+    if (dtype == kF16) return FN<F16, 64>(__VA_ARGS__);                             \
+    return FN<BF16, 64>(__VA_ARGS__);                                               \
+  }                                                                                 \
+  if (dtype == kF32) return FN<F32, 128>(__VA_ARGS__);                              \
+  if (dtype == kF16) return FN<F16, 128>(__VA_ARGS__);                              \
+  return FN<BF16, 128>(__VA_ARGS__);
+
+int append8_dispatch(int dtype, int head_dim, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn,
+                     const void* vn, int BH, int n_new, int start, int sink, int ring, hipStream_t stream) {
+  AppendRows a{n_new, 0, 0, 0, start, sink, ring};
+  surviving_rows(start, n_new, sink, ring, &a.n_a, &a.i_b, &a.n_b);
+  GKI_BY_TYPE(append8, kc, vc, ks, vs, kn, vn, BH, a, stream)
+}
+
+int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const uint8_t* ks, const uint8_t* vs,
+                  void* ko, void* vo, int64_t* positions, int BH, int length, int sink, int ring,
+                  hipStream_t stream) {
+  HeldRows a{};
+  a.n_sink = length < sink ? length : sink;
+  a.lo = length - ring > sink ? length - ring : sink;
+  a.n = a.n_sink + (length > a.lo ? length - a.lo : 0);
+  a.sink = sink;
+  a.ring = ring;
+  if (a.n == 0) return 0;
+  GKI_BY_TYPE(held_rows, kc, vc, ks, vs, ko, vo, positions, BH, a, stream)
+}
+
+int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                     const uint8_t* ks, const uint8_t* vs, void* o, float* lse, int ring, float* ws, int n_splits,
+                     hipStream_t stream) {
+  RingStream src;
+  ring_stream(g.n_kv, g.n_q, g.sink, g.window, ring, &src.n_sink, &src.w_lo, &src.base, &src.n_tokens);
+  src.sink = g.sink;
+  src.ring = ring;
+  src.q_off = g.q_off;
+  src.window = g.window;
+  StreamArgs a{};
+  a.q = q, a.k = k, a.v = v, a.ks = ks, a.vs = vs, a.o = o, a.lse = lse;
+  a.H_kv = g.H_kv;
+  a.rb = a.n_rows = g.group * g.n_q;
+  a.n_q = g.n_q;
+  a.q_stride = g.H * g.n_q;
+  a.kv_rows = g.sink + ring;
+  a.n_splits = a.n_parts = n_splits;
+  a.acc = ws;
+  a.ml = ws + (size_t)g.B * g.H * g.n_q * n_splits * head_dim;
+  a.scale_log2 = g.qk_scale_log2;
+  a.q_sign = g.scale == 0.f ? 0.f : g.scale < 0.f ? -1.f : 1.f;
+  GKI_BY_TYPE(attend8, a, src, g.B * g.H_kv, stream)
+}
+
+}  // namespace gki

@@ -58,6 +58,12 @@ SIGNATURES = {
                                                                        _c_int, _c_ptr]),
     "gki_rolling_decode_noalloc": (ctypes.c_int, [_c_ptr] * 5 + [_c_int] * 9
                                    + [_c_i64, _c_float, _c_int, _c_ptr]),
+    "gki_stream_splits": (ctypes.c_int, [_c_int] * 6 + [_c_i64]),
+    "gki_stream_workspace_floats": (ctypes.c_int64, [_c_int] * 5),
+    "gki_rolling8_append": (ctypes.c_int, [_c_ptr] * 6 + [_c_int] * 6 + [_c_i64, _c_int, _c_ptr]),
+    "gki_rolling_read": (ctypes.c_int, [_c_ptr] * 7 + [_c_int] * 6 + [_c_i64, _c_ptr]),
+    "gki_rolling8_decode": (ctypes.c_int, [_c_ptr] * 7 + [_c_int] * 9 + [_c_i64, _c_float, _c_ptr,
+                                                                        _c_int, _c_ptr]),
     "gki_read_probe_words": (ctypes.c_int64, [_c_int]),
     "gki_read_probe": (ctypes.c_int, [_c_ptr, _c_ptr, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_ptr,
                                       _c_i64, _c_ptr]),

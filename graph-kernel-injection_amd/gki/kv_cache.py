@@ -19,6 +19,11 @@ mask and ``is_causal=True``), so both give the same bits.
 
 For c4's shape (B8 H32 D128 bf16, S4 W2048) the cache holds 2055 of 100000
 positions: 2 x 135 MB instead of 2 x 6.55 GB.
+
+``storage_dtype=torch.float8_e4m3fn`` holds each row in 8 bits: e4m3 codes and one
+power of two (``k_scale`` / ``v_scale``), the smallest 2^e with the row's largest
+magnitude at most 448 * 2^e. Rows are quantised as they are appended, attention runs
+over the stored values (code * 2^e), and ``read`` gives back what either kind holds.
 """
 
 from __future__ import annotations
@@ -62,13 +67,21 @@ class StreamingKVCache:
     ``H`` = ``heads`` = the K/V heads. Queries may have any multiple of ``heads``
     (grouped-query attention: q head h reads kv head h // (Hq // heads)).
     ``length`` counts the positions appended so far (0 .. length-1).
+
+    ``storage_dtype``: what the cache holds its rows in, ``dtype`` (the default) or
+    ``torch.float8_e4m3fn``. In 8 bits ``k_cache`` / ``v_cache`` are the codes and
+    ``k_scale`` / ``v_scale`` (``float8_e8m0fnu``, ``[B, H, sink_size + ring_size]``)
+    the rows' powers of two; infinities and NaN are stored as NaN, and tokens, queries
+    and outputs keep ``dtype``. No gradient flows through the cache.
     """
 
     def __init__(self, batch: int, heads: int, head_dim: int, spec: StreamingMaskSpec,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda",
-                 max_query: int = 4) -> None:
+                 max_query: int = 4, storage_dtype: Optional[torch.dtype] = None) -> None:
         if dtype not in _DTYPE_CODE:
             raise ValueError(f"dtype must be one of float32/float16/bfloat16, got {dtype}")
+        if storage_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise ValueError(f"storage_dtype must be {dtype} or torch.float8_e4m3fn, got {storage_dtype}")
         if head_dim not in _DECODE_HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {_DECODE_HEAD_DIMS}, got {head_dim}")
         max_q = _lib.tile_sizes()["decode_max_q"]
@@ -89,9 +102,16 @@ class StreamingKVCache:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         shape = (self.batch, self.heads, self.sink_size + self.ring_size, self.head_dim)
-        self.k_cache = torch.zeros(shape, dtype=dtype, device=self.device)
-        self.v_cache = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.storage_dtype = storage_dtype or dtype
+        self.k_cache = torch.zeros(shape, dtype=self.storage_dtype, device=self.device)
+        self.v_cache = torch.zeros(shape, dtype=self.storage_dtype, device=self.device)
+        self.k_scale = self.v_scale = None
+        if self.storage_dtype != dtype:
+            self.k_scale, self.v_scale = (
+                torch.zeros(shape[:3], dtype=torch.uint8, device=self.device).view(torch.float8_e8m0fnu)
+                for _ in range(2))
         self.length = 0
+        self._plans: dict = {}           # (Hq, n_q, tokens) -> launch plan of an 8-bit attend
 
     @property
     def capacity(self) -> int:
@@ -125,11 +145,40 @@ class StreamingKVCache:
         lib = _lib.load()
         with _on_device(self.device):
             stream = _current_stream(self.device)
-            _lib.check(lib.gki_rolling_append(
-                self.k_cache.data_ptr(), self.v_cache.data_ptr(), k.data_ptr(), v.data_ptr(),
-                _DTYPE_CODE[self.dtype], self.batch, self.heads, self.head_dim, self.sink_size,
-                self.ring_size, self.length, n, stream), "gki_rolling_append")
+            if self.k_scale is None:
+                _lib.check(lib.gki_rolling_append(
+                    self.k_cache.data_ptr(), self.v_cache.data_ptr(), k.data_ptr(), v.data_ptr(),
+                    _DTYPE_CODE[self.dtype], self.batch, self.heads, self.head_dim, self.sink_size,
+                    self.ring_size, self.length, n, stream), "gki_rolling_append")
+            else:
+                _lib.check(lib.gki_rolling8_append(
+                    self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_scale.data_ptr(),
+                    self.v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[self.dtype],
+                    self.batch, self.heads, self.head_dim, self.sink_size, self.ring_size, self.length,
+                    n, stream), "gki_rolling8_append")
         self.length += n
+
+    def read(self) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """What the cache holds: ``(positions, k, v)``, the held positions ascending
+        (``int64 [n]``: the sinks, then the last ``ring_size``) and their keys and
+        values ``[B, H, n, D]`` in ``dtype`` -- from 8 bits the stored values, those
+        past ``dtype``'s range as its infinities."""
+        n = min(self.length, self.sink_size) + max(
+            0, self.length - max(self.sink_size, self.length - self.ring_size))
+        positions = torch.empty(n, dtype=torch.int64, device=self.device)
+        shape = (self.batch, self.heads, n, self.head_dim)
+        k, v = (torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
+        if n:
+            lib = _lib.load()
+            eight = self.k_scale is not None
+            with _on_device(self.device):
+                _lib.check(lib.gki_rolling_read(
+                    self.k_cache.data_ptr(), self.v_cache.data_ptr(),
+                    self.k_scale.data_ptr() if eight else 0, self.v_scale.data_ptr() if eight else 0,
+                    k.data_ptr(), v.data_ptr(), positions.data_ptr(), _DTYPE_CODE[self.dtype],
+                    self.batch, self.heads, self.head_dim, self.sink_size, self.ring_size, self.length,
+                    _current_stream(self.device)), "gki_rolling_read")
+        return positions, k, v
 
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
                return_lse: bool = False):
@@ -146,6 +195,8 @@ class StreamingKVCache:
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(self.head_dim)
         q = _aligned(q)
+        if self.k_scale is not None:
+            return self._attend8(q, n_q, float(softmax_scale), return_lse)
         _, _, n_tokens = rolling_stream(self.length, n_q, self.sink_size, self.window_size,
                                         self.ring_size)
         B, H, H_kv = self.batch, int(q.shape[1]), self.heads
@@ -164,6 +215,35 @@ class StreamingKVCache:
                 self.window_size, self.ring_size, self.length, float(softmax_scale),
                 scratch.data_ptr() + 4 * pad if ws_floats else 0, n_splits, stream),
                 "gki_rolling_decode")
+        if not return_lse:
+            return o
+        return o, scratch[:B * H * n_q].view(B, H, n_q).clone()
+
+    def _attend8(self, q: torch.Tensor, n_q: int, softmax_scale: float, return_lse: bool):
+        """The decode over 8-bit rows."""
+        lib = _lib.load()
+        B, H, D, length = self.batch, int(q.shape[1]), self.head_dim, self.length
+        n_tokens = min(length, self.sink_size) + max(
+            0, length - max(self.sink_size, length - n_q - self.window_size + 1))
+        dtype = _DTYPE_CODE[self.dtype]
+        plan = self._plans.get((H, n_q, n_tokens))
+        if plan is None:
+            if len(self._plans) >= 4096:     # a filling window adds one key per step
+                self._plans.clear()
+            splits = int(lib.gki_stream_splits(dtype, B, H, self.heads, n_q, D, n_tokens))
+            plan = self._plans[H, n_q, n_tokens] = (
+                splits, int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits)))
+        n_splits, ws_floats = plan
+        o = torch.empty_like(q)
+        pad = (B * H * n_q + 63) & ~63
+        scratch = torch.empty(pad + ws_floats, dtype=torch.float32, device=self.device)
+        with _on_device(self.device):
+            rc = lib.gki_rolling8_decode(
+                q.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_scale.data_ptr(),
+                self.v_scale.data_ptr(), o.data_ptr(), scratch.data_ptr(), dtype, B, H, self.heads, n_q, D,
+                self.sink_size, self.window_size, self.ring_size, length, softmax_scale,
+                scratch.data_ptr() + 4 * pad if ws_floats else 0, n_splits, _current_stream(self.device))
+        _lib.check(rc, "gki_rolling8_decode")
         if not return_lse:
             return o
         return o, scratch[:B * H * n_q].view(B, H, n_q).clone()

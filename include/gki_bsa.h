@@ -259,6 +259,49 @@ int gki_rolling_decode_noalloc(const void* q, const void* k_cache, const void* v
                                int32_t window_size, int32_t ring_size, int64_t length,
                                float softmax_scale, int32_t n_splits, void* stream);
 
+/* ---- Rolling cache held in 8 bits -------------------------------------------
+ * No reference counterpart. The cache above with each row of head_dim values
+ * stored as head_dim e4m3 codes (k_codes / v_codes, uint8 [B, H, sink_size +
+ * ring_size, head_dim]) and one byte (k_scale / v_scale, uint8 [B, H, sink_size +
+ * ring_size]) e + 127, e the smallest integer >= -117 with max |x| <= 448 * 2^e
+ * over the row's finite values: a value is code * 2^e, code the e4m3 number
+ * nearest to x * 2^-e (ties to even). Infinities and NaN are stored as NaN.
+ * `dtype` is that of the rows outside (k_new, q, o); head_dim 64 or 128. */
+
+/* Quantise n_new tokens as they are written at positions start_pos ..
+ * start_pos + n_new - 1; rules as gki_rolling_append. */
+int gki_rolling8_append(void* k_codes, void* v_codes, void* k_scale, void* v_scale,
+                        const void* k_new, const void* v_new, int32_t dtype, int32_t B, int32_t H,
+                        int32_t head_dim, int32_t sink_size, int32_t ring_size, int64_t start_pos,
+                        int32_t n_new, void* stream);
+
+/* What a rolling cache of `length` positions holds: the n = min(length, sink_size)
+ * + max(0, length - max(sink_size, length - ring_size)) positions, ascending, into
+ * positions[n], and their rows as `dtype` into k_out / v_out [B, H, n, head_dim].
+ * k_scale and v_scale: the 8-bit cache's (its k_codes / v_codes as k_cache /
+ * v_cache), or both NULL for a cache that holds `dtype` itself. */
+int gki_rolling_read(const void* k_cache, const void* v_cache, const void* k_scale,
+                     const void* v_scale, void* k_out, void* v_out, int64_t* positions,
+                     int32_t dtype, int32_t B, int32_t H, int32_t head_dim, int32_t sink_size,
+                     int32_t ring_size, int64_t length, void* stream);
+
+/* Slices that the decode calls below cut each stream of n_tokens tokens into for a
+ * full card (any n_splits >= 1 is right), and the floats of 16-byte aligned
+ * workspace that n_parts states per query row need (0 for one). */
+int gki_stream_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
+                          int32_t head_dim, int64_t n_tokens);
+int64_t gki_stream_workspace_floats(int32_t B, int32_t H, int32_t n_q, int32_t head_dim,
+                                    int32_t n_parts);
+
+/* Decode step over the 8-bit cache: as gki_rolling_decode, over the stored
+ * values. Any number of q heads per K/V head; workspace of
+ * gki_stream_workspace_floats(B, H, n_q, head_dim, n_splits) floats. */
+int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes, const void* k_scale,
+                        const void* v_scale, void* o, float* lse, int32_t dtype, int32_t B, int32_t H,
+                        int32_t H_kv, int32_t n_q, int32_t head_dim, int32_t sink_size,
+                        int32_t window_size, int32_t ring_size, int64_t length, float softmax_scale,
+                        float* workspace, int32_t n_splits, void* stream);
+
 /* Measurement helper, no counterpart in the reference: reads exactly the K and V
  * bytes a single-position StreamingLLM decode step reads from a full cache --
  * per (b, kv head) slice of bh slices of n_kv rows of row_bytes (a multiple of
