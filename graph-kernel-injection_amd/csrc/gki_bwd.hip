@@ -69,21 +69,34 @@ __device__ inline uint4 and4(const uint4& v, uint32_t m) {
 struct KvItem {
   int kt, it0, it1, pslot;
 };
-__device__ inline KvItem kv_item_of(int b, int BH, const KvWork& w, int& bh) {
+// Item i of one (b, kv head): listed, or part i % parts of kv tile i / parts's walk.
+__device__ inline int q_tiles_of(const Geom& g) { return (g.n_q + kTileM - 1) / kTileM; }
+template <bool DENSE>
+__device__ inline KvItem kv_item(const Geom& g, const KvWork& w, int i) {
+  if constexpr (DENSE) {
+    const int kt = i / w.parts, c = i - kt * w.parts;
+    const int64_t n_it = (int64_t)q_tiles_of(g) * g.group;
+    return {kt, (int)(n_it * c / w.parts), (int)(n_it * (c + 1) / w.parts), w.parts > 1 ? i : -1};
+  } else {
+    const int4 t = ((const int4*)w.items)[i];
+    return {t.x, t.y, t.z, t.w};
+  }
+}
+template <bool DENSE>
+__device__ inline KvItem kv_item_of(int b, int BH, const Geom& g, const KvWork& w, int& bh) {
   const int wg = xcd_remap(b, w.n_items * BH);
   bh = wg / w.n_items;
-  const int4 t = ((const int4*)w.items)[wg - bh * w.n_items];
-  return {t.x, t.y, t.z, t.w};
+  return kv_item<DENSE>(g, w, wg - bh * w.n_items);
 }
 
 // The same for items cut into `parts` workgroups each (work_parts_grid); bh < 0
 // for a workgroup past the last.
-__device__ inline KvItem kv_item_part_of(int b, int BH, int parts, const KvWork& w, int& bh, int& part) {
+template <bool DENSE>
+__device__ inline KvItem kv_item_part_of(int b, int BH, int parts, const Geom& g, const KvWork& w, int& bh, int& part) {
   const int wg = work_part_of(b, w.n_items * BH, parts, nullptr, part);
   bh = wg < 0 ? -1 : wg / w.n_items;
   if (wg < 0) return {0, 0, 0, -1};
-  const int4 t = ((const int4*)w.items)[wg - bh * w.n_items];
-  return {t.x, t.y, t.z, t.w};
+  return kv_item<DENSE>(g, w, wg - bh * w.n_items);
 }
 
 // Sum of a split column's fp32 partials, in item order, cast to the storage
@@ -93,7 +106,7 @@ __device__ inline KvItem kv_item_part_of(int b, int BH, int parts, const KvWork&
 template <int D>
 constexpr int kReduceWgPerTile = 2 * kTileN * D / (256 * 4);
 
-template <typename T, int D>
+template <typename T, int D, bool DENSE>
 __global__ __launch_bounds__(256) void dkdv_reduce_kernel(Geom g, KvWork w,
                                                           typename T::storage* __restrict__ dK,
                                                           typename T::storage* __restrict__ dV) {
@@ -102,7 +115,10 @@ __global__ __launch_bounds__(256) void dkdv_reduce_kernel(Geom g, KvWork w,
   constexpr int WGT = kReduceWgPerTile<D>;
   const int rest = blockIdx.x / WGT, part = blockIdx.x - rest * WGT;
   const int bh = rest / w.n_split, s = rest - bh * w.n_split;
-  const int kt = w.split[3 * s], p0 = w.split[3 * s + 1], np = w.split[3 * s + 2];
+  const int kt = DENSE ? s : w.split[3 * s], p0 = DENSE ? s * w.parts : w.split[3 * s + 1];
+  int np = DENSE ? w.parts : w.split[3 * s + 2];
+  if constexpr (DENSE)       // past the entry's keys there are no partials, and the sums are zeros
+    if (kt * kTileN >= own_keys(g, bh / g.H_kv)) np = 0;
   const int idx = (part * 256 + threadIdx.x) * 4;      // first float of this thread
   const float4* src = (const float4*)(w.partials + ((size_t)bh * w.n_pslots + p0) * 2 * TILE + idx);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -158,7 +174,7 @@ __global__ __launch_bounds__(256) void dkdv_reduce_kernel(Geom g, KvWork w,
 // and this form, 7% fewer cycles at a 10% lower clock, ran 2-3% slower than the
 // 16x16x32 quadrants below.
 // FORM: Geom::bwd_form. A template parameter, so no form carries a branch.
-template <typename T, int D, int FORM>
+template <typename T, int D, int FORM, bool DENSE>
 __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void dkdv_kernel_16(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ dO, uint16_t* __restrict__ dK,
@@ -181,11 +197,20 @@ __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void 
   // over (q head of the group, CSC list entry), accumulated in registers
   const int BH = g.B * g.H_kv;
   int bh;
-  const KvItem item = kv_item_of(blockIdx.x, BH, w, bh);
+  KvItem item = kv_item_of<DENSE>(blockIdx.x, BH, g, w, bh);
   // an empty column (no kept q tile) only writes zeros: its K / V rows are not read
-  const bool has_work = item.it1 > item.it0;
   const int kt = item.kt;
   const size_t kb = (size_t)bh * g.n_kv * D;
+  const int n_rows = g.n_kv;                   // rows of dK / dV
+  if constexpr (DENSE) {
+    // a kv tile past the entry's keys: zeros (from the reduce where the column is split)
+    g.n_kv = own_keys(g, bh / g.H_kv);
+    if (kt * kTileN >= g.n_kv) {
+      if (item.pslot >= 0) return;
+      item.it1 = item.it0;
+    }
+  }
+  const bool has_work = item.it1 > item.it0;
   const int bhq0 = (bh / g.H_kv) * g.H + (bh % g.H_kv) * g.group;   // first q head
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, hi = lane >> 5, col = lane & 31;
@@ -210,7 +235,8 @@ __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void 
 #pragma unroll
   for (int i = 0; i < DT; ++i) dk[i] = dv[i] = splat16(0.f);
 
-  const int e_beg = col_ptr[kt], e_end = col_ptr[kt + 1];
+  const int e_beg = DENSE ? 0 : col_ptr[kt], e_end = DENSE ? q_tiles_of(g) : col_ptr[kt + 1];
+  auto entry = [&](int e) { return walk_entry<DENSE>(col_idx, e); };
   DmaTile<D, 4, true> dma;
   dma.init(tid);
   // Rows past n_q are zeros in Q and dO (the DMA's range check); LSE / Delta
@@ -231,21 +257,21 @@ __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void 
   const int n_it = item.it1 - item.it0;
   const int h0 = L > 0 ? item.it0 / L : 0;
   int e_nx = e_beg + (item.it0 - h0 * L), q_nx = bhq0 + h0;
-  if (n_it > 0) load_tile((col_idx[e_nx] & kIdxMask) * kTileM, q_nx, 0);
+  if (n_it > 0) load_tile((entry(e_nx) & kIdxMask) * kTileM, q_nx, 0);
   dma_wait();
   __syncthreads();
 
   const int kv_hi_wave = min(k_w + 31, g.n_kv - 1);
   for (int it = 0; it < n_it; ++it) {
     const int buf = it & 1;
-    const int ent = col_idx[e_nx];
+    const int ent = entry(e_nx);
     if (++e_nx == e_end) {
       e_nx = e_beg;
       ++q_nx;
     }
     const int q0 = (ent & kIdxMask) * kTileM;
     const bool partial = (ent >> kPartialBit) & 1;
-    if (it + 1 < n_it) load_tile((col_idx[e_nx] & kIdxMask) * kTileM, q_nx, buf ^ 1);
+    if (it + 1 < n_it) load_tile((entry(e_nx) & kIdxMask) * kTileM, q_nx, buf ^ 1);
     const uint16_t* cq = stile + buf * TILE;
     const uint16_t* cdo = stile + (2 + buf) * TILE;
     const int qw0 = q0 + 32 * qh;              // the wave's first q row
@@ -351,7 +377,7 @@ __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void 
   if (qh == 1) return;
   const bool split = item.pslot >= 0;          // a split column: fp32 partials for the reduce
   const int row = 32 * kh + (lane_e & 31);     // of the kv tile
-  if (!split && kt * kTileN + row >= g.n_kv) return;
+  if (!split && kt * kTileN + row >= n_rows) return;
   float* part = w.partials + ((size_t)bh * w.n_pslots + (split ? item.pslot : 0)) * 2 * TILE + (size_t)row * D;
   const size_t out = kb + (size_t)(kt * kTileN + row) * D;
 #pragma unroll
@@ -388,7 +414,7 @@ __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void 
 // 32 x 32 blocks they cannot see: B4 H16 N8192 W1024 fp16 backward 0.586 ->
 // 0.577 ms (level on walks of 65, B1 H16 N131072 W4096).
 // ---------------------------------------------------------------------------
-template <typename T, bool PRE>
+template <typename T, bool PRE, bool DENSE>
 __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ dO, uint16_t* __restrict__ dK,
@@ -404,11 +430,20 @@ __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
 
   const int BH = g.B * g.H_kv;
   int bh;
-  const KvItem item = kv_item_of(blockIdx.x, BH, w, bh);
+  KvItem item = kv_item_of<DENSE>(blockIdx.x, BH, g, w, bh);
   // an empty column (no kept q tile) only writes zeros: its K / V rows are not read
-  const bool has_work = item.it1 > item.it0;
   const int kt = item.kt;
   const size_t kb = (size_t)bh * g.n_kv * D;
+  const int n_rows = g.n_kv;                   // rows of dK / dV
+  if constexpr (DENSE) {
+    // a kv tile past the entry's keys: zeros (from the reduce where the column is split)
+    g.n_kv = own_keys(g, bh / g.H_kv);
+    if (kt * kTileN >= g.n_kv) {
+      if (item.pslot >= 0) return;
+      item.it1 = item.it0;
+    }
+  }
+  const bool has_work = item.it1 > item.it0;
   const int bhq0 = (bh / g.H_kv) * g.H + (bh % g.H_kv) * g.group;   // first q head
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int grp = lane >> 4, col = lane & 15;
@@ -434,7 +469,8 @@ __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
 #pragma unroll
     for (int i = 0; i < DT; ++i) dk[b][i] = dv[b][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int e_beg = col_ptr[kt], e_end = col_ptr[kt + 1];
+  const int e_beg = DENSE ? 0 : col_ptr[kt], e_end = DENSE ? q_tiles_of(g) : col_ptr[kt + 1];
+  auto entry = [&](int e) { return walk_entry<DENSE>(col_idx, e); };
   DmaTile<D> dma;
   dma.init(tid);
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
@@ -451,21 +487,21 @@ __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
   const int n_it = item.it1 - item.it0;
   const int h0 = L > 0 ? item.it0 / L : 0;
   int e_nx = e_beg + (item.it0 - h0 * L), q_nx = bhq0 + h0;
-  if (n_it > 0) load_tile((col_idx[e_nx] & kIdxMask) * kTileM, q_nx, 0);
+  if (n_it > 0) load_tile((entry(e_nx) & kIdxMask) * kTileM, q_nx, 0);
   dma_wait();
   __syncthreads();
 
   const int kv_hi_wave = min(k_w + 31, g.n_kv - 1);
   for (int it = 0; it < n_it; ++it) {
     const int buf = it & 1;
-    const int ent = col_idx[e_nx];
+    const int ent = entry(e_nx);
     if (++e_nx == e_end) {
       e_nx = e_beg;
       ++q_nx;
     }
     const int q0 = (ent & kIdxMask) * kTileM;
     const bool partial = (ent >> kPartialBit) & 1;
-    if (it + 1 < n_it) load_tile((col_idx[e_nx] & kIdxMask) * kTileM, q_nx, buf ^ 1);
+    if (it + 1 < n_it) load_tile((entry(e_nx) & kIdxMask) * kTileM, q_nx, buf ^ 1);
     const uint16_t* cq = sq[buf];
     const uint16_t* cdo = sdo[buf];
     const int qw0 = q0 + 32 * qh;              // the wave's first q row
@@ -591,7 +627,7 @@ __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = k_w + 16 * b + 4 * grp + i;
-      if (row < g.n_kv) {
+      if (row < n_rows) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           dK[kb + (size_t)row * D + 16 * dt + col] = T::from_float(dk[b][dt][i]);
@@ -613,7 +649,7 @@ __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
 // shares of the q rows of each staged step (16 rows each; two subtiles when
 // KB = 4), and an item of the work list is 4 / KB workgroups. The shares' sums
 // meet through LDS at the end, in order.
-template <int D, int KB>
+template <int D, int KB, bool DENSE>
 __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void dkdv_kernel_32(
     Geom g, const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ dO, float* __restrict__ dK, float* __restrict__ dV,
@@ -634,12 +670,21 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
 
   const int BH = g.B * g.H_kv;
   int bh, part;
-  const KvItem item = kv_item_part_of(blockIdx.x, BH, QS, w, bh, part);
+  KvItem item = kv_item_part_of<DENSE>(blockIdx.x, BH, QS, g, w, bh, part);
   if (bh < 0) return;
   // an empty column (no kept q tile) only writes zeros: its K / V rows are not read
-  const bool has_work = item.it1 > item.it0;
   const int kt = item.kt;
   const size_t kb = (size_t)bh * g.n_kv * D;
+  const int n_rows = g.n_kv;                   // rows of dK / dV
+  if constexpr (DENSE) {
+    // a kv tile past the entry's keys: zeros (from the reduce where the column is split)
+    g.n_kv = own_keys(g, bh / g.H_kv);
+    if (kt * kTileN >= g.n_kv) {
+      if (item.pslot >= 0) return;
+      item.it1 = item.it0;
+    }
+  }
+  const bool has_work = item.it1 > item.it0;
   const int bhq0 = (bh / g.H_kv) * g.H + (bh % g.H_kv) * g.group;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = lane >> 4, col = lane & 15;
@@ -663,7 +708,8 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
 #pragma unroll
     for (int e = 0; e < DE; ++e) dk[v][e] = dv[v][e] = ck[v][e] = cv[v][e] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int e_beg = col_ptr[kt], e_end = col_ptr[kt + 1];
+  const int e_beg = DENSE ? 0 : col_ptr[kt], e_end = DENSE ? q_tiles_of(g) : col_ptr[kt + 1];
+  auto entry = [&](int e) { return walk_entry<DENSE>(col_idx, e); };
   DmaTileF32<D, TR> dma;
   dma.init(tid);
   const int L = e_end - e_beg;
@@ -671,7 +717,7 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
   const int h0 = L > 0 ? item.it0 / L : 0;
   int e_nx = e_beg + (item.it0 - h0 * L), q_nx = bhq0 + h0;
   auto stage = [&](int s, int buf) {
-    const int q0 = (col_idx[e_nx] & kIdxMask) * kTileM + (s % HALVES) * TR;
+    const int q0 = (entry(e_nx) & kIdxMask) * kTileM + (s % HALVES) * TR;
     const size_t qb = (size_t)q_nx * g.n_q * D;
     dma.load(Q + qb, q0, g.n_q, sq[buf]);
     dma.load(dO + qb, q0, g.n_q, sdo[buf]);
@@ -688,7 +734,7 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
   const int kv_hi = min(k_w + 15, g.n_kv - 1);
   for (int s = 0; s < n_step; ++s) {
     const int buf = s & 1;
-    const int ent = col_idx[e_nx];
+    const int ent = entry(e_nx);
     if (s % HALVES == HALVES - 1 && ++e_nx == e_end) {
       e_nx = e_beg;
       ++q_nx;
@@ -810,7 +856,7 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 4 * grp + i;
-    if (!split && k_w + row >= g.n_kv) continue;
+    if (!split && k_w + row >= n_rows) continue;
 #pragma unroll
     for (int v = 0; v < DV; ++v) {
       const int c = row * D + 64 * v + DE * col;
@@ -836,7 +882,7 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
 // halves' fp32 sums meet once, through LDS, at the end (the kh = 0 wave adds
 // the kh = 1 wave's, a fixed order).
 // ---------------------------------------------------------------------------
-template <typename T, int D, int FORM>
+template <typename T, int D, int FORM, bool DENSE>
 __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ O, const uint16_t* __restrict__ dO,
@@ -857,6 +903,7 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
+  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const Lane32<D> at(lane);
@@ -908,22 +955,23 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
 #pragma unroll
   for (int i = 0; i < DT; ++i) dq[i] = splat16(0.f);
 
-  const int e_beg = row_ptr[qt], e_end = row_ptr[qt + 1];
+  const int e_beg = DENSE ? 0 : row_ptr[qt], e_end = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1];
+  auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTile<D, 4, true> dma;
   dma.init(tid);
   auto stage = [&](int k0, int buf) {
     dma.load(K + kb, k0, g.n_kv, stile + buf * TILE);
     dma.load(V + kb, k0, g.n_kv, stile + (2 + buf) * TILE);
   };
-  if (e_beg < e_end) stage((row_idx[e_beg] & kIdxMask) * kTileN, 0);
+  if (e_beg < e_end) stage((entry(e_beg) & kIdxMask) * kTileN, 0);
   dma_wait();
   __syncthreads();
   for (int e = e_beg; e < e_end; ++e) {
     const int buf = (e - e_beg) & 1;
-    const int ent = row_idx[e];
+    const int ent = entry(e);
     const int k0 = (ent & kIdxMask) * kTileN;
     const bool partial = (ent >> kPartialBit) & 1;
-    if (e + 1 < e_end) stage((row_idx[e + 1] & kIdxMask) * kTileN, buf ^ 1);
+    if (e + 1 < e_end) stage((entry(e + 1) & kIdxMask) * kTileN, buf ^ 1);
     const uint16_t* ck = stile + buf * TILE;
     const uint16_t* cv = stile + (2 + buf) * TILE;
     const int kw0 = k0 + 32 * kh;              // the wave's first kv row
@@ -1007,7 +1055,7 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
 // tile instead of 32. The two kv halves' fp32 dQ sums meet once, through LDS,
 // at the end (the kh = 0 wave adds the kh = 1 wave's, a fixed order).
 // ---------------------------------------------------------------------------
-template <typename T, bool PRE>
+template <typename T, bool PRE, bool DENSE>
 __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ O, const uint16_t* __restrict__ dO,
@@ -1024,6 +1072,7 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
+  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int grp = lane >> 4, col = lane & 15;
   const int qh = __builtin_amdgcn_readfirstlane(wave >> 1), kh = __builtin_amdgcn_readfirstlane(wave & 1);
@@ -1069,23 +1118,24 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
 #pragma unroll
     for (int i = 0; i < DT; ++i) dq[b][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int e_beg = row_ptr[qt], e_end = row_ptr[qt + 1];
+  const int e_beg = DENSE ? 0 : row_ptr[qt], e_end = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1];
+  auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTile<D> dma;
   dma.init(tid);
   auto stage = [&](int k0, int buf) {
     dma.load(K + kb, k0, g.n_kv, sk[buf]);
     dma.load(V + kb, k0, g.n_kv, sv[buf]);
   };
-  if (e_beg < e_end) stage((row_idx[e_beg] & kIdxMask) * kTileN, 0);
+  if (e_beg < e_end) stage((entry(e_beg) & kIdxMask) * kTileN, 0);
   dma_wait();
   __syncthreads();
   const int q_hi_wave = min(q0w + 31, g.n_q - 1);
   for (int e = e_beg; e < e_end; ++e) {
     const int buf = (e - e_beg) & 1;
-    const int ent = row_idx[e];
+    const int ent = entry(e);
     const int k0 = (ent & kIdxMask) * kTileN;
     const bool partial = (ent >> kPartialBit) & 1;
-    if (e + 1 < e_end) stage((row_idx[e + 1] & kIdxMask) * kTileN, buf ^ 1);
+    if (e + 1 < e_end) stage((entry(e + 1) & kIdxMask) * kTileN, buf ^ 1);
     const uint16_t* ck = sk[buf];
     const uint16_t* cv = sv[buf];
     const int kw0 = k0 + 32 * kh;              // the wave's first kv row
@@ -1189,7 +1239,7 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
 // Blocks and shares as in the forward (QB blocks of 16 q rows x 4 / QB shares
 // of the keys). Also Delta = rowsum(O dO) of its rows, for itself and for the
 // dK/dV kernel, which runs next.
-template <int D, int QB>
+template <int D, int QB, bool DENSE>
 __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_kernel_32(
     Geom g, const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ O, const float* __restrict__ dO, float* __restrict__ dQ,
@@ -1211,6 +1261,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
+  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = lane >> 4, col = lane & 15;
   const int share = wave / QB;
@@ -1243,11 +1294,13 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
 #pragma unroll
     for (int e = 0; e < DE; ++e) dq[v][e] = cq[v][e] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int e_beg = row_ptr[qt], n_step = (row_ptr[qt + 1] - e_beg) * HALVES;
+  const int e_beg = DENSE ? 0 : row_ptr[qt];
+  const int n_step = (DENSE ? kv_tiles_of(g) : row_ptr[qt + 1] - e_beg) * HALVES;
+  auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTileF32<D, TR> dma;
   dma.init(tid);
   auto step_k0 = [&](int s) {
-    return (row_idx[e_beg + s / HALVES] & kIdxMask) * kTileN + (s % HALVES) * TR;
+    return (entry(e_beg + s / HALVES) & kIdxMask) * kTileN + (s % HALVES) * TR;
   };
   auto stage = [&](int s, int buf) {
     const int k0 = step_k0(s);
@@ -1261,7 +1314,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
   const int q_hi = min(q0 + 15, g.n_q - 1);
   for (int s = 0; s < n_step; ++s) {
     const int buf = s & 1;
-    const bool partial = (row_idx[e_beg + s / HALVES] >> kPartialBit) & 1;
+    const bool partial = (entry(e_beg + s / HALVES) >> kPartialBit) & 1;
     if (s + 1 < n_step) stage(s + 1, buf ^ 1);
     const float *ck = sk[buf], *cv = sv[buf];
     const int r0 = 16 * SUBS * share;
@@ -1364,7 +1417,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
 
 // dQ first: it also produces the -Delta and LSE rows, which dK/dV reads
 // from the two halves of the row-term workspace
-template <typename T, int D, int FORM>
+template <typename T, int D, int FORM, bool DENSE>
 void launch_bwd16_as(const Geom& g, const void* q, const void* k, const void* v, const void* o,
                      const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                      const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* dq_order,
@@ -1373,29 +1426,29 @@ void launch_bwd16_as(const Geom& g, const void* q, const void* k, const void* v,
   const float* lse2 = delta + (size_t)BH * g.n_q;
   if constexpr (D == 64) {
     constexpr bool PRE = FORM == kBwdPre;
-    hipLaunchKernelGGL((dq_kernel_q64<T, PRE>), dim3(n_qt * BH), dim3(256), 0, stream, g,
+    hipLaunchKernelGGL((dq_kernel_q64<T, PRE, DENSE>), dim3(n_qt * BH), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o,
                        (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order);
-    hipLaunchKernelGGL((dkdv_kernel_q64<T, PRE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
+    hipLaunchKernelGGL((dkdv_kernel_q64<T, PRE, DENSE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout,
                        (uint16_t*)dk, (uint16_t*)dv, lse2, delta, col_ptr, col_idx, w);
   } else {
-    hipLaunchKernelGGL((dq_kernel_16<T, D, FORM>), dim3(n_qt * BH), dim3(256), 0, stream, g,
+    hipLaunchKernelGGL((dq_kernel_16<T, D, FORM, DENSE>), dim3(n_qt * BH), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o,
                        (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order);
-    hipLaunchKernelGGL((dkdv_kernel_16<T, D, FORM>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
+    hipLaunchKernelGGL((dkdv_kernel_16<T, D, FORM, DENSE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout,
                        (uint16_t*)dk, (uint16_t*)dv, lse2, delta, col_ptr, col_idx, w);
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool DENSE>
 void launch_bwd16(const Geom& g, const void* q, const void* k, const void* v, const void* o,
                   const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                   const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* dq_order,
                   const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, hipStream_t stream) {
 #define GKI_BWD16(FORM)                                                                             \
-  launch_bwd16_as<T, D, FORM>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,  \
+  launch_bwd16_as<T, D, FORM, DENSE>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,  \
                               dq_order, col_ptr, col_idx, w, stream)
   // head_dim 64 forms P by an fma of the base-2 LSE, so its first two forms are one
   if (g.bwd_form == kBwdPre) GKI_BWD16(kBwdPre);
@@ -1404,7 +1457,7 @@ void launch_bwd16(const Geom& g, const void* q, const void* k, const void* v, co
 #undef GKI_BWD16
 }
 
-template <int D>
+template <int D, bool DENSE>
 int launch_bwd(int dtype, const Geom& g, const void* q, const void* k, const void* v, const void* o,
                const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* dq_order,
@@ -1415,14 +1468,14 @@ int launch_bwd(int dtype, const Geom& g, const void* q, const void* k, const voi
     // dQ first: it also writes Delta, which dK/dV reads
     const int qgrid = n_qt * BH, kgrid = w.n_items * BHkv;
 #define GKI_DQ32(QB)                                                                                \
-  hipLaunchKernelGGL((dq_kernel_32<D, QB>), dim3(work_parts_grid(qgrid, 4 / QB)), dim3(256), 0,     \
+  hipLaunchKernelGGL((dq_kernel_32<D, QB, DENSE>), dim3(work_parts_grid(qgrid, 4 / QB)), dim3(256), 0,     \
                      stream, g, (const float*)q, (const float*)k, (const float*)v, (const float*)o, \
                      (const float*)dout, (float*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order)
 #define GKI_DKDV32(KB)                                                                              \
-  hipLaunchKernelGGL((dkdv_kernel_32<D, KB>), dim3(work_parts_grid(kgrid, 4 / KB)), dim3(256), 0,   \
+  hipLaunchKernelGGL((dkdv_kernel_32<D, KB, DENSE>), dim3(work_parts_grid(kgrid, 4 / KB)), dim3(256), 0,   \
                      stream, g, (const float*)q, (const float*)k, (const float*)v,                  \
                      (const float*)dout, (float*)dk, (float*)dv, lse, delta, col_ptr, col_idx, w)
-    const int qblocks = f32_row_blocks(D, qgrid, row_kv_tiles(g, kTileM));
+    const int qblocks = f32_row_blocks(D, qgrid, DENSE ? kv_tiles_of(g) : row_kv_tiles(g, kTileM));
     if (qblocks == 1) GKI_DQ32(1);
     else if (qblocks == 2) GKI_DQ32(2);
     else GKI_DQ32(4);
@@ -1433,22 +1486,22 @@ int launch_bwd(int dtype, const Geom& g, const void* q, const void* k, const voi
 #undef GKI_DQ32
 #undef GKI_DKDV32
     if (w.n_split > 0)
-      hipLaunchKernelGGL((dkdv_reduce_kernel<F32, D>), red_grid, dim3(256), 0, stream, g, w,
+      hipLaunchKernelGGL((dkdv_reduce_kernel<F32, D, DENSE>), red_grid, dim3(256), 0, stream, g, w,
                          (float*)dk, (float*)dv);
   } else if (dtype == kF16) {
-    launch_bwd16<F16, D>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,
+    launch_bwd16<F16, D, DENSE>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,
                          dq_order, col_ptr, col_idx, w, stream);
     if (w.n_split > 0)
-      hipLaunchKernelGGL((dkdv_reduce_kernel<F16, D>), red_grid, dim3(256), 0, stream, g, w,
+      hipLaunchKernelGGL((dkdv_reduce_kernel<F16, D, DENSE>), red_grid, dim3(256), 0, stream, g, w,
                          (uint16_t*)dk, (uint16_t*)dv);
   } else {
-    launch_bwd16<BF16, D>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,
+    launch_bwd16<BF16, D, DENSE>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,
                           dq_order, col_ptr, col_idx, w, stream);
     if (w.n_split > 0)
-      hipLaunchKernelGGL((dkdv_reduce_kernel<BF16, D>), red_grid, dim3(256), 0, stream, g, w,
+      hipLaunchKernelGGL((dkdv_reduce_kernel<BF16, D, DENSE>), red_grid, dim3(256), 0, stream, g, w,
                          (uint16_t*)dk, (uint16_t*)dv);
   }
-  return check_launch("gki_bsa_bwd");
+  return check_launch(DENSE ? "gki_cross_bwd" : "gki_bsa_bwd");
 }
 
 }  // namespace
@@ -1460,7 +1513,7 @@ int bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
                  hipStream_t stream) {
 #define GKI_BWD_CASE(DD)                                                                          \
   case DD:                                                                                        \
-    return launch_bwd<DD>(dtype, g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx,   \
+    return launch_bwd<DD, false>(dtype, g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx,   \
                           n_qt, dq_order, col_ptr, col_idx, w, stream);
   switch (head_dim) {
     GKI_BWD_CASE(16)
@@ -1470,6 +1523,29 @@ int bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
     default: return fail(2, "unsupported head_dim " + std::to_string(head_dim));
   }
 #undef GKI_BWD_CASE
+}
+
+int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                       const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
+                       int parts, float* partials, hipStream_t stream) {
+  const int n_kt = kv_tiles_of(g);
+  KvWork w{};
+  w.parts = parts;
+  w.n_items = n_kt * parts;
+  if (parts > 1) w.n_split = n_kt, w.n_pslots = w.n_items;
+  w.partials = partials;
+#define GKI_CROSS_CASE(DD)                                                                                 \
+  case DD:                                                                                                 \
+    return launch_bwd<DD, true>(dtype, g, q, k, v, o, dout, lse, dq, dk, dv, delta, nullptr, nullptr,      \
+                                (g.n_q + kTileM - 1) / kTileM, nullptr, nullptr, nullptr, w, stream);
+  switch (head_dim) {
+    GKI_CROSS_CASE(16)
+    GKI_CROSS_CASE(32)
+    GKI_CROSS_CASE(64)
+    GKI_CROSS_CASE(128)
+    default: return fail(2, "unsupported head_dim " + std::to_string(head_dim));
+  }
+#undef GKI_CROSS_CASE
 }
 
 }  // namespace gki

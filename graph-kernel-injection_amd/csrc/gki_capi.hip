@@ -58,6 +58,13 @@ int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const
 int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                      const uint8_t* ks, const uint8_t* vs, void* o, float* lse, int ring, float* ws, int n_splits,
                      hipStream_t stream);
+int cross_fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
+                       float* lse, hipStream_t stream);
+int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
+                          float* lse, float* ws, int n_splits, hipStream_t stream);
+int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                       const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
+                       int parts, float* partials, hipStream_t stream);
 int64_t read_probe_words(int BH);
 int read_probe_dispatch(const void* k, const void* v, int BH, int64_t n_kv, int row_bytes, int n_sink,
                         int64_t w_lo, uint32_t* out, hipStream_t stream);
@@ -240,6 +247,34 @@ int rolling8_args(const char* what, int dtype, int B, int H, int head_dim, int s
               w + "B and H must be positive and B * H not too large");
   GKI_REQUIRE(sink_size >= 0 && ring_size >= 1 && (int64_t)sink_size + ring_size < (1ll << kPartialBit), 1,
               w + "sink_size must be >= 0, ring_size >= 1 and their sum below 2^30");
+  return 0;
+}
+
+// Geometry of a cross attention: every key of the entry's own visible to every query.
+int cross_geom(Geom& g, int dtype, int B, int H, int H_kv, int n_q, int n_kv, int head_dim, const int32_t* kv_len,
+               float scale) {
+  GKI_REQUIRE(dtype == kF32 || dtype == kF16 || dtype == kBF16, 2,
+              "unsupported dtype code " + std::to_string(dtype) + " (0=fp32, 1=fp16, 2=bf16)");
+  GKI_REQUIRE(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128, 2,
+              "unsupported head_dim " + std::to_string(head_dim) + " (supported: 16, 32, 64, 128)");
+  GKI_REQUIRE(B > 0 && H > 0 && n_q > 0 && n_kv > 0, 1, "B, H, n_q and n_kv must be positive");
+  GKI_REQUIRE(H_kv > 0 && H % H_kv == 0, 1, "H_kv must be positive and divide H (grouped-query attention)");
+  GKI_REQUIRE((int64_t)B * H < (1ll << 31) / 4096, 1, "B * H too large");
+  GKI_REQUIRE((int64_t)n_q < (1ll << kPartialBit) && (int64_t)n_kv < (1ll << kPartialBit), 1,
+              "n_q and n_kv must be below 2^30");
+  GKI_REQUIRE(std::isfinite(scale), 1, "softmax_scale must be finite");
+  g = Geom{};
+  g.B = B;
+  g.H = H;
+  g.H_kv = H_kv;
+  g.group = H / H_kv;
+  g.n_q = n_q;
+  g.n_kv = n_kv;
+  g.q_off = n_kv - n_q;
+  set_scale(g, scale);
+  g.bwd_form = bwd_form_of(dtype, scale);
+  g.n_qb = g.n_kb = g.bm = g.bn = 1;
+  g.kv_len = kv_len;
   return 0;
 }
 
@@ -589,6 +624,59 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
                           rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale), q, k_codes,
                           v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, o, lse, ring_size, workspace,
                           n_splits, (hipStream_t)stream);
+}
+
+int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
+                     int32_t head_dim) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0 || !cross_as_streams(dtype, head_dim, H / H_kv, n_q))
+    return 0;
+  return gki_stream_splits(dtype, B, H, H_kv, n_q, head_dim, n_kv);
+}
+
+int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int32_t dtype, int32_t B, int32_t H,
+                  int32_t H_kv, int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* kv_len, float softmax_scale,
+                  float* workspace, int32_t n_splits, void* stream) {
+  Geom g;
+  if (int rc = cross_geom(g, dtype, B, H, H_kv, n_q, n_kv, head_dim, kv_len, softmax_scale)) return rc;
+  GKI_REQUIRE(q && k && v && o && lse, 1, "gki_cross_fwd: null pointer");
+  GKI_REQUIRE(all_aligned16(q, k, v, o, workspace), 1, "gki_cross_fwd: q, k, v, o and the workspace must be 16-byte aligned");
+  const int tm = fwd_tile_m(dtype);
+  if (n_splits == 0) {
+    GKI_REQUIRE((int64_t)((n_q + tm - 1) / tm) * B * H < (1ll << 24), 1, "gki_cross_fwd: grid too large");
+    return cross_fwd_dispatch(dtype, head_dim, g, q, k, v, o, lse, (hipStream_t)stream);
+  }
+  GKI_REQUIRE(dtype != kF32 && (head_dim == 64 || head_dim == 128), 2,
+              "gki_cross_fwd: streams take fp16 or bf16 and head_dim 64 or 128");
+  GKI_REQUIRE(n_splits > 0 && (int64_t)g.group * n_q < (1ll << kPartialBit) &&
+                  (int64_t)n_splits * B * H_kv * ((g.group * (int64_t)n_q + 15) / 16) < (1ll << 23), 1,
+              "gki_cross_fwd: n_splits must not be negative and the grid must fit");
+  GKI_REQUIRE(n_splits == 1 || workspace, 1, "gki_cross_fwd: null workspace");
+  return cross_stream_dispatch(dtype, head_dim, g, q, k, v, o, lse, workspace, n_splits, (hipStream_t)stream);
+}
+
+int gki_cross_bwd_parts(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
+                        int32_t head_dim) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0) return 1;
+  const int64_t walk = ((int64_t)n_q + kTileM - 1) / kTileM * (H / H_kv);
+  return cross_kv_parts(dtype, head_dim, walk, ((int64_t)n_kv + kTileN - 1) / kTileN * B * H_kv);
+}
+
+int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                  void* dq, void* dk, void* dv, float* delta, int32_t dtype, int32_t B, int32_t H, int32_t H_kv,
+                  int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* kv_len, float softmax_scale,
+                  int32_t parts, float* kv_partials, void* stream) {
+  Geom g;
+  if (int rc = cross_geom(g, dtype, B, H, H_kv, n_q, n_kv, head_dim, kv_len, softmax_scale)) return rc;
+  GKI_REQUIRE(q && k && v && o && dout && lse && dq && dk && dv && delta, 1, "gki_cross_bwd: null tensor");
+  GKI_REQUIRE(all_aligned16(q, k, v, o, dout, dq, dk, dv, kv_partials), 1,
+              "gki_cross_bwd: q, k, v, o, dout, dq, dk, dv and kv_partials must be 16-byte aligned");
+  GKI_REQUIRE(parts >= 1 && (parts == 1 || kv_partials), 1,
+              "gki_cross_bwd: parts must be positive, and several need kv_partials");
+  const int64_t n_qt = (n_q + kTileM - 1) / kTileM, n_kt = kv_tiles_of(g);
+  GKI_REQUIRE(n_qt * g.group < (1ll << 30) && n_qt * B * H < (1ll << 24) && n_kt * parts * B * H_kv < (1ll << 24) &&
+                  (parts == 1 || n_kt * B * H_kv * (head_dim / 8) < (1ll << 24)), 1, "gki_cross_bwd: grid too large");
+  return cross_bwd_dispatch(dtype, head_dim, g, q, k, v, o, dout, lse, dq, dk, dv, delta, parts, kv_partials,
+                            (hipStream_t)stream);
 }
 
 int64_t gki_read_probe_words(int32_t bh) { return bh > 0 ? read_probe_words(bh) : 0; }

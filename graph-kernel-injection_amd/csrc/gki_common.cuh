@@ -579,6 +579,9 @@ struct Geom {
   // original block mask (used only for tiles flagged partial)
   const int32_t* mask;
   int n_qb, n_kb, bm, bn;
+  // dense walks (cross attention): the keys of each batch entry that are valid, the
+  // first kv_len[b] of n_kv; null: all
+  const int32_t* kv_len;
 };
 
 // Work list of the dK / dV grid (built on the host by gki_dkdv_items). A kv
@@ -595,7 +598,22 @@ struct KvWork {
   int n_split;
   int n_pslots;           // partial slots per (b, kv head)
   float* partials;        // [B * H_kv][n_pslots][2 (dK, dV)][64][D] fp32
+  int parts;              // dense walks: items per kv tile (no list: item i is part i % parts of tile i / parts)
 };
+
+// Dense walks: the kernels' DENSE forms read no list. A q tile visits every kv tile
+// of its batch entry's own keys, a kv tile every q tile; entry e of either walk is
+// tile e.
+template <bool DENSE>
+__device__ inline int walk_entry(const int32_t* list, int e) {
+  return DENSE ? e : list[e];
+}
+__host__ __device__ inline int kv_tiles_of(const Geom& g) { return (g.n_kv + kTileN - 1) / kTileN; }
+// Valid keys of batch entry b (a length outside 0 .. n_kv counts as the nearest of them).
+__device__ inline int own_keys(const Geom& g, int b) {
+  if (g.kv_len == nullptr) return g.n_kv;
+  return max(0, min(__builtin_amdgcn_readfirstlane(g.kv_len[b]), g.n_kv));
+}
 
 // A 16-byte Q fragment as the unscaled-max kernels read it (see Geom::q_and).
 __device__ inline uint4 q_words(const Geom& g, uint4 w) {
@@ -843,6 +861,34 @@ inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
   const int64_t target = head_dim >= 128 ? 512 : 1024;
   const int64_t want = (target + n_workgroups - 1) / n_workgroups;
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, n_tokens / 128));
+}
+
+// Does a cross attention run its query rows as streams (a whole group's rows against
+// each read of K and V) or as q tiles of each head? 16-bit, head_dim 64 or 128.
+inline bool cross_as_streams(int dtype, int head_dim, int group, int n_q) {
+  return dtype != kF32 && (head_dim == 64 || head_dim == 128) && group * n_q <= 32;
+}
+
+// Parts that a dense walk of dK/dV is cut into: each of `columns` kv tiles (over all
+// (b, kv head)) is walked by `walk` = q tiles * group iterations. A column is one
+// item where the columns fill the card, else pieces of about a 512th of the work, of 8
+// iterations or more (2 for fp32); never more than about 8192 items in all.
+inline int cross_kv_parts(int dtype, int head_dim, int64_t walk, int64_t columns) {
+  const int64_t total = walk * columns;
+  int64_t chunk;
+  if (dtype == kF32) {
+    chunk = columns >= 512 ? walk : std::max<int64_t>(2, (total + 511) / 512);
+  } else {
+    int64_t spread = std::max<int64_t>(8, (total + 511) / 512);
+    const int64_t few = head_dim >= 64 ? 128 : 192, brief = head_dim >= 64 ? 32 : 16;
+    if (columns >= 512) spread = std::max(spread, walk);
+    else if (columns >= few && walk <= brief) spread = std::max<int64_t>(std::max<int64_t>(spread, 16), walk);
+    const bool middling = head_dim < 128 && columns >= 512 && columns < 1024;
+    const int64_t whole = middling ? 48 : 80, piece = middling ? 32 : 80;
+    chunk = std::min(walk <= whole ? std::max<int64_t>(32, walk) : piece, spread);
+  }
+  chunk = std::max<int64_t>(std::max<int64_t>(chunk, 1), (total + 8191) / 8192);
+  return (int)((walk + chunk - 1) / chunk);
 }
 
 // XCD-aware remap: hardware dispatches workgroup b to XCD b % 8. Give each XCD

@@ -81,7 +81,7 @@ constexpr int kFwdThreads = 256;
 // N8192 D64 W1024 fp16 0.174 -> 0.168, B1 H16 N131072 D64 W4096 bf16 2.20 ->
 // 2.16, 500 queries behind 8500 keys D128 0.0525 -> 0.0467, B4 H8 N2000 D32
 // 0.0177 -> 0.0150.
-template <typename T, int D, bool PIPE>
+template <typename T, int D, bool PIPE, bool DENSE>
 __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, uint16_t* __restrict__ O, float* __restrict__ LSE,
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
+  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const Lane32<D> at(lane);
@@ -201,20 +202,21 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
       lsum = T::mfma(ones, p[st], lsum);
     }
   };
-  const int e_beg = row_ptr[qt], e_end = row_ptr[qt + 1];
+  const int e_beg = DENSE ? 0 : row_ptr[qt], e_end = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1];
+  auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   if constexpr (!PIPE) {
     if (e_beg < e_end) {
-      stage(K, tile_k0(row_idx[e_beg]), sk[0]);
-      stage(V, tile_k0(row_idx[e_beg]), sv[0]);
+      stage(K, tile_k0(entry(e_beg)), sk[0]);
+      stage(V, tile_k0(entry(e_beg)), sv[0]);
     }
     dma_wait();
     __syncthreads();
 
     // unrolled by two so that the buffers are constants of the instructions
     auto step = [&](int e, int buf) {
-      const int ent = row_idx[e];
+      const int ent = entry(e);
       if (e + 1 < e_end) {
-        const int k1 = tile_k0(row_idx[e + 1]);
+        const int k1 = tile_k0(entry(e + 1));
         stage(K, k1, sk[buf ^ 1]);
         stage(V, k1, sv[buf ^ 1]);
       }
@@ -248,16 +250,16 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
     floatx16 sa[2], sb[2];
     // Prologue: K_0, V_0 and K_1 in LDS, S_0 with its maxima.
     if (n > 0) {
-      const int k0 = tile_k0(row_idx[e_beg]);
+      const int k0 = tile_k0(entry(e_beg));
       stage(K, k0, sk[0]);
       stage(V, k0, sv[0]);
-      if (n > 1) stage(K, tile_k0(row_idx[e_beg + 1]), sk[1]);
+      if (n > 1) stage(K, tile_k0(entry(e_beg + 1)), sk[1]);
     }
     dma_wait();
     __syncthreads();
     if (n > 0) {
       scores(sk[0], sa);
-      apply_mask(row_idx[e_beg], sa);
+      apply_mask(entry(e_beg), sa);
       move_max(lane_max(sa));
     }
     __syncthreads();   // every wave is done with K_0 before iteration 0 refills its buffer
@@ -266,9 +268,9 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
     // becomes P_j; O += V_j P_j while sn's maxima are taken.
     auto step = [&](int j, int par, floatx16 (&s)[2], floatx16 (&sn)[2]) {   // par = j & 1
       const int e = e_beg + j;
-      const int ent1 = row_idx[e + 1];
+      const int ent1 = entry(e + 1);
       // LDS: K_{j+1} in sk[(j+1)&1], V_j in sv[j&1]; refill the other halves
-      if (j + 2 < n) stage(K, tile_k0(row_idx[e + 2]), sk[par]);
+      if (j + 2 < n) stage(K, tile_k0(entry(e + 2)), sk[par]);
       stage(V, tile_k0(ent1), sv[par ^ 1]);
 
       uint4 p[4];
@@ -358,7 +360,7 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
 // times, us: 500 queries behind 8500 keys, B1 H32, D128 (128 tiles) 46.8 -> 30.6;
 // B1 H8 N1000 D64 (64) 20.7 -> 12.9; B1 H4 N1000 D128 (32) 18.2 -> 13.6.
 // ---------------------------------------------------------------------------
-template <typename T, int D>
+template <typename T, int D, bool DENSE>
 __global__ __launch_bounds__(512, 2) void fwd_split_16(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, uint16_t* __restrict__ O, float* __restrict__ LSE,
@@ -382,6 +384,7 @@ __global__ __launch_bounds__(512, 2) void fwd_split_16(
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
+  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const Lane32<D> at(lane);
@@ -389,8 +392,8 @@ __global__ __launch_bounds__(512, 2) void fwd_split_16(
   const int qw = qt * kTileMF + 32 * (part * QB + blk);   // first row of this wave
   if (qt * kTileMF + 32 * QB * part >= g.n_q) return;     // a part past the last row
 
-  const int e_beg = row_ptr[qt], n = row_ptr[qt + 1] - e_beg;
-  const int32_t* const ents = row_idx + e_beg;
+  const int e_beg = DENSE ? 0 : row_ptr[qt], n = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1] - e_beg;
+  auto entry = [&](int i) { return walk_entry<DENSE>(row_idx, e_beg + i); };
   DmaTile<D, NW, true> dma;
   dma.init(tid);
   auto tile_k0 = [&](int ent) { return (ent & kIdxMask) * kTileN; };
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(512, 2) void fwd_split_16(
 #pragma unroll
     for (int j = 0; j < TPS; ++j)
       if (TPS * s + j < n) {
-        const int k0 = tile_k0(ents[TPS * s + j]);
+        const int k0 = tile_k0(entry(TPS * s + j));
         uint16_t* const dst = stile + (2 * TPS * (s & 1) + 2 * j) * TILE;
         dma.load(K + kb, k0, g.n_kv, dst);
         dma.load(V + kb, k0, g.n_kv, dst + TILE);
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(512, 2) void fwd_split_16(
     if (st + 1 < steps) stage(st + 1);
     const int e = TPS * st + tj;
     if (e < n) {
-      const int ent = ents[e];
+      const int ent = entry(e);
       const int k0 = tile_k0(ent), kw = k0 + 32 * th;
       const bool partial = (ent >> kPartialBit) & 1;
       const uint16_t* ck = stile + (2 * TPS * (st & 1) + 2 * tj) * TILE + 32 * D * th;
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(512, 2) void fwd_split_16(
 // waves keep a softmax state each and merge through LDS at the end: a grid too
 // short for the card (B1 H4 N1024: 64 tiles, 29 us) then runs on four times the
 // workgroups, each a quarter of the serial chain (11.6 us).
-template <int D, int QB>
+template <int D, int QB, bool DENSE>
 __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 1 ? 4 : 2) >= 256 ? 2 : 3) void fwd_kernel_32(
     Geom g, const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     float* __restrict__ O, float* __restrict__ LSE, const int32_t* __restrict__ row_ptr,
@@ -568,6 +571,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
+  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = lane >> 4, col = lane & 15;
   const int share = wave / QB;
@@ -590,11 +594,13 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
   // the LSE of a 1024-key row 9% above one rounding (8% per 64 keys, now 6%)
   float m = kNegInf, l = 0.f, lc = 0.f;
 
-  const int e_beg = row_ptr[qt], n_step = (row_ptr[qt + 1] - e_beg) * HALVES;
+  const int e_beg = DENSE ? 0 : row_ptr[qt];
+  const int n_step = (DENSE ? kv_tiles_of(g) : row_ptr[qt + 1] - e_beg) * HALVES;
+  auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTileF32<D, TR> dma;
   dma.init(tid);
   auto step_k0 = [&](int s) {
-    return (row_idx[e_beg + s / HALVES] & kIdxMask) * kTileN + (s % HALVES) * TR;
+    return (entry(e_beg + s / HALVES) & kIdxMask) * kTileN + (s % HALVES) * TR;
   };
   auto stage = [&](int s, int buf) {
     const int k0 = step_k0(s);
@@ -608,7 +614,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
   const int q_hi = min(q0 + 15, g.n_q - 1);
   for (int s = 0; s < n_step; ++s) {
     const int buf = s & 1;
-    const bool partial = (row_idx[e_beg + s / HALVES] >> kPartialBit) & 1;
+    const bool partial = (entry(e_beg + s / HALVES) >> kPartialBit) & 1;
     if (s + 1 < n_step) stage(s + 1, buf ^ 1);
     const float *ck = sk[buf], *cv = sv[buf];
     const int k0 = step_k0(s) + 16 * SUBS * share;       // the wave's first key
@@ -771,7 +777,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
 template <int D>
 constexpr bool kFwdPipe = D >= 128;
 
-template <typename T, int D>
+template <typename T, int D, bool DENSE>
 void launch_fwd16(const Geom& g, const void* q, const void* k, const void* v, void* o, float* lse,
                   const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* wg_order,
                   hipStream_t stream) {
@@ -780,34 +786,34 @@ void launch_fwd16(const Geom& g, const void* q, const void* k, const void* v, vo
   hipLaunchKernelGGL(KERNEL, dim3(GRID), dim3(THREADS), 0, stream, g, (const uint16_t*)q,          \
                      (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, lse, row_ptr, row_idx,  \
                      n_qt, wg_order)
-  if (fwd_shares_keys(D, grid, row_kv_tiles(g, kTileMF)))
-    GKI_FWD16((fwd_split_16<T, D>), work_parts_grid(grid, 2), 512);
+  if (fwd_shares_keys(D, grid, DENSE ? kv_tiles_of(g) : row_kv_tiles(g, kTileMF)))
+    GKI_FWD16((fwd_split_16<T, D, DENSE>), work_parts_grid(grid, 2), 512);
   else
-    GKI_FWD16((fwd_kernel_16<T, D, kFwdPipe<D>>), grid, kFwdThreads);
+    GKI_FWD16((fwd_kernel_16<T, D, kFwdPipe<D>, DENSE>), grid, kFwdThreads);
 #undef GKI_FWD16
 }
 
-template <int D>
+template <int D, bool DENSE>
 int launch_fwd(int dtype, const Geom& g, const void* q, const void* k, const void* v, void* o,
                float* lse, const int32_t* row_ptr, const int32_t* row_idx, int n_qt,
                const int32_t* wg_order, hipStream_t stream) {
   const int grid = n_qt * g.B * g.H;
   if (dtype == kF32) {
 #define GKI_FWD32(QB)                                                                               \
-  hipLaunchKernelGGL((fwd_kernel_32<D, QB>), dim3(work_parts_grid(grid, 4 / QB)), dim3(256), 0,     \
+  hipLaunchKernelGGL((fwd_kernel_32<D, QB, DENSE>), dim3(work_parts_grid(grid, 4 / QB)), dim3(256), 0,     \
                      stream, g, (const float*)q, (const float*)k, (const float*)v, (float*)o, lse,  \
                      row_ptr, row_idx, n_qt, wg_order)
-    const int blocks = f32_row_blocks(D, grid, row_kv_tiles(g, kTileM));
+    const int blocks = f32_row_blocks(D, grid, DENSE ? kv_tiles_of(g) : row_kv_tiles(g, kTileM));
     if (blocks == 1) GKI_FWD32(1);
     else if (blocks == 2) GKI_FWD32(2);
     else GKI_FWD32(4);
 #undef GKI_FWD32
   } else if (dtype == kF16) {
-    launch_fwd16<F16, D>(g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    launch_fwd16<F16, D, DENSE>(g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
   } else {
-    launch_fwd16<BF16, D>(g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    launch_fwd16<BF16, D, DENSE>(g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
   }
-  return check_launch("gki_bsa_fwd");
+  return check_launch(DENSE ? "gki_cross_fwd" : "gki_bsa_fwd");
 }
 
 }  // namespace
@@ -818,12 +824,27 @@ int fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
                  void* o, float* lse, const int32_t* row_ptr, const int32_t* row_idx, int n_qt,
                  const int32_t* wg_order, hipStream_t stream) {
   switch (head_dim) {
-    case 16: return launch_fwd<16>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
-    case 32: return launch_fwd<32>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
-    case 64: return launch_fwd<64>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
-    case 128: return launch_fwd<128>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    case 16: return launch_fwd<16, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    case 32: return launch_fwd<32, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    case 64: return launch_fwd<64, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    case 128: return launch_fwd<128, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
     default: return fail(2, "unsupported head_dim " + std::to_string(head_dim));
   }
+}
+
+int cross_fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
+                       float* lse, hipStream_t stream) {
+  const int tm = fwd_tile_m(dtype), n_qt = (g.n_q + tm - 1) / tm;
+#define GKI_CROSS_CASE(DD) \
+  case DD: return launch_fwd<DD, true>(dtype, g, q, k, v, o, lse, nullptr, nullptr, n_qt, nullptr, stream);
+  switch (head_dim) {
+    GKI_CROSS_CASE(16)
+    GKI_CROSS_CASE(32)
+    GKI_CROSS_CASE(64)
+    GKI_CROSS_CASE(128)
+    default: return fail(2, "unsupported head_dim " + std::to_string(head_dim));
+  }
+#undef GKI_CROSS_CASE
 }
 
 }  // namespace gki

@@ -1,5 +1,5 @@
-// Attention of few query rows over long streams of keys and values: the rolling
-// cache held in 8 bits, for gfx950.
+// Attention of few query rows over long streams of keys and values (the rolling cache
+// held in 8 bits, cross attention of single tokens), for gfx950.
 //
 // A stream is the K / V rows of one (b, kv head); the rows that read it are the
 // group * n_q query rows of that head's group. For each of them
@@ -178,6 +178,18 @@ struct RingStream {
   }
 };
 
+// A contiguous stream per (b, kv head): all its rows, or the first len[b] of them (a
+// length outside 0 .. n counts as the nearest).
+struct DenseStream {
+  const int32_t* len;
+  int n, H_kv;
+  __device__ inline int count(int s) const {
+    return len == nullptr ? n : max(0, min(__builtin_amdgcn_readfirstlane(len[s / H_kv]), n));
+  }
+  __device__ inline int row(int t) const { return t; }
+  __device__ inline bool visible(int, int) const { return true; }
+};
+
 struct StreamArgs {
   const void *q, *k, *v;
   const uint8_t *ks, *vs;      // exponents of the 8-bit rows
@@ -197,125 +209,81 @@ struct StreamArgs {
 // bits), so that products with the stored values are those of the queries themselves.
 template <typename T> constexpr int kPieces = std::is_same<T, BF16>::value ? 1 : std::is_same<T, F16>::value ? 2 : 3;
 
-template <int NPC>
+template <typename C, int NPC>
 __device__ inline void split8(float (&f)[8], uint4 (&piece)[NPC]) {
 #pragma unroll
   for (int n = 0; n < NPC; ++n) {
-    piece[n] = make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]),
-                          pack2<BF16>(f[6], f[7]));
+    piece[n] = make_uint4(pack2<C>(f[0], f[1]), pack2<C>(f[2], f[3]), pack2<C>(f[4], f[5]), pack2<C>(f[6], f[7]));
     if (n + 1 < NPC) {
       const uint16_t* h = (const uint16_t*)&piece[n];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] -= BF16::to_float(h[i]);
+      for (int i = 0; i < 8; ++i) f[i] -= C::to_float(h[i]);
     }
   }
 }
 
-// A workgroup of four waves: 16 NB query rows (columns of S^T = K Q^T on
-// v_mfma_f32_16x16x32_bf16) against a slice of the stream, 64 tokens at a time, 16
-// per wave. The tokens' codes come by 16-byte loads into registers, two steps ahead,
-// and are written to LDS as bfloat16 (v_cvt_scalef32_pk_bf16_fp8 applies the scale);
-// V^T operands by one transposed LDS read each. Each wave keeps a softmax state of
-// its own tokens; they meet in LDS at the end. fp16 and fp32 queries, and their
-// probabilities, are 2 and 3 bfloat16 pieces: 2 and 3 times the products, of which
-// the memory-bound stream leaves room for. bf16: P is rounded to bfloat16 for P V, as
-// in the 16-bit decode (half a unit of 2^-8 of each weight, averaged over the keys);
-// the row sums add the fp32 P.
-template <typename T, int D, int NB, bool RULE, class Src>
-__global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
-  constexpr int NPC = kPieces<T>;
-  constexpr int KS = D / 32, DT = D / 16;
-  constexpr int UPR = D / 16;                  // 16-byte units per row
-  constexpr int NU = kTileN * UPR / 256;       // units per thread and tile
-  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
-  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int grp = lane >> 4, col = lane & 15;
-  int lb = xcd_remap(blockIdx.x, gridDim.x);
-  const int rt = lb % a.row_tiles;
-  lb /= a.row_tiles;
-  const int split = lb % a.n_splits, s_id = lb / a.n_splits;
-  const int row0 = rt * 16 * NB;
-  const size_t q_row0 = (size_t)(s_id / a.H_kv) * a.q_stride + (size_t)(s_id % a.H_kv) * a.rb;
-  const size_t kb = (size_t)s_id * a.kv_rows;
-  const int n_tok = src.count(s_id);
-  const int g0 = (int)(((int64_t)n_tok * split) / a.n_splits);
-  const int g1 = (int)(((int64_t)n_tok * (split + 1)) / a.n_splits);
-  const int n_chunks = (g1 - g0 + kTileN - 1) / kTileN;
-  const uint8_t *K = (const uint8_t*)a.k, *V = (const uint8_t*)a.v;
-
-  struct Raw {
-    uint4 k[NU], v[NU];
-    uint8_t ks[NU], vs[NU];
-  };
-  // tokens past the slice repeat its last one and are masked when consumed
-  auto fetch = [&](int c, Raw& r) {
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int unit = u * 256 + tid;
-      const size_t at = kb + src.row(min(g0 + c * kTileN + unit / UPR, g1 - 1));
-      r.k[u] = ld_nt16(K + at * D + 16 * (unit % UPR));
-      r.ks[u] = a.ks[at];
-      r.v[u] = ld_nt16(V + at * D + 16 * (unit % UPR));
-      r.vs[u] = a.vs[at];
-    }
-  };
-  auto put16 = [&](uint16_t* tile, int row, int c16, const uint4& w, float scale) {
-    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-    uint32_t out[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], scale, false));
-      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], scale, true));
-    }
-    *(uint4*)(tile + lds_off<D>(row, 16 * c16)) = make_uint4(out[0], out[1], out[2], out[3]);
-    *(uint4*)(tile + lds_off<D>(row, 16 * c16 + 8)) = make_uint4(out[4], out[5], out[6], out[7]);
-  };
-  auto put = [&](const Raw& r, int b) {
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int unit = u * 256 + tid;
-      put16(sk[b], unit / UPR, unit % UPR, r.k[u], scale_of(r.ks[u]));
-      put16(sv[b], unit / UPR, unit % UPR, r.v[u], scale_of(r.vs[u]));
-    }
-  };
-
-  Raw ra, rc;
-  if (n_chunks > 0) fetch(0, ra);
-  if (n_chunks > 1) fetch(1, rc);
-
-  // Q^T operand of column block h: lane (grp, col) holds elements 32 ks + 8 grp .. +7
-  // of row row0 + 16 h + col
-  uint4 qf[NB][KS][NPC];
-  int my_q[NB];
-#pragma unroll
-  for (int h = 0; h < NB; ++h) {
-    const int r = row0 + 16 * h + col;
-    my_q[h] = r % a.n_q;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      float f[8];
-      load8<T>((const typename T::storage*)a.q + (q_row0 + (r < a.n_rows ? r : 0)) * D + 32 * ks + 8 * grp, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = r < a.n_rows && a.q_sign != 0.f ? f[i] * a.q_sign : 0.f;
-      split8<NPC>(f, qf[h][ks]);
-    }
+// Where a workgroup works: 16 NB query rows (from row0 on) of stream s against the
+// slice [g0, g1) of its tokens. Row tiles of a slice are neighbours on one XCD.
+struct StreamPlace {
+  int s, row0, split, g0, g1;
+  size_t q_row0, kb;           // the stream's first row of Q, of K and V
+  template <class Src>
+  __device__ inline StreamPlace(const StreamArgs& a, const Src& src, int rows_tile) {
+    int lb = xcd_remap(blockIdx.x, gridDim.x);
+    row0 = lb % a.row_tiles * rows_tile;
+    lb /= a.row_tiles;
+    split = lb % a.n_splits;
+    s = lb / a.n_splits;
+    q_row0 = (size_t)(s / a.H_kv) * a.q_stride + (size_t)(s % a.H_kv) * a.rb;
+    kb = (size_t)s * a.kv_rows;
+    const int n_tok = src.count(s);
+    g0 = (int)(((int64_t)n_tok * split) / a.n_splits);
+    g1 = (int)(((int64_t)n_tok * (split + 1)) / a.n_splits);
   }
+  __device__ inline int chunks() const { return (g1 - g0 + kTileN - 1) / kTileN; }
+};
 
+// A wave's share of a workgroup of four: 16 NB query rows, as columns of S^T = K Q^T on
+// v_mfma_f32_16x16x32, against 16 of the 64 tokens of each step (tiles of element
+// type C in LDS), with a softmax state of its own. NPC: pieces of the queries and of
+// the probabilities. The reference max is lazy: it moves when a score exceeds it by
+// the slack, so that the rescale almost never runs.
+template <typename T, typename C, int D, int NB, int NPC, bool RULE>
+struct StreamWave {
+  static constexpr int KS = D / 32, DT = D / 16;
+  uint4 qf[NB][KS][NPC];
   floatx4 o[NB][DT];
   float lsum[NB], m[NB];
+  int my_q[NB], wave, lane, grp, col;
+
+  __device__ inline StreamWave(const StreamArgs& a, const StreamPlace& at) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    grp = lane >> 4, col = lane & 15;
+    // Q^T operand of column block h: lane (grp, col) holds elements 32 ks + 8 grp .. +7
+    // of row row0 + 16 h + col
 #pragma unroll
-  for (int h = 0; h < NB; ++h) {
+    for (int h = 0; h < NB; ++h) {
+      const int r = at.row0 + 16 * h + col;
+      my_q[h] = r % a.n_q;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[h][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
-    lsum[h] = 0.f;
-    m[h] = kNegInf;
+      for (int ks = 0; ks < KS; ++ks) {
+        float f[8];
+        load8<T>((const typename T::storage*)a.q + (at.q_row0 + (r < a.n_rows ? r : 0)) * D + 32 * ks + 8 * grp, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = r < a.n_rows && a.q_sign != 0.f ? f[i] * a.q_sign : 0.f;
+        split8<C>(f, qf[h][ks]);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[h][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+      lsum[h] = 0.f;
+      m[h] = kNegInf;
+    }
   }
 
-  auto consume = [&](int c, int b) {
-    const uint16_t *ck = sk[b], *cv = sv[b];
+  // The wave's 16 tokens of the step that starts at token t; g1 ends the slice.
+  template <class Src>
+  __device__ inline void step(const StreamArgs& a, const Src& src, const uint16_t* ck, const uint16_t* cv, int t, int g1) {
     floatx4 s[NB];
 #pragma unroll
     for (int h = 0; h < NB; ++h) s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -325,10 +293,10 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
 #pragma unroll
       for (int h = 0; h < NB; ++h)
 #pragma unroll
-        for (int n = 0; n < NPC; ++n) s[h] = BF16::mfma(x, qf[h][ks][n], s[h]);
+        for (int n = 0; n < NPC; ++n) s[h] = C::mfma(x, qf[h][ks][n], s[h]);
     }
     // lane (grp, col): s[h][i] = score of token t0 + i for row row0 + 16 h + col
-    const int t0 = g0 + c * kTileN + 16 * wave + 4 * grp;
+    const int t0 = t + 16 * wave + 4 * grp;
     uint2 pb[NB][NPC];
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
@@ -355,11 +323,11 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
       lsum[h] += (s[h][0] + s[h][1]) + (s[h][2] + s[h][3]);
 #pragma unroll
       for (int n = 0; n < NPC; ++n) {
-        pb[h][n] = make_uint2(pack2<BF16>(s[h][0], s[h][1]), pack2<BF16>(s[h][2], s[h][3]));
+        pb[h][n] = make_uint2(pack2<C>(s[h][0], s[h][1]), pack2<C>(s[h][2], s[h][3]));
         if (n + 1 < NPC) {
           const uint16_t* p = (const uint16_t*)&pb[h][n];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][i] -= BF16::to_float(p[i]);
+          for (int i = 0; i < 4; ++i) s[h][i] -= C::to_float(p[i]);
         }
       }
     }
@@ -369,16 +337,120 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
 #pragma unroll
       for (int h = 0; h < NB; ++h)
 #pragma unroll
-        for (int n = 0; n < NPC; ++n) o[h][dt] = mfma16k<BF16>(x, pb[h][n], o[h][dt]);
+        for (int n = 0; n < NPC; ++n) o[h][dt] = mfma16k<C>(x, pb[h][n], o[h][dt]);
+    }
+  }
+
+  // The four waves' states meet in LDS (wacc: 64 D floats, wml: 128), one column block
+  // at a time: lane (grp, col) holds O^T rows 16 dt + 4 grp + i of row row0 + 16 h + col.
+  __device__ inline void finish(const StreamArgs& a, const StreamPlace& at, float* wacc, float* wml) {
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+      const float lw = wave_sum16x4(lsum[h]);
+      __syncthreads();                         // the tiles' (or the previous block's) readers are done
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *(floatx4*)(wacc + (wave * 16 + col) * D + 16 * dt + 4 * grp) = o[h][dt];
+      if (grp == 0) {
+        wml[(wave * 16 + col) * 2] = m[h];
+        wml[(wave * 16 + col) * 2 + 1] = lw;
+      }
+      __syncthreads();
+      const int rows_h = min(16, a.n_rows - at.row0 - 16 * h);
+      for (int idx = threadIdx.x; idx < rows_h * (D / 4); idx += 256) {
+        const int rl = idx / (D / 4), d = 4 * (idx % (D / 4));
+        const size_t row = at.q_row0 + at.row0 + 16 * h + rl;
+        float M = kNegInf;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, wml[(w * 16 + rl) * 2]);
+        const float Mu = M == kNegInf ? 0.f : M;
+        float L = 0.f;
+        floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = __builtin_amdgcn_exp2f(wml[(w * 16 + rl) * 2] - Mu);
+          L += wml[(w * 16 + rl) * 2 + 1] * f;
+          x += *(const floatx4*)(wacc + (w * 16 + rl) * D + d) * f;
+        }
+        if (a.n_parts == 1) {
+          x = x / (L == 0.f ? 1.f : L);        // no visible token: 0; NaN stays NaN
+          typename T::storage* dst = (typename T::storage*)a.o + row * D + d;
+          if constexpr (T::is_f32) *(floatx4*)dst = x;
+          else *(uint2*)dst = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+          if (d == 0) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
+        } else {
+          *(floatx4*)(a.acc + (row * a.n_parts + at.split) * D + d) = x;
+          if (d == 0) *(float2*)(a.ml + (row * a.n_parts + at.split) * 2) = make_float2(M, L);
+        }
+      }
+    }
+  }
+};
+
+// Over 8-bit rows. The tokens' codes come by 16-byte loads into registers, two steps
+// ahead, and are written to LDS as bfloat16 (v_cvt_scalef32_pk_bf16_fp8 applies the
+// scale). fp16 and fp32 queries, and their probabilities, are 2 and 3 bfloat16
+// pieces: 2 and 3 times the products, for which the memory-bound stream leaves room.
+// bf16: P is rounded to bfloat16 for P V, as in the 16-bit decode (half a unit of
+// 2^-8 of each weight, averaged over the keys); the row sums add the fp32 P.
+template <typename T, int D, int NB, bool RULE, class Src>
+__global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
+  constexpr int UPR = D / 16;                  // 16-byte units per row
+  constexpr int NU = kTileN * UPR / 256;       // units per thread and tile
+  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
+  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  const int tid = threadIdx.x;
+  const StreamPlace at(a, src, 16 * NB);
+  const int n_chunks = at.chunks();
+  const uint8_t *K = (const uint8_t*)a.k, *V = (const uint8_t*)a.v;
+
+  struct Raw {
+    uint4 k[NU], v[NU];
+    uint8_t ks[NU], vs[NU];
+  };
+  // tokens past the slice repeat its last one and are masked when consumed
+  auto fetch = [&](int c, Raw& r) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int unit = u * 256 + tid;
+      const size_t row = at.kb + src.row(min(at.g0 + c * kTileN + unit / UPR, at.g1 - 1));
+      r.k[u] = ld_nt16(K + row * D + 16 * (unit % UPR));
+      r.ks[u] = a.ks[row];
+      r.v[u] = ld_nt16(V + row * D + 16 * (unit % UPR));
+      r.vs[u] = a.vs[row];
     }
   };
+  auto put16 = [&](uint16_t* tile, int row, int c16, const uint4& w, float scale) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t out[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], scale, false));
+      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], scale, true));
+    }
+    *(uint4*)(tile + lds_off<D>(row, 16 * c16)) = make_uint4(out[0], out[1], out[2], out[3]);
+    *(uint4*)(tile + lds_off<D>(row, 16 * c16 + 8)) = make_uint4(out[4], out[5], out[6], out[7]);
+  };
+  auto put = [&](const Raw& r, int b) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int unit = u * 256 + tid;
+      put16(sk[b], unit / UPR, unit % UPR, r.k[u], scale_of(r.ks[u]));
+      put16(sv[b], unit / UPR, unit % UPR, r.v[u], scale_of(r.vs[u]));
+    }
+  };
+
+  Raw ra, rc;
+  if (n_chunks > 0) fetch(0, ra);
+  if (n_chunks > 1) fetch(1, rc);
+  StreamWave<T, BF16, D, NB, kPieces<T>, RULE> w(a, at);
   // One barrier per step: a buffer is rewritten two steps on, when every wave has
   // passed the barrier of the step between.
   auto step = [&](int c, int b, Raw& r) {
     put(r, b);
     if (c + 2 < n_chunks) fetch(c + 2, r);
     __syncthreads();
-    consume(c, b);
+    w.step(a, src, sk[b], sv[b], at.g0 + c * kTileN, at.g1);
   };
   int c = 0;
   for (; c + 1 < n_chunks; c += 2) {
@@ -386,52 +458,52 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
     step(c + 1, 1, rc);
   }
   if (c < n_chunks) step(c, 0, ra);
+  w.finish(a, at, (float*)&sk[0][0], (float*)&sv[0][0]);
+}
 
-  // The four waves' states meet, one column block at a time: lane (grp, col) holds
-  // O^T rows 16 dt + 4 grp + i of row row0 + 16 h + col.
-  float* wacc = (float*)&sk[0][0];             // [4][16][D]: both K buffers
-  float* wml = (float*)&sv[0][0];              // [4][16][2]
+// Over 16-bit rows: gathered into LDS by LDS-DMA, two steps in flight, so that no
+// registers hold loads.
+template <typename T, int D, int NB, bool RULE, class Src>
+__global__ __launch_bounds__(256) void stream16_kernel(StreamArgs a, Src src) {
+  constexpr int NP = D / 32;                   // 1 KB LDS blocks per wave and 64-row tile
+  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
+  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const StreamPlace at(a, src, 16 * NB);
+  const int n_chunks = at.chunks();
+  const uint16_t *K = (const uint16_t*)a.k + at.kb * D, *V = (const uint16_t*)a.v + at.kb * D;
+  StreamWave<T, T, D, NB, 1, RULE> w(a, at);
+  dma_wait();   // the Q loads are complete before any LDS-DMA is in flight
+
+  // the lane's chunk of LDS block 4 p + wave of a tile: row, swizzled column
+  int drow[NP], dcol[NP];
 #pragma unroll
-  for (int h = 0; h < NB; ++h) {
-    const float lw = wave_sum16x4(lsum[h]);
-    __syncthreads();                           // the buffers' (or the previous block's) readers are done
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      *(floatx4*)(wacc + (wave * 16 + col) * D + 16 * dt + 4 * grp) = o[h][dt];
-    if (grp == 0) {
-      wml[(wave * 16 + col) * 2] = m[h];
-      wml[(wave * 16 + col) * 2 + 1] = lw;
-    }
-    __syncthreads();
-    const int rows_h = min(16, a.n_rows - row0 - 16 * h);
-    for (int idx = tid; idx < rows_h * (D / 4); idx += 256) {
-      const int rl = idx / (D / 4), d = 4 * (idx % (D / 4));
-      const size_t row = q_row0 + row0 + 16 * h + rl;
-      float M = kNegInf;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, wml[(w * 16 + rl) * 2]);
-      const float Mu = M == kNegInf ? 0.f : M;
-      float L = 0.f;
-      floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(wml[(w * 16 + rl) * 2] - Mu);
-        L += wml[(w * 16 + rl) * 2 + 1] * f;
-        x += *(const floatx4*)(wacc + (w * 16 + rl) * D + d) * f;
-      }
-      if (a.n_parts == 1) {
-        const float den = L == 0.f ? 1.f : L;  // no visible token: 0; NaN stays NaN
-        x = x / den;
-        typename T::storage* dst = (typename T::storage*)a.o + row * D + d;
-        if constexpr (T::is_f32) *(floatx4*)dst = x;
-        else *(uint2*)dst = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-        if (d == 0) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
-      } else {
-        *(floatx4*)(a.acc + (row * a.n_parts + split) * D + d) = x;
-        if (d == 0) *(float2*)(a.ml + (row * a.n_parts + split) * 2) = make_float2(M, L);
-      }
-    }
+  for (int p = 0; p < NP; ++p) {
+    const int e = (4 * p + wave) * 512 + 8 * lane;
+    drow[p] = e / D;
+    dcol[p] = (((e % D) >> 3) ^ lds_swz<D>(drow[p])) << 3;
   }
+  // tokens past the slice repeat its last one and are masked when consumed
+  auto issue = [&](int c, int b) {
+    const uint32_t lk = lds_addr(sk[b]), lv = lds_addr(sv[b]);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const size_t off = (size_t)src.row(min(at.g0 + c * kTileN + drow[p], at.g1 - 1)) * D + dcol[p];
+      dma_load16(K + off, lk + (4 * p + wave) * 1024);
+      dma_load16(V + off, lv + (4 * p + wave) * 1024);
+    }
+  };
+  if (n_chunks > 0) issue(0, 0);
+  if (n_chunks > 1) issue(1, 1);
+  for (int c = 0; c < n_chunks; ++c) {
+    const int b = c & 1;
+    wait_chunks<NP, 2>(min(1, n_chunks - 1 - c));   // chunk c has landed
+    __syncthreads();
+    w.step(a, src, sk[b], sv[b], at.g0 + c * kTileN, at.g1);
+    __syncthreads();                           // every wave is done with buffer b
+    if (c + 2 < n_chunks) issue(c + 2, b);
+  }
+  w.finish(a, at, (float*)&sk[0][0], (float*)&sv[0][0]);
 }
 
 // The states of a row's n_parts slices joined: a wave per row.
@@ -476,6 +548,22 @@ void launch_stream8(const StreamArgs& a, const RingStream& src, int n_streams, h
   const dim3 grid(n_streams * a.n_splits * a.row_tiles);
   if (a.n_q == 1) hipLaunchKernelGGL((stream8_kernel<T, D, NB, false, RingStream>), grid, dim3(256), 0, stream, a, src);
   else hipLaunchKernelGGL((stream8_kernel<T, D, NB, true, RingStream>), grid, dim3(256), 0, stream, a, src);
+}
+
+template <typename T, int D, int NB>
+void launch_stream16(const StreamArgs& a, const DenseStream& src, int n_streams, hipStream_t stream) {
+  hipLaunchKernelGGL((stream16_kernel<T, D, NB, false, DenseStream>), dim3(n_streams * a.n_splits * a.row_tiles),
+                     dim3(256), 0, stream, a, src);
+}
+
+template <typename T, int D>
+int cross_stream(StreamArgs a, const DenseStream& src, int n_streams, hipStream_t stream) {
+  const int tile = stream_rows_tile(false, a.n_rows);
+  a.row_tiles = (a.n_rows + tile - 1) / tile;
+  if (tile == 32) launch_stream16<T, D, 2>(a, src, n_streams, stream);
+  else launch_stream16<T, D, 1>(a, src, n_streams, stream);
+  if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
+  return check_launch("gki_cross_fwd");
 }
 
 template <typename T, int D>
@@ -529,6 +617,25 @@ int held_rows(const void* kc, const void* vc, const uint8_t* ks, const uint8_t* 
   if (dtype == kF16) return FN<F16, 128>(__VA_ARGS__);                              \
   return FN<BF16, 128>(__VA_ARGS__);
 
+namespace {
+StreamArgs stream_args(const Geom& g, const void* q, const void* k, const void* v, const uint8_t* ks,
+                       const uint8_t* vs, void* o, float* lse, int kv_rows, float* ws, int n_splits, int head_dim) {
+  StreamArgs a{};
+  a.q = q, a.k = k, a.v = v, a.ks = ks, a.vs = vs, a.o = o, a.lse = lse;
+  a.H_kv = g.H_kv;
+  a.rb = a.n_rows = g.group * g.n_q;
+  a.n_q = g.n_q;
+  a.q_stride = g.H * g.n_q;
+  a.kv_rows = kv_rows;
+  a.n_splits = a.n_parts = n_splits;
+  a.acc = ws;
+  a.ml = ws + (size_t)g.B * g.H * g.n_q * n_splits * head_dim;
+  a.scale_log2 = g.qk_scale_log2;
+  a.q_sign = g.scale == 0.f ? 0.f : g.scale < 0.f ? -1.f : 1.f;
+  return a;
+}
+}  // namespace
+
 int append8_dispatch(int dtype, int head_dim, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn,
                      const void* vn, int BH, int n_new, int start, int sink, int ring, hipStream_t stream) {
   AppendRows a{n_new, 0, 0, 0, start, sink, ring};
@@ -558,19 +665,18 @@ int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, cons
   src.ring = ring;
   src.q_off = g.q_off;
   src.window = g.window;
-  StreamArgs a{};
-  a.q = q, a.k = k, a.v = v, a.ks = ks, a.vs = vs, a.o = o, a.lse = lse;
-  a.H_kv = g.H_kv;
-  a.rb = a.n_rows = g.group * g.n_q;
-  a.n_q = g.n_q;
-  a.q_stride = g.H * g.n_q;
-  a.kv_rows = g.sink + ring;
-  a.n_splits = a.n_parts = n_splits;
-  a.acc = ws;
-  a.ml = ws + (size_t)g.B * g.H * g.n_q * n_splits * head_dim;
-  a.scale_log2 = g.qk_scale_log2;
-  a.q_sign = g.scale == 0.f ? 0.f : g.scale < 0.f ? -1.f : 1.f;
+  const StreamArgs a = stream_args(g, q, k, v, ks, vs, o, lse, g.sink + ring, ws, n_splits, head_dim);
   GKI_BY_TYPE(attend8, a, src, g.B * g.H_kv, stream)
+}
+
+int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
+                          float* lse, float* ws, int n_splits, hipStream_t stream) {
+  const DenseStream src{g.kv_len, g.n_kv, g.H_kv};
+  const StreamArgs a = stream_args(g, q, k, v, nullptr, nullptr, o, lse, g.n_kv, ws, n_splits, head_dim);
+  const int n = g.B * g.H_kv;
+  if (dtype == kF16)
+    return head_dim == 64 ? cross_stream<F16, 64>(a, src, n, stream) : cross_stream<F16, 128>(a, src, n, stream);
+  return head_dim == 64 ? cross_stream<BF16, 64>(a, src, n, stream) : cross_stream<BF16, 128>(a, src, n, stream);
 }
 
 }  // namespace gki

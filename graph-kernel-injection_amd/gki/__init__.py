@@ -5,6 +5,7 @@ kept-block lists, the autograd bridge over the HIP kernels in
 ``libgki_bsa.so``, and the torch.fx pass that injects it.
 """
 
+from .cross import cross_attention
 from .fx_pass import (
     BlockSparseAttentionInjector,
     InjectionConfig,
@@ -30,6 +31,7 @@ __all__ = [
     "block_sparse_attention",
     "build_block_lists",
     "clear_schedule_cache",
+    "cross_attention",
     "make_dense_mask",
     "make_streaming_mask",
     "pretty_print_graph",

@@ -1,0 +1,160 @@
+"""Cross attention: queries over another sequence's keys, padded to a common length.
+
+The second attention of an encoder-decoder layer. Every query row of batch entry ``b``
+sees the first ``kv_lengths[b]`` keys (all of them without lengths); nothing is causal
+and no mask is built: the kernels walk the tiles an entry has, forward (``gki_cross_fwd``)
+and backward (``gki_cross_bwd``). A decoder's step -- up to 32 query rows per K/V head
+-- reads each key once for a whole group of heads, cut into slices that fill the card.
+
+There is no CPU or eager fallback: a missing library raises ``RuntimeError``.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _DTYPE_CODE, _HEAD_DIMS, _aligned, _current_stream, _on_device
+
+# launch plans: (dtype, B, H, H_kv, n_q, n_kv, D) -> (slices, their workspace floats)
+_PLANS: dict = {}
+
+
+def _fwd_plan(lib, key) -> Tuple[int, int]:
+    plan = _PLANS.get(key)
+    if plan is None:
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        _, B, H, _, n_q, _, D = key
+        splits = int(lib.gki_cross_splits(*key))
+        plan = _PLANS[key] = (splits, int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits)))
+    return plan
+
+
+def _check(q, k, v, kv_lengths, enable_gqa) -> None:
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("Q/K/V must be 4-D [B, H, N, D] tensors")
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise ValueError("All inputs must live on a CUDA device")
+    if q.device != k.device or q.device != v.device:
+        raise ValueError("Q/K/V must live on one device")
+    if k.shape != v.shape:
+        raise ValueError("K and V must share shape")
+    B, H, _, D = q.shape
+    H_kv = k.shape[1]
+    if k.shape[0] != B or k.shape[-1] != D or not (
+            H_kv == H or (enable_gqa and H_kv > 0 and H % H_kv == 0)):
+        raise ValueError("Q/K/V batch/head/dim mismatch")
+    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in _DTYPE_CODE:
+        raise ValueError(f"Q/K/V must share one dtype among float32/float16/bfloat16, got "
+                         f"{q.dtype}/{k.dtype}/{v.dtype}")
+    if D not in _HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {_HEAD_DIMS}, got {D}")
+    if kv_lengths is not None:
+        if kv_lengths.dtype not in (torch.int32, torch.int64) or kv_lengths.shape != (B,):
+            raise ValueError(f"kv_lengths must be an int32 or int64 tensor [{B}], got {kv_lengths.dtype} "
+                             f"{tuple(kv_lengths.shape)}")
+        if kv_lengths.device != q.device:
+            raise ValueError(f"kv_lengths must live on {q.device}")
+
+
+def _forward(q, k, v, kv_lengths, scale):
+    """(o, lse, q, k, v, kv_lengths) with the inputs as the kernels read them."""
+    lib = _lib.load()
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    if kv_lengths is not None:
+        if kv_lengths.dtype != torch.int32:
+            kv_lengths = kv_lengths.clamp(0, k.shape[2]).to(torch.int32)
+        kv_lengths = kv_lengths.contiguous()
+    B, H, n_q, D = q.shape
+    H_kv, n_kv = k.shape[1], k.shape[2]
+    o = torch.empty_like(q)
+    rows = B * H * n_q
+    if rows == 0 or n_kv == 0:
+        return o.zero_(), torch.zeros((B, H, n_q), dtype=torch.float32, device=q.device), q, k, v, kv_lengths
+    key = (_DTYPE_CODE[q.dtype], B, H, H_kv, n_q, n_kv, D)
+    splits, ws_floats = _fwd_plan(lib, key)
+    # the LSE rows (padded to 256 bytes), then the slices' states: one allocation
+    pad = (rows + 63) & ~63 if ws_floats else rows
+    scratch = torch.empty(pad + ws_floats, dtype=torch.float32, device=q.device)
+    with _on_device(q.device):
+        rc = lib.gki_cross_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), scratch.data_ptr(), *key,
+            0 if kv_lengths is None else kv_lengths.data_ptr(), scale,
+            scratch.data_ptr() + 4 * pad if ws_floats else 0, splits, _current_stream(q.device))
+    _lib.check(rc, "gki_cross_fwd")
+    return o, scratch, q, k, v, kv_lengths
+
+
+class _CrossAttention(torch.autograd.Function):
+    """Autograd bridge between PyTorch and the gfx950 kernels."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lengths, scale):  # type: ignore[override]
+        o, lse, q, k, v, kv_lengths = _forward(q, k, v, kv_lengths, scale)
+        B, H, n_q, _ = q.shape
+        rows = lse.view(-1)[:B * H * n_q]
+        # a step's states follow its LSE rows: they need not outlive the forward
+        ctx.save_for_backward(q, k, v, o, rows if rows.numel() == lse.numel() else rows.clone(), kv_lengths)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):  # type: ignore[override]
+        lib = _lib.load()
+        q, k, v, o, lse, kv_lengths = ctx.saved_tensors
+        B, H, n_q, D = q.shape
+        H_kv, n_kv = k.shape[1], k.shape[2]
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        if q.numel() == 0 or k.numel() == 0:
+            return dq.zero_(), dk.zero_(), dv.zero_(), None, None
+        do = _aligned(do.to(q.dtype))
+        shape = (_DTYPE_CODE[q.dtype], B, H, H_kv, n_q, n_kv, D)
+        parts = int(lib.gki_cross_bwd_parts(*shape))
+        tile = _lib.tile_sizes()["tile_n"]
+        # row terms (Delta, then a form of the LSE), then the parts' fp32 dK / dV sums
+        pad = (2 * B * H * n_q + 63) & ~63
+        sums = B * H_kv * -(-n_kv // tile) * parts * 2 * tile * D if parts > 1 else 0
+        scratch = torch.empty(pad + sums, dtype=torch.float32, device=q.device)
+        with _on_device(q.device):
+            rc = lib.gki_cross_bwd(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), scratch.data_ptr(), *shape,
+                0 if kv_lengths is None else kv_lengths.data_ptr(), ctx.scale, parts,
+                scratch.data_ptr() + 4 * pad if sums else 0, _current_stream(q.device))
+        _lib.check(rc, "gki_cross_bwd")
+        return dq, dk, dv, None, None
+
+
+def cross_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    kv_lengths: Optional[torch.Tensor] = None,
+    softmax_scale: Optional[float] = None,
+    enable_gqa: bool = False,
+) -> torch.Tensor:
+    """Differentiable attention of ``q`` (``[B, H, N_Q, D]``) over another sequence's
+    ``k``, ``v`` (``[B, H, N_KV, D]``), every visible key for every query.
+
+    One dtype among fp32/fp16/bf16, ``D`` in {16, 32, 64, 128}, any ``N_Q`` and
+    ``N_KV``. ``kv_lengths``: int32 or int64 ``[B]`` on the same device, the valid keys of
+    each batch entry (the first ones; a value outside ``0 .. N_KV`` counts as the nearest
+    of them, as the device is not asked); keys past them are not read and get zero
+    gradients, an entry without keys gives zeros (and zero gradients).
+    ``softmax_scale`` defaults to ``1/sqrt(D)``, any finite value is taken.
+    ``enable_gqa``: K and V may have ``H_kv`` heads dividing Q's ``H``, as in
+    ``block_sparse_attention``. Differentiable once.
+    """
+    _check(q, k, v, kv_lengths, enable_gqa)
+    scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"softmax_scale must be finite, got {scale}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossAttention.apply(q, k, v, kv_lengths, scale)
+    return _forward(q, k, v, kv_lengths, scale)[0]

@@ -302,6 +302,40 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
                         int32_t window_size, int32_t ring_size, int64_t length, float softmax_scale,
                         float* workspace, int32_t n_splits, void* stream);
 
+/* ---- Cross attention ----------------------------------------------------------
+ * No reference counterpart. Every query row of batch entry b over its first
+ * kv_len[b] keys (int32 [B] on the device; a length outside 0 .. n_kv counts as the
+ * nearest of them; NULL: all n_kv), not causal. An entry without keys has O = 0,
+ * LSE = 0 and zero gradients; keys past an entry's length are not read and have
+ * zero gradients. Grouped-query heads as above. */
+
+/* Slices per K/V head for gki_cross_fwd: 0 where the rows run as q tiles. */
+int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
+                     int32_t head_dim);
+
+/* O and LSE (natural). n_splits 0: a workgroup per q tile and head. n_splits >= 1
+ * (fp16 / bf16, head_dim 64 or 128): the group's rows of a K/V head against slices of
+ * its keys, for few query rows; 16-byte aligned workspace of
+ * gki_stream_workspace_floats(B, H, n_q, head_dim, n_splits) floats. */
+int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int32_t dtype,
+                  int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                  const int32_t* kv_len, float softmax_scale, float* workspace, int32_t n_splits,
+                  void* stream);
+
+/* Parts per kv tile that gki_cross_bwd cuts dK/dV into for a full card (any
+ * parts >= 1 is right). */
+int gki_cross_bwd_parts(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
+                        int32_t n_kv, int32_t head_dim);
+
+/* dQ, dK, dV (fully written) from the forward's O and LSE. delta: fp32
+ * [2, B, H, n_q] workspace as in gki_bsa_bwd; kv_partials: 16-byte aligned fp32
+ * workspace [B * H_kv][ceil(n_kv / 64) * parts][2][64][head_dim] when parts > 1. */
+int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                  const float* lse, void* dq, void* dk, void* dv, float* delta, int32_t dtype,
+                  int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                  const int32_t* kv_len, float softmax_scale, int32_t parts, float* kv_partials,
+                  void* stream);
+
 /* Measurement helper, no counterpart in the reference: reads exactly the K and V
  * bytes a single-position StreamingLLM decode step reads from a full cache --
  * per (b, kv head) slice of bh slices of n_kv rows of row_bytes (a multiple of
