@@ -65,6 +65,10 @@ int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q,
 int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                        const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                        int parts, float* partials, hipStream_t stream);
+int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                           const uint8_t* ks, const uint8_t* vs, const void* prefix_k, const void* prefix_v, int n_prefix,
+                           void* o, float* lse, int ring, float* ws, int n_prefix_splits, int n_splits,
+                           hipStream_t stream);
 int64_t read_probe_words(int BH);
 int read_probe_dispatch(const void* k, const void* v, int BH, int64_t n_kv, int row_bytes, int n_sink,
                         int64_t w_lo, uint32_t* out, hipStream_t stream);
@@ -624,6 +628,37 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
                           rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale), q, k_codes,
                           v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, o, lse, ring_size, workspace,
                           n_splits, (hipStream_t)stream);
+}
+
+int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
+                      int32_t n_prefix) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_prefix <= 0) return 1;
+  const int64_t rows = (int64_t)B * (H / H_kv) * n_q;
+  const int64_t tile = prefix_as_streams(rows) ? stream_rows_tile(false, (int)rows) : kTileMF;
+  return stream_splits(head_dim, H_kv * ((rows + tile - 1) / tile), n_prefix);
+}
+
+int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+                              const void* v_scale, const void* prefix_k, const void* prefix_v, int32_t n_prefix,
+                              void* o, float* lse, int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
+                              int32_t head_dim, int32_t sink_size, int32_t window_size, int32_t ring_size,
+                              int64_t length, float softmax_scale, float* workspace, int32_t n_prefix_splits,
+                              int32_t n_splits, void* stream) {
+  if (int rc = rolling_decode_args(dtype, B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, length,
+                                   softmax_scale, q, k_cache, v_cache, o, lse, n_splits))
+    return rc;
+  GKI_REQUIRE(dtype != kF32, 2, "gki_rolling_prefix_decode: fp16 or bf16");
+  GKI_REQUIRE(prefix_k && prefix_v && workspace && !k_scale == !v_scale, 1, "gki_rolling_prefix_decode: null pointer");
+  GKI_REQUIRE(all_aligned16(prefix_k, prefix_v, o, workspace), 1,
+              "gki_rolling_prefix_decode: the prefix, o and the workspace must be 16-byte aligned");
+  GKI_REQUIRE(n_prefix >= 1 && n_prefix < (1 << kPartialBit), 1, "gki_rolling_prefix_decode: n_prefix must be in [1, 2^30)");
+  const int64_t tiles = ((int64_t)B * (H / H_kv) * n_q + 15) / 16 * H_kv;
+  GKI_REQUIRE(n_prefix_splits >= 1 && tiles * n_prefix_splits < (1ll << 23), 1,
+              "gki_rolling_prefix_decode: n_prefix_splits must be >= 1 and the grid must fit");
+  return prefix_decode_dispatch(dtype, head_dim,
+                                rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale), q, k_cache,
+                                v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale, prefix_k, prefix_v, n_prefix,
+                                o, lse, ring_size, workspace, n_prefix_splits, n_splits, (hipStream_t)stream);
 }
 
 int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,

@@ -584,6 +584,16 @@ struct Geom {
   const int32_t* kv_len;
 };
 
+// Rows of several sequences against one K / V (a shared prefix): row r of kv head h is
+// row h rb + (r / rb) q_stride + r % rb of Q, rb = group * n_q rows that one sequence
+// has of it. A workgroup takes a slice of the keys and writes its state, part
+// part0 + slice of the row's n_parts: acc [rows][n_parts][D], ml [rows][n_parts][2].
+struct SharedRows {
+  int n_rows, rb, q_stride, n_splits, part0, n_parts;
+  float *acc, *ml;
+  __device__ inline size_t row(int h, int r) const { return (size_t)h * rb + (size_t)(r / rb) * q_stride + r % rb; }
+};
+
 // Work list of the dK / dV grid (built on the host by gki_dkdv_items). A kv
 // tile's walk -- group x (its kept q tiles) iterations, iteration i visiting
 // list entry i % L of q head i / L -- is cut into items of at most a chunk of
@@ -600,6 +610,10 @@ struct KvWork {
   float* partials;        // [B * H_kv][n_pslots][2 (dK, dV)][64][D] fp32
   int parts;              // dense walks: items per kv tile (no list: item i is part i % parts of tile i / parts)
 };
+
+// Walks of the 16-bit forward: listed tiles, every tile of an entry's own keys, a
+// slice of a shared prefix's.
+enum Walk : int { kListed = 0, kDense = 1, kShared = 2 };
 
 // Dense walks: the kernels' DENSE forms read no list. A q tile visits every kv tile
 // of its batch entry's own keys, a kv tile every q tile; entry e of either walk is
@@ -853,6 +867,9 @@ inline void surviving_rows(int start, int n_new, int sink, int ring, int* n_a, i
 // Query rows per workgroup of the stream kernels: one block of 16, or two where a
 // stream has more (fp32: its three pieces of each operand leave registers for one).
 inline int stream_rows_tile(bool f32, int n_rows) { return f32 || n_rows <= 16 ? 16 : 32; }
+
+// Does a shared prefix run its rows as streams (blocks of 16, few rows) or as 128-row tiles?
+inline bool prefix_as_streams(int64_t n_rows) { return n_rows <= 64; }
 
 // Slices of each stream: enough workgroups for two rounds of what the card holds at
 // once (two per CU at head_dim 128, four at 64, by their 64 KB and 32 KB of LDS), of

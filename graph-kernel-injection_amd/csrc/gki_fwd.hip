@@ -81,25 +81,27 @@ constexpr int kFwdThreads = 256;
 // N8192 D64 W1024 fp16 0.174 -> 0.168, B1 H16 N131072 D64 W4096 bf16 2.20 ->
 // 2.16, 500 queries behind 8500 keys D128 0.0525 -> 0.0467, B4 H8 N2000 D32
 // 0.0177 -> 0.0150.
-template <typename T, int D, bool PIPE, bool DENSE>
+template <typename T, int D, bool PIPE, int WALK>
 __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
     Geom g, const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
     const uint16_t* __restrict__ V, uint16_t* __restrict__ O, float* __restrict__ LSE,
     const int32_t* __restrict__ row_ptr, const int32_t* __restrict__ row_idx, int n_qt,
-    const int32_t* __restrict__ wg_order) {
+    const int32_t* __restrict__ wg_order, SharedRows sh) {
+  constexpr bool DENSE = WALK != kListed, SHARED = WALK == kShared;
   constexpr int KS = D / 16;                   // k-steps of the QK^T contraction
   constexpr int DT = D >= 32 ? D / 32 : 1;     // 32-row tiles of O^T
   constexpr int NW = 4;
   __shared__ __align__(16) uint16_t sk[2][kTileN * D];
   __shared__ __align__(16) uint16_t sv[2][kTileN * D];
 
-  const int n_wg = n_qt * g.B * g.H;
+  const int n_wg = SHARED ? gridDim.x : n_qt * g.B * g.H;
   const int wg = work_of(blockIdx.x, n_wg, wg_order);
   if (wg < 0) return;
+  // SHARED: the row tiles of a slice are neighbours, its head is bh / n_splits
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
-  const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
-  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
+  const size_t kb = (size_t)(SHARED ? bh / sh.n_splits : kv_bh(g, bh)) * g.n_kv * D;
+  if constexpr (WALK == kDense) g.n_kv = own_keys(g, bh / g.H);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const Lane32<D> at(lane);
@@ -108,8 +110,13 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
   uint4 qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    const uint4 v = q_words(g, row16_or_zero<D>(Q + qb, qw + col, g.n_q, 16 * ks + 8 * hi));
-    qf[ks] = qw + col < g.n_q ? v : make_uint4(0, 0, 0, 0);
+    if constexpr (SHARED) {
+      const int r = min(qw + col, g.n_q - 1), d = 16 * ks + 8 * hi;
+      qf[ks] = q_words(g, *(const uint4*)(Q + sh.row(bh / sh.n_splits, r) * D + d));
+    } else {
+      const uint4 v = q_words(g, row16_or_zero<D>(Q + qb, qw + col, g.n_q, 16 * ks + 8 * hi));
+      qf[ks] = qw + col < g.n_q ? v : make_uint4(0, 0, 0, 0);
+    }
   }
 
   floatx16 o[DT];
@@ -202,7 +209,9 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
       lsum = T::mfma(ones, p[st], lsum);
     }
   };
-  const int e_beg = DENSE ? 0 : row_ptr[qt], e_end = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1];
+  const int n_kt = kv_tiles_of(g), slice = SHARED ? bh % sh.n_splits : 0;
+  const int e_beg = SHARED ? (int)((int64_t)n_kt * slice / sh.n_splits) : DENSE ? 0 : row_ptr[qt];
+  const int e_end = SHARED ? (int)((int64_t)n_kt * (slice + 1) / sh.n_splits) : DENSE ? n_kt : row_ptr[qt + 1];
   auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   if constexpr (!PIPE) {
     if (e_beg < e_end) {
@@ -332,6 +341,18 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
   const int hi_e = lane_e >> 5;
   const int my_q = qw + (lane_e & 31);
   const float l_tot = lsum[0];
+  if constexpr (SHARED) {
+    if (my_q >= g.n_q) return;
+    const size_t at = sh.row(bh / sh.n_splits, my_q) * sh.n_parts + sh.part0 + slice;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *(floatx4*)(sh.acc + at * D + 32 * dt + 8 * r + 4 * hi_e) =
+            floatx4{o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]};
+    if (hi_e == 0) *(float2*)(sh.ml + at * 2) = make_float2(l_tot == 0.f ? kNegInf : -nm, l_tot);
+    return;
+  }
   const bool valid = l_tot > 0.f;
   const float inv = valid ? 1.f / l_tot : 1.f;
   if (my_q < g.n_q) {
@@ -782,14 +803,14 @@ void launch_fwd16(const Geom& g, const void* q, const void* k, const void* v, vo
                   const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* wg_order,
                   hipStream_t stream) {
   const int grid = n_qt * g.B * g.H;
-#define GKI_FWD16(KERNEL, GRID, THREADS)                                                           \
+#define GKI_FWD16(KERNEL, GRID, THREADS, ...)                                                           \
   hipLaunchKernelGGL(KERNEL, dim3(GRID), dim3(THREADS), 0, stream, g, (const uint16_t*)q,          \
                      (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)o, lse, row_ptr, row_idx,  \
-                     n_qt, wg_order)
+                     n_qt, wg_order __VA_OPT__(,) __VA_ARGS__)
   if (fwd_shares_keys(D, grid, DENSE ? kv_tiles_of(g) : row_kv_tiles(g, kTileMF)))
     GKI_FWD16((fwd_split_16<T, D, DENSE>), work_parts_grid(grid, 2), 512);
   else
-    GKI_FWD16((fwd_kernel_16<T, D, kFwdPipe<D>, DENSE>), grid, kFwdThreads);
+    GKI_FWD16((fwd_kernel_16<T, D, kFwdPipe<D>, DENSE ? kDense : kListed>), grid, kFwdThreads, SharedRows{});
 #undef GKI_FWD16
 }
 
@@ -830,6 +851,25 @@ int fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
     case 128: return launch_fwd<128, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
     default: return fail(2, "unsupported head_dim " + std::to_string(head_dim));
   }
+}
+
+namespace {
+template <typename T, int D>
+int launch_prefix(const Geom& g, const void* q, const void* k, const void* v, const SharedRows& sh, hipStream_t stream) {
+  const int n_qt = (g.n_q + kTileMF - 1) / kTileMF;
+  hipLaunchKernelGGL((fwd_kernel_16<T, D, kFwdPipe<D>, kShared>), dim3(n_qt * sh.n_splits * g.H_kv), dim3(kFwdThreads),
+                     0, stream, g, (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)nullptr,
+                     (float*)nullptr, (const int32_t*)nullptr, (const int32_t*)nullptr, n_qt, (const int32_t*)nullptr, sh);
+  return check_launch("gki_rolling_prefix_decode");
+}
+}  // namespace
+
+// The rows of a batch against a prefix that its sequences share: g.n_q rows of each of
+// g.H_kv heads over g.n_kv keys.
+int prefix_tiles_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                          const SharedRows& sh, hipStream_t stream) {
+  if (dtype == kF16) return head_dim == 64 ? launch_prefix<F16, 64>(g, q, k, v, sh, stream) : launch_prefix<F16, 128>(g, q, k, v, sh, stream);
+  return head_dim == 64 ? launch_prefix<BF16, 64>(g, q, k, v, sh, stream) : launch_prefix<BF16, 128>(g, q, k, v, sh, stream);
 }
 
 int cross_fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,

@@ -26,6 +26,9 @@
 #include "gki_common.cuh"
 
 namespace gki {
+int prefix_tiles_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                          const SharedRows& sh, hipStream_t stream);
+
 namespace {
 
 constexpr int kMinExponent = -117;           // 2^-9 (the smallest code) * 2^-117 is a normal float
@@ -200,7 +203,8 @@ struct StreamArgs {
   int n_q, q_stride;           // q_stride = H * n_q rows of Q between batch entries
   int kv_rows;                 // rows that K and V hold per stream
   int n_rows, row_tiles;       // query rows of a stream, and tiles of them
-  int n_splits, n_parts;       // slices here; states per row in the workspace (1: O and LSE are written here)
+  int n_splits;                // slices here: parts part0 .. of the n_parts states that a row has in the
+  int part0, n_parts;          // workspace (n_parts 1: O and LSE are written here)
   float scale_log2;            // |scale| log2 e (log2 e for scale 0), the sign in q_sign
   float q_sign;                // 1, -1, or 0: the scores are those of q_sign * q
 };
@@ -240,6 +244,10 @@ struct StreamPlace {
     g0 = (int)(((int64_t)n_tok * split) / a.n_splits);
     g1 = (int)(((int64_t)n_tok * (split + 1)) / a.n_splits);
   }
+  // Row r of the stream in Q: a shared prefix is read by rb rows of each sequence.
+  __device__ inline size_t q_row(const StreamArgs& a, int r) const {
+    return a.n_rows == a.rb ? q_row0 + r : q_row0 + (size_t)(r / a.rb) * a.q_stride + r % a.rb;
+  }
   __device__ inline int chunks() const { return (g1 - g0 + kTileN - 1) / kTileN; }
 };
 
@@ -269,7 +277,7 @@ struct StreamWave {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         float f[8];
-        load8<T>((const typename T::storage*)a.q + (at.q_row0 + (r < a.n_rows ? r : 0)) * D + 32 * ks + 8 * grp, f);
+        load8<T>((const typename T::storage*)a.q + at.q_row(a, r < a.n_rows ? r : 0) * D + 32 * ks + 8 * grp, f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = r < a.n_rows && a.q_sign != 0.f ? f[i] * a.q_sign : 0.f;
         split8<C>(f, qf[h][ks]);
@@ -359,7 +367,7 @@ struct StreamWave {
       const int rows_h = min(16, a.n_rows - at.row0 - 16 * h);
       for (int idx = threadIdx.x; idx < rows_h * (D / 4); idx += 256) {
         const int rl = idx / (D / 4), d = 4 * (idx % (D / 4));
-        const size_t row = at.q_row0 + at.row0 + 16 * h + rl;
+        const size_t row = at.q_row(a, at.row0 + 16 * h + rl);
         float M = kNegInf;
 #pragma unroll
         for (int w = 0; w < 4; ++w) M = fmaxf(M, wml[(w * 16 + rl) * 2]);
@@ -379,8 +387,8 @@ struct StreamWave {
           else *(uint2*)dst = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
           if (d == 0) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
         } else {
-          *(floatx4*)(a.acc + (row * a.n_parts + at.split) * D + d) = x;
-          if (d == 0) *(float2*)(a.ml + (row * a.n_parts + at.split) * 2) = make_float2(M, L);
+          *(floatx4*)(a.acc + (row * a.n_parts + a.part0 + at.split) * D + d) = x;
+          if (d == 0) *(float2*)(a.ml + (row * a.n_parts + a.part0 + at.split) * 2) = make_float2(M, L);
         }
       }
     }
@@ -543,41 +551,68 @@ void launch_join(const StreamArgs& a, int64_t n_rows, hipStream_t stream) {
                      (typename T::storage*)a.o, a.lse, n_rows, a.n_parts);
 }
 
-template <typename T, int D, int NB>
-void launch_stream8(const StreamArgs& a, const RingStream& src, int n_streams, hipStream_t stream) {
+// The streams of a launch in row tiles of the size that their rows take.
+template <typename T, int D, bool EIGHT, class Src>
+void launch_streams(StreamArgs a, const Src& src, int n_streams, hipStream_t stream) {
+  const int tile = stream_rows_tile(T::is_f32, a.n_rows);
+  a.row_tiles = (a.n_rows + tile - 1) / tile;
   const dim3 grid(n_streams * a.n_splits * a.row_tiles);
-  if (a.n_q == 1) hipLaunchKernelGGL((stream8_kernel<T, D, NB, false, RingStream>), grid, dim3(256), 0, stream, a, src);
-  else hipLaunchKernelGGL((stream8_kernel<T, D, NB, true, RingStream>), grid, dim3(256), 0, stream, a, src);
-}
-
-template <typename T, int D, int NB>
-void launch_stream16(const StreamArgs& a, const DenseStream& src, int n_streams, hipStream_t stream) {
-  hipLaunchKernelGGL((stream16_kernel<T, D, NB, false, DenseStream>), dim3(n_streams * a.n_splits * a.row_tiles),
-                     dim3(256), 0, stream, a, src);
+#define GKI_STREAM(NB, RULE)                                                                                      \
+  do {                                                                                                            \
+    if constexpr (EIGHT) hipLaunchKernelGGL((stream8_kernel<T, D, NB, RULE, Src>), grid, dim3(256), 0, stream, a, src); \
+    else hipLaunchKernelGGL((stream16_kernel<T, D, NB, RULE, Src>), grid, dim3(256), 0, stream, a, src);            \
+  } while (0)
+  if constexpr (std::is_same<Src, DenseStream>::value) {     // every token is visible to every row
+    if (tile == 32) GKI_STREAM(2, false);
+    else GKI_STREAM(1, false);
+  } else if constexpr (T::is_f32) {
+    if (a.n_q == 1) GKI_STREAM(1, false);
+    else GKI_STREAM(1, true);
+  } else {
+    if (a.n_q == 1 && tile == 32) GKI_STREAM(2, false);
+    else if (a.n_q == 1) GKI_STREAM(1, false);
+    else if (tile == 32) GKI_STREAM(2, true);
+    else GKI_STREAM(1, true);
+  }
+#undef GKI_STREAM
 }
 
 template <typename T, int D>
-int cross_stream(StreamArgs a, const DenseStream& src, int n_streams, hipStream_t stream) {
-  const int tile = stream_rows_tile(false, a.n_rows);
-  a.row_tiles = (a.n_rows + tile - 1) / tile;
-  if (tile == 32) launch_stream16<T, D, 2>(a, src, n_streams, stream);
-  else launch_stream16<T, D, 1>(a, src, n_streams, stream);
+int cross_stream(const StreamArgs& a, const DenseStream& src, int n_streams, hipStream_t stream) {
+  launch_streams<T, D, false>(a, src, n_streams, stream);
   if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
   return check_launch("gki_cross_fwd");
 }
 
 template <typename T, int D>
-int attend8(StreamArgs a, const RingStream& src, int n_streams, hipStream_t stream) {
-  const int tile = stream_rows_tile(T::is_f32, a.n_rows);
-  a.row_tiles = (a.n_rows + tile - 1) / tile;
-  if constexpr (!T::is_f32) {
-    if (tile == 32) launch_stream8<T, D, 2>(a, src, n_streams, stream);
-    else launch_stream8<T, D, 1>(a, src, n_streams, stream);
-  } else {
-    launch_stream8<T, D, 1>(a, src, n_streams, stream);
-  }
+int attend8(const StreamArgs& a, const RingStream& src, int n_streams, hipStream_t stream) {
+  launch_streams<T, D, true>(a, src, n_streams, stream);
   if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
   return check_launch("gki_rolling8_decode");
+}
+
+// A prefix that the sequences share, then each sequence's own cache, then their states
+// joined. `own` and `shared` differ in the rows, the keys and the parts.
+template <typename T, int D>
+int prefix_decode(const Geom& g, const StreamArgs& own, const RingStream& ring, const StreamArgs& shared, int n_prefix,
+                  hipStream_t stream) {
+  if (prefix_as_streams(shared.n_rows)) {
+    launch_streams<T, D, false>(shared, DenseStream{nullptr, n_prefix, g.H_kv}, g.H_kv, stream);
+  } else {
+    Geom pg = g;
+    pg.n_q = shared.n_rows;
+    pg.n_kv = n_prefix;
+    pg.causal = 0;
+    const SharedRows sh{shared.n_rows, shared.rb, shared.q_stride, shared.n_splits, shared.part0, shared.n_parts,
+                        shared.acc, shared.ml};
+    if (int rc = prefix_tiles_dispatch(std::is_same<T, F16>::value ? kF16 : kBF16, D, pg, shared.q, shared.k, shared.v,
+                                       sh, stream))
+      return rc;
+  }
+  if (own.ks) launch_streams<T, D, true>(own, ring, g.B * g.H_kv, stream);
+  else launch_streams<T, D, false>(own, ring, g.B * g.H_kv, stream);
+  launch_join<T, D>(own, (int64_t)g.B * g.H * g.n_q, stream);
+  return check_launch("gki_rolling_prefix_decode");
 }
 
 // A workgroup per 256 lanes of work, up to a grid whose lanes a launch can count.
@@ -634,6 +669,15 @@ StreamArgs stream_args(const Geom& g, const void* q, const void* k, const void* 
   a.q_sign = g.scale == 0.f ? 0.f : g.scale < 0.f ? -1.f : 1.f;
   return a;
 }
+RingStream ring_args(const Geom& g, int ring) {
+  RingStream src;
+  ring_stream(g.n_kv, g.n_q, g.sink, g.window, ring, &src.n_sink, &src.w_lo, &src.base, &src.n_tokens);
+  src.sink = g.sink;
+  src.ring = ring;
+  src.q_off = g.q_off;
+  src.window = g.window;
+  return src;
+}
 }  // namespace
 
 int append8_dispatch(int dtype, int head_dim, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn,
@@ -659,12 +703,7 @@ int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const
 int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                      const uint8_t* ks, const uint8_t* vs, void* o, float* lse, int ring, float* ws, int n_splits,
                      hipStream_t stream) {
-  RingStream src;
-  ring_stream(g.n_kv, g.n_q, g.sink, g.window, ring, &src.n_sink, &src.w_lo, &src.base, &src.n_tokens);
-  src.sink = g.sink;
-  src.ring = ring;
-  src.q_off = g.q_off;
-  src.window = g.window;
+  const RingStream src = ring_args(g, ring);
   const StreamArgs a = stream_args(g, q, k, v, ks, vs, o, lse, g.sink + ring, ws, n_splits, head_dim);
   GKI_BY_TYPE(attend8, a, src, g.B * g.H_kv, stream)
 }
@@ -677,6 +716,25 @@ int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q,
   if (dtype == kF16)
     return head_dim == 64 ? cross_stream<F16, 64>(a, src, n, stream) : cross_stream<F16, 128>(a, src, n, stream);
   return head_dim == 64 ? cross_stream<BF16, 64>(a, src, n, stream) : cross_stream<BF16, 128>(a, src, n, stream);
+}
+
+int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
+                           const uint8_t* ks, const uint8_t* vs, const void* prefix_k, const void* prefix_v, int n_prefix,
+                           void* o, float* lse, int ring, float* ws, int n_prefix_splits, int n_splits,
+                           hipStream_t stream) {
+  const int n_parts = n_prefix_splits + n_splits;
+  StreamArgs own = stream_args(g, q, k, v, ks, vs, o, lse, g.sink + ring, ws, n_parts, head_dim);
+  own.n_splits = n_splits;
+  own.part0 = n_prefix_splits;
+  StreamArgs shared = stream_args(g, q, prefix_k, prefix_v, nullptr, nullptr, o, lse, n_prefix, ws, n_parts, head_dim);
+  shared.n_splits = n_prefix_splits;
+  shared.n_rows = g.B * shared.rb;
+  const RingStream src = ring_args(g, ring);
+  if (dtype == kF16)
+    return head_dim == 64 ? prefix_decode<F16, 64>(g, own, src, shared, n_prefix, stream)
+                          : prefix_decode<F16, 128>(g, own, src, shared, n_prefix, stream);
+  return head_dim == 64 ? prefix_decode<BF16, 64>(g, own, src, shared, n_prefix, stream)
+                        : prefix_decode<BF16, 128>(g, own, src, shared, n_prefix, stream);
 }
 
 }  // namespace gki

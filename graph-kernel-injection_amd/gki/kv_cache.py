@@ -24,6 +24,10 @@ positions: 2 x 135 MB instead of 2 x 6.55 GB.
 power of two (``k_scale`` / ``v_scale``), the smallest 2^e with the row's largest
 magnitude at most 448 * 2^e. Rows are quantised as they are appended, attention runs
 over the stored values (code * 2^e), and ``read`` gives back what either kind holds.
+
+``set_prefix`` puts keys and values that all sequences of the batch share (a system
+prompt, a document) in front of every sequence's own positions, held once: the decode
+runs the queries of all sequences against each read of them.
 """
 
 from __future__ import annotations
@@ -111,14 +115,41 @@ class StreamingKVCache:
                 torch.zeros(shape[:3], dtype=torch.uint8, device=self.device).view(torch.float8_e8m0fnu)
                 for _ in range(2))
         self.length = 0
-        self._plans: dict = {}           # (Hq, n_q, tokens) -> launch plan of an 8-bit attend
+        self._prefix: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+        self._plans: dict = {}           # (Hq, n_q, tokens, prefix) -> launch plan of _attend_streams
 
     @property
     def capacity(self) -> int:
         return self.sink_size + self.ring_size
 
     def reset(self) -> None:
+        """Forget every sequence's positions (not the shared prefix)."""
         self.length = 0
+
+    def set_prefix(self, k: Optional[torch.Tensor], v: Optional[torch.Tensor]) -> None:
+        """Keys and values ``[1, H, P, D]`` in ``dtype`` (float16 or bfloat16) that every
+        query of every sequence sees in full, whatever the window, beside its own
+        positions; ``None, None`` (or ``P = 0``) removes them. Positions and ``length``
+        count the sequences' own tokens only. Contiguous, 16-byte aligned tensors are
+        kept, not copied: they must not change while the cache uses them."""
+        if k is None and v is None:
+            self._prefix = None
+            return
+        if k is None or v is None:
+            raise ValueError("the prefix needs both keys and values")
+        if self.dtype == torch.float32:
+            raise ValueError("a shared prefix takes a float16 or bfloat16 cache")
+        for name, t in (("k", k), ("v", v)):
+            if t.dim() != 4 or t.shape[:2] != (1, self.heads) or t.shape[3] != self.head_dim:
+                raise ValueError(f"prefix {name} must be [1, {self.heads}, P, {self.head_dim}], "
+                                 f"got {tuple(t.shape)}")
+            if t.dtype != self.dtype:
+                raise ValueError(f"prefix {name} must be {self.dtype}, got {t.dtype}")
+            if t.device != self.device:
+                raise ValueError(f"prefix {name} must live on {self.device}")
+        if k.shape != v.shape:
+            raise ValueError("prefix k and v must share shape")
+        self._prefix = (_aligned(k.detach()), _aligned(v.detach())) if k.shape[2] else None
 
     def _check_tokens(self, name: str, t: torch.Tensor, grouped: bool = False) -> None:
         heads_ok = t.dim() == 4 and (t.shape[1] == self.heads or
@@ -183,8 +214,8 @@ class StreamingKVCache:
     def attend(self, q: torch.Tensor, softmax_scale: Optional[float] = None,
                return_lse: bool = False):
         """Decode attention of ``q`` (``[B, Hq, n_q, D]``, the last n_q positions
-        of the cache; Hq a multiple of the cache's heads) over the visible
-        tokens: ``O`` (and the natural-log LSE ``[B, Hq, n_q]`` fp32 when
+        of the cache; Hq a multiple of the cache's heads) over the shared prefix,
+        if there is one, and the visible tokens: ``O`` (and the natural-log LSE ``[B, Hq, n_q]`` fp32 when
         ``return_lse``)."""
         self._check_tokens("q", q, grouped=True)
         n_q = int(q.shape[2])
@@ -195,8 +226,8 @@ class StreamingKVCache:
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(self.head_dim)
         q = _aligned(q)
-        if self.k_scale is not None:
-            return self._attend8(q, n_q, float(softmax_scale), return_lse)
+        if self.k_scale is not None or self._prefix is not None:
+            return self._attend_streams(q, n_q, float(softmax_scale), return_lse)
         _, _, n_tokens = rolling_stream(self.length, n_q, self.sink_size, self.window_size,
                                         self.ring_size)
         B, H, H_kv = self.batch, int(q.shape[1]), self.heads
@@ -219,31 +250,46 @@ class StreamingKVCache:
             return o
         return o, scratch[:B * H * n_q].view(B, H, n_q).clone()
 
-    def _attend8(self, q: torch.Tensor, n_q: int, softmax_scale: float, return_lse: bool):
-        """The decode over 8-bit rows."""
+    def _attend_streams(self, q: torch.Tensor, n_q: int, softmax_scale: float, return_lse: bool):
+        """The decode over 8-bit rows, or behind a shared prefix."""
         lib = _lib.load()
-        B, H, D, length = self.batch, int(q.shape[1]), self.head_dim, self.length
+        B, H, H_kv, D, length = self.batch, int(q.shape[1]), self.heads, self.head_dim, self.length
         n_tokens = min(length, self.sink_size) + max(
             0, length - max(self.sink_size, length - n_q - self.window_size + 1))
+        prefix = self._prefix
+        n_prefix = int(prefix[0].shape[2]) if prefix is not None else 0
         dtype = _DTYPE_CODE[self.dtype]
-        plan = self._plans.get((H, n_q, n_tokens))
+        key = (H, n_q, n_tokens, n_prefix)
+        plan = self._plans.get(key)
         if plan is None:
             if len(self._plans) >= 4096:     # a filling window adds one key per step
                 self._plans.clear()
-            splits = int(lib.gki_stream_splits(dtype, B, H, self.heads, n_q, D, n_tokens))
-            plan = self._plans[H, n_q, n_tokens] = (
-                splits, int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits)))
-        n_splits, ws_floats = plan
+            splits = int(lib.gki_stream_splits(dtype, B, H, H_kv, n_q, D, n_tokens))
+            shared = int(lib.gki_prefix_splits(dtype, B, H, H_kv, n_q, D, n_prefix)) if n_prefix else 0
+            plan = self._plans[key] = (
+                splits, shared, int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits + shared)))
+        n_splits, n_shared, ws_floats = plan
         o = torch.empty_like(q)
+        # the LSE rows (padded to 256 bytes), then the slices' states: one allocation
         pad = (B * H * n_q + 63) & ~63
         scratch = torch.empty(pad + ws_floats, dtype=torch.float32, device=self.device)
+        lse = scratch.data_ptr()
+        ws = lse + 4 * pad if ws_floats else 0
+        eight = self.k_scale is not None
+        k_scale, v_scale = (self.k_scale.data_ptr(), self.v_scale.data_ptr()) if eight else (0, 0)
+        place = (dtype, B, H, H_kv, n_q, D, self.sink_size, self.window_size, self.ring_size, length, softmax_scale, ws)
         with _on_device(self.device):
-            rc = lib.gki_rolling8_decode(
-                q.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(), self.k_scale.data_ptr(),
-                self.v_scale.data_ptr(), o.data_ptr(), scratch.data_ptr(), dtype, B, H, self.heads, n_q, D,
-                self.sink_size, self.window_size, self.ring_size, length, softmax_scale,
-                scratch.data_ptr() + 4 * pad if ws_floats else 0, n_splits, _current_stream(self.device))
-        _lib.check(rc, "gki_rolling8_decode")
+            stream = _current_stream(self.device)
+            if n_prefix:
+                rc = lib.gki_rolling_prefix_decode(
+                    q.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(), k_scale, v_scale,
+                    prefix[0].data_ptr(), prefix[1].data_ptr(), n_prefix, o.data_ptr(), lse, *place, n_shared,
+                    n_splits, stream)
+            else:
+                rc = lib.gki_rolling8_decode(
+                    q.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(), k_scale, v_scale,
+                    o.data_ptr(), lse, *place, n_splits, stream)
+        _lib.check(rc, "gki_rolling_prefix_decode" if n_prefix else "gki_rolling8_decode")
         if not return_lse:
             return o
         return o, scratch[:B * H * n_q].view(B, H, n_q).clone()

@@ -302,6 +302,25 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
                         int32_t window_size, int32_t ring_size, int64_t length, float softmax_scale,
                         float* workspace, int32_t n_splits, void* stream);
 
+/* Decode step behind a prefix that every sequence of the batch shares: n_prefix keys
+ * and values (prefix_k / prefix_v: [H_kv, n_prefix, head_dim] in `dtype`, fp16 or bf16)
+ * that all query rows see in full, then each sequence's own rolling cache as in
+ * gki_rolling_decode (k_scale = v_scale = NULL) or gki_rolling8_decode. The rows of all
+ * sequences run against each read of the prefix. workspace: 16-byte aligned,
+ * gki_stream_workspace_floats(B, H, n_q, head_dim, n_prefix_splits + n_splits) floats;
+ * n_prefix_splits and n_splits >= 1, for a full card from gki_prefix_splits and
+ * gki_stream_splits. */
+int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
+                      int32_t head_dim, int32_t n_prefix);
+int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_cache,
+                              const void* k_scale, const void* v_scale, const void* prefix_k,
+                              const void* prefix_v, int32_t n_prefix, void* o, float* lse,
+                              int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
+                              int32_t head_dim, int32_t sink_size, int32_t window_size,
+                              int32_t ring_size, int64_t length, float softmax_scale,
+                              float* workspace, int32_t n_prefix_splits, int32_t n_splits,
+                              void* stream);
+
 /* ---- Cross attention ----------------------------------------------------------
  * No reference counterpart. Every query row of batch entry b over its first
  * kv_len[b] keys (int32 [B] on the device; a length outside 0 .. n_kv counts as the
