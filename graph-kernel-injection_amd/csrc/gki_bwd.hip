@@ -84,7 +84,7 @@ __device__ inline KvItem kv_item(const Geom& g, const KvWork& w, int i) {
 }
 template <bool DENSE>
 __device__ inline KvItem kv_item_of(int b, int BH, const Geom& g, const KvWork& w, int& bh) {
-  const int wg = xcd_remap(b, w.n_items * BH);
+  const int wg = work_of(b, w.n_items * BH, nullptr, entries_of<DENSE>(g));
   bh = wg / w.n_items;
   return kv_item<DENSE>(g, w, wg - bh * w.n_items);
 }
@@ -93,7 +93,7 @@ __device__ inline KvItem kv_item_of(int b, int BH, const Geom& g, const KvWork& 
 // for a workgroup past the last.
 template <bool DENSE>
 __device__ inline KvItem kv_item_part_of(int b, int BH, int parts, const Geom& g, const KvWork& w, int& bh, int& part) {
-  const int wg = work_part_of(b, w.n_items * BH, parts, nullptr, part);
+  const int wg = work_part_of(b, w.n_items * BH, parts, nullptr, part, entries_of<DENSE>(g));
   bh = wg < 0 ? -1 : wg / w.n_items;
   if (wg < 0) return {0, 0, 0, -1};
   return kv_item<DENSE>(g, w, wg - bh * w.n_items);
@@ -898,7 +898,7 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
   __shared__ __align__(16) uint16_t stile[LDS16];      // K, K, V, V; the waves' sums at the end
 
   const int n_wg = n_qt * g.B * g.H;
-  const int wg = work_of(blockIdx.x, n_wg, dq_order);
+  const int wg = work_of(blockIdx.x, n_wg, dq_order, entries_of<DENSE>(g));
   if (wg < 0) return;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
@@ -1067,7 +1067,7 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
   __shared__ __align__(16) uint16_t sv[2][64 * D];
 
   const int n_wg = n_qt * g.B * g.H;
-  const int wg = work_of(blockIdx.x, n_wg, dq_order);
+  const int wg = work_of(blockIdx.x, n_wg, dq_order, entries_of<DENSE>(g));
   if (wg < 0) return;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
@@ -1256,7 +1256,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
   __shared__ __align__(16) float sv[2][TR * D];
 
   int part;
-  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, KB, dq_order, part);
+  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, KB, dq_order, part, entries_of<DENSE>(g));
   if (wg < 0) return;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;

@@ -634,8 +634,9 @@ int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t
                       int32_t n_prefix) {
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_prefix <= 0) return 1;
   const int64_t rows = (int64_t)B * (H / H_kv) * n_q;
-  const int64_t tile = prefix_as_streams(rows) ? stream_rows_tile(false, (int)rows) : kTileMF;
-  return stream_splits(head_dim, H_kv * ((rows + tile - 1) / tile), n_prefix);
+  const bool streams = prefix_as_streams(rows);
+  const int64_t tile = streams ? stream_rows_tile(false, (int)rows) : kTileMF;
+  return prefix_splits(streams, H_kv * ((rows + tile - 1) / tile), n_prefix);
 }
 
 int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,

@@ -623,6 +623,11 @@ __device__ inline int walk_entry(const int32_t* list, int e) {
   return DENSE ? e : list[e];
 }
 __host__ __device__ inline int kv_tiles_of(const Geom& g) { return (g.n_kv + kTileN - 1) / kTileN; }
+// Entries of different lengths share the card evenly where every XCD has a range of
+// each: one range of all units, as the listed walks have it, gives the XCDs of the
+// longest entry the most work (@@).
+template <bool DENSE>
+__device__ inline int entries_of(const Geom& g) { return DENSE && g.kv_len != nullptr ? g.B : 1; }
 // Valid keys of batch entry b (a length outside 0 .. n_kv counts as the nearest of them).
 __device__ inline int own_keys(const Geom& g, int b) {
   if (g.kv_len == nullptr) return g.n_kv;
@@ -871,13 +876,28 @@ inline int stream_rows_tile(bool f32, int n_rows) { return f32 || n_rows <= 16 ?
 // Does a shared prefix run its rows as streams (blocks of 16, few rows) or as 128-row tiles?
 inline bool prefix_as_streams(int64_t n_rows) { return n_rows <= 64; }
 
-// Slices of each stream: enough workgroups for two rounds of what the card holds at
-// once (two per CU at head_dim 128, four at 64, by their 64 KB and 32 KB of LDS), of
-// at least 128 tokens each.
+// Slices of each stream: about a workgroup per CU at head_dim 128, two at 64, of at
+// least 128 tokens each (a step of 64 takes about 0.5 us of latency, and a slice more
+// to join 0.05); a short stream stays whole, as joining two slices costs a launch.
+// us with 1 / 2 / 4 / 8 / 16 slices:
+//   8-bit   64 streams of 2052 tokens, D128    30.4 / 21.1 / 14.8 / 14.9 / 21.0
+//           16 of 8192 (16-bit), D128          82.2 / 46.0 / 26.5 / 17.6 / 16.6
+//           512 of 8196, D128                  168 / 170 / 176 / 188 / 226
+//           256 of 2000 (16-bit), D64          18.6 / 18.0 / 19.5 / 19.8 / 24.8
+//           256 of 600, D64                    10.4 / 12.8 / 13.0 / 15.7
 inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
-  const int64_t target = head_dim >= 128 ? 512 : 1024;
-  const int64_t want = (target + n_workgroups - 1) / n_workgroups;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, n_tokens / 128));
+  if (n_tokens < 768) return 1;
+  const int64_t target = head_dim >= 128 ? 256 : 512;
+  return (int)std::max<int64_t>(1, std::min((target + n_workgroups - 1) / n_workgroups, n_tokens / 128));
+}
+
+// Slices of a shared prefix (their states are joined with the sequences' own in any
+// case): a workgroup per CU; 128-row tiles of at least 256 keys. us with 4 / 8 / 16 / 32 /
+// 64 slices: 8 row tiles over 8192 keys 29.3 at 16, 29.4 at 32, 38.8 at 64; 16 over 32768
+// (8-bit sequences of 2052) 95.0 at 16, 98.1 at 32; 8 streams of 20000 keys 82.8 / 50.6 /
+// 34.6 / 30.8 / 35.8.
+inline int prefix_splits(bool streams, int64_t n_workgroups, int64_t n_keys) {
+  return (int)std::max<int64_t>(1, std::min((256 + n_workgroups - 1) / n_workgroups, n_keys / (streams ? 128 : 256)));
 }
 
 // Does a cross attention run its query rows as streams (a whole group's rows against
@@ -887,24 +907,18 @@ inline bool cross_as_streams(int dtype, int head_dim, int group, int n_q) {
 }
 
 // Parts that a dense walk of dK/dV is cut into: each of `columns` kv tiles (over all
-// (b, kv head)) is walked by `walk` = q tiles * group iterations. A column is one
-// item where the columns fill the card, else pieces of about a 512th of the work, of 8
-// iterations or more (2 for fp32); never more than about 8192 items in all.
+// (b, kv head)) is walked by `walk` = q tiles * group iterations, all alike. 512 columns
+// fill the card whole, as do 128 (192 below head_dim 64) short ones (16-bit); fewer are
+// cut into about 512 items of 8 iterations or more (2 for fp32). Never more than about
+// 8192 items in all. Backward us with 1 / 2 / 4 / 8 / 16 parts:
+//   1024 columns of 128, D128     828 / 850 / 859 / 951 / 1136
+//   3072 columns of 7, D64        109 / 144 / 201
+//   64 columns of 256, D64        232 / 139 / 93 / 82 / 87
+//   128 columns of 64, D128 fp32  662 / 622 / 625 / 637 / 608
 inline int cross_kv_parts(int dtype, int head_dim, int64_t walk, int64_t columns) {
-  const int64_t total = walk * columns;
-  int64_t chunk;
-  if (dtype == kF32) {
-    chunk = columns >= 512 ? walk : std::max<int64_t>(2, (total + 511) / 512);
-  } else {
-    int64_t spread = std::max<int64_t>(8, (total + 511) / 512);
-    const int64_t few = head_dim >= 64 ? 128 : 192, brief = head_dim >= 64 ? 32 : 16;
-    if (columns >= 512) spread = std::max(spread, walk);
-    else if (columns >= few && walk <= brief) spread = std::max<int64_t>(std::max<int64_t>(spread, 16), walk);
-    const bool middling = head_dim < 128 && columns >= 512 && columns < 1024;
-    const int64_t whole = middling ? 48 : 80, piece = middling ? 32 : 80;
-    chunk = std::min(walk <= whole ? std::max<int64_t>(32, walk) : piece, spread);
-  }
-  chunk = std::max<int64_t>(std::max<int64_t>(chunk, 1), (total + 8191) / 8192);
+  const int64_t total = walk * columns, few = head_dim >= 64 ? 128 : 192, brief = head_dim >= 64 ? 32 : 16;
+  if (columns >= 512 || (dtype != kF32 && columns >= few && walk <= brief)) return 1;
+  const int64_t chunk = std::max({(int64_t)(dtype == kF32 ? 2 : 8), (total + 511) / 512, (total + 8191) / 8192});
   return (int)((walk + chunk - 1) / chunk);
 }
 
@@ -939,8 +953,13 @@ __device__ inline void mfma_priority_lo() {
 // id, or, with an order table (gki_fwd_order), the unit that table lists at
 // that id (each XCD's range sorted heaviest first, so the units dispatched last
 // are the short ones and the launch ends with less idle tail). -1 (the
-// workgroup exits) for a table entry outside 0 .. n-1.
-__device__ inline int work_of(int b, int n, const int32_t* order) {
+// workgroup exits) for a table entry outside 0 .. n-1. `entries` > 1: an XCD has its
+// range of each of that many equal runs of units, not of all of them.
+__device__ inline int work_of(int b, int n, const int32_t* order, int entries = 1) {
+  if (entries > 1) {
+    const int per = n / entries, e = b / per;
+    return e * per + xcd_remap(b - e * per, per);
+  }
   const int l = xcd_remap(b, n);
   if (order == nullptr) return l;
   const int w = __builtin_amdgcn_readfirstlane(order[l]);
@@ -950,10 +969,10 @@ __device__ inline int work_of(int b, int n, const int32_t* order) {
 // The same for units cut into `parts` workgroups each (grid work_parts_grid):
 // the parts of a unit run on one XCD, one after the other.
 inline int work_parts_grid(int n, int parts) { return parts == 1 ? n : kXcd * parts * ((n + kXcd - 1) / kXcd); }
-__device__ inline int work_part_of(int b, int n, int parts, const int32_t* order, int& part) {
+__device__ inline int work_part_of(int b, int n, int parts, const int32_t* order, int& part, int entries = 1) {
   const int x = b % kXcd, k = b / kXcd, slot = x + kXcd * (k / parts);
   part = k % parts;
-  return slot < n ? work_of(slot, n, order) : -1;
+  return slot < n ? work_of(slot, n, order, entries) : -1;
 }
 
 // Reductions across the 4 lane groups (lanes l, l^16, l^32, l^48) with the

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kFwdThreads, D <= 64 ? 4 : 2) void fwd_kernel_16(
   __shared__ __align__(16) uint16_t sv[2][kTileN * D];
 
   const int n_wg = SHARED ? gridDim.x : n_qt * g.B * g.H;
-  const int wg = work_of(blockIdx.x, n_wg, wg_order);
+  const int wg = work_of(blockIdx.x, n_wg, wg_order, entries_of<WALK == kDense>(g));
   if (wg < 0) return;
   // SHARED: the row tiles of a slice are neighbours, its head is bh / n_splits
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(512, 2) void fwd_split_16(
   __shared__ float sm[NW][32], sl[NW][32];
 
   int part;
-  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, 4 / QB, wg_order, part);
+  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, 4 / QB, wg_order, part, entries_of<DENSE>(g));
   if (wg < 0) return;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
   __shared__ __align__(16) float sv[2][TR * D];
 
   int part;
-  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, KB, wg_order, part);
+  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, KB, wg_order, part, entries_of<DENSE>(g));
   if (wg < 0) return;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
