@@ -56,8 +56,8 @@ int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const
                   void* ko, void* vo, int64_t* positions, int BH, int length, int sink, int ring,
                   hipStream_t stream);
 int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
-                     const uint8_t* ks, const uint8_t* vs, void* o, float* lse, int ring, float* ws, int n_splits,
-                     hipStream_t stream);
+                     const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new, void* o, float* lse,
+                     int ring, float* ws, int n_splits, hipStream_t stream);
 int cross_fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
                        float* lse, hipStream_t stream);
 int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
@@ -66,9 +66,9 @@ int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, co
                        const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                        int parts, float* partials, hipStream_t stream);
 int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
-                           const uint8_t* ks, const uint8_t* vs, const void* prefix_k, const void* prefix_v, int n_prefix,
-                           void* o, float* lse, int ring, float* ws, int n_prefix_splits, int n_splits,
-                           hipStream_t stream);
+                           const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new,
+                           const void* prefix_k, const void* prefix_v, int n_prefix, void* o, float* lse, int ring,
+                           float* ws, int n_prefix_splits, int n_splits, hipStream_t stream);
 int64_t read_probe_words(int BH);
 int read_probe_dispatch(const void* k, const void* v, int BH, int64_t n_kv, int row_bytes, int n_sink,
                         int64_t w_lo, uint32_t* out, hipStream_t stream);
@@ -280,6 +280,37 @@ int cross_geom(Geom& g, int dtype, int B, int H, int H_kv, int n_q, int n_kv, in
   g.n_qb = g.n_kb = g.bm = g.bn = 1;
   g.kv_len = kv_len;
   return 0;
+}
+
+// A decode over an 8-bit cache (k_scale), behind a shared prefix (n_prefix > 0) or both;
+// with k_new the n_q tokens are written too.
+int rolling_wide(const void* q, const void* k_new, const void* v_new, const void* k_cache, const void* v_cache,
+                 const void* k_scale, const void* v_scale, const void* prefix_k, const void* prefix_v, int n_prefix,
+                 void* o, float* lse, int dtype, int B, int H, int H_kv, int n_q, int head_dim, int sink_size,
+                 int window_size, int ring_size, int64_t length, float softmax_scale, float* workspace,
+                 int n_prefix_splits, int n_splits, void* stream) {
+  if (int rc = rolling_decode_args(dtype, B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, length,
+                                   softmax_scale, q, k_cache, v_cache, o, lse, n_splits))
+    return rc;
+  GKI_REQUIRE(!k_scale == !v_scale, 1, "rolling cache: one scale without the other");
+  GKI_REQUIRE(all_aligned16(o, workspace), 1, "rolling cache: o and the workspace must be 16-byte aligned");
+  const int64_t rows = (int64_t)(H / H_kv) * n_q;
+  GKI_REQUIRE((rows + 15) / 16 * n_splits * B * H_kv < (1ll << 23), 1, "rolling cache: the grid must fit");
+  const Geom g = rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale);
+  if (n_prefix == 0) {
+    GKI_REQUIRE(n_splits == 1 || workspace, 1, "rolling cache: null workspace");
+    return attend8_dispatch(dtype, head_dim, g, q, k_cache, v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
+                            k_new, v_new, o, lse, ring_size, workspace, n_splits, (hipStream_t)stream);
+  }
+  GKI_REQUIRE(dtype != kF32, 2, "shared prefix: fp16 or bf16");
+  GKI_REQUIRE(prefix_k && prefix_v && workspace, 1, "shared prefix: null pointer");
+  GKI_REQUIRE(all_aligned16(prefix_k, prefix_v), 1, "shared prefix: keys and values must be 16-byte aligned");
+  GKI_REQUIRE(n_prefix > 0 && n_prefix < (1 << kPartialBit), 1, "shared prefix: n_prefix must be in [1, 2^30)");
+  GKI_REQUIRE(n_prefix_splits >= 1 && (rows * B + 15) / 16 * H_kv * n_prefix_splits < (1ll << 22), 1,
+              "shared prefix: n_prefix_splits must be >= 1 and the grid must fit");
+  return prefix_decode_dispatch(dtype, head_dim, g, q, k_cache, v_cache, (const uint8_t*)k_scale,
+                                (const uint8_t*)v_scale, k_new, v_new, prefix_k, prefix_v, n_prefix, o, lse, ring_size,
+                                workspace, n_prefix_splits, n_splits, (hipStream_t)stream);
 }
 
 }  // namespace
@@ -574,7 +605,7 @@ int gki_rolling_decode_noalloc(const void* q, const void* k_cache, const void* v
 int gki_stream_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
                           int64_t n_tokens) {
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_tokens < 0) return 1;
-  const int rows = H / H_kv * n_q, tile = stream_rows_tile(dtype == kF32, rows);
+  const int rows = H / H_kv * n_q, tile = stream_rows_tile(dtype != kBF16, rows);
   return stream_splits(head_dim, (int64_t)B * H_kv * ((rows + tile - 1) / tile), n_tokens);
 }
 
@@ -617,26 +648,18 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
                         const void* v_scale, void* o, float* lse, int32_t dtype, int32_t B, int32_t H, int32_t H_kv,
                         int32_t n_q, int32_t head_dim, int32_t sink_size, int32_t window_size, int32_t ring_size,
                         int64_t length, float softmax_scale, float* workspace, int32_t n_splits, void* stream) {
-  if (int rc = rolling_decode_args(dtype, B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, length,
-                                   softmax_scale, q, k_codes, v_codes, o, lse, n_splits))
-    return rc;
   GKI_REQUIRE(k_scale && v_scale, 1, "gki_rolling8_decode: null scale");
-  GKI_REQUIRE((((uintptr_t)o | (uintptr_t)workspace) & 15) == 0, 1,
-              "gki_rolling8_decode: o and the workspace must be 16-byte aligned");
-  GKI_REQUIRE(n_splits == 1 || workspace, 1, "gki_rolling8_decode: null workspace");
-  return attend8_dispatch(dtype, head_dim,
-                          rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale), q, k_codes,
-                          v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, o, lse, ring_size, workspace,
-                          n_splits, (hipStream_t)stream);
+  return rolling_wide(q, nullptr, nullptr, k_codes, v_codes, k_scale, v_scale, nullptr, nullptr, 0, o, lse, dtype, B, H,
+                      H_kv, n_q, head_dim, sink_size, window_size, ring_size, length, softmax_scale, workspace, 0,
+                      n_splits, stream);
 }
 
 int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
                       int32_t n_prefix) {
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_prefix <= 0) return 1;
   const int64_t rows = (int64_t)B * (H / H_kv) * n_q;
-  const bool streams = prefix_as_streams(rows);
-  const int64_t tile = streams ? stream_rows_tile(false, (int)rows) : kTileMF;
-  return prefix_splits(streams, H_kv * ((rows + tile - 1) / tile), n_prefix);
+  const int64_t tile = prefix_as_streams(rows) ? 32 : kTileMF;
+  return prefix_splits(H_kv * ((rows + tile - 1) / tile), n_prefix);
 }
 
 int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
@@ -645,21 +668,24 @@ int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_
                               int32_t head_dim, int32_t sink_size, int32_t window_size, int32_t ring_size,
                               int64_t length, float softmax_scale, float* workspace, int32_t n_prefix_splits,
                               int32_t n_splits, void* stream) {
-  if (int rc = rolling_decode_args(dtype, B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, length,
-                                   softmax_scale, q, k_cache, v_cache, o, lse, n_splits))
-    return rc;
-  GKI_REQUIRE(dtype != kF32, 2, "gki_rolling_prefix_decode: fp16 or bf16");
-  GKI_REQUIRE(prefix_k && prefix_v && workspace && !k_scale == !v_scale, 1, "gki_rolling_prefix_decode: null pointer");
-  GKI_REQUIRE(all_aligned16(prefix_k, prefix_v, o, workspace), 1,
-              "gki_rolling_prefix_decode: the prefix, o and the workspace must be 16-byte aligned");
-  GKI_REQUIRE(n_prefix >= 1 && n_prefix < (1 << kPartialBit), 1, "gki_rolling_prefix_decode: n_prefix must be in [1, 2^30)");
-  const int64_t tiles = ((int64_t)B * (H / H_kv) * n_q + 15) / 16 * H_kv;
-  GKI_REQUIRE(n_prefix_splits >= 1 && tiles * n_prefix_splits < (1ll << 23), 1,
-              "gki_rolling_prefix_decode: n_prefix_splits must be >= 1 and the grid must fit");
-  return prefix_decode_dispatch(dtype, head_dim,
-                                rolling_geom(B, H, H_kv, n_q, sink_size, window_size, length, softmax_scale), q, k_cache,
-                                v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale, prefix_k, prefix_v, n_prefix,
-                                o, lse, ring_size, workspace, n_prefix_splits, n_splits, (hipStream_t)stream);
+  GKI_REQUIRE(n_prefix >= 1, 1, "gki_rolling_prefix_decode: n_prefix must be positive");
+  return rolling_wide(q, nullptr, nullptr, k_cache, v_cache, k_scale, v_scale, prefix_k, prefix_v, n_prefix, o, lse,
+                      dtype, B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, length, softmax_scale,
+                      workspace, n_prefix_splits, n_splits, stream);
+}
+
+int gki_rolling_step(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, void* k_scale,
+                     void* v_scale, const void* prefix_k, const void* prefix_v, int32_t n_prefix, void* o, float* lse,
+                     int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
+                     int32_t sink_size, int32_t window_size, int32_t ring_size, int64_t start_pos, float softmax_scale,
+                     float* workspace, int32_t n_prefix_splits, int32_t n_splits, void* stream) {
+  GKI_REQUIRE(start_pos >= 0 && start_pos < (1ll << kPartialBit), 1, "gki_rolling_step: start_pos must be in [0, 2^30)");
+  GKI_REQUIRE(k_new && v_new && all_aligned16(k_new, v_new), 1,
+              "gki_rolling_step: k_new and v_new must not be null and 16-byte aligned");
+  GKI_REQUIRE(k_scale || n_prefix > 0, 2, "gki_rolling_step: an 8-bit cache or a prefix");
+  return rolling_wide(q, k_new, v_new, k_cache, v_cache, k_scale, v_scale, prefix_k, prefix_v, n_prefix, o, lse, dtype,
+                      B, H, H_kv, n_q, head_dim, sink_size, window_size, ring_size, start_pos + n_q, softmax_scale,
+                      workspace, n_prefix_splits, n_splits, stream);
 }
 
 int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,

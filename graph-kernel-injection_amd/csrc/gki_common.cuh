@@ -625,7 +625,8 @@ __device__ inline int walk_entry(const int32_t* list, int e) {
 __host__ __device__ inline int kv_tiles_of(const Geom& g) { return (g.n_kv + kTileN - 1) / kTileN; }
 // Entries of different lengths share the card evenly where every XCD has a range of
 // each: one range of all units, as the listed walks have it, gives the XCDs of the
-// longest entry the most work (@@).
+// longest entry the most work (B4 H16/4 2048 x 4096
+// D128, 72% of the keys valid: forward 261 -> 189 us, dQ 414 -> 298).
 template <bool DENSE>
 __device__ inline int entries_of(const Geom& g) { return DENSE && g.kv_len != nullptr ? g.B : 1; }
 // Valid keys of batch entry b (a length outside 0 .. n_kv counts as the nearest of them).
@@ -870,11 +871,14 @@ inline void surviving_rows(int start, int n_new, int sink, int ring, int* n_a, i
 }
 
 // Query rows per workgroup of the stream kernels: one block of 16, or two where a
-// stream has more (fp32: its three pieces of each operand leave registers for one).
-inline int stream_rows_tile(bool f32, int n_rows) { return f32 || n_rows <= 16 ? 16 : 32; }
+// stream has more (not for 8-bit rows under fp16 or fp32 queries: their two or three
+// pieces of each operand leave registers for one).
+inline int stream_rows_tile(bool pieces, int n_rows) { return pieces || n_rows <= 16 ? 16 : 32; }
 
-// Does a shared prefix run its rows as streams (blocks of 16, few rows) or as 128-row tiles?
-inline bool prefix_as_streams(int64_t n_rows) { return n_rows <= 64; }
+// Does a shared prefix run its rows as streams (32 of them) or as 128-row tiles? 8 heads
+// over 4000 keys, D128, us: 24 / 32 / 48 / 64 rows as streams 16.0 / 16.8 / 19.0 / 19.7, 65 as
+// tiles 17.2.
+inline bool prefix_as_streams(int64_t n_rows) { return n_rows <= 32; }
 
 // Slices of each stream: about a workgroup per CU at head_dim 128, two at 64, of at
 // least 128 tokens each (a step of 64 takes about 0.5 us of latency, and a slice more
@@ -892,12 +896,12 @@ inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
 }
 
 // Slices of a shared prefix (their states are joined with the sequences' own in any
-// case): a workgroup per CU; 128-row tiles of at least 256 keys. us with 4 / 8 / 16 / 32 /
-// 64 slices: 8 row tiles over 8192 keys 29.3 at 16, 29.4 at 32, 38.8 at 64; 16 over 32768
-// (8-bit sequences of 2052) 95.0 at 16, 98.1 at 32; 8 streams of 20000 keys 82.8 / 50.6 /
-// 34.6 / 30.8 / 35.8.
-inline int prefix_splits(bool streams, int64_t n_workgroups, int64_t n_keys) {
-  return (int)std::max<int64_t>(1, std::min((256 + n_workgroups - 1) / n_workgroups, n_keys / (streams ? 128 : 256)));
+// case): a workgroup for every other CU, beside the sequences' own, of at least 256 keys.
+// us with 4 / 8 / 16 / 32 slices: 8 row tiles over 8192 keys (sequences of 304)
+// - / 27.8 / 22.7 / 24.8, over 2000 16.6 / 14.7 / 16.8; 16 over 32768 (8-bit sequences of
+// 2052) - / 89.3 / 92.9 / 96; 8 streams of 20000 keys 64.8 / 39.1 / 26.7 / 26.1.
+inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
+  return (int)std::max<int64_t>(1, std::min((128 + n_workgroups - 1) / n_workgroups, n_keys / 256));
 }
 
 // Does a cross attention run its query rows as streams (a whole group's rows against

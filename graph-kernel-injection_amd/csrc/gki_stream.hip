@@ -23,12 +23,9 @@
 #include <algorithm>
 #include <string>
 
-#include "gki_common.cuh"
+#include "gki_rows16.cuh"
 
 namespace gki {
-int prefix_tiles_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
-                          const SharedRows& sh, hipStream_t stream);
-
 namespace {
 
 constexpr int kMinExponent = -117;           // 2^-9 (the smallest code) * 2^-117 is a normal float
@@ -51,7 +48,8 @@ __device__ inline void load8(const typename T::storage* p, float (&f)[8]) {
   }
 }
 
-// Slot of new row r of the launch (rows_of_append): its source row and cache slot.
+// Rows that a launch writes into a rolling cache: of n_new from position start on, the
+// first n_a and n_b from the i_b-th on (surviving_rows).
 struct AppendRows {
   int n_new, n_a, i_b, n_b, start, sink, ring;
   __device__ inline int source(int r) const { return r < n_a ? r : i_b + (r - n_a); }
@@ -60,51 +58,78 @@ struct AppendRows {
     return p < sink ? p : sink + (p - sink) % ring;
   }
 };
+struct AppendArgs {
+  void *kc, *vc;
+  uint8_t *ks, *vs;            // exponents of the 8-bit rows
+  const void *kn, *vn;
+  int BH;
+  AppendRows rows;
+  int n_blocks;                // workgroups that write (0: none)
+};
 
-// One row of K or V per D / 8 lanes (16 or 8): the largest finite magnitude across
-// them, the exponent from its bits, eight codes per lane. Bound by HBM: reads the
-// rows once, writes D + 1 bytes each.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void append8_kernel(
-    uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, uint8_t* __restrict__ ks, uint8_t* __restrict__ vs,
-    const typename T::storage* __restrict__ kn, const typename T::storage* __restrict__ vn, int BH,
-    AppendRows a) {
+// Eight elements of a row, and the largest finite magnitude among them.
+template <typename T>
+__device__ inline float load8_top(const typename T::storage* p, float (&f)[8]) {
+  load8<T>(p, f);
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = fabsf(f[j]);
+    top = fmaxf(top, x < __builtin_huge_valf() ? x : 0.f);     // false for NaN too
+  }
+  return top;
+}
+// The exponent of a row: top = (1 + m / 2^23) 2^k <= 448 * 2^e = 1.75 * 2^(8 + e).
+__device__ inline int exponent_of(float top) {
+  const uint32_t bits = __float_as_uint(top);
+  return max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0), kMinExponent);
+}
+// The codes of eight elements of a row of exponent e.
+__device__ inline uint2 codes8(const float (&f)[8], int e) {
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = fabsf(f[j]) < __builtin_huge_valf() ? f[j] * inv : __builtin_nanf("");
+  int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w0, true);
+  int w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+  w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w1, true);
+  return make_uint2((uint32_t)w0, (uint32_t)w1);
+}
+
+// D / 8 lanes per row of K or V, eight elements each; in 8 bits the largest magnitude
+// goes round among them. Bound by HBM: reads the rows once, writes them once.
+template <typename T, int D, bool EIGHT>
+__device__ inline void append_rows(const AppendArgs& a, int block) {
+  using S = typename T::storage;
   constexpr int LPR = D / 8;                   // lanes per row
-  const int rows = a.n_a + a.n_b;
+  const int rows = a.rows.n_a + a.rows.n_b;
   const int ch = threadIdx.x % LPR;
-  const int64_t n = (int64_t)BH * rows;
+  const int64_t n = (int64_t)a.BH * rows;
   // whole rows: the lanes of a row leave together
-  for (int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR; row < 2 * n;
-       row += (int64_t)gridDim.x * (256 / LPR)) {
+  for (int64_t row = ((int64_t)block * 256 + threadIdx.x) / LPR; row < 2 * n; row += (int64_t)a.n_blocks * (256 / LPR)) {
     const bool is_v = row >= n;
     const int64_t rr = is_v ? row - n : row;
-    const int bh = (int)(rr / rows), i = a.source((int)(rr % rows));
-    float f[8];
-    load8<T>((is_v ? vn : kn) + ((size_t)bh * a.n_new + i) * D + 8 * ch, f);
-    float top = 0.f;
+    const int bh = (int)(rr / rows), i = a.rows.source((int)(rr % rows));
+    const S* src = (const S*)(is_v ? a.vn : a.kn) + ((size_t)bh * a.rows.n_new + i) * D + 8 * ch;
+    const size_t dst = (size_t)bh * (a.rows.sink + a.rows.ring) + a.rows.slot(i);
+    if constexpr (EIGHT) {
+      float f[8];
+      float top = load8_top<T>(src, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = fabsf(f[j]);
-      top = fmaxf(top, x < __builtin_huge_valf() ? x : 0.f);     // false for NaN too
+      for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+      const int e = exponent_of(top);
+      *(uint2*)((uint8_t*)(is_v ? a.vc : a.kc) + dst * D + 8 * ch) = codes8(f, e);
+      if (ch == 0) (is_v ? a.vs : a.ks)[dst] = (uint8_t)(e + 127);
+    } else {
+      static_assert(!T::is_f32 || EIGHT, "16-bit rows");
+      *(uint4*)((S*)(is_v ? a.vc : a.kc) + dst * D + 8 * ch) = *(const uint4*)src;
     }
-#pragma unroll
-    for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-    // top = (1 + m / 2^23) 2^k <= 448 * 2^e = 1.75 * 2^(8 + e)
-    const uint32_t bits = __float_as_uint(top);
-    const int e = max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0), kMinExponent);
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      y[j] = fabsf(f[j]) < __builtin_huge_valf() ? f[j] * inv : __builtin_nanf("");
-    int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w0, true);
-    int w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
-    w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w1, true);
-    const size_t dst = (size_t)bh * (a.sink + a.ring) + a.slot(i);
-    *(uint2*)((is_v ? vc : kc) + dst * D + 8 * ch) = make_uint2((uint32_t)w0, (uint32_t)w1);
-    if (ch == 0) (is_v ? vs : ks)[dst] = (uint8_t)(e + 127);
   }
+}
+template <typename T, int D>
+__global__ __launch_bounds__(256) void append8_kernel(AppendArgs a) {
+  append_rows<T, D, true>(a, blockIdx.x);
 }
 
 // Two e4m3 codes of a word (its low or high half) times 2^e: exact in fp32.
@@ -167,6 +192,7 @@ __global__ __launch_bounds__(256) void held_rows_kernel(
 // The tokens of a rolling cache that some of its n_q last positions see: sinks
 // 0 .. n_sink - 1, then positions w_lo .. length - 1.
 struct RingStream {
+  static constexpr bool kSteps = true;         // a step's own tokens may be among them
   int n_tokens, n_sink, w_lo, sink, ring, base, q_off, window;   // base: (w_lo - sink) mod ring
   __device__ inline int count(int) const { return n_tokens; }
   __device__ inline int row(int t) const {
@@ -174,9 +200,21 @@ struct RingStream {
     const int j = base + (t - n_sink);
     return sink + (j >= ring ? j - ring : j);
   }
+  __device__ inline int position(int t) const { return t < n_sink ? t : w_lo + (t - n_sink); }
+  // Do tokens t .. t + n - 1 lie in consecutive rows (all sinks, or window tokens that
+  // the ring does not turn between)?
+  __device__ inline bool consecutive(int t, int n) const {
+    return t + n <= n_sink || (t >= n_sink && (base + (t - n_sink) >= ring || base + (t - n_sink) + n <= ring));
+  }
+  // Does some row not see some of them?
+  __device__ inline bool partly_hidden(int t, int n) const {
+    const int p0 = position(t), p1 = position(t + n - 1);
+    return p1 > q_off || (p1 >= sink && max(p0, sink) <= n_tok_last() - window);
+  }
+  __device__ inline int n_tok_last() const { return w_lo + (n_tokens - n_sink) - 1; }   // the last query's position
   // token rule of query position i
   __device__ inline bool visible(int i, int t) const {
-    const int p = t < n_sink ? t : w_lo + (t - n_sink), qa = q_off + i;
+    const int p = position(t), qa = q_off + i;
     return (p <= qa) & ((p < sink) | (p > qa - window));
   }
 };
@@ -184,12 +222,16 @@ struct RingStream {
 // A contiguous stream per (b, kv head): all its rows, or the first len[b] of them (a
 // length outside 0 .. n counts as the nearest).
 struct DenseStream {
+  static constexpr bool kSteps = false;
   const int32_t* len;
   int n, H_kv;
   __device__ inline int count(int s) const {
     return len == nullptr ? n : max(0, min(__builtin_amdgcn_readfirstlane(len[s / H_kv]), n));
   }
   __device__ inline int row(int t) const { return t; }
+  __device__ inline int position(int t) const { return t; }
+  __device__ inline bool consecutive(int, int) const { return true; }
+  __device__ inline bool partly_hidden(int, int) const { return false; }
   __device__ inline bool visible(int, int) const { return true; }
 };
 
@@ -203,10 +245,16 @@ struct StreamArgs {
   int n_q, q_stride;           // q_stride = H * n_q rows of Q between batch entries
   int kv_rows;                 // rows that K and V hold per stream
   int n_rows, row_tiles;       // query rows of a stream, and tiles of them
+  int n_blocks;                // workgroups: streams * n_splits * row_tiles
   int n_splits;                // slices here: parts part0 .. of the n_parts states that a row has in the
   int part0, n_parts;          // workspace (n_parts 1: O and LSE are written here)
   float scale_log2;            // |scale| log2 e (log2 e for scale 0), the sign in q_sign
   float q_sign;                // 1, -1, or 0: the scores are those of q_sign * q
+  // A step's own tokens, positions start .. of which each stream has n_new rows here, are
+  // taken from these rows: the cache's are being written by the same launch. (Their
+  // slots held positions at least `ring` older, which no row of the step sees.)
+  const void *k_new, *v_new;
+  int n_new, start;            // no such tokens: start past every position
 };
 
 // Queries as 1, 2 or 3 bfloat16 pieces whose sum they are (8, 11 and 24 significant
@@ -232,8 +280,8 @@ struct StreamPlace {
   int s, row0, split, g0, g1;
   size_t q_row0, kb;           // the stream's first row of Q, of K and V
   template <class Src>
-  __device__ inline StreamPlace(const StreamArgs& a, const Src& src, int rows_tile) {
-    int lb = xcd_remap(blockIdx.x, gridDim.x);
+  __device__ inline StreamPlace(const StreamArgs& a, const Src& src, int rows_tile, int block) {
+    int lb = xcd_remap(block, a.n_blocks);
     row0 = lb % a.row_tiles * rows_tile;
     lb /= a.row_tiles;
     split = lb % a.n_splits;
@@ -303,17 +351,21 @@ struct StreamWave {
 #pragma unroll
         for (int n = 0; n < NPC; ++n) s[h] = C::mfma(x, qf[h][ks][n], s[h]);
     }
-    // lane (grp, col): s[h][i] = score of token t0 + i for row row0 + 16 h + col
-    const int t0 = t + 16 * wave + 4 * grp;
+    // lane (grp, col): s[h][i] = score of token t + 16 wave + 4 grp + i for row row0 + 16 h + col
+    if (t + kTileN > g1 || (RULE && src.partly_hidden(t, kTileN))) {
+      const int t0 = t + 16 * wave + 4 * grp;
+#pragma unroll
+      for (int h = 0; h < NB; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bool ok = t0 + i < g1;
+          if constexpr (RULE) ok = ok && src.visible(my_q[h], t0 + i);
+          s[h][i] = ok ? s[h][i] : kNegInf;
+        }
+    }
     uint2 pb[NB][NPC];
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bool ok = t0 + i < g1;
-        if constexpr (RULE) ok = ok && src.visible(my_q[h], t0 + i);
-        s[h][i] = ok ? s[h][i] : kNegInf;
-      }
       float mx = fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3]));
       if (__any(mx * a.scale_log2 > m[h] + kStreamSlack)) {
         mx = wave_max16x4(mx) * a.scale_log2;
@@ -402,30 +454,63 @@ struct StreamWave {
 // bf16: P is rounded to bfloat16 for P V, as in the 16-bit decode (half a unit of
 // 2^-8 of each weight, averaged over the keys); the row sums add the fp32 P.
 template <typename T, int D, int NB, bool RULE, class Src>
-__global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
+__device__ inline void stream8_rows(const StreamArgs& a, const Src& src, int block, uint16_t* sk, uint16_t* sv) {
+  using S = typename T::storage;
   constexpr int UPR = D / 16;                  // 16-byte units per row
   constexpr int NU = kTileN * UPR / 256;       // units per thread and tile
-  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
-  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  constexpr int TILE = kTileN * D;
   const int tid = threadIdx.x;
-  const StreamPlace at(a, src, 16 * NB);
+  const StreamPlace at(a, src, 16 * NB, block);
   const int n_chunks = at.chunks();
-  const uint8_t *K = (const uint8_t*)a.k, *V = (const uint8_t*)a.v;
+  const uint8_t *K = (const uint8_t*)a.k + at.kb * D, *V = (const uint8_t*)a.v + at.kb * D;
+  const uint8_t *Ks = a.ks + at.kb, *Vs = a.vs + at.kb;
 
   struct Raw {
     uint4 k[NU], v[NU];
     uint8_t ks[NU], vs[NU];
   };
-  // tokens past the slice repeat its last one and are masked when consumed
   auto fetch = [&](int c, Raw& r) {
+    const int t = at.g0 + c * kTileN;
+    int row[NU];
+    if (t + kTileN <= at.g1 && src.consecutive(t, kTileN)) {
+      const int first = src.row(t);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) row[u] = first + (u * 256 + tid) / UPR;
+    } else {
+      // tokens past the slice repeat its last one and are masked when consumed
+#pragma unroll
+      for (int u = 0; u < NU; ++u) row[u] = src.row(min(t + (u * 256 + tid) / UPR, at.g1 - 1));
+    }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int unit = u * 256 + tid;
-      const size_t row = at.kb + src.row(min(at.g0 + c * kTileN + unit / UPR, at.g1 - 1));
-      r.k[u] = ld_nt16(K + row * D + 16 * (unit % UPR));
-      r.ks[u] = a.ks[row];
-      r.v[u] = ld_nt16(V + row * D + 16 * (unit % UPR));
-      r.vs[u] = a.vs[row];
+      const size_t off = (size_t)row[u] * D + 16 * (tid % UPR);
+      r.k[u] = ld_nt16(K + off);
+      r.ks[u] = Ks[row[u]];
+      r.v[u] = ld_nt16(V + off);
+      r.vs[u] = Vs[row[u]];
+    }
+    // the step's own tokens, quantised here as append_rows quantises them
+    if (src.position(min(t + kTileN - 1, at.g1 - 1)) >= a.start) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int unit = u * 256 + tid;
+        const int p = src.position(min(t + unit / UPR, at.g1 - 1)) - a.start;
+        const size_t off = ((size_t)at.s * a.n_new + max(p, 0)) * D + 16 * (unit % UPR);
+        auto quantised = [&](const void* rows, uint4& codes, uint8_t& scale) {
+          float lo[8], hi[8];
+          float top = fmaxf(load8_top<T>((const S*)rows + off, lo), load8_top<T>((const S*)rows + off + 8, hi));
+#pragma unroll
+          for (int o = 1; o < UPR; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+          const int e = exponent_of(top);
+          const uint2 x = codes8(lo, e), y = codes8(hi, e);
+          if (p >= 0) {
+            codes = make_uint4(x.x, x.y, y.x, y.y);
+            scale = (uint8_t)(e + 127);
+          }
+        };
+        quantised(a.k_new, r.k[u], r.ks[u]);
+        quantised(a.v_new, r.v[u], r.vs[u]);
+      }
     }
   };
   auto put16 = [&](uint16_t* tile, int row, int c16, const uint4& w, float scale) {
@@ -443,8 +528,8 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int unit = u * 256 + tid;
-      put16(sk[b], unit / UPR, unit % UPR, r.k[u], scale_of(r.ks[u]));
-      put16(sv[b], unit / UPR, unit % UPR, r.v[u], scale_of(r.vs[u]));
+      put16(sk + b * TILE, unit / UPR, unit % UPR, r.k[u], scale_of(r.ks[u]));
+      put16(sv + b * TILE, unit / UPR, unit % UPR, r.v[u], scale_of(r.vs[u]));
     }
   };
 
@@ -458,7 +543,7 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
     put(r, b);
     if (c + 2 < n_chunks) fetch(c + 2, r);
     __syncthreads();
-    w.step(a, src, sk[b], sv[b], at.g0 + c * kTileN, at.g1);
+    w.step(a, src, sk + b * TILE, sv + b * TILE, at.g0 + c * kTileN, at.g1);
   };
   int c = 0;
   for (; c + 1 < n_chunks; c += 2) {
@@ -466,18 +551,17 @@ __global__ __launch_bounds__(256) void stream8_kernel(StreamArgs a, Src src) {
     step(c + 1, 1, rc);
   }
   if (c < n_chunks) step(c, 0, ra);
-  w.finish(a, at, (float*)&sk[0][0], (float*)&sv[0][0]);
+  w.finish(a, at, (float*)sk, (float*)sv);
 }
 
 // Over 16-bit rows: gathered into LDS by LDS-DMA, two steps in flight, so that no
 // registers hold loads.
 template <typename T, int D, int NB, bool RULE, class Src>
-__global__ __launch_bounds__(256) void stream16_kernel(StreamArgs a, Src src) {
+__device__ inline void stream16_rows(const StreamArgs& a, const Src& src, int block, uint16_t* sk, uint16_t* sv) {
   constexpr int NP = D / 32;                   // 1 KB LDS blocks per wave and 64-row tile
-  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
-  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  constexpr int TILE = kTileN * D;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const StreamPlace at(a, src, 16 * NB);
+  const StreamPlace at(a, src, 16 * NB, block);
   const int n_chunks = at.chunks();
   const uint16_t *K = (const uint16_t*)a.k + at.kb * D, *V = (const uint16_t*)a.v + at.kb * D;
   StreamWave<T, T, D, NB, 1, RULE> w(a, at);
@@ -491,14 +575,36 @@ __global__ __launch_bounds__(256) void stream16_kernel(StreamArgs a, Src src) {
     drow[p] = e / D;
     dcol[p] = (((e % D) >> 3) ^ lds_swz<D>(drow[p])) << 3;
   }
-  // tokens past the slice repeat its last one and are masked when consumed
   auto issue = [&](int c, int b) {
-    const uint32_t lk = lds_addr(sk[b]), lv = lds_addr(sv[b]);
+    const uint32_t lk = lds_addr(sk + b * TILE), lv = lds_addr(sv + b * TILE);
+    const int t = at.g0 + c * kTileN, n = min(kTileN, at.g1 - t);
+    if (src.consecutive(t, n) && src.position(t + n - 1) < a.start) {
+      // rows one after another: resources over those that the slice has (past them zeros),
+      // the lane's offsets the same for every step
+      const size_t row = (size_t)src.row(t) * D;
+      const i32x4 rk = buffer_rsrc(K + row, n * D * 2), rv = buffer_rsrc(V + row, n * D * 2);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const int off = 2 * (drow[p] * D + dcol[p]);
+        dma_buf16(rk, off, lk + (4 * p + wave) * 1024);
+        dma_buf16(rv, off, lv + (4 * p + wave) * 1024);
+      }
+      return;
+    }
+    // tokens past the slice repeat its last one and are masked when consumed
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const size_t off = (size_t)src.row(min(at.g0 + c * kTileN + drow[p], at.g1 - 1)) * D + dcol[p];
-      dma_load16(K + off, lk + (4 * p + wave) * 1024);
-      dma_load16(V + off, lv + (4 * p + wave) * 1024);
+      const int x = min(t + drow[p], at.g1 - 1);
+      const uint16_t *kt = K + (size_t)src.row(x) * D, *vt = V + (size_t)src.row(x) * D;
+      if constexpr (Src::kSteps) {
+        const int i = src.position(x) - a.start;
+        if (i >= 0) {
+          const size_t own = ((size_t)at.s * a.n_new + i) * D;
+          kt = (const uint16_t*)a.k_new + own, vt = (const uint16_t*)a.v_new + own;
+        }
+      }
+      dma_load16(kt + dcol[p], lk + (4 * p + wave) * 1024);
+      dma_load16(vt + dcol[p], lv + (4 * p + wave) * 1024);
     }
   };
   if (n_chunks > 0) issue(0, 0);
@@ -507,11 +613,67 @@ __global__ __launch_bounds__(256) void stream16_kernel(StreamArgs a, Src src) {
     const int b = c & 1;
     wait_chunks<NP, 2>(min(1, n_chunks - 1 - c));   // chunk c has landed
     __syncthreads();
-    w.step(a, src, sk[b], sv[b], at.g0 + c * kTileN, at.g1);
+    w.step(a, src, sk + b * TILE, sv + b * TILE, at.g0 + c * kTileN, at.g1);
     __syncthreads();                           // every wave is done with buffer b
     if (c + 2 < n_chunks) issue(c + 2, b);
   }
-  w.finish(a, at, (float*)&sk[0][0], (float*)&sv[0][0]);
+  w.finish(a, at, (float*)sk, (float*)sv);
+}
+
+template <typename T, int D, int NB, bool RULE, bool EIGHT, class Src>
+__device__ inline void stream_rows(const StreamArgs& a, const Src& src, int block, uint16_t* sk, uint16_t* sv) {
+  if constexpr (EIGHT) stream8_rows<T, D, NB, RULE>(a, src, block, sk, sv);
+  else stream16_rows<T, D, NB, RULE>(a, src, block, sk, sv);
+}
+
+// Waves per SIMD that the registers must leave room for: as many workgroups per CU as
+// their LDS allows (two at head_dim 128, four at 64, one less there with two row blocks
+// or three pieces).
+template <typename T, int D, int NB> constexpr int kStreamWaves = D >= 128 ? 2 : NB == 1 && !T::is_f32 ? 4 : 3;
+
+// Streams, then the workgroups that write a step's tokens into the cache.
+template <typename T, int D, int NB, bool RULE, bool EIGHT, class Src>
+__global__ __launch_bounds__(256, (kStreamWaves<T, D, NB>)) void stream_kernel(StreamArgs a, Src src, AppendArgs ap) {
+  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
+  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  if constexpr (Src::kSteps) {
+    if ((int)blockIdx.x >= a.n_blocks) {
+      append_rows<T, D, EIGHT>(ap, blockIdx.x - a.n_blocks);
+      return;
+    }
+  }
+  stream_rows<T, D, NB, RULE, EIGHT>(a, src, blockIdx.x, &sk[0][0], &sv[0][0]);
+}
+
+// The sequences' own streams in a launch with the shared prefix's workgroups, which come
+// first: with about one of those per CU each CU gets one of the matrix cores' kind and
+// one of the memory's (in turn, they went by two of a kind to each CU).
+template <typename T, int D, int NB, bool EIGHT>
+struct OwnStreams {
+  StreamArgs a;
+  RingStream src;
+  AppendArgs ap;
+  int shared_blocks;           // a multiple of the XCDs
+  // Is the workgroup one of these? Its index among its kind.
+  __device__ inline bool takes(int& block) const {
+    const int own = block - shared_blocks;
+    block = own >= 0 ? own : block;
+    return own >= 0;
+  }
+  __device__ inline void run(int block, uint16_t* sk, uint16_t* sv) const {
+    if (block < a.n_blocks) stream_rows<T, D, NB, true, EIGHT>(a, src, block, sk, sv);
+    else if (block < a.n_blocks + ap.n_blocks) append_rows<T, D, EIGHT>(ap, block - a.n_blocks);
+  }
+};
+
+// A shared prefix of few rows as streams, and the sequences' own.
+template <typename T, int D, class Beside>
+__global__ __launch_bounds__(256, (kStreamWaves<T, D, 2>)) void prefix_streams_kernel(StreamArgs a, DenseStream src, Beside beside) {
+  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
+  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  int block = blockIdx.x;
+  if (beside.takes(block)) beside.run(block, &sk[0][0], &sv[0][0]);
+  else if (block < a.n_blocks) stream_rows<T, D, 2, false, false>(a, src, block, &sk[0][0], &sv[0][0]);
 }
 
 // The states of a row's n_parts slices joined: a wave per row.
@@ -551,21 +713,32 @@ void launch_join(const StreamArgs& a, int64_t n_rows, hipStream_t stream) {
                      (typename T::storage*)a.o, a.lse, n_rows, a.n_parts);
 }
 
+// A workgroup per 256 lanes of work, up to a grid whose lanes a launch can count.
+inline dim3 row_grid(int64_t lanes) { return dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)); }
+
+// Workgroups that write the rows of `a`.
+inline int append_blocks(const AppendArgs& a, int head_dim) {
+  const int64_t lanes = 2 * (int64_t)a.BH * (a.rows.n_a + a.rows.n_b) * (head_dim / 8);
+  return (int)row_grid(lanes).x;
+}
+
+inline void set_rows(StreamArgs& a, int n_streams, int tile) {
+  a.row_tiles = (a.n_rows + tile - 1) / tile;
+  a.n_blocks = n_streams * a.n_splits * a.row_tiles;
+}
+
 // The streams of a launch in row tiles of the size that their rows take.
 template <typename T, int D, bool EIGHT, class Src>
-void launch_streams(StreamArgs a, const Src& src, int n_streams, hipStream_t stream) {
-  const int tile = stream_rows_tile(T::is_f32, a.n_rows);
-  a.row_tiles = (a.n_rows + tile - 1) / tile;
-  const dim3 grid(n_streams * a.n_splits * a.row_tiles);
-#define GKI_STREAM(NB, RULE)                                                                                      \
-  do {                                                                                                            \
-    if constexpr (EIGHT) hipLaunchKernelGGL((stream8_kernel<T, D, NB, RULE, Src>), grid, dim3(256), 0, stream, a, src); \
-    else hipLaunchKernelGGL((stream16_kernel<T, D, NB, RULE, Src>), grid, dim3(256), 0, stream, a, src);            \
-  } while (0)
-  if constexpr (std::is_same<Src, DenseStream>::value) {     // every token is visible to every row
+void launch_streams(StreamArgs a, const Src& src, int n_streams, const AppendArgs& ap, hipStream_t stream) {
+  const int tile = stream_rows_tile(EIGHT && kPieces<T> > 1, a.n_rows);
+  set_rows(a, n_streams, tile);
+#define GKI_STREAM(NB, RULE)                                                                              \
+  hipLaunchKernelGGL((stream_kernel<T, D, NB, RULE, EIGHT, Src>), dim3(a.n_blocks + ap.n_blocks), dim3(256), \
+                     0, stream, a, src, ap)
+  if constexpr (!Src::kSteps) {     // every token is visible to every row
     if (tile == 32) GKI_STREAM(2, false);
     else GKI_STREAM(1, false);
-  } else if constexpr (T::is_f32) {
+  } else if constexpr (kPieces<T> > 1) {
     if (a.n_q == 1) GKI_STREAM(1, false);
     else GKI_STREAM(1, true);
   } else {
@@ -579,53 +752,70 @@ void launch_streams(StreamArgs a, const Src& src, int n_streams, hipStream_t str
 
 template <typename T, int D>
 int cross_stream(const StreamArgs& a, const DenseStream& src, int n_streams, hipStream_t stream) {
-  launch_streams<T, D, false>(a, src, n_streams, stream);
+  launch_streams<T, D, false>(a, src, n_streams, AppendArgs{}, stream);
   if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
   return check_launch("gki_cross_fwd");
 }
 
 template <typename T, int D>
-int attend8(const StreamArgs& a, const RingStream& src, int n_streams, hipStream_t stream) {
-  launch_streams<T, D, true>(a, src, n_streams, stream);
+int attend8(const StreamArgs& a, const RingStream& src, int n_streams, const AppendArgs& ap, hipStream_t stream) {
+  launch_streams<T, D, true>(a, src, n_streams, ap, stream);
   if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
   return check_launch("gki_rolling8_decode");
 }
 
-// A prefix that the sequences share, then each sequence's own cache, then their states
-// joined. `own` and `shared` differ in the rows, the keys and the parts.
-template <typename T, int D>
-int prefix_decode(const Geom& g, const StreamArgs& own, const RingStream& ring, const StreamArgs& shared, int n_prefix,
-                  hipStream_t stream) {
+template <typename T, int D, int NB, bool EIGHT>
+void launch_prefix(const Geom& g, OwnStreams<T, D, NB, EIGHT> own, StreamArgs shared, int n_prefix, hipStream_t stream) {
+  set_rows(own.a, g.B * g.H_kv, 16 * NB);
+  const int n_own = own.a.n_blocks + own.ap.n_blocks;
   if (prefix_as_streams(shared.n_rows)) {
-    launch_streams<T, D, false>(shared, DenseStream{nullptr, n_prefix, g.H_kv}, g.H_kv, stream);
-  } else {
-    Geom pg = g;
-    pg.n_q = shared.n_rows;
-    pg.n_kv = n_prefix;
-    pg.causal = 0;
-    const SharedRows sh{shared.n_rows, shared.rb, shared.q_stride, shared.n_splits, shared.part0, shared.n_parts,
-                        shared.acc, shared.ml};
-    if (int rc = prefix_tiles_dispatch(std::is_same<T, F16>::value ? kF16 : kBF16, D, pg, shared.q, shared.k, shared.v,
-                                       sh, stream))
-      return rc;
+    set_rows(shared, g.H_kv, 32);
+    own.shared_blocks = kXcd * ((shared.n_blocks + kXcd - 1) / kXcd);
+    hipLaunchKernelGGL((prefix_streams_kernel<T, D, OwnStreams<T, D, NB, EIGHT>>), dim3(own.shared_blocks + n_own), dim3(256), 0,
+                       stream, shared, DenseStream{nullptr, n_prefix, g.H_kv}, own);
+    return;
   }
-  if (own.ks) launch_streams<T, D, true>(own, ring, g.B * g.H_kv, stream);
-  else launch_streams<T, D, false>(own, ring, g.B * g.H_kv, stream);
+  Geom pg = g;
+  pg.n_q = shared.n_rows;
+  pg.n_kv = n_prefix;
+  pg.causal = 0;
+  const SharedRows sh{shared.n_rows, shared.rb, shared.q_stride, shared.n_splits, shared.part0, shared.n_parts,
+                      shared.acc, shared.ml};
+  const int n_qt = (shared.n_rows + kTileMF - 1) / kTileMF;
+  own.shared_blocks = kXcd * ((n_qt * sh.n_splits * g.H_kv + kXcd - 1) / kXcd);
+  hipLaunchKernelGGL((fwd_kernel_16<T, D, kFwdPipe<D>, kShared, OwnStreams<T, D, NB, EIGHT>>), dim3(own.shared_blocks + n_own),
+                     dim3(kFwdThreads), 0, stream, pg, (const uint16_t*)shared.q, (const uint16_t*)shared.k,
+                     (const uint16_t*)shared.v, (uint16_t*)nullptr, (float*)nullptr, (const int32_t*)nullptr,
+                     (const int32_t*)nullptr, n_qt, (const int32_t*)nullptr, sh, own);
+}
+
+// A prefix that the sequences share and each sequence's own cache in one launch, then
+// their states joined. `own` and `shared` differ in the rows, the keys and the parts.
+template <typename T, int D>
+int prefix_decode(const Geom& g, const StreamArgs& own, const RingStream& ring, const AppendArgs& ap,
+                  const StreamArgs& shared, int n_prefix, hipStream_t stream) {
+#define GKI_PREFIX(NB, EIGHT) \
+  launch_prefix<T, D, NB, EIGHT>(g, OwnStreams<T, D, NB, EIGHT>{own, ring, ap, 0}, shared, n_prefix, stream)
+  const bool wide = stream_rows_tile(own.ks && kPieces<T> > 1, own.n_rows) == 32;
+  if (own.ks) {
+    if constexpr (kPieces<T> == 1) {
+      if (wide) GKI_PREFIX(2, true);
+      else GKI_PREFIX(1, true);
+    } else {
+      GKI_PREFIX(1, true);
+    }
+  } else if (wide) GKI_PREFIX(2, false);
+  else GKI_PREFIX(1, false);
+#undef GKI_PREFIX
   launch_join<T, D>(own, (int64_t)g.B * g.H * g.n_q, stream);
   return check_launch("gki_rolling_prefix_decode");
 }
 
-// A workgroup per 256 lanes of work, up to a grid whose lanes a launch can count.
-inline dim3 row_grid(int64_t lanes) { return dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)); }
-
 template <typename T, int D>
-int append8(uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn, const void* vn, int BH,
-            const AppendRows& a, hipStream_t stream) {
-  const int64_t lanes = 2 * (int64_t)BH * (a.n_a + a.n_b) * (D / 8);
-  if (lanes == 0) return 0;
-  using S = typename T::storage;
-  hipLaunchKernelGGL((append8_kernel<T, D>), row_grid(lanes), dim3(256), 0, stream, kc, vc, ks,
-                     vs, (const S*)kn, (const S*)vn, BH, a);
+int append8(AppendArgs a, hipStream_t stream) {
+  a.n_blocks = append_blocks(a, D);
+  if (a.n_blocks == 0) return 0;
+  hipLaunchKernelGGL((append8_kernel<T, D>), dim3(a.n_blocks), dim3(256), 0, stream, a);
   return check_launch("gki_rolling8_append");
 }
 
@@ -667,7 +857,27 @@ StreamArgs stream_args(const Geom& g, const void* q, const void* k, const void* 
   a.ml = ws + (size_t)g.B * g.H * g.n_q * n_splits * head_dim;
   a.scale_log2 = g.qk_scale_log2;
   a.q_sign = g.scale == 0.f ? 0.f : g.scale < 0.f ? -1.f : 1.f;
+  a.start = 1 << kPartialBit;
   return a;
+}
+
+AppendArgs append_args(void* kc, void* vc, uint8_t* ks, uint8_t* vs, const void* kn, const void* vn, int BH, int n_new,
+                       int start, int sink, int ring) {
+  AppendArgs a{kc, vc, ks, vs, kn, vn, BH, AppendRows{n_new, 0, 0, 0, start, sink, ring}, 0};
+  surviving_rows(start, n_new, sink, ring, &a.rows.n_a, &a.rows.i_b, &a.rows.n_b);
+  return a;
+}
+
+// A step: its n_q tokens (k_new, v_new) are written by the launch that attends them.
+void set_step(const Geom& g, StreamArgs& a, AppendArgs& ap, const void* k_new, const void* v_new, int ring, int head_dim) {
+  if (!k_new) return;
+  a.k_new = k_new;
+  a.v_new = v_new;
+  a.n_new = g.n_q;
+  a.start = g.q_off;
+  ap = append_args((void*)a.k, (void*)a.v, (uint8_t*)a.ks, (uint8_t*)a.vs, k_new, v_new, g.B * g.H_kv, g.n_q, g.q_off,
+                   g.sink, ring);
+  ap.n_blocks = append_blocks(ap, head_dim);
 }
 RingStream ring_args(const Geom& g, int ring) {
   RingStream src;
@@ -682,9 +892,8 @@ RingStream ring_args(const Geom& g, int ring) {
 
 int append8_dispatch(int dtype, int head_dim, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, const void* kn,
                      const void* vn, int BH, int n_new, int start, int sink, int ring, hipStream_t stream) {
-  AppendRows a{n_new, 0, 0, 0, start, sink, ring};
-  surviving_rows(start, n_new, sink, ring, &a.n_a, &a.i_b, &a.n_b);
-  GKI_BY_TYPE(append8, kc, vc, ks, vs, kn, vn, BH, a, stream)
+  const AppendArgs a = append_args(kc, vc, ks, vs, kn, vn, BH, n_new, start, sink, ring);
+  GKI_BY_TYPE(append8, a, stream)
 }
 
 int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const uint8_t* ks, const uint8_t* vs,
@@ -701,11 +910,13 @@ int read_dispatch(int dtype, int head_dim, const void* kc, const void* vc, const
 }
 
 int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
-                     const uint8_t* ks, const uint8_t* vs, void* o, float* lse, int ring, float* ws, int n_splits,
-                     hipStream_t stream) {
+                     const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new, void* o, float* lse,
+                     int ring, float* ws, int n_splits, hipStream_t stream) {
   const RingStream src = ring_args(g, ring);
-  const StreamArgs a = stream_args(g, q, k, v, ks, vs, o, lse, g.sink + ring, ws, n_splits, head_dim);
-  GKI_BY_TYPE(attend8, a, src, g.B * g.H_kv, stream)
+  StreamArgs a = stream_args(g, q, k, v, ks, vs, o, lse, g.sink + ring, ws, n_splits, head_dim);
+  AppendArgs ap{};
+  set_step(g, a, ap, k_new, v_new, ring, head_dim);
+  GKI_BY_TYPE(attend8, a, src, g.B * g.H_kv, ap, stream)
 }
 
 int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
@@ -719,22 +930,24 @@ int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q,
 }
 
 int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
-                           const uint8_t* ks, const uint8_t* vs, const void* prefix_k, const void* prefix_v, int n_prefix,
-                           void* o, float* lse, int ring, float* ws, int n_prefix_splits, int n_splits,
-                           hipStream_t stream) {
+                           const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new,
+                           const void* prefix_k, const void* prefix_v, int n_prefix, void* o, float* lse, int ring,
+                           float* ws, int n_prefix_splits, int n_splits, hipStream_t stream) {
   const int n_parts = n_prefix_splits + n_splits;
   StreamArgs own = stream_args(g, q, k, v, ks, vs, o, lse, g.sink + ring, ws, n_parts, head_dim);
   own.n_splits = n_splits;
   own.part0 = n_prefix_splits;
+  AppendArgs ap{};
+  set_step(g, own, ap, k_new, v_new, ring, head_dim);
   StreamArgs shared = stream_args(g, q, prefix_k, prefix_v, nullptr, nullptr, o, lse, n_prefix, ws, n_parts, head_dim);
   shared.n_splits = n_prefix_splits;
   shared.n_rows = g.B * shared.rb;
   const RingStream src = ring_args(g, ring);
   if (dtype == kF16)
-    return head_dim == 64 ? prefix_decode<F16, 64>(g, own, src, shared, n_prefix, stream)
-                          : prefix_decode<F16, 128>(g, own, src, shared, n_prefix, stream);
-  return head_dim == 64 ? prefix_decode<BF16, 64>(g, own, src, shared, n_prefix, stream)
-                        : prefix_decode<BF16, 128>(g, own, src, shared, n_prefix, stream);
+    return head_dim == 64 ? prefix_decode<F16, 64>(g, own, src, ap, shared, n_prefix, stream)
+                          : prefix_decode<F16, 128>(g, own, src, ap, shared, n_prefix, stream);
+  return head_dim == 64 ? prefix_decode<BF16, 64>(g, own, src, ap, shared, n_prefix, stream)
+                        : prefix_decode<BF16, 128>(g, own, src, ap, shared, n_prefix, stream);
 }
 
 }  // namespace gki

@@ -250,10 +250,13 @@ class StreamingKVCache:
             return o
         return o, scratch[:B * H * n_q].view(B, H, n_q).clone()
 
-    def _attend_streams(self, q: torch.Tensor, n_q: int, softmax_scale: float, return_lse: bool):
-        """The decode over 8-bit rows, or behind a shared prefix."""
+    def _attend_streams(self, q: torch.Tensor, n_q: int, softmax_scale: float, return_lse: bool,
+                        new: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+        """The decode over 8-bit rows, or behind a shared prefix. ``new``: the keys and
+        values of the n_q tokens, which the same launch writes (``length`` is not moved)."""
         lib = _lib.load()
-        B, H, H_kv, D, length = self.batch, int(q.shape[1]), self.heads, self.head_dim, self.length
+        B, H, H_kv, D = self.batch, int(q.shape[1]), self.heads, self.head_dim
+        length = self.length + (n_q if new else 0)
         n_tokens = min(length, self.sink_size) + max(
             0, length - max(self.sink_size, length - n_q - self.window_size + 1))
         prefix = self._prefix
@@ -274,22 +277,28 @@ class StreamingKVCache:
         pad = (B * H * n_q + 63) & ~63
         scratch = torch.empty(pad + ws_floats, dtype=torch.float32, device=self.device)
         lse = scratch.data_ptr()
+        rows = (self.k_cache.data_ptr(), self.v_cache.data_ptr())
+        scales = (0, 0) if self.k_scale is None else (self.k_scale.data_ptr(), self.v_scale.data_ptr())
+        shared = (prefix[0].data_ptr(), prefix[1].data_ptr(), n_prefix) if n_prefix else (0, 0, 0)
+        place = (dtype, B, H, H_kv, n_q, D, self.sink_size, self.window_size, self.ring_size)
         ws = lse + 4 * pad if ws_floats else 0
-        eight = self.k_scale is not None
-        k_scale, v_scale = (self.k_scale.data_ptr(), self.v_scale.data_ptr()) if eight else (0, 0)
-        place = (dtype, B, H, H_kv, n_q, D, self.sink_size, self.window_size, self.ring_size, length, softmax_scale, ws)
         with _on_device(self.device):
             stream = _current_stream(self.device)
-            if n_prefix:
-                rc = lib.gki_rolling_prefix_decode(
-                    q.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(), k_scale, v_scale,
-                    prefix[0].data_ptr(), prefix[1].data_ptr(), n_prefix, o.data_ptr(), lse, *place, n_shared,
-                    n_splits, stream)
+            if new:
+                what = "gki_rolling_step"
+                rc = lib.gki_rolling_step(q.data_ptr(), new[0].data_ptr(), new[1].data_ptr(), *rows, *scales, *shared,
+                                          o.data_ptr(), lse, *place, self.length, softmax_scale, ws, n_shared,
+                                          n_splits, stream)
+            elif n_prefix:
+                what = "gki_rolling_prefix_decode"
+                rc = lib.gki_rolling_prefix_decode(q.data_ptr(), *rows, *scales, *shared, o.data_ptr(), lse, *place,
+                                                   length, softmax_scale, ws, n_shared, n_splits, stream)
             else:
-                rc = lib.gki_rolling8_decode(
-                    q.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(), k_scale, v_scale,
-                    o.data_ptr(), lse, *place, n_splits, stream)
-        _lib.check(rc, "gki_rolling_prefix_decode" if n_prefix else "gki_rolling8_decode")
+                what = "gki_rolling8_decode"
+                rc = lib.gki_rolling8_decode(q.data_ptr(), *rows, *scales, o.data_ptr(), lse, *place, length,
+                                             softmax_scale, ws, n_splits, stream)
+        if rc:
+            _lib.check(rc, what)
         if not return_lse:
             return o
         return o, scratch[:B * H * n_q].view(B, H, n_q).clone()
@@ -297,5 +306,18 @@ class StreamingKVCache:
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
              softmax_scale: Optional[float] = None) -> torch.Tensor:
         """One decode step: append the new tokens' K / V, then attend with q."""
+        if (self.k_scale is not None or self._prefix is not None) and q.dim() == 4 and k.dim() == 4 \
+                and 1 <= q.shape[2] == k.shape[2] <= self.max_query:
+            # the tokens are written by the launch that attends them
+            self._check_tokens("q", q, grouped=True)
+            self._check_tokens("k", k)
+            self._check_tokens("v", v)
+            if k.shape != v.shape:
+                raise ValueError("k and v must share shape")
+            scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
+            n = int(q.shape[2])
+            o = self._attend_streams(_aligned(q), n, scale, False, (_aligned(k), _aligned(v)))
+            self.length += n
+            return o
         self.append(k, v)
         return self.attend(q, softmax_scale)

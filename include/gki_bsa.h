@@ -321,6 +321,19 @@ int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_
                               float* workspace, int32_t n_prefix_splits, int32_t n_splits,
                               void* stream);
 
+/* gki_rolling8_append / gki_rolling_append of n_q tokens (k_new / v_new: [B, H_kv, n_q,
+ * head_dim] at positions start_pos ..) and the decode of q at those positions, in one
+ * launch and the join: over an 8-bit cache (k_scale, v_scale), behind a prefix
+ * (n_prefix > 0; n_prefix_splits is not read without one), or both. The same results as
+ * the calls apart. */
+int gki_rolling_step(const void* q, const void* k_new, const void* v_new, void* k_cache,
+                     void* v_cache, void* k_scale, void* v_scale, const void* prefix_k,
+                     const void* prefix_v, int32_t n_prefix, void* o, float* lse, int32_t dtype,
+                     int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
+                     int32_t sink_size, int32_t window_size, int32_t ring_size, int64_t start_pos,
+                     float softmax_scale, float* workspace, int32_t n_prefix_splits,
+                     int32_t n_splits, void* stream);
+
 /* ---- Cross attention ----------------------------------------------------------
  * No reference counterpart. Every query row of batch entry b over its first
  * kv_len[b] keys (int32 [B] on the device; a length outside 0 .. n_kv counts as the

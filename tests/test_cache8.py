@@ -65,6 +65,14 @@ def test_c_entries_refuse_before_launch():
     assert decode(D=32) == 2 and decode(n_q=5) == 2 and decode(H=3, H_kv=2) == 1 and decode(ring=3) == 1
     assert decode(s=math.inf) == 1 and decode(scale=0) == 1 and decode(splits=2) == 1 and decode(splits=0) == 1
     assert decode(o=24) == 1 and decode(ws=24, splits=2) == 1 and decode(length=0) == 1
+
+    def step(k_new=16, k_scale=16, n_prefix=0, start=5, ws=0, splits=1, dtype=2):
+        return lib.gki_rolling_step(16, k_new, 16, 16, 16, k_scale, k_scale, 0, 0, n_prefix, 16, 16, dtype, 1, 2, 1, 1, 64,
+                                    0, 8, 8, start, 0.1, ws, 0, splits, null)
+
+    assert step(k_new=0) == 1 and step(k_new=8) == 1 and step(k_scale=0) == 2 and step(start=-1) == 1
+    assert step(start=2**30) == 1 and step(splits=2) == 1 and step(n_prefix=3) == 1 and step(dtype=8) == 2
+    assert step(n_prefix=-1) == 1
     read = (16, 16, 16, 16, 16, 16, 16)
     assert lib.gki_rolling_read(*read, 2, 1, 1, 64, 4, 8, -1, null) == 1
     assert lib.gki_rolling_read(16, 16, 16, 0, 16, 16, 16, 2, 1, 1, 64, 4, 8, 3, null) == 1    # one scale
@@ -227,6 +235,56 @@ def test_steps_over_a_turning_ring_and_large_logits():
     cache.reset()
     cache.append(ks[:, :, :3], vs[:, :, :3])
     _check_attend(cache, torch.randn((B, 2, 1, D), device=DEV).to(dtype), ks[:, :, :3], vs[:, :, :3])
+
+
+def _twins(dtype, head_dim, sink, window, max_q, B, H_kv, storage, prefix=0, seed=8):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    caches = [StreamingKVCache(B, H_kv, head_dim, StreamingMaskSpec(sink, window), dtype, DEV, max_q, storage_dtype=storage)
+              for _ in range(2)]
+    if prefix:
+        pk, pv = (torch.randn((1, H_kv, prefix, head_dim), generator=gen, device=DEV).to(dtype) for _ in range(2))
+        for c in caches:
+            c.set_prefix(pk, pv)
+    return caches, gen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,storage,prefix", [(torch.bfloat16, F8, 0), (torch.float16, F8, 0), (torch.float32, F8, 0),
+                                                  (torch.bfloat16, F8, 70), (torch.float16, None, 70)])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("sink,window,max_q,n_q,heads", [(4, 20, 4, 1, 2), (2, 70, 3, 3, 4), (0, 1, 1, 1, 2), (5, 0, 2, 2, 2),
+                                                         (3, 130, 4, 4, 32), (0, 0, 4, 3, 2), (1, 1, 2, 2, 40)])
+def test_a_step_is_the_append_and_the_attend(dtype, storage, prefix, head_dim, sink, window, max_q, n_q, heads):
+    """Same outputs and same cache, byte for byte, at every length across the sinks, the
+    filling of the ring and its turn."""
+    B, H_kv = 2, 2
+    (one, two), gen = _twins(dtype, head_dim, sink, window, max_q, B, H_kv, storage, prefix)
+    for t in range(0, 2 * (sink + window) + 9, n_q):
+        k, v = (torch.randn((B, H_kv, n_q, head_dim), generator=gen, device=DEV).to(dtype) for _ in range(2))
+        q = torch.randn((B, heads, n_q, head_dim), generator=gen, device=DEV).to(dtype)
+        got = one.step(q, k, v)
+        two.append(k, v)
+        assert torch.equal(got, two.attend(q)), t
+        assert one.length == two.length
+    for name in ("k_cache", "v_cache") + (("k_scale", "v_scale") if storage else ()):
+        a, b = (getattr(c, name).view(torch.uint8) for c in (one, two))
+        assert torch.equal(a, b), name
+
+
+@pytest.mark.gpu
+def test_a_step_of_unlike_counts_and_a_refused_one():
+    (one, two), gen = _twins(torch.bfloat16, 64, 4, 30, 4, 1, 2, F8)
+    k, v = (torch.randn((1, 2, 9, 64), generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn((1, 2, 2, 64), generator=gen, device=DEV).to(torch.bfloat16)
+    got = one.step(q, k, v)                                      # nine tokens, two queries
+    two.append(k, v)
+    assert torch.equal(got, two.attend(q))
+    with pytest.raises(ValueError, match="share shape|must be"):
+        one.step(q, k[:, :, :2], v[:, :1, :2])
+    with pytest.raises(ValueError, match="multiple of 2"):
+        one.step(q[:, :1], k[:, :, :2], v[:, :, :2])
+    assert one.length == 9                                       # a refused step writes nothing
+    assert torch.equal(one.attend(q), got)
 
 
 @pytest.mark.gpu
