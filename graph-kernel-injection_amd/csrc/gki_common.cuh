@@ -880,19 +880,25 @@ inline int stream_rows_tile(bool pieces, int n_rows) { return pieces || n_rows <
 // tiles 17.2.
 inline bool prefix_as_streams(int64_t n_rows) { return n_rows <= 32; }
 
-// Slices of each stream: about a workgroup per CU at head_dim 128, two at 64, of at
-// least 128 tokens each (a step of 64 takes about 0.5 us of latency, and a slice more
-// to join 0.05); a short stream stays whole, as joining two slices costs a launch.
-// us with 1 / 2 / 4 / 8 / 16 slices:
-//   8-bit   64 streams of 2052 tokens, D128    30.4 / 21.1 / 14.8 / 14.9 / 21.0
-//           16 of 8192 (16-bit), D128          82.2 / 46.0 / 26.5 / 17.6 / 16.6
-//           512 of 8196, D128                  168 / 170 / 176 / 188 / 226
-//           256 of 2000 (16-bit), D64          18.6 / 18.0 / 19.5 / 19.8 / 24.8
-//           256 of 600, D64                    10.4 / 12.8 / 13.0 / 15.7
-inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
+// Slices of each stream: about a workgroup per CU, of at least 128 tokens each (a step
+// of 64 takes 0.5 to 0.9 us of latency, a slice more to join 0.05); a short stream stays
+// whole, as joining two slices costs a launch. us with 1 / 2 / 4 / 8 / 16 slices:
+//   8-bit   64 streams of 2052 tokens, D128    31.9 / 21.7 / 15.0 / 14.7 / 20.7
+//           16 of 8192 (16-bit), D128          76.5 / 43.4 / 24.2 / 16.2 / 16.3
+//           512 of 8196, D128                  166 / 177 / 175 / 188 / 225
+//           256 of 2000 (16-bit), D64          17.9 / 19.7 / 19.9 / 20.8 / 24.9
+//           256 of 600, D64                    10.6 / 12.7 / 12.7 / 16.0
+inline int stream_splits(int64_t n_workgroups, int64_t n_tokens) {
   if (n_tokens < 768) return 1;
-  const int64_t target = head_dim >= 128 ? 256 : 512;
-  return (int)std::max<int64_t>(1, std::min((target + n_workgroups - 1) / n_workgroups, n_tokens / 128));
+  return (int)std::max<int64_t>(1, std::min((256 + n_workgroups - 1) / n_workgroups, n_tokens / 128));
+}
+// The same behind a shared prefix, where the states are joined in any case: long streams
+// in up to about 1024 pieces of 512 tokens or more, which even out the CUs that the
+// prefix loads. us with 1 / 2 / 4: 256 streams of 2052 (16-bit) 62.3 / 60.8 / 57.2, 512 of
+// 2052 (8-bit) 89.3 / 87.5 / 93.5, 256 of 304 22.7 / 23.0 / 24.7.
+inline int stream_splits_beside(int64_t n_workgroups, int64_t n_tokens) {
+  const int64_t even = std::min((1024 + n_workgroups - 1) / n_workgroups, n_tokens / 512);
+  return (int)std::max<int64_t>(stream_splits(n_workgroups, n_tokens), even);
 }
 
 // Slices of a shared prefix (their states are joined with the sequences' own in any

@@ -20,19 +20,34 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .ops import _DTYPE_CODE, _HEAD_DIMS, _aligned, _current_stream, _on_device
 
-# launch plans: (dtype, B, H, H_kv, n_q, n_kv, D) -> (slices, their workspace floats)
-_PLANS: dict = {}
+# launch plans: (dtype, B, H, H_kv, n_q, n_kv, D) -> (slices, floats of the LSE rows, of
+# the slices' states) of a forward, (parts, floats of the row terms, of the parts' sums) of
+# a backward
+_FWD_PLANS: dict = {}
+_BWD_PLANS: dict = {}
 
 
-def _fwd_plan(lib, key) -> Tuple[int, int]:
-    plan = _PLANS.get(key)
+def _planned(plans: dict, key: tuple, make) -> Tuple[int, int, int]:
+    plan = plans.get(key)
     if plan is None:
-        if len(_PLANS) >= 4096:
-            _PLANS.clear()
-        _, B, H, _, n_q, _, D = key
-        splits = int(lib.gki_cross_splits(*key))
-        plan = _PLANS[key] = (splits, int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits)))
+        if len(plans) >= 4096:
+            plans.clear()
+        plan = plans[key] = make(_lib.load(), *key)
     return plan
+
+
+def _make_fwd_plan(lib, dtype, B, H, H_kv, n_q, n_kv, D) -> Tuple[int, int, int]:
+    splits = int(lib.gki_cross_splits(dtype, B, H, H_kv, n_q, n_kv, D))
+    states = int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits))
+    rows = B * H * n_q
+    return splits, (rows + 63) & ~63 if states else rows, states     # the states 256-byte aligned
+
+
+def _make_bwd_plan(lib, dtype, B, H, H_kv, n_q, n_kv, D) -> Tuple[int, int, int]:
+    parts = int(lib.gki_cross_bwd_parts(dtype, B, H, H_kv, n_q, n_kv, D))
+    tile = _lib.tile_sizes()["tile_n"]
+    sums = B * H_kv * -(-n_kv // tile) * parts * 2 * tile * D if parts > 1 else 0
+    return parts, (2 * B * H * n_q + 63) & ~63, sums
 
 
 def _check(q, k, v, kv_lengths, enable_gqa) -> None:
@@ -63,31 +78,26 @@ def _check(q, k, v, kv_lengths, enable_gqa) -> None:
 
 
 def _forward(q, k, v, kv_lengths, scale):
-    """(o, lse, q, k, v, kv_lengths) with the inputs as the kernels read them."""
-    lib = _lib.load()
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    if kv_lengths is not None:
-        if kv_lengths.dtype != torch.int32:
-            kv_lengths = kv_lengths.clamp(0, k.shape[2]).to(torch.int32)
-        kv_lengths = kv_lengths.contiguous()
+    """(o, lse rows and behind them the slices' states, key) of aligned inputs; key None:
+    nothing to compute."""
     B, H, n_q, D = q.shape
-    H_kv, n_kv = k.shape[1], k.shape[2]
+    n_kv = k.shape[2]
     o = torch.empty_like(q)
-    rows = B * H * n_q
-    if rows == 0 or n_kv == 0:
-        return o.zero_(), torch.zeros((B, H, n_q), dtype=torch.float32, device=q.device), q, k, v, kv_lengths
-    key = (_DTYPE_CODE[q.dtype], B, H, H_kv, n_q, n_kv, D)
-    splits, ws_floats = _fwd_plan(lib, key)
-    # the LSE rows (padded to 256 bytes), then the slices' states: one allocation
-    pad = (rows + 63) & ~63 if ws_floats else rows
-    scratch = torch.empty(pad + ws_floats, dtype=torch.float32, device=q.device)
+    if q.numel() == 0 or n_kv == 0:
+        return o.zero_(), torch.zeros(B * H * n_q, dtype=torch.float32, device=q.device), None
+    key = (_DTYPE_CODE[q.dtype], B, H, k.shape[1], n_q, n_kv, D)
+    splits, rows, states = _planned(_FWD_PLANS, key, _make_fwd_plan)
+    scratch = torch.empty(rows + states, dtype=torch.float32, device=q.device)
+    lse = scratch.data_ptr()
+    lib = _lib.load()
     with _on_device(q.device):
         rc = lib.gki_cross_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), scratch.data_ptr(), *key,
-            0 if kv_lengths is None else kv_lengths.data_ptr(), scale,
-            scratch.data_ptr() + 4 * pad if ws_floats else 0, splits, _current_stream(q.device))
-    _lib.check(rc, "gki_cross_fwd")
-    return o, scratch, q, k, v, kv_lengths
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse, *key,
+            0 if kv_lengths is None else kv_lengths.data_ptr(), scale, lse + 4 * rows if states else 0, splits,
+            _current_stream(q.device))
+    if rc:
+        _lib.check(rc, "gki_cross_fwd")
+    return o, scratch, key
 
 
 class _CrossAttention(torch.autograd.Function):
@@ -95,39 +105,34 @@ class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, kv_lengths, scale):  # type: ignore[override]
-        o, lse, q, k, v, kv_lengths = _forward(q, k, v, kv_lengths, scale)
-        B, H, n_q, _ = q.shape
-        rows = lse.view(-1)[:B * H * n_q]
-        # a step's states follow its LSE rows: they need not outlive the forward
-        ctx.save_for_backward(q, k, v, o, rows if rows.numel() == lse.numel() else rows.clone(), kv_lengths)
-        ctx.scale = scale
+        o, lse, key = _forward(q, k, v, kv_lengths, scale)
+        if key is not None and _FWD_PLANS[key][2]:
+            lse = lse[:o.numel() // o.shape[3]].clone()     # the states need not outlive the forward
+        ctx.save_for_backward(q, k, v, o, lse, kv_lengths)
+        ctx.call = key, scale
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):  # type: ignore[override]
-        lib = _lib.load()
         q, k, v, o, lse, kv_lengths = ctx.saved_tensors
-        B, H, n_q, D = q.shape
-        H_kv, n_kv = k.shape[1], k.shape[2]
+        key, scale = ctx.call
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        if q.numel() == 0 or k.numel() == 0:
+        if key is None:
             return dq.zero_(), dk.zero_(), dv.zero_(), None, None
-        do = _aligned(do.to(q.dtype))
-        shape = (_DTYPE_CODE[q.dtype], B, H, H_kv, n_q, n_kv, D)
-        parts = int(lib.gki_cross_bwd_parts(*shape))
-        tile = _lib.tile_sizes()["tile_n"]
-        # row terms (Delta, then a form of the LSE), then the parts' fp32 dK / dV sums
-        pad = (2 * B * H * n_q + 63) & ~63
-        sums = B * H_kv * -(-n_kv // tile) * parts * 2 * tile * D if parts > 1 else 0
-        scratch = torch.empty(pad + sums, dtype=torch.float32, device=q.device)
+        do = _aligned(do if do.dtype == q.dtype else do.to(q.dtype))
+        parts, terms, sums = _planned(_BWD_PLANS, key, _make_bwd_plan)
+        scratch = torch.empty(terms + sums, dtype=torch.float32, device=q.device)
+        delta = scratch.data_ptr()
+        lib = _lib.load()
         with _on_device(q.device):
             rc = lib.gki_cross_bwd(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), scratch.data_ptr(), *shape,
-                0 if kv_lengths is None else kv_lengths.data_ptr(), ctx.scale, parts,
-                scratch.data_ptr() + 4 * pad if sums else 0, _current_stream(q.device))
-        _lib.check(rc, "gki_cross_bwd")
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, *key,
+                0 if kv_lengths is None else kv_lengths.data_ptr(), scale, parts,
+                delta + 4 * terms if sums else 0, _current_stream(q.device))
+        if rc:
+            _lib.check(rc, "gki_cross_bwd")
         return dq, dk, dv, None, None
 
 
@@ -155,6 +160,12 @@ def cross_attention(
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
     if not math.isfinite(scale):
         raise ValueError(f"softmax_scale must be finite, got {scale}")
+    if kv_lengths is not None:
+        if kv_lengths.dtype != torch.int32:
+            kv_lengths = kv_lengths.clamp(0, k.shape[2]).to(torch.int32)
+        kv_lengths = kv_lengths.contiguous()
+    # copies of strided inputs are made here, where autograd sees them
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossAttention.apply(q, k, v, kv_lengths, scale)
     return _forward(q, k, v, kv_lengths, scale)[0]

@@ -267,8 +267,13 @@ class StreamingKVCache:
         if plan is None:
             if len(self._plans) >= 4096:     # a filling window adds one key per step
                 self._plans.clear()
-            splits = int(lib.gki_stream_splits(dtype, B, H, H_kv, n_q, D, n_tokens))
-            shared = int(lib.gki_prefix_splits(dtype, B, H, H_kv, n_q, D, n_prefix)) if n_prefix else 0
+            shared = 0
+            if n_prefix:
+                own = ctypes.c_int32()
+                shared = int(lib.gki_prefix_splits(dtype, B, H, H_kv, n_q, n_prefix, n_tokens, ctypes.byref(own)))
+                splits = own.value
+            else:
+                splits = int(lib.gki_stream_splits(dtype, B, H, H_kv, n_q, D, n_tokens))
             plan = self._plans[key] = (
                 splits, shared, int(lib.gki_stream_workspace_floats(B, H, n_q, D, splits + shared)))
         n_splits, n_shared, ws_floats = plan

@@ -172,7 +172,7 @@ def test_larger_grids(dtype, B, H, H_kv, n_q, n_kv, D):
 def test_single_tokens_at_any_number_of_slices(dtype, D, splits, monkeypatch):
     from gki import cross
 
-    monkeypatch.setattr(cross, "_PLANS", {})
+    monkeypatch.setattr(cross, "_FWD_PLANS", {})
     lib = _lib.load()
     monkeypatch.setattr(lib, "gki_cross_splits", lambda *a: splits)
     for H, H_kv, n_q, n_kv in ((4, 4, 1, 900), (8, 2, 2, 130), (16, 1, 2, 70), (20, 1, 4, 257), (5, 1, 1, 1)):

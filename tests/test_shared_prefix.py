@@ -38,8 +38,11 @@ def test_c_entry_refuses_before_launch():
     assert call(n_ps=0) == 1 and call(n_s=0) == 1 and call(H=3) == 1 and call(ring=2) == 1 and call(s=math.nan) == 1
     assert call(n_ps=2**24) == 1
     for rows in ((1, 1), (8, 8), (64, 8), (1024, 8)):
-        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 128, 100) == 1
-        assert 1 <= lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 128, 100000) <= 100000 // 128
+        own = ctypes.c_int32()
+        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 100, 100, ctypes.byref(own)) == 1 and own.value == 1
+        assert 1 <= lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 100000, 5000, ctypes.byref(own)) <= 100000 // 256
+        assert 1 <= own.value <= 5000 // 128
+        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 100, 100, None) == 1
 
 
 def _check(cache, q, pk, pv, k, v, scale=None, tag=""):
@@ -97,8 +100,12 @@ def test_decode_against_64_bits(dtype, bits, D, B, H, H_kv, n_q, P, length, sink
 @pytest.mark.parametrize("n_ps,n_s", [(1, 1), (3, 2), (40, 5)])
 def test_any_number_of_slices(B, n_ps, n_s, monkeypatch):
     lib = _lib.load()
-    monkeypatch.setattr(lib, "gki_prefix_splits", lambda *a: n_ps)
-    monkeypatch.setattr(lib, "gki_stream_splits", lambda *a: n_s)
+
+    def splits(*a):
+        a[-1]._obj.value = n_s
+        return n_ps
+
+    monkeypatch.setattr(lib, "gki_prefix_splits", splits)
     for bits in (16, 8):
         _check(*_make(B, 8, 2, 1, 300, 150, 128, torch.bfloat16, 3, bits=bits))
 
