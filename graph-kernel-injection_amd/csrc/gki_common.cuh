@@ -332,6 +332,20 @@ __device__ inline void dma_buf16(i32x4 rsrc, int voff, uint32_t lds) {
                "s"(lds)
                : "memory", "m0");
 }
+// Either for data that is read once (`once`: non-temporal) or again.
+__device__ inline void dma_buf16(i32x4 rsrc, int voff, uint32_t lds, bool once) {
+  if (once)
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" ::"v"(voff), "s"(rsrc), "s"(lds)
+                 : "memory", "m0");
+  else
+    dma_buf16(rsrc, voff, lds);
+}
+__device__ inline void dma_load16(const void* src, uint32_t lds, bool once) {
+  if (once)
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "s"(lds) : "memory", "m0");
+  else
+    dma_load16(src, lds);
+}
 // 4-byte variant: lane i writes lds + 4 i.
 __device__ inline void dma_load4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds)
@@ -880,34 +894,36 @@ inline int stream_rows_tile(bool pieces, int n_rows) { return pieces || n_rows <
 // tiles 17.2.
 inline bool prefix_as_streams(int64_t n_rows) { return n_rows <= 32; }
 
-// Slices of each stream: about a workgroup per CU, of at least 128 tokens each (a step
-// of 64 takes 0.5 to 0.9 us of latency, a slice more to join 0.05); a short stream stays
-// whole, as joining two slices costs a launch. us with 1 / 2 / 4 / 8 / 16 slices:
-//   8-bit   64 streams of 2052 tokens, D128    31.9 / 21.7 / 15.0 / 14.7 / 20.7
-//           16 of 8192 (16-bit), D128          76.5 / 43.4 / 24.2 / 16.2 / 16.3
-//           512 of 8196, D128                  166 / 177 / 175 / 188 / 225
-//           256 of 2000 (16-bit), D64          17.9 / 19.7 / 19.9 / 20.8 / 24.9
-//           256 of 600, D64                    10.6 / 12.7 / 12.7 / 16.0
-inline int stream_splits(int64_t n_workgroups, int64_t n_tokens) {
+// Slices of each stream: about a workgroup per CU at head_dim 128, two at 64, of at
+// least 128 tokens each; a short stream stays whole, as joining two slices costs a
+// launch. us with 1 / 2 / 4 / 8 / 16 slices:
+//   8-bit   64 streams of 2052 tokens, D128    22.3 / 17.0 / 13.0 / 14.1 / 19.3
+//           512 of 8196, D128                  163 / 177 / 166 / 167 / 191
+//           256 of 600, D64                    10.2 / 12.9 / 13.0 / 15.0
+//   16-bit  16 of 8192, D128                   91.9 / 51.9 / 30.1 / 19.4 / 15.6
+//           256 of 2000, D64                   21.2 / 19.4 / 19.5 / 20.0 / 25.1
+inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
   if (n_tokens < 768) return 1;
-  return (int)std::max<int64_t>(1, std::min((256 + n_workgroups - 1) / n_workgroups, n_tokens / 128));
+  const int64_t target = head_dim >= 128 ? 256 : 512;
+  return (int)std::max<int64_t>(1, std::min((target + n_workgroups - 1) / n_workgroups, n_tokens / 128));
 }
 // The same behind a shared prefix, where the states are joined in any case: long streams
 // in up to about 1024 pieces of 512 tokens or more, which even out the CUs that the
-// prefix loads. us with 1 / 2 / 4: 256 streams of 2052 (16-bit) 62.3 / 60.8 / 57.2, 512 of
-// 2052 (8-bit) 89.3 / 87.5 / 93.5, 256 of 304 22.7 / 23.0 / 24.7.
-inline int stream_splits_beside(int64_t n_workgroups, int64_t n_tokens) {
+// prefix loads. us with 1 / 2 / 4, the prefix in 8 slices: 256 streams of 2052 (16-bit)
+// 58.7 / 59.3 / 56.4, 512 of 2052 (8-bit) 87.4 / 86.2 / 86.6.
+inline int stream_splits_beside(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
   const int64_t even = std::min((1024 + n_workgroups - 1) / n_workgroups, n_tokens / 512);
-  return (int)std::max<int64_t>(stream_splits(n_workgroups, n_tokens), even);
+  return (int)std::max<int64_t>(stream_splits(head_dim, n_workgroups, n_tokens), even);
 }
 
 // Slices of a shared prefix (their states are joined with the sequences' own in any
-// case): a workgroup for every other CU, beside the sequences' own, of at least 256 keys.
-// us with 4 / 8 / 16 / 32 slices: 8 row tiles over 8192 keys (sequences of 304)
-// - / 27.8 / 22.7 / 24.8, over 2000 16.6 / 14.7 / 16.8; 16 over 32768 (8-bit sequences of
-// 2052) - / 89.3 / 92.9 / 96; 8 streams of 20000 keys 64.8 / 39.1 / 26.7 / 26.1.
-inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
-  return (int)std::max<int64_t>(1, std::min((128 + n_workgroups - 1) / n_workgroups, n_keys / 256));
+// case), of at least 256 keys: a workgroup per CU as streams, for every other CU as row
+// tiles, beside the sequences' own. us with 4 / 8 / 16 / 32 slices: 8 row tiles over 8192
+// keys (sequences of 304) - / 27.7 / 23.1 / 27.0, over 2000 15.9 / 14.1 / 14.3; 16 over 32768
+// (8-bit sequences of 2052) - / 89.7 / 97.8; 8 streams of 20000 keys 77.5 / 43.9 / 28.7 / 24.4.
+inline int prefix_splits(bool streams, int64_t n_workgroups, int64_t n_keys) {
+  const int64_t target = streams ? 256 : 128;
+  return (int)std::max<int64_t>(1, std::min((target + n_workgroups - 1) / n_workgroups, n_keys / 256));
 }
 
 // Does a cross attention run its query rows as streams (a whole group's rows against

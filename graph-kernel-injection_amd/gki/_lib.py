@@ -64,7 +64,7 @@ SIGNATURES = {
     "gki_rolling_read": (ctypes.c_int, [_c_ptr] * 7 + [_c_int] * 6 + [_c_i64, _c_ptr]),
     "gki_rolling8_decode": (ctypes.c_int, [_c_ptr] * 7 + [_c_int] * 9 + [_c_i64, _c_float, _c_ptr,
                                                                         _c_int, _c_ptr]),
-    "gki_prefix_splits": (ctypes.c_int, [_c_int] * 6 + [_c_i64, _c_ptr]),
+    "gki_prefix_splits": (ctypes.c_int, [_c_int] * 7 + [_c_i64, _c_ptr]),
     "gki_rolling_prefix_decode": (ctypes.c_int, [_c_ptr] * 7 + [_c_int] + [_c_ptr] * 2 + [_c_int] * 9
                                   + [_c_i64, _c_float, _c_ptr, _c_int, _c_int, _c_ptr]),
     "gki_rolling_step": (ctypes.c_int, [_c_ptr] * 9 + [_c_int] + [_c_ptr] * 2 + [_c_int] * 9

@@ -270,7 +270,7 @@ class StreamingKVCache:
             shared = 0
             if n_prefix:
                 own = ctypes.c_int32()
-                shared = int(lib.gki_prefix_splits(dtype, B, H, H_kv, n_q, n_prefix, n_tokens, ctypes.byref(own)))
+                shared = int(lib.gki_prefix_splits(dtype, B, H, H_kv, n_q, D, n_prefix, n_tokens, ctypes.byref(own)))
                 splits = own.value
             else:
                 splits = int(lib.gki_stream_splits(dtype, B, H, H_kv, n_q, D, n_tokens))

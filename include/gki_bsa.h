@@ -311,7 +311,7 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
  * n_prefix_splits and n_splits >= 1, for a full card what gki_prefix_splits returns and
  * writes to own_splits (for n_tokens visible tokens of each sequence). */
 int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
-                      int32_t n_prefix, int64_t n_tokens, int32_t* own_splits);
+                      int32_t head_dim, int32_t n_prefix, int64_t n_tokens, int32_t* own_splits);
 int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_cache,
                               const void* k_scale, const void* v_scale, const void* prefix_k,
                               const void* prefix_v, int32_t n_prefix, void* o, float* lse,

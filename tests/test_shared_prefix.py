@@ -39,10 +39,10 @@ def test_c_entry_refuses_before_launch():
     assert call(n_ps=2**24) == 1
     for rows in ((1, 1), (8, 8), (64, 8), (1024, 8)):
         own = ctypes.c_int32()
-        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 100, 100, ctypes.byref(own)) == 1 and own.value == 1
-        assert 1 <= lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 100000, 5000, ctypes.byref(own)) <= 100000 // 256
+        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 128, 100, 100, ctypes.byref(own)) == 1 and own.value == 1
+        assert 1 <= lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 128, 100000, 5000, ctypes.byref(own)) <= 100000 // 256
         assert 1 <= own.value <= 5000 // 128
-        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 100, 100, None) == 1
+        assert lib.gki_prefix_splits(2, rows[0], rows[1], 1, 1, 128, 100, 100, None) == 1
 
 
 def _check(cache, q, pk, pv, k, v, scale=None, tag=""):
