@@ -659,10 +659,9 @@ int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t
   if (own_splits) *own_splits = 1;
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_prefix <= 0 || n_tokens < 0) return 1;
   const int64_t own = (int64_t)(H / H_kv) * n_q, rows = B * own;
-  const bool streams = prefix_as_streams(rows);
-  const int64_t tile = streams ? 32 : kTileMF, own_tile = stream_rows_tile(dtype != kBF16, (int)own);
+  const int64_t tile = prefix_as_streams(rows) ? 32 : kTileMF, own_tile = stream_rows_tile(dtype != kBF16, (int)own);
   if (own_splits) *own_splits = stream_splits_beside(head_dim, (int64_t)B * H_kv * ((own + own_tile - 1) / own_tile), n_tokens);
-  return prefix_splits(streams, H_kv * ((rows + tile - 1) / tile), n_prefix);
+  return prefix_splits(H_kv * ((rows + tile - 1) / tile), n_prefix);
 }
 
 int gki_rolling_prefix_decode(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,

@@ -917,13 +917,14 @@ inline int stream_splits_beside(int head_dim, int64_t n_workgroups, int64_t n_to
 }
 
 // Slices of a shared prefix (their states are joined with the sequences' own in any
-// case), of at least 256 keys: a workgroup per CU as streams, for every other CU as row
-// tiles, beside the sequences' own. us with 4 / 8 / 16 / 32 slices: 8 row tiles over 8192
-// keys (sequences of 304) - / 27.7 / 23.1 / 27.0, over 2000 15.9 / 14.1 / 14.3; 16 over 32768
-// (8-bit sequences of 2052) - / 89.7 / 97.8; 8 streams of 20000 keys 77.5 / 43.9 / 28.7 / 24.4.
-inline int prefix_splits(bool streams, int64_t n_workgroups, int64_t n_keys) {
-  const int64_t target = streams ? 256 : 128;
-  return (int)std::max<int64_t>(1, std::min((target + n_workgroups - 1) / n_workgroups, n_keys / 256));
+// case): a workgroup per CU, beside the sequences' own, of 512 keys or more (256 up to
+// eight slices). us with 4 / 8 / 16 / 32 slices, the sequences' in 1 or 2: 8 row tiles
+// over 8192 keys (sequences of 304) - / 27.7 / 23.1 / 27.0, over 2000 15.9 / 14.1 / 14.3, over
+// 20000 (of 1004, 8 bits) - / - / 33.0 / 29.7; 16 over 32768 (of 2052, 8 bits, past the
+// caches) - / 96.6 / 91.9 / 104; 8 streams of 20000 keys 77.5 / 43.9 / 28.7 / 24.4.
+inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
+  const int64_t most = std::max(n_keys / 512, std::min<int64_t>(8, n_keys / 256));
+  return (int)std::max<int64_t>(1, std::min((256 + n_workgroups - 1) / n_workgroups, most));
 }
 
 // Does a cross attention run its query rows as streams (a whole group's rows against
