@@ -887,7 +887,7 @@ inline void surviving_rows(int start, int n_new, int sink, int ring, int* n_a, i
 // Query rows per workgroup of the stream kernels: one block of 16, or two where a
 // stream has more (not for 8-bit rows under fp16 or fp32 queries: their two or three
 // pieces of each operand leave registers for one).
-inline int stream_rows_tile(bool pieces, int n_rows) { return pieces || n_rows <= 16 ? 16 : 32; }
+inline int stream_rows_tile(bool pieces, int64_t n_rows) { return pieces || n_rows <= 16 ? 16 : 32; }
 
 // Does a shared prefix run its rows as streams (32 of them) or as 128-row tiles? 8 heads
 // over 4000 keys, D128, us: 24 / 32 / 48 / 64 rows as streams 16.0 / 16.8 / 19.0 / 19.7, 65 as
@@ -930,22 +930,21 @@ inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
 // Does a cross attention run its query rows as streams (a whole group's rows against
 // each read of K and V) or as q tiles of each head? 16-bit, head_dim 64 or 128.
 inline bool cross_as_streams(int dtype, int head_dim, int group, int n_q) {
-  return dtype != kF32 && (head_dim == 64 || head_dim == 128) && group * n_q <= 32;
+  return dtype != kF32 && (head_dim == 64 || head_dim == 128) && (int64_t)group * n_q <= 32;
 }
 
 // Parts that a dense walk of dK/dV is cut into: each of `columns` kv tiles (over all
 // (b, kv head)) is walked by `walk` = q tiles * group iterations, all alike. 512 columns
 // fill the card whole, as do 128 (192 below head_dim 64) short ones (16-bit); fewer are
-// cut into about 512 items of 8 iterations or more (2 for fp32). Never more than about
-// 8192 items in all. Backward us with 1 / 2 / 4 / 8 / 16 parts:
+// cut into about 512 items of 8 iterations or more (2 for fp32). Backward us with
+// 1 / 2 / 4 / 8 / 16 parts:
 //   1024 columns of 128, D128     828 / 850 / 859 / 951 / 1136
-//   3072 columns of 7, D64        109 / 144 / 201
 //   64 columns of 256, D64        232 / 139 / 93 / 82 / 87
 //   128 columns of 64, D128 fp32  662 / 622 / 625 / 637 / 608
 inline int cross_kv_parts(int dtype, int head_dim, int64_t walk, int64_t columns) {
-  const int64_t total = walk * columns, few = head_dim >= 64 ? 128 : 192, brief = head_dim >= 64 ? 32 : 16;
+  const int64_t few = head_dim >= 64 ? 128 : 192, brief = head_dim >= 64 ? 32 : 16;
   if (columns >= 512 || (dtype != kF32 && columns >= few && walk <= brief)) return 1;
-  const int64_t chunk = std::max({(int64_t)(dtype == kF32 ? 2 : 8), (total + 511) / 512, (total + 8191) / 8192});
+  const int64_t chunk = std::max((int64_t)(dtype == kF32 ? 2 : 8), (walk * columns + 511) / 512);
   return (int)((walk + chunk - 1) / chunk);
 }
 

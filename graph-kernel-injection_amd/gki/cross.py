@@ -106,7 +106,7 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_lengths, scale):  # type: ignore[override]
         o, lse, key = _forward(q, k, v, kv_lengths, scale)
-        if key is not None and _FWD_PLANS[key][2]:
+        if key is not None and lse.numel() > o.numel() // o.shape[3]:
             lse = lse[:o.numel() // o.shape[3]].clone()     # the states need not outlive the forward
         ctx.save_for_backward(q, k, v, o, lse, kv_lengths)
         ctx.call = key, scale

@@ -289,7 +289,7 @@ int gki_rolling_read(const void* k_cache, const void* v_cache, const void* k_sca
  * full card (any n_splits >= 1 is right), and the floats of 16-byte aligned
  * workspace that n_parts states per query row need (0 for one). */
 int gki_stream_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
-                          int32_t head_dim, int64_t n_tokens);
+                      int32_t head_dim, int64_t n_tokens);
 int64_t gki_stream_workspace_floats(int32_t B, int32_t H, int32_t n_q, int32_t head_dim,
                                     int32_t n_parts);
 

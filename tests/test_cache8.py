@@ -306,6 +306,21 @@ def test_unseen_slots_do_not_matter():
 
 
 @pytest.mark.gpu
+def test_slots_past_2_31_elements():
+    B, H, D, window = 34, 8, 128, 65536               # 2.3e9 elements of K and of V
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    k, v = (torch.randn((B, H, 70, D), generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn((B, H, 1, D), generator=gen, device=DEV).to(torch.bfloat16)
+    cache = StreamingKVCache(B, H, D, StreamingMaskSpec(4, window), torch.bfloat16, DEV, storage_dtype=F8)
+    assert cache.k_cache.numel() > 2**31
+    cache.append(k, v)
+    _check_attend(cache, q, k, v)
+    _, kr, vr = cache.read()
+    for x, got in ((k, kr), (v, vr)):
+        _same(got, cache8.stored_values(x.double().cpu().numpy()))
+
+
+@pytest.mark.gpu
 def test_strided_tokens_side_stream_and_graph():
     dtype, B, H, D = torch.bfloat16, 2, 4, 64
     gen = torch.Generator(device=DEV).manual_seed(7)

@@ -52,6 +52,7 @@ def test_c_entries_refuse_before_launch():
 
 def test_launch_rules():
     lib = _lib.load()
+    assert lib.gki_cross_splits(2, 1, 4, 1, 2**29, 2000, 64) == 0         # group * n_q past 31 bits
     assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 64) >= 1          # a step: streams
     assert lib.gki_cross_splits(0, 16, 16, 16, 1, 2000, 64) == 0          # fp32: q tiles
     assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 32) == 0
@@ -212,6 +213,38 @@ def test_padding_may_hold_anything(dtype, D, n_q):
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     _compare(want, q, k, v, do, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q", [2, 70])
+def test_keys_past_2_31_elements(n_q):
+    n_kv, held = 9_000_000, 200                       # entry 2 starts 2.3e9 elements into K and V
+    q, k0, v0, do = _inputs(3, 2, 1, n_q, held, 128, torch.bfloat16, seed=13)
+    k, v = (torch.full((3, 1, n_kv, 128), math.nan, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    k[:, :, :held], v[:, :, :held] = k0, v0
+    n = torch.tensor([1, 0, held], dtype=torch.int32, device=DEV)
+    out, dq, dk, dv = _run(q, k, v, do, n)
+    assert not dk[:, :, held:].any() and not dv[:, :, held:].any()
+    _compare((out, dq, dk[:, :, :held], dv[:, :, :held]), q, k0, v0, do, n)
+
+
+@pytest.mark.gpu
+def test_strided_lengths_and_two_graphs():
+    """Lengths from a strided tensor; two captured graphs of one shape replayed in turn."""
+    q, k, v, _ = _inputs(2, 8, 2, 1, 3000, 128, torch.bfloat16, seed=17)
+    pairs = torch.tensor([[3000, 5], [1234, 7]], dtype=torch.int32, device=DEV)
+    want = [cross_attention(q, k, v, pairs[:, i].contiguous(), enable_gqa=True) for i in range(2)]
+    assert all(torch.equal(cross_attention(q, k, v, pairs[:, i], enable_gqa=True), want[i]) for i in range(2))
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            outs.append(cross_attention(q, k, v, pairs[:, i], enable_gqa=True))
+    for _ in range(3):
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 @pytest.mark.gpu
