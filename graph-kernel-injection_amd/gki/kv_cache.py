@@ -151,17 +151,21 @@ class StreamingKVCache:
             raise ValueError("prefix k and v must share shape")
         self._prefix = (_aligned(k.detach()), _aligned(v.detach())) if k.shape[2] else None
 
-    def _check_tokens(self, name: str, t: torch.Tensor, grouped: bool = False) -> None:
-        heads_ok = t.dim() == 4 and (t.shape[1] == self.heads or
-                                     (grouped and t.shape[1] % self.heads == 0 and t.shape[1] > 0))
-        if t.dim() != 4 or t.shape[0] != self.batch or not heads_ok or t.shape[3] != self.head_dim:
+    def _check_tokens(self, name: str, t: torch.Tensor, grouped: bool = False) -> int:
+        """The tokens of ``t``, which must be ``[B, H, n, D]`` of the cache."""
+        shape = t.shape                      # read once: a decode step's host time counts
+        if len(shape) == 4:
+            b, h, n, d = shape
+            heads_ok = h == self.heads or (grouped and h > 0 and h % self.heads == 0)
+        if len(shape) != 4 or b != self.batch or not heads_ok or d != self.head_dim:
             want = "a multiple of " + str(self.heads) if grouped else str(self.heads)
             raise ValueError(f"{name} must be [{self.batch}, {want}, n, {self.head_dim}], "
-                             f"got {tuple(t.shape)}")
+                             f"got {tuple(shape)}")
         if t.dtype != self.dtype:
             raise ValueError(f"{name} must be {self.dtype}, got {t.dtype}")
         if t.device != self.device:
             raise ValueError(f"{name} must live on {self.device}")
+        return n
 
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Append ``[B, H, n, D]`` keys / values at positions length .. length+n-1."""
@@ -257,8 +261,8 @@ class StreamingKVCache:
         lib = _lib.load()
         B, H, H_kv, D = self.batch, int(q.shape[1]), self.heads, self.head_dim
         length = self.length + (n_q if new else 0)
-        n_tokens = min(length, self.sink_size) + max(
-            0, length - max(self.sink_size, length - n_q - self.window_size + 1))
+        oldest = length - n_q - self.window_size + 1         # of the positions that some row's window holds
+        n_tokens = length if oldest <= self.sink_size else self.sink_size + length - oldest
         prefix = self._prefix
         n_prefix = int(prefix[0].shape[2]) if prefix is not None else 0
         dtype = _DTYPE_CODE[self.dtype]
@@ -311,18 +315,15 @@ class StreamingKVCache:
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
              softmax_scale: Optional[float] = None) -> torch.Tensor:
         """One decode step: append the new tokens' K / V, then attend with q."""
-        if (self.k_scale is not None or self._prefix is not None) and q.dim() == 4 and k.dim() == 4 \
-                and 1 <= q.shape[2] == k.shape[2] <= self.max_query:
-            # the tokens are written by the launch that attends them
-            self._check_tokens("q", q, grouped=True)
-            self._check_tokens("k", k)
-            self._check_tokens("v", v)
-            if k.shape != v.shape:
+        if self.k_scale is not None or self._prefix is not None:
+            n = self._check_tokens("q", q, grouped=True)
+            n_k = self._check_tokens("k", k)
+            if n_k != self._check_tokens("v", v):
                 raise ValueError("k and v must share shape")
-            scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
-            n = int(q.shape[2])
-            o = self._attend_streams(_aligned(q), n, scale, False, (_aligned(k), _aligned(v)))
-            self.length += n
-            return o
+            if 1 <= n == n_k <= self.max_query:      # the tokens are written by the launch that attends them
+                scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
+                o = self._attend_streams(_aligned(q), n, scale, False, (_aligned(k), _aligned(v)))
+                self.length += n
+                return o
         self.append(k, v)
         return self.attend(q, softmax_scale)
