@@ -692,7 +692,8 @@ int gki_rolling_step(const void* q, const void* k_new, const void* v_new, void* 
 
 int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
                      int32_t head_dim) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0 || !cross_as_streams(dtype, head_dim, H / H_kv, n_q))
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0 ||
+      !cross_as_streams(dtype, head_dim, B, H, H_kv, n_q, n_kv))
     return 0;
   return gki_stream_splits(dtype, B, H, H_kv, n_q, head_dim, n_kv);
 }

@@ -928,9 +928,25 @@ inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
 }
 
 // Does a cross attention run its query rows as streams (a whole group's rows against
-// each read of K and V) or as q tiles of each head? 16-bit, head_dim 64 or 128.
-inline bool cross_as_streams(int dtype, int head_dim, int group, int n_q) {
-  return dtype != kF32 && (head_dim == 64 || head_dim == 128) && (int64_t)group * n_q <= 32;
+// slices of its keys, 32 a workgroup) or as 128-row q tiles of each head? Streams take
+// 16 bits and head_dim 64 or 128: up to 32 rows always, more where the tiles are too few
+// or too empty for the card. Both times are estimated in tokens that a stream's
+// workgroup walks: n_kv / slices, times the rounds of 512 (head_dim 128: 256)
+// workgroups, and 700 (500) for the join; a tile walks a token in 0.5 (0.62) of that,
+// in rounds of 128 tiles. us, tiles / streams, of 8192 keys and of 1500:
+//   D64   H8 n_q 64, 512       46.1, 46.7 / 16.5, 33.1     12.5, 12.6 / 13.7, 15.2
+//         H32/8 n_q 256        47.0 / 53.4                 13.0 / 19.9
+//         B8 H32/8 n_q 16, 64  85.0, 72.7 / 32.9, 90.8     20.7, 19.3 / 15.3, 23.0
+//   D128  H8 n_q 64, 512       74.5, 77.5 / 18.9, 64.1     18.8, 19.3 / 15.1, 22.4
+//         B8 H32/8 n_q 32, 128  135, 151 / 114, 265        29.4, 32.3 / 27.8, 64.2
+inline bool cross_as_streams(int dtype, int head_dim, int64_t B, int64_t H, int64_t H_kv, int64_t n_q, int64_t n_kv) {
+  const int64_t rows = H / H_kv * n_q, workgroups = B * H_kv * ((rows + 31) / 32), tiles = B * H * ((n_q + 127) / 128);
+  if (dtype == kF32 || (head_dim != 64 && head_dim != 128)) return false;
+  if (rows <= 32) return true;
+  const int64_t slices = stream_splits(head_dim, workgroups, n_kv), round = head_dim == 64 ? 512 : 256;
+  const double streams = (double)n_kv / slices * std::max(1.0, (double)workgroups * slices / round) +
+                         (slices > 1 ? (head_dim == 64 ? 700 : 500) : 0);
+  return streams < (head_dim == 64 ? 0.5 : 0.62) * n_kv * std::max(1.0, (double)tiles / 128);
 }
 
 // Parts that a dense walk of dK/dV is cut into: each of `columns` kv tiles (over all

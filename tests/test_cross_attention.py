@@ -53,6 +53,8 @@ def test_c_entries_refuse_before_launch():
 def test_launch_rules():
     lib = _lib.load()
     assert lib.gki_cross_splits(2, 1, 4, 1, 2**29, 2000, 64) == 0         # group * n_q past 31 bits
+    assert lib.gki_cross_splits(2, 1, 8, 8, 200, 8000, 128) > 1           # few tiles, long keys: streams
+    assert lib.gki_cross_splits(2, 16, 16, 16, 200, 8000, 128) == 0
     assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 64) >= 1          # a step: streams
     assert lib.gki_cross_splits(0, 16, 16, 16, 1, 2000, 64) == 0          # fp32: q tiles
     assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 32) == 0
@@ -157,6 +159,7 @@ def test_forward_and_gradients(dtype, head_dim, H, H_kv, n_q, n_kv, lengths):
     (3, 16, 16, 700, 500, 64),      # grids past the ones whose tiles share their keys
     (2, 32, 4, 600, 1500, 128), (1, 4, 1, 3000, 100, 32),    # long walks of few kv tiles: cut into parts
     (1, 2, 2, 5000, 130, 128), (9, 16, 8, 130, 640, 16),
+    (2, 8, 1, 37, 3000, 128), (1, 2, 2, 333, 5000, 64), (8, 16, 2, 5, 1700, 128),    # few tiles: streams of several row tiles
 ])
 def test_larger_grids(dtype, B, H, H_kv, n_q, n_kv, D):
     q, k, v, do = _inputs(B, H, H_kv, n_q, n_kv, D, dtype, seed=7)
