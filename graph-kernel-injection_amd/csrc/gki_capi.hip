@@ -59,7 +59,7 @@ int attend8_dispatch(int dtype, int head_dim, const Geom& g, const void* q, cons
                      const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new, void* o, float* lse,
                      int ring, float* ws, int n_splits, hipStream_t stream);
 int cross_fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
-                       float* lse, hipStream_t stream);
+                       float* lse, float* ws, int n_slices, hipStream_t stream);
 int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
                           float* lse, float* ws, int n_splits, hipStream_t stream);
 int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
@@ -692,9 +692,12 @@ int gki_rolling_step(const void* q, const void* k_new, const void* v_new, void* 
 
 int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
                      int32_t head_dim) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0 ||
-      !cross_as_streams(dtype, head_dim, B, H, H_kv, n_q, n_kv))
-    return 0;
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0) return 0;
+  if (dtype == kF32) {
+    const int n = f32_slices(head_dim, (int64_t)B * H, n_q, n_kv);
+    return n > 1 ? n : 0;
+  }
+  if (!cross_as_streams(dtype, head_dim, B, H, H_kv, n_q, n_kv)) return 0;
   return gki_stream_splits(dtype, B, H, H_kv, n_q, head_dim, n_kv);
 }
 
@@ -706,16 +709,17 @@ int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* l
   GKI_REQUIRE(q && k && v && o && lse, 1, "gki_cross_fwd: null pointer");
   GKI_REQUIRE(all_aligned16(q, k, v, o, workspace), 1, "gki_cross_fwd: q, k, v, o and the workspace must be 16-byte aligned");
   const int tm = fwd_tile_m(dtype);
-  if (n_splits == 0) {
-    GKI_REQUIRE((int64_t)((n_q + tm - 1) / tm) * B * H < (1ll << 24), 1, "gki_cross_fwd: grid too large");
-    return cross_fwd_dispatch(dtype, head_dim, g, q, k, v, o, lse, (hipStream_t)stream);
+  GKI_REQUIRE(n_splits >= 0, 1, "gki_cross_fwd: n_splits must not be negative");
+  GKI_REQUIRE(n_splits <= 1 || workspace, 1, "gki_cross_fwd: null workspace");
+  if (n_splits == 0 || dtype == kF32) {
+    const int64_t units = (int64_t)((n_q + tm - 1) / tm) * B * H;
+    GKI_REQUIRE(units < (1ll << 24) && (n_splits <= 1 || units < (1ll << 21) / n_splits), 1, "gki_cross_fwd: grid too large");
+    return cross_fwd_dispatch(dtype, head_dim, g, q, k, v, o, lse, workspace, n_splits, (hipStream_t)stream);
   }
-  GKI_REQUIRE(dtype != kF32 && (head_dim == 64 || head_dim == 128), 2,
-              "gki_cross_fwd: streams take fp16 or bf16 and head_dim 64 or 128");
-  GKI_REQUIRE(n_splits > 0 && (int64_t)g.group * n_q < (1ll << kPartialBit) &&
+  GKI_REQUIRE(head_dim >= 32, 2, "gki_cross_fwd: streams take head_dim 32, 64 or 128");
+  GKI_REQUIRE((int64_t)g.group * n_q < (1ll << kPartialBit) &&
                   (int64_t)n_splits * B * H_kv * ((g.group * (int64_t)n_q + 15) / 16) < (1ll << 23), 1,
-              "gki_cross_fwd: n_splits must not be negative and the grid must fit");
-  GKI_REQUIRE(n_splits == 1 || workspace, 1, "gki_cross_fwd: null workspace");
+              "gki_cross_fwd: the grid must fit");
   return cross_stream_dispatch(dtype, head_dim, g, q, k, v, o, lse, workspace, n_splits, (hipStream_t)stream);
 }
 

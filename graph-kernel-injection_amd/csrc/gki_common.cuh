@@ -608,6 +608,13 @@ struct SharedRows {
   __device__ inline size_t row(int h, int r) const { return (size_t)h * rb + (size_t)(r / rb) * q_stride + r % rb; }
 };
 
+// Slices of a q tile's keys (fp32 cross attention of few rows), whose states are joined:
+// acc [rows][n][D], ml [rows][n][2].
+struct KeySlices {
+  int n = 1;
+  float *acc = nullptr, *ml = nullptr;
+};
+
 // Work list of the dK / dV grid (built on the host by gki_dkdv_items). A kv
 // tile's walk -- group x (its kept q tiles) iterations, iteration i visiting
 // list entry i % L of q head i / L -- is cut into items of at most a chunk of
@@ -927,9 +934,32 @@ inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
   return (int)std::max<int64_t>(1, std::min((256 + n_workgroups - 1) / n_workgroups, most));
 }
 
+// fp32 cross attention: workgroups per 64-row tile of `rows` = 16 QB rows each. A lone
+// short tile has only those that hold rows (empty ones, which leave at once, would take
+// their turn among the CUs: one query of 8 heads over 8192 keys in slices 31.7 -> 18.2 us).
+__host__ __device__ inline int f32_tile_parts(int n_q, int rows) {
+  return n_q >= kTileM ? kTileM / rows : (n_q + rows - 1) / rows;
+}
+// 16-row blocks that hold rows, and the blocks per workgroup for as many tiles.
+inline int64_t f32_full_blocks(int64_t BH, int64_t n_q) { return BH * ((n_q + 15) / 16); }
+inline int f32_dense_row_blocks(int head_dim, int64_t BH, int64_t n_q, int kv_tiles) {
+  return f32_row_blocks(head_dim, (int)((f32_full_blocks(BH, n_q) + 3) / 4), kv_tiles);
+}
+// Slices of the keys for an fp32 forward of few rows: as many as run at once beside the
+// one-block workgroups, of three kv tiles or more, where they shorten the walk (1.9 us a
+// kv tile at head_dim 128, 1.0 at 64) by three or four times the join. One query, D64 / D128:
+// 8 heads over 8192 keys 134, 246 -> 18.2, 21.9 us; over 2000, 8 batches of 16 heads (D64)
+// and of 32 of 8 (D128: one slice) 54.9, 158 -> 26.4, 70.4.
+inline int f32_slices(int head_dim, int64_t BH, int64_t n_q, int64_t n_kv) {
+  const int64_t kv_tiles = (n_kv + kTileN - 1) / kTileN, blocks = f32_full_blocks(BH, n_q);
+  const int64_t n = std::min((head_dim >= 128 ? 256 : head_dim == 64 ? 512 : 1024) / blocks, kv_tiles / 3);
+  if (n < 2 || kv_tiles - (kv_tiles + n - 1) / n < (head_dim >= 128 ? 8 : head_dim == 64 ? 16 : 24)) return 1;
+  return (int)n;
+}
+
 // Does a cross attention run its query rows as streams (a whole group's rows against
 // slices of its keys, 32 a workgroup) or as 128-row q tiles of each head? Streams take
-// 16 bits and head_dim 64 or 128: up to 32 rows always, more where the tiles are too few
+// 16 bits and head_dim 32 or more: up to 32 rows always, more where the tiles are too few
 // or too empty for the card. Both times are estimated in tokens that a stream's
 // workgroup walks: n_kv / slices, times the rounds of 512 (head_dim 128: 256)
 // workgroups, and 700 (500) for the join; a tile walks a token in 0.5 (0.62) of that,
@@ -941,12 +971,12 @@ inline int prefix_splits(int64_t n_workgroups, int64_t n_keys) {
 //         B8 H32/8 n_q 32, 128  135, 151 / 114, 265        29.4, 32.3 / 27.8, 64.2
 inline bool cross_as_streams(int dtype, int head_dim, int64_t B, int64_t H, int64_t H_kv, int64_t n_q, int64_t n_kv) {
   const int64_t rows = H / H_kv * n_q, workgroups = B * H_kv * ((rows + 31) / 32), tiles = B * H * ((n_q + 127) / 128);
-  if (dtype == kF32 || (head_dim != 64 && head_dim != 128)) return false;
+  if (dtype == kF32 || head_dim < 32) return false;
   if (rows <= 32) return true;
-  const int64_t slices = stream_splits(head_dim, workgroups, n_kv), round = head_dim == 64 ? 512 : 256;
+  const int64_t slices = stream_splits(head_dim, workgroups, n_kv), round = head_dim < 128 ? 512 : 256;
   const double streams = (double)n_kv / slices * std::max(1.0, (double)workgroups * slices / round) +
-                         (slices > 1 ? (head_dim == 64 ? 700 : 500) : 0);
-  return streams < (head_dim == 64 ? 0.5 : 0.62) * n_kv * std::max(1.0, (double)tiles / 128);
+                         (slices > 1 ? (head_dim < 128 ? 700 : 500) : 0);
+  return streams < (head_dim < 128 ? 0.5 : 0.62) * n_kv * std::max(1.0, (double)tiles / 128);
 }
 
 // Parts that a dense walk of dK/dV is cut into: each of `columns` kv tiles (over all

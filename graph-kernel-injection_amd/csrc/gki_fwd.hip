@@ -36,6 +36,7 @@
 // the LDS reads per flop, two waves per SIMD, every product slotted between
 // softmax operations by hand) ran 6% (head_dim 64) and 28% (128) slower.
 // The fp32 path uses v_mfma_f32_16x16x4f32 on 64-row tiles (16 rows per wave).
+#include "gki_join.cuh"
 #include "gki_rows16.cuh"
 
 namespace gki {
@@ -248,7 +249,7 @@ template <int D, int QB, bool DENSE>
 __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 1 ? 4 : 2) >= 256 ? 2 : 3) void fwd_kernel_32(
     Geom g, const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     float* __restrict__ O, float* __restrict__ LSE, const int32_t* __restrict__ row_ptr,
-    const int32_t* __restrict__ row_idx, int n_qt, const int32_t* __restrict__ wg_order) {
+    const int32_t* __restrict__ row_idx, int n_qt, const int32_t* __restrict__ wg_order, KeySlices ks) {
   constexpr int DJ = D / 16;                 // 16-byte chunks of a row per lane; output tiles
   constexpr int KB = 4 / QB;                 // key shares
   constexpr int TR = KB == 4 ? 64 : 32;      // keys per staged step
@@ -260,12 +261,18 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
   __shared__ __align__(16) float sv[2][TR * D];
 
   int part;
-  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, KB, wg_order, part, entries_of<DENSE>(g));
+  int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H * (DENSE ? ks.n : 1), DENSE ? f32_tile_parts(g.n_q, 16 * QB) : KB,
+                        wg_order, part, entries_of<DENSE>(g));
   if (wg < 0) return;
+  int slice = 0;
+  if constexpr (DENSE) slice = wg % ks.n, wg /= ks.n;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
-  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
+  if constexpr (DENSE) {
+    if (qt * kTileM + 16 * part * QB >= g.n_q) return;     // blocks behind the last row
+    g.n_kv = own_keys(g, bh / g.H);
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = lane >> 4, col = lane & 15;
   const int share = wave / QB;
@@ -288,8 +295,9 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
   // the LSE of a 1024-key row 9% above one rounding (8% per 64 keys, now 6%)
   float m = kNegInf, l = 0.f, lc = 0.f;
 
-  const int e_beg = DENSE ? 0 : row_ptr[qt];
-  const int n_step = (DENSE ? kv_tiles_of(g) : row_ptr[qt + 1] - e_beg) * HALVES;
+  auto slice_end = [&](int x) { return ks.n == 1 ? x * kv_tiles_of(g) : (int)((int64_t)kv_tiles_of(g) * x / ks.n); };
+  const int e_beg = DENSE ? slice_end(slice) : row_ptr[qt];
+  const int n_step = ((DENSE ? slice_end(slice + 1) : row_ptr[qt + 1]) - e_beg) * HALVES;
   auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTileF32<D, TR> dma;
   dma.init(tid);
@@ -446,6 +454,20 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : D * (QB == 
           o[v][e][i] = a;
         }
   }
+  if constexpr (DENSE) {
+    if (ks.n > 1) {
+      if (my_q >= g.n_q) return;
+      const size_t state = ((size_t)bh * g.n_q + my_q) * ks.n + slice;
+#pragma unroll
+      for (int v = 0; v < DV; ++v)
+#pragma unroll
+        for (int e = 0; e < DE; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ks.acc[state * D + 64 * v + DE * (4 * grp + i) + e] = o[v][e][i];
+      if (grp == 0) *(float2*)(ks.ml + 2 * state) = make_float2(m, l);
+      return;
+    }
+  }
   const bool valid = l > 0.f;
   if (my_q < g.n_q) {
     const float den = valid ? l : 1.f;
@@ -484,18 +506,22 @@ void launch_fwd16(const Geom& g, const void* q, const void* k, const void* v, vo
 template <int D, bool DENSE>
 int launch_fwd(int dtype, const Geom& g, const void* q, const void* k, const void* v, void* o,
                float* lse, const int32_t* row_ptr, const int32_t* row_idx, int n_qt,
-               const int32_t* wg_order, hipStream_t stream) {
+               const int32_t* wg_order, const KeySlices& ks, hipStream_t stream) {
   const int grid = n_qt * g.B * g.H;
   if (dtype == kF32) {
 #define GKI_FWD32(QB)                                                                               \
-  hipLaunchKernelGGL((fwd_kernel_32<D, QB, DENSE>), dim3(work_parts_grid(grid, 4 / QB)), dim3(256), 0,     \
+  hipLaunchKernelGGL((fwd_kernel_32<D, QB, DENSE>),                                                 \
+                     dim3(work_parts_grid(grid * ks.n, DENSE ? f32_tile_parts(g.n_q, 16 * QB) : 4 / QB)), dim3(256), 0, \
                      stream, g, (const float*)q, (const float*)k, (const float*)v, (float*)o, lse,  \
-                     row_ptr, row_idx, n_qt, wg_order)
-    const int blocks = f32_row_blocks(D, grid, DENSE ? kv_tiles_of(g) : row_kv_tiles(g, kTileM));
+                     row_ptr, row_idx, n_qt, wg_order, ks)
+    const int blocks = ks.n > 1 ? 1 : DENSE ? f32_dense_row_blocks(D, g.B * g.H, g.n_q, kv_tiles_of(g))
+                                            : f32_row_blocks(D, grid, row_kv_tiles(g, kTileM));
     if (blocks == 1) GKI_FWD32(1);
     else if (blocks == 2) GKI_FWD32(2);
     else GKI_FWD32(4);
 #undef GKI_FWD32
+    if constexpr (DENSE)
+      if (ks.n > 1) launch_join<F32, D, true>(ks.acc, ks.ml, o, lse, (int64_t)g.B * g.H * g.n_q, ks.n, stream);
   } else if (dtype == kF16) {
     launch_fwd16<F16, D, DENSE>(g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
   } else {
@@ -512,19 +538,21 @@ int fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
                  void* o, float* lse, const int32_t* row_ptr, const int32_t* row_idx, int n_qt,
                  const int32_t* wg_order, hipStream_t stream) {
   switch (head_dim) {
-    case 16: return launch_fwd<16, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
-    case 32: return launch_fwd<32, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
-    case 64: return launch_fwd<64, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
-    case 128: return launch_fwd<128, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, stream);
+    case 16: return launch_fwd<16, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, KeySlices{}, stream);
+    case 32: return launch_fwd<32, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, KeySlices{}, stream);
+    case 64: return launch_fwd<64, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, KeySlices{}, stream);
+    case 128: return launch_fwd<128, false>(dtype, g, q, k, v, o, lse, row_ptr, row_idx, n_qt, wg_order, KeySlices{}, stream);
     default: return fail(2, "unsupported head_dim " + std::to_string(head_dim));
   }
 }
 
 int cross_fwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v, void* o,
-                       float* lse, hipStream_t stream) {
+                       float* lse, float* ws, int n_slices, hipStream_t stream) {
   const int tm = fwd_tile_m(dtype), n_qt = (g.n_q + tm - 1) / tm;
+  KeySlices ks;
+  if (n_slices > 1) ks = {n_slices, ws, ws + (size_t)g.B * g.H * g.n_q * n_slices * head_dim};
 #define GKI_CROSS_CASE(DD) \
-  case DD: return launch_fwd<DD, true>(dtype, g, q, k, v, o, lse, nullptr, nullptr, n_qt, nullptr, stream);
+  case DD: return launch_fwd<DD, true>(dtype, g, q, k, v, o, lse, nullptr, nullptr, n_qt, nullptr, ks, stream);
   switch (head_dim) {
     GKI_CROSS_CASE(16)
     GKI_CROSS_CASE(32)

@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <string>
 
+#include "gki_join.cuh"
 #include "gki_rows16.cuh"
 
 namespace gki {
@@ -794,43 +795,6 @@ __global__ __launch_bounds__(256, (kStreamWaves<T, D, 2>)) void prefix_streams_k
   else if (block < a.n_blocks) stream_rows<T, D, 2, false, false>(a, src, block, &sk[0][0], &sv[0][0]);
 }
 
-// The states of a row's n_parts slices joined: a wave per row.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ acc, const float* __restrict__ ml,
-                                                   typename T::storage* __restrict__ O, float* __restrict__ LSE,
-                                                   int64_t n_rows, int n_parts) {
-  constexpr int E = D / 64;                    // elements per lane
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= n_rows) return;
-  const float2* st = (const float2*)ml + row * n_parts;
-  const float* x = acc + row * n_parts * D + E * lane;
-  float M = kNegInf;
-#pragma unroll 4
-  for (int p = 0; p < n_parts; ++p) M = fmaxf(M, st[p].x);
-  const float Mu = M == kNegInf ? 0.f : M;
-  float L = 0.f, a[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) a[e] = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < n_parts; ++p) {
-    const float f = __builtin_amdgcn_exp2f(st[p].x - Mu);
-    L += st[p].y * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) a[e] += x[(size_t)p * D + e] * f;
-  }
-  typename T::storage* dst = O + row * D + E * lane;
-#pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = T::from_float(a[e] / (L == 0.f ? 1.f : L));
-  if (lane == 0) LSE[row] = L == 0.f ? 0.f : lse_natural(M, L);
-}
-
-template <typename T, int D>
-void launch_join(const StreamArgs& a, int64_t n_rows, hipStream_t stream) {
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, stream, a.acc, a.ml,
-                     (typename T::storage*)a.o, a.lse, n_rows, a.n_parts);
-}
-
 // A workgroup per 256 lanes of work, up to a grid whose lanes a launch can count.
 inline dim3 row_grid(int64_t lanes) { return dim3((unsigned)std::min<int64_t>((lanes + 255) / 256, 1 << 20)); }
 
@@ -871,14 +835,14 @@ void launch_streams(StreamArgs a, const Src& src, int n_streams, const AppendArg
 template <typename T, int D>
 int cross_stream(const StreamArgs& a, const DenseStream& src, int n_streams, hipStream_t stream) {
   launch_streams<T, D, false>(a, src, n_streams, AppendArgs{}, stream);
-  if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
+  if (a.n_parts > 1) launch_join<T, D, false>(a.acc, a.ml, a.o, a.lse, (int64_t)n_streams * a.rb, a.n_parts, stream);
   return check_launch("gki_cross_fwd");
 }
 
 template <typename T, int D>
 int attend8(const StreamArgs& a, const RingStream& src, int n_streams, const AppendArgs& ap, hipStream_t stream) {
   launch_streams<T, D, true>(a, src, n_streams, ap, stream);
-  if (a.n_parts > 1) launch_join<T, D>(a, (int64_t)n_streams * a.rb, stream);
+  if (a.n_parts > 1) launch_join<T, D, false>(a.acc, a.ml, a.o, a.lse, (int64_t)n_streams * a.rb, a.n_parts, stream);
   return check_launch("gki_rolling8_decode");
 }
 
@@ -925,7 +889,7 @@ int prefix_decode(const Geom& g, const StreamArgs& own, const RingStream& ring, 
   } else if (wide) GKI_PREFIX(2, false);
   else GKI_PREFIX(1, false);
 #undef GKI_PREFIX
-  launch_join<T, D>(own, (int64_t)g.B * g.H * g.n_q, stream);
+  launch_join<T, D, false>(own.acc, own.ml, own.o, own.lse, (int64_t)g.B * g.H * g.n_q, own.n_parts, stream);
   return check_launch("gki_rolling_prefix_decode");
 }
 
@@ -1042,9 +1006,12 @@ int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q,
   const DenseStream src{g.kv_len, g.n_kv, g.H_kv};
   const StreamArgs a = stream_args(g, q, k, v, nullptr, nullptr, o, lse, g.n_kv, ws, n_splits, head_dim);
   const int n = g.B * g.H_kv;
-  if (dtype == kF16)
-    return head_dim == 64 ? cross_stream<F16, 64>(a, src, n, stream) : cross_stream<F16, 128>(a, src, n, stream);
-  return head_dim == 64 ? cross_stream<BF16, 64>(a, src, n, stream) : cross_stream<BF16, 128>(a, src, n, stream);
+#define GKI_CROSS_STREAM(DD) \
+  return dtype == kF16 ? cross_stream<F16, DD>(a, src, n, stream) : cross_stream<BF16, DD>(a, src, n, stream)
+  if (head_dim == 32) GKI_CROSS_STREAM(32);
+  if (head_dim == 64) GKI_CROSS_STREAM(64);
+  GKI_CROSS_STREAM(128);
+#undef GKI_CROSS_STREAM
 }
 
 int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,

@@ -341,13 +341,14 @@ int gki_rolling_step(const void* q, const void* k_new, const void* v_new, void* 
  * LSE = 0 and zero gradients; keys past an entry's length are not read and have
  * zero gradients. Grouped-query heads as above. */
 
-/* Slices per K/V head for gki_cross_fwd: 0 where the rows run as q tiles. */
+/* Slices of the keys for gki_cross_fwd: 0 where a workgroup walks all keys of a q tile. */
 int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
                      int32_t head_dim);
 
-/* O and LSE (natural). n_splits 0: a workgroup per q tile and head. n_splits >= 1
- * (fp16 / bf16, head_dim 64 or 128): the group's rows of a K/V head against slices of
- * its keys, for few query rows; 16-byte aligned workspace of
+/* O and LSE (natural). n_splits 0: a workgroup per q tile and head. n_splits >= 1, for
+ * few query rows: slices of the keys, against the group's rows of a K/V head (fp16 /
+ * bf16, head_dim 32, 64 or 128) or against a head's q tile (fp32), joined when there are
+ * several; 16-byte aligned workspace of
  * gki_stream_workspace_floats(B, H, n_q, head_dim, n_splits) floats. */
 int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int32_t dtype,
                   int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv, int32_t head_dim,

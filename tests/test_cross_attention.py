@@ -44,7 +44,7 @@ def test_c_entries_refuse_before_launch():
     assert fwd(dtype=9) == 2 and fwd(D=48) == 2 and fwd(H_kv=3) == 1 and fwd(n_q=0) == 1 and fwd(n_kv=0) == 1
     assert fwd(q=0) == 1 and fwd(q=20) == 1 and fwd(scale=math.nan) == 1 and fwd(splits=-1) == 1
     assert fwd(splits=2) == 1 and b"workspace" in lib.gki_last_error()
-    assert fwd(splits=1, dtype=0) == 2 and fwd(splits=1, D=32) == 2 and fwd(ws=20, splits=2) == 1
+    assert fwd(splits=2, dtype=0) == 1 and fwd(splits=1, D=16) == 2 and fwd(ws=20, splits=2) == 1
     assert fwd(n_kv=2**30) == 1
     assert bwd(dtype=9) == 2 and bwd(D=8) == 2 and bwd(H_kv=3) == 1 and bwd(dq=0) == 1 and bwd(dq=8) == 1
     assert bwd(parts=0) == 1 and bwd(parts=2) == 1 and bwd(partials=8) == 1 and bwd(scale=math.inf) == 1
@@ -56,8 +56,10 @@ def test_launch_rules():
     assert lib.gki_cross_splits(2, 1, 8, 8, 200, 8000, 128) > 1           # few tiles, long keys: streams
     assert lib.gki_cross_splits(2, 16, 16, 16, 200, 8000, 128) == 0
     assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 64) >= 1          # a step: streams
-    assert lib.gki_cross_splits(0, 16, 16, 16, 1, 2000, 64) == 0          # fp32: q tiles
-    assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 32) == 0
+    assert lib.gki_cross_splits(0, 16, 16, 16, 300, 2000, 64) == 0        # fp32: q tiles
+    assert lib.gki_cross_splits(0, 1, 8, 8, 1, 2000, 64) > 1              # or slices of their keys
+    assert lib.gki_cross_splits(0, 1, 8, 8, 1, 300, 64) == 0
+    assert lib.gki_cross_splits(2, 16, 16, 16, 1, 2000, 16) == 0
     assert lib.gki_cross_splits(2, 16, 16, 16, 500, 2000, 64) == 0
     for dtype in (0, 2):
         for n_q, n_kv, H, H_kv, D in ((1, 1, 1, 1, 16), (2048, 64, 32, 4, 128), (70000, 50, 8, 1, 64), (64, 8192, 4, 4, 32)):
@@ -170,16 +172,19 @@ def test_larger_grids(dtype, B, H, H_kv, n_q, n_kv, D):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
 @pytest.mark.parametrize("splits", [0, 1, 2, 5, 33])
 def test_single_tokens_at_any_number_of_slices(dtype, D, splits, monkeypatch):
+    if D == 16 and dtype != torch.float32:
+        splits = 0                                # no streams
+
     from gki import cross
 
     monkeypatch.setattr(cross, "_FWD_PLANS", {})
     lib = _lib.load()
     monkeypatch.setattr(lib, "gki_cross_splits", lambda *a: splits)
-    for H, H_kv, n_q, n_kv in ((4, 4, 1, 900), (8, 2, 2, 130), (16, 1, 2, 70), (20, 1, 4, 257), (5, 1, 1, 1)):
+    for H, H_kv, n_q, n_kv in ((4, 4, 1, 900), (8, 2, 2, 130), (16, 1, 2, 70), (20, 1, 4, 257), (5, 1, 1, 1), (2, 1, 70, 300)):
         q, k, v, _ = _inputs(3, H, H_kv, n_q, n_kv, D, dtype, seed=splits)
         n = torch.tensor([n_kv, n_kv // 2, 0], device=DEV)          # int64
         out = cross_attention(q, k, v, n, enable_gqa=True)
