@@ -99,6 +99,39 @@ __device__ inline KvItem kv_item_part_of(int b, int BH, int parts, const Geom& g
   return kv_item<DENSE>(g, w, wg - bh * w.n_items);
 }
 
+// Dense dQ walks in slices (KeySlices, acc [slice][B * H * n_q][D]): the first kv tile of
+// slice x, and where a slice's sums go.
+__device__ inline int slice_begin(const Geom& g, const KeySlices& s, int x) {
+  return s.n == 1 ? x * kv_tiles_of(g) : (int)((int64_t)kv_tiles_of(g) * x / s.n);
+}
+template <int D>
+__device__ inline float* slice_rows(const Geom& g, const KeySlices& s, int x) {
+  return s.acc + (size_t)x * g.B * g.H * g.n_q * D;
+}
+// The slices' sums added in order, compensated for fp32, four elements a thread; bound
+// by L2, which still holds them. Forward + backward of 64 rows of 8 heads over 8192 keys,
+// D128 bf16: 155 -> 77 us; 4 heads over 4096, fp32: 224 -> 78.
+template <typename T>
+__global__ __launch_bounds__(256) void dq_reduce_kernel(KeySlices s, int64_t n, typename T::storage* __restrict__ dQ) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  floatx4 sum = floatx4{0.f, 0.f, 0.f, 0.f}, comp = sum;
+#pragma unroll 4
+  for (int x = 0; x < s.n; ++x) {
+    const floatx4 y = *(const floatx4*)(s.acc + (size_t)x * n + i) - comp, t = sum + y;
+    if constexpr (T::is_f32) comp = (t - sum) - y;
+    sum = t;
+  }
+  if constexpr (T::is_f32) *(floatx4*)(dQ + i) = sum;
+  else *(uint2*)(dQ + i) = make_uint2(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]));
+}
+template <typename T>
+void launch_dq_reduce(const KeySlices& s, const Geom& g, int head_dim, void* dq, hipStream_t stream) {
+  const int64_t n = (int64_t)g.B * g.H * g.n_q * head_dim;
+  hipLaunchKernelGGL((dq_reduce_kernel<T>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, stream, s, n,
+                     (typename T::storage*)dq);
+}
+
 // Sum of a split column's fp32 partials, in item order, cast to the storage
 // type. A split column's 2 x 64 x D partial floats (dK then dV) are spread
 // over D / 8 workgroups, one float4 per thread; the loads of four partials are
@@ -888,7 +921,7 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ O, const uint16_t* __restrict__ dO,
     uint16_t* __restrict__ dQ, const float* __restrict__ LSE, float* __restrict__ Delta,
     const int32_t* __restrict__ row_ptr, const int32_t* __restrict__ row_idx, int n_qt,
-    const int32_t* __restrict__ dq_order) {
+    const int32_t* __restrict__ dq_order, KeySlices slices) {
   constexpr bool ROW = FORM != kBwdPlain, PRE = FORM == kBwdPre;
   constexpr int kAhead = 4;                    // operands read ahead
   constexpr int KS = D / 16;
@@ -898,8 +931,10 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
   __shared__ __align__(16) uint16_t stile[LDS16];      // K, K, V, V; the waves' sums at the end
 
   const int n_wg = n_qt * g.B * g.H;
-  const int wg = work_of(blockIdx.x, n_wg, dq_order, entries_of<DENSE>(g));
+  int wg = work_of(blockIdx.x, n_wg * (DENSE ? slices.n : 1), dq_order, entries_of<DENSE>(g));
   if (wg < 0) return;
+  int slice = 0;
+  if constexpr (DENSE) slice = wg % slices.n, wg /= slices.n;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
@@ -946,7 +981,7 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
       if constexpr (FORM == kBwdRow) qf[ks] = and4(qf[ks], g.q_and);
       if constexpr (PRE) df[ks] = scale8<T>(df[ks], g.scale);
     }
-    if (ok && hi == 0 && kh == 0) {            // the two kv-half waves hold the same rows
+    if (ok && hi == 0 && kh == 0 && slice == 0) {   // the two kv-half waves (and the slices) hold the same rows
       Delta[(size_t)bh * g.n_q + my_q] = ndlt;
       Delta[(size_t)g.B * g.H * g.n_q + (size_t)bh * g.n_q + my_q] = lse2;
     }
@@ -955,7 +990,8 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
 #pragma unroll
   for (int i = 0; i < DT; ++i) dq[i] = splat16(0.f);
 
-  const int e_beg = DENSE ? 0 : row_ptr[qt], e_end = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1];
+  const int e_beg = DENSE ? slice_begin(g, slices, slice) : row_ptr[qt];
+  const int e_end = DENSE ? slice_begin(g, slices, slice + 1) : row_ptr[qt + 1];
   auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTile<D, 4, true> dma;
   dma.init(tid);
@@ -1041,6 +1077,13 @@ __global__ __launch_bounds__(256, D > 64 ? 2 : 4) void dq_kernel_16(
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = dq[dt][4 * q + i] + r[i];
+      if constexpr (DENSE) {
+        if (slices.n > 1) {
+          float* dst = slice_rows<D>(g, slices, slice) + qb + (size_t)my_q * D + 32 * dt + 8 * q + 4 * hi_e;
+          *(floatx4*)dst = floatx4{v[0], v[1], v[2], v[3]};
+          continue;
+        }
+      }
       *(uint2*)(dQ + qb + (size_t)my_q * D + 32 * dt + 8 * q + 4 * hi_e) =
           make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     }
@@ -1061,14 +1104,16 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
     const uint16_t* __restrict__ V, const uint16_t* __restrict__ O, const uint16_t* __restrict__ dO,
     uint16_t* __restrict__ dQ, const float* __restrict__ LSE, float* __restrict__ Delta,
     const int32_t* __restrict__ row_ptr, const int32_t* __restrict__ row_idx, int n_qt,
-    const int32_t* __restrict__ dq_order) {
+    const int32_t* __restrict__ dq_order, KeySlices slices) {
   constexpr int D = 64, KS = 2, DT = 4;
   __shared__ __align__(16) uint16_t sk[2][64 * D];
   __shared__ __align__(16) uint16_t sv[2][64 * D];
 
   const int n_wg = n_qt * g.B * g.H;
-  const int wg = work_of(blockIdx.x, n_wg, dq_order, entries_of<DENSE>(g));
+  int wg = work_of(blockIdx.x, n_wg * (DENSE ? slices.n : 1), dq_order, entries_of<DENSE>(g));
   if (wg < 0) return;
+  int slice = 0;
+  if constexpr (DENSE) slice = wg % slices.n, wg /= slices.n;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
@@ -1106,7 +1151,7 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) df[b][ks] = scale8<T>(df[b][ks], g.scale);
     }
-    if (ok && grp == 0 && kh == 0) {     // the two kv-half waves hold the same rows
+    if (ok && grp == 0 && kh == 0 && slice == 0) {     // the two kv-half waves (and the slices) hold the same rows
       Delta[(size_t)bh * g.n_q + my_q] = ndlt[b];
       Delta[(size_t)g.B * g.H * g.n_q + (size_t)bh * g.n_q + my_q] = lse2[b];
     }
@@ -1118,7 +1163,8 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
 #pragma unroll
     for (int i = 0; i < DT; ++i) dq[b][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int e_beg = DENSE ? 0 : row_ptr[qt], e_end = DENSE ? kv_tiles_of(g) : row_ptr[qt + 1];
+  const int e_beg = DENSE ? slice_begin(g, slices, slice) : row_ptr[qt];
+  const int e_end = DENSE ? slice_begin(g, slices, slice + 1) : row_ptr[qt + 1];
   auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTile<D> dma;
   dma.init(tid);
@@ -1227,6 +1273,12 @@ __global__ __launch_bounds__(256, 4) void dq_kernel_q64(
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const floatx4 o = dq[b][dt] + red[(b * DT + dt) * 64 + lane_e];
+      if constexpr (DENSE) {
+        if (slices.n > 1) {
+          *(floatx4*)(slice_rows<D>(g, slices, slice) + qb + (size_t)my_q * D + 16 * dt + 4 * grp_e) = o;
+          continue;
+        }
+      }
       const uint2 w = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
       *(uint2*)(dQ + qb + (size_t)my_q * D + 16 * dt + 4 * grp_e) = w;
     }
@@ -1244,7 +1296,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
     Geom g, const float* __restrict__ Q, const float* __restrict__ K, const float* __restrict__ V,
     const float* __restrict__ O, const float* __restrict__ dO, float* __restrict__ dQ,
     const float* __restrict__ LSE, float* __restrict__ Delta, const int32_t* __restrict__ row_ptr,
-    const int32_t* __restrict__ row_idx, int n_qt, const int32_t* __restrict__ dq_order) {
+    const int32_t* __restrict__ row_idx, int n_qt, const int32_t* __restrict__ dq_order, KeySlices slices) {
   constexpr int DJ = D / 16;
   constexpr int KB = 4 / QB;
   constexpr int TR = KB == 4 ? 64 : 32;
@@ -1256,12 +1308,18 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
   __shared__ __align__(16) float sv[2][TR * D];
 
   int part;
-  const int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H, KB, dq_order, part, entries_of<DENSE>(g));
+  int wg = work_part_of(blockIdx.x, n_qt * g.B * g.H * (DENSE ? slices.n : 1), DENSE ? f32_tile_parts(g.n_q, 16 * QB) : KB,
+                        dq_order, part, entries_of<DENSE>(g));
   if (wg < 0) return;
+  int slice = 0;
+  if constexpr (DENSE) slice = wg % slices.n, wg /= slices.n;
   const int bh = wg / n_qt, qt = wg - bh * n_qt;
   const size_t qb = (size_t)bh * g.n_q * D;
   const size_t kb = (size_t)kv_bh(g, bh) * g.n_kv * D;
-  if constexpr (DENSE) g.n_kv = own_keys(g, bh / g.H);
+  if constexpr (DENSE) {
+    if (qt * kTileM + 16 * part * QB >= g.n_q) return;     // blocks behind the last row
+    g.n_kv = own_keys(g, bh / g.H);
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = lane >> 4, col = lane & 15;
   const int share = wave / QB;
@@ -1287,15 +1345,15 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
     for (int j = 0; j < n; ++j) part_d[j] += part_d[j + n];
   const float dlt = wave_sum16x4(part_d[0]);
   const float lse = my_q < g.n_q ? LSE[(size_t)bh * g.n_q + my_q] : 0.f;   // natural
-  if (my_q < g.n_q && grp == 0 && share == 0) Delta[(size_t)bh * g.n_q + my_q] = dlt;
+  if (my_q < g.n_q && grp == 0 && share == 0 && slice == 0) Delta[(size_t)bh * g.n_q + my_q] = dlt;
   floatx4 dq[DV][DE], cq[DV][DE];      // running sum and its compensation (two_sum_fold)
 #pragma unroll
   for (int v = 0; v < DV; ++v)
 #pragma unroll
     for (int e = 0; e < DE; ++e) dq[v][e] = cq[v][e] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int e_beg = DENSE ? 0 : row_ptr[qt];
-  const int n_step = (DENSE ? kv_tiles_of(g) : row_ptr[qt + 1] - e_beg) * HALVES;
+  const int e_beg = DENSE ? slice_begin(g, slices, slice) : row_ptr[qt];
+  const int n_step = ((DENSE ? slice_begin(g, slices, slice + 1) : row_ptr[qt + 1]) - e_beg) * HALVES;
   auto entry = [&](int e) { return walk_entry<DENSE>(row_idx, e); };
   DmaTileF32<D, TR> dma;
   dma.init(tid);
@@ -1404,7 +1462,7 @@ __global__ __launch_bounds__(256, D * (QB == 1 ? 4 : 2) >= 512 ? 1 : 2) void dq_
     for (int v = 0; v < DV; ++v)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float* dst = dQ + qb + (size_t)my_q * D + 64 * v + DE * (4 * grp + i);
+        float* dst = (DENSE && slices.n > 1 ? slice_rows<D>(g, slices, slice) : dQ) + qb + (size_t)my_q * D + 64 * v + DE * (4 * grp + i);
         if constexpr (DE == 4) {
           *(floatx4*)dst = floatx4{dq[v][0][i], dq[v][1][i], dq[v][2][i], dq[v][3][i]};
         } else {
@@ -1421,21 +1479,22 @@ template <typename T, int D, int FORM, bool DENSE>
 void launch_bwd16_as(const Geom& g, const void* q, const void* k, const void* v, const void* o,
                      const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                      const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* dq_order,
-                     const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, hipStream_t stream) {
+                     const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, const KeySlices& slices,
+                     hipStream_t stream) {
   const int BH = g.B * g.H, BHkv = g.B * g.H_kv;
   const float* lse2 = delta + (size_t)BH * g.n_q;
   if constexpr (D == 64) {
     constexpr bool PRE = FORM == kBwdPre;
-    hipLaunchKernelGGL((dq_kernel_q64<T, PRE, DENSE>), dim3(n_qt * BH), dim3(256), 0, stream, g,
+    hipLaunchKernelGGL((dq_kernel_q64<T, PRE, DENSE>), dim3(n_qt * BH * slices.n), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o,
-                       (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order);
+                       (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order, slices);
     hipLaunchKernelGGL((dkdv_kernel_q64<T, PRE, DENSE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout,
                        (uint16_t*)dk, (uint16_t*)dv, lse2, delta, col_ptr, col_idx, w);
   } else {
-    hipLaunchKernelGGL((dq_kernel_16<T, D, FORM, DENSE>), dim3(n_qt * BH), dim3(256), 0, stream, g,
+    hipLaunchKernelGGL((dq_kernel_16<T, D, FORM, DENSE>), dim3(n_qt * BH * slices.n), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o,
-                       (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order);
+                       (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order, slices);
     hipLaunchKernelGGL((dkdv_kernel_16<T, D, FORM, DENSE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout,
                        (uint16_t*)dk, (uint16_t*)dv, lse2, delta, col_ptr, col_idx, w);
@@ -1446,10 +1505,11 @@ template <typename T, int D, bool DENSE>
 void launch_bwd16(const Geom& g, const void* q, const void* k, const void* v, const void* o,
                   const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                   const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* dq_order,
-                  const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, hipStream_t stream) {
+                  const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, const KeySlices& slices,
+                  hipStream_t stream) {
 #define GKI_BWD16(FORM)                                                                             \
   launch_bwd16_as<T, D, FORM, DENSE>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,  \
-                              dq_order, col_ptr, col_idx, w, stream)
+                              dq_order, col_ptr, col_idx, w, slices, stream)
   // head_dim 64 forms P by an fma of the base-2 LSE, so its first two forms are one
   if (g.bwd_form == kBwdPre) GKI_BWD16(kBwdPre);
   else if (g.bwd_form == kBwdRow && D != 64) GKI_BWD16((D != 64 ? kBwdRow : kBwdPlain));
@@ -1461,21 +1521,24 @@ template <int D, bool DENSE>
 int launch_bwd(int dtype, const Geom& g, const void* q, const void* k, const void* v, const void* o,
                const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
                const int32_t* row_ptr, const int32_t* row_idx, int n_qt, const int32_t* dq_order,
-               const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, hipStream_t stream) {
+               const int32_t* col_ptr, const int32_t* col_idx, const KvWork& w, const KeySlices& slices,
+               hipStream_t stream) {
   const int BH = g.B * g.H, BHkv = g.B * g.H_kv;
   const dim3 red_grid(w.n_split * BHkv * kReduceWgPerTile<D>);
   if (dtype == kF32) {
     // dQ first: it also writes Delta, which dK/dV reads
     const int qgrid = n_qt * BH, kgrid = w.n_items * BHkv;
 #define GKI_DQ32(QB)                                                                                \
-  hipLaunchKernelGGL((dq_kernel_32<D, QB, DENSE>), dim3(work_parts_grid(qgrid, 4 / QB)), dim3(256), 0,     \
-                     stream, g, (const float*)q, (const float*)k, (const float*)v, (const float*)o, \
-                     (const float*)dout, (float*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order)
+  hipLaunchKernelGGL((dq_kernel_32<D, QB, DENSE>),                                                  \
+                     dim3(work_parts_grid(qgrid * slices.n, DENSE ? f32_tile_parts(g.n_q, 16 * QB) : 4 / QB)), \
+                     dim3(256), 0, stream, g, (const float*)q, (const float*)k, (const float*)v, (const float*)o, \
+                     (const float*)dout, (float*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order, slices)
 #define GKI_DKDV32(KB)                                                                              \
   hipLaunchKernelGGL((dkdv_kernel_32<D, KB, DENSE>), dim3(work_parts_grid(kgrid, 4 / KB)), dim3(256), 0,   \
                      stream, g, (const float*)q, (const float*)k, (const float*)v,                  \
                      (const float*)dout, (float*)dk, (float*)dv, lse, delta, col_ptr, col_idx, w)
-    const int qblocks = f32_row_blocks(D, qgrid, DENSE ? kv_tiles_of(g) : row_kv_tiles(g, kTileM));
+    const int qblocks = slices.n > 1 ? 1 : DENSE ? f32_dense_row_blocks(D, BH, g.n_q, kv_tiles_of(g))
+                                                 : f32_row_blocks(D, qgrid, row_kv_tiles(g, kTileM));
     if (qblocks == 1) GKI_DQ32(1);
     else if (qblocks == 2) GKI_DQ32(2);
     else GKI_DQ32(4);
@@ -1490,16 +1553,23 @@ int launch_bwd(int dtype, const Geom& g, const void* q, const void* k, const voi
                          (float*)dk, (float*)dv);
   } else if (dtype == kF16) {
     launch_bwd16<F16, D, DENSE>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,
-                         dq_order, col_ptr, col_idx, w, stream);
+                         dq_order, col_ptr, col_idx, w, slices, stream);
     if (w.n_split > 0)
       hipLaunchKernelGGL((dkdv_reduce_kernel<F16, D, DENSE>), red_grid, dim3(256), 0, stream, g, w,
                          (uint16_t*)dk, (uint16_t*)dv);
   } else {
     launch_bwd16<BF16, D, DENSE>(g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx, n_qt,
-                          dq_order, col_ptr, col_idx, w, stream);
+                          dq_order, col_ptr, col_idx, w, slices, stream);
     if (w.n_split > 0)
       hipLaunchKernelGGL((dkdv_reduce_kernel<BF16, D, DENSE>), red_grid, dim3(256), 0, stream, g, w,
                          (uint16_t*)dk, (uint16_t*)dv);
+  }
+  if constexpr (DENSE) {
+    if (slices.n > 1) {
+      if (dtype == kF32) launch_dq_reduce<F32>(slices, g, D, dq, stream);
+      else if (dtype == kF16) launch_dq_reduce<F16>(slices, g, D, dq, stream);
+      else launch_dq_reduce<BF16>(slices, g, D, dq, stream);
+    }
   }
   return check_launch(DENSE ? "gki_cross_bwd" : "gki_bsa_bwd");
 }
@@ -1514,7 +1584,7 @@ int bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
 #define GKI_BWD_CASE(DD)                                                                          \
   case DD:                                                                                        \
     return launch_bwd<DD, false>(dtype, g, q, k, v, o, dout, lse, dq, dk, dv, delta, row_ptr, row_idx,   \
-                          n_qt, dq_order, col_ptr, col_idx, w, stream);
+                          n_qt, dq_order, col_ptr, col_idx, w, KeySlices{}, stream);
   switch (head_dim) {
     GKI_BWD_CASE(16)
     GKI_BWD_CASE(32)
@@ -1527,7 +1597,7 @@ int bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const vo
 
 int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                        const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
-                       int parts, float* partials, hipStream_t stream) {
+                       int parts, float* partials, int dq_slices, float* dq_sums, hipStream_t stream) {
   const int n_kt = kv_tiles_of(g);
   KvWork w{};
   w.parts = parts;
@@ -1537,7 +1607,7 @@ int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, co
 #define GKI_CROSS_CASE(DD)                                                                                 \
   case DD:                                                                                                 \
     return launch_bwd<DD, true>(dtype, g, q, k, v, o, dout, lse, dq, dk, dv, delta, nullptr, nullptr,      \
-                                (g.n_q + kTileM - 1) / kTileM, nullptr, nullptr, nullptr, w, stream);
+                                (g.n_q + kTileM - 1) / kTileM, nullptr, nullptr, nullptr, w, KeySlices{dq_slices, dq_sums, nullptr}, stream);
   switch (head_dim) {
     GKI_CROSS_CASE(16)
     GKI_CROSS_CASE(32)

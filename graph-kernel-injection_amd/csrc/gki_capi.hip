@@ -64,7 +64,7 @@ int cross_stream_dispatch(int dtype, int head_dim, const Geom& g, const void* q,
                           float* lse, float* ws, int n_splits, hipStream_t stream);
 int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                        const void* o, const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
-                       int parts, float* partials, hipStream_t stream);
+                       int parts, float* partials, int dq_slices, float* dq_sums, hipStream_t stream);
 int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q, const void* k, const void* v,
                            const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new,
                            const void* prefix_k, const void* prefix_v, int n_prefix, void* o, float* lse, int ring,
@@ -724,8 +724,10 @@ int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* l
 }
 
 int gki_cross_bwd_parts(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv,
-                        int32_t head_dim) {
+                        int32_t head_dim, int32_t* dq_slices) {
+  if (dq_slices) *dq_slices = 1;
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_kv <= 0) return 1;
+  if (dq_slices) *dq_slices = cross_dq_slices(dtype, head_dim, (int64_t)B * H, n_q, n_kv);
   const int64_t walk = ((int64_t)n_q + kTileM - 1) / kTileM * (H / H_kv);
   return cross_kv_parts(dtype, head_dim, walk, ((int64_t)n_kv + kTileN - 1) / kTileN * B * H_kv);
 }
@@ -733,19 +735,22 @@ int gki_cross_bwd_parts(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32
 int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
                   void* dq, void* dk, void* dv, float* delta, int32_t dtype, int32_t B, int32_t H, int32_t H_kv,
                   int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* kv_len, float softmax_scale,
-                  int32_t parts, float* kv_partials, void* stream) {
+                  int32_t parts, float* kv_partials, int32_t dq_slices, float* dq_sums, void* stream) {
   Geom g;
   if (int rc = cross_geom(g, dtype, B, H, H_kv, n_q, n_kv, head_dim, kv_len, softmax_scale)) return rc;
   GKI_REQUIRE(q && k && v && o && dout && lse && dq && dk && dv && delta, 1, "gki_cross_bwd: null tensor");
-  GKI_REQUIRE(all_aligned16(q, k, v, o, dout, dq, dk, dv, kv_partials), 1,
-              "gki_cross_bwd: q, k, v, o, dout, dq, dk, dv and kv_partials must be 16-byte aligned");
+  GKI_REQUIRE(all_aligned16(q, k, v, o, dout, dq, dk, dv, kv_partials, dq_sums), 1,
+              "gki_cross_bwd: q, k, v, o, dout, dq, dk, dv, kv_partials and dq_sums must be 16-byte aligned");
   GKI_REQUIRE(parts >= 1 && (parts == 1 || kv_partials), 1,
               "gki_cross_bwd: parts must be positive, and several need kv_partials");
+  GKI_REQUIRE(dq_slices >= 1 && (dq_slices == 1 || dq_sums), 1,
+              "gki_cross_bwd: dq_slices must be positive, and several need dq_sums");
   const int64_t n_qt = (n_q + kTileM - 1) / kTileM, n_kt = kv_tiles_of(g);
+  GKI_REQUIRE(dq_slices == 1 || (n_qt * B * H < (1ll << 21) / dq_slices), 1, "gki_cross_bwd: dQ grid too large");
   GKI_REQUIRE(n_qt * g.group < (1ll << 30) && n_qt * B * H < (1ll << 24) && n_kt * parts * B * H_kv < (1ll << 24) &&
                   (parts == 1 || n_kt * B * H_kv * (head_dim / 8) < (1ll << 24)), 1, "gki_cross_bwd: grid too large");
   return cross_bwd_dispatch(dtype, head_dim, g, q, k, v, o, dout, lse, dq, dk, dv, delta, parts, kv_partials,
-                            (hipStream_t)stream);
+                            dq_slices, dq_sums, (hipStream_t)stream);
 }
 
 int64_t gki_read_probe_words(int32_t bh) { return bh > 0 ? read_probe_words(bh) : 0; }

@@ -608,8 +608,8 @@ struct SharedRows {
   __device__ inline size_t row(int h, int r) const { return (size_t)h * rb + (size_t)(r / rb) * q_stride + r % rb; }
 };
 
-// Slices of a q tile's keys (fp32 cross attention of few rows), whose states are joined:
-// acc [rows][n][D], ml [rows][n][2].
+// Slices of a q tile's keys (cross attention of few rows): the fp32 forward's, whose states
+// are joined, acc [rows][n][D], ml [rows][n][2]; dQ's, whose sums are added.
 struct KeySlices {
   int n = 1;
   float *acc = nullptr, *ml = nullptr;
@@ -945,16 +945,27 @@ inline int64_t f32_full_blocks(int64_t BH, int64_t n_q) { return BH * ((n_q + 15
 inline int f32_dense_row_blocks(int head_dim, int64_t BH, int64_t n_q, int kv_tiles) {
   return f32_row_blocks(head_dim, (int)((f32_full_blocks(BH, n_q) + 3) / 4), kv_tiles);
 }
-// Slices of the keys for an fp32 forward of few rows: as many as run at once beside the
-// one-block workgroups, of three kv tiles or more, where they shorten the walk (1.9 us a
-// kv tile at head_dim 128, 1.0 at 64) by three or four times the join. One query, D64 / D128:
-// 8 heads over 8192 keys 134, 246 -> 18.2, 21.9 us; over 2000, 8 batches of 16 heads (D64)
-// and of 32 of 8 (D128: one slice) 54.9, 158 -> 26.4, 70.4.
+// Slices of the keys for an fp32 forward of few rows: to a workgroup per CU (two share its
+// matrix cores: 8 heads of 333 rows over 777 keys, D64, 20 -> 23 us in three), of three kv
+// tiles or more, where they shorten the walk (1.9 us a kv tile at head_dim 128, 1.0 at 64)
+// by twice the join. One query, D64 / D128: 8 heads over 8192 keys 134, 246 -> 14.7, 21.7
+// us; over 2000, 8 batches of 16 heads (D64) and of 32 on 8 (D128: one slice) 54.9, 158 ->
+// 26.1, 70.3.
 inline int f32_slices(int head_dim, int64_t BH, int64_t n_q, int64_t n_kv) {
   const int64_t kv_tiles = (n_kv + kTileN - 1) / kTileN, blocks = f32_full_blocks(BH, n_q);
-  const int64_t n = std::min((head_dim >= 128 ? 256 : head_dim == 64 ? 512 : 1024) / blocks, kv_tiles / 3);
-  if (n < 2 || kv_tiles - (kv_tiles + n - 1) / n < (head_dim >= 128 ? 8 : head_dim == 64 ? 16 : 24)) return 1;
+  const int64_t n = std::min((head_dim >= 64 ? 256 : 512) / blocks, kv_tiles / 3);
+  if (n < 2 || kv_tiles - (kv_tiles + n - 1) / n < (head_dim >= 128 ? 4 : head_dim == 64 ? 8 : 12)) return 1;
   return (int)n;
+}
+
+// The same for dQ: 16-bit workgroups of 64 rows to two a CU or fp32 ones of 16, four kv
+// tiles or more each.
+inline int cross_dq_slices(int dtype, int head_dim, int64_t BH, int64_t n_q, int64_t n_kv) {
+  const int64_t kv_tiles = (n_kv + kTileN - 1) / kTileN;
+  const int64_t blocks = dtype == kF32 ? f32_full_blocks(BH, n_q) : BH * ((n_q + kTileM - 1) / kTileM);
+  const int64_t room = dtype == kF32 && head_dim >= 64 ? 256 : 512;
+  const int64_t n = std::min(room / blocks, kv_tiles / 4), brief = dtype != kF32 ? 12 : head_dim >= 128 ? 4 : 8;
+  return n < 2 || kv_tiles - (kv_tiles + n - 1) / n < brief ? 1 : (int)n;
 }
 
 // Does a cross attention run its query rows as streams (a whole group's rows against
@@ -962,8 +973,8 @@ inline int f32_slices(int head_dim, int64_t BH, int64_t n_q, int64_t n_kv) {
 // 16 bits and head_dim 32 or more: up to 32 rows always, more where the tiles are too few
 // or too empty for the card. Both times are estimated in tokens that a stream's
 // workgroup walks: n_kv / slices, times the rounds of 512 (head_dim 128: 256)
-// workgroups, and 700 (500) for the join; a tile walks a token in 0.5 (0.62) of that,
-// in rounds of 128 tiles. us, tiles / streams, of 8192 keys and of 1500:
+// workgroups, and 700 (500) for the join; a tile walks a token in 0.5 (0.62, head_dim 32 0.7)
+// of that, in rounds of 128 tiles. us, tiles / streams, of 8192 keys and of 1500:
 //   D64   H8 n_q 64, 512       46.1, 46.7 / 16.5, 33.1     12.5, 12.6 / 13.7, 15.2
 //         H32/8 n_q 256        47.0 / 53.4                 13.0 / 19.9
 //         B8 H32/8 n_q 16, 64  85.0, 72.7 / 32.9, 90.8     20.7, 19.3 / 15.3, 23.0
@@ -976,7 +987,7 @@ inline bool cross_as_streams(int dtype, int head_dim, int64_t B, int64_t H, int6
   const int64_t slices = stream_splits(head_dim, workgroups, n_kv), round = head_dim < 128 ? 512 : 256;
   const double streams = (double)n_kv / slices * std::max(1.0, (double)workgroups * slices / round) +
                          (slices > 1 ? (head_dim < 128 ? 700 : 500) : 0);
-  return streams < (head_dim < 128 ? 0.5 : 0.62) * n_kv * std::max(1.0, (double)tiles / 128);
+  return streams < (head_dim == 32 ? 0.7 : head_dim == 64 ? 0.5 : 0.62) * n_kv * std::max(1.0, (double)tiles / 128);
 }
 
 // Parts that a dense walk of dK/dV is cut into: each of `columns` kv tiles (over all

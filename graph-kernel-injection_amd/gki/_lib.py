@@ -71,8 +71,9 @@ SIGNATURES = {
                          + [_c_i64, _c_float, _c_ptr, _c_int, _c_int, _c_ptr]),
     "gki_cross_splits": (ctypes.c_int, [_c_int] * 7),
     "gki_cross_fwd": (ctypes.c_int, [_c_ptr] * 5 + [_c_int] * 7 + [_c_ptr, _c_float, _c_ptr, _c_int, _c_ptr]),
-    "gki_cross_bwd_parts": (ctypes.c_int, [_c_int] * 7),
-    "gki_cross_bwd": (ctypes.c_int, [_c_ptr] * 10 + [_c_int] * 7 + [_c_ptr, _c_float, _c_int, _c_ptr, _c_ptr]),
+    "gki_cross_bwd_parts": (ctypes.c_int, [_c_int] * 7 + [_c_ptr]),
+    "gki_cross_bwd": (ctypes.c_int, [_c_ptr] * 10 + [_c_int] * 7 + [_c_ptr, _c_float, _c_int, _c_ptr, _c_int, _c_ptr,
+                                                                     _c_ptr]),
     "gki_read_probe_words": (ctypes.c_int64, [_c_int]),
     "gki_read_probe": (ctypes.c_int, [_c_ptr, _c_ptr, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_ptr,
                                       _c_i64, _c_ptr]),

@@ -11,6 +11,7 @@ There is no CPU or eager fallback: a missing library raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -21,13 +22,13 @@ from . import _lib
 from .ops import _DTYPE_CODE, _HEAD_DIMS, _aligned, _current_stream, _on_device
 
 # launch plans: (dtype, B, H, H_kv, n_q, n_kv, D) -> (slices, floats of the LSE rows, of
-# the slices' states) of a forward, (parts, floats of the row terms, of the parts' sums) of
-# a backward
+# the slices' states) of a forward, (parts of dK/dV, slices of dQ, floats of the row terms,
+# of the parts' sums, of the slices') of a backward
 _FWD_PLANS: dict = {}
 _BWD_PLANS: dict = {}
 
 
-def _planned(plans: dict, key: tuple, make) -> Tuple[int, int, int]:
+def _planned(plans: dict, key: tuple, make) -> Tuple[int, ...]:
     plan = plans.get(key)
     if plan is None:
         if len(plans) >= 4096:
@@ -43,11 +44,13 @@ def _make_fwd_plan(lib, dtype, B, H, H_kv, n_q, n_kv, D) -> Tuple[int, int, int]
     return splits, (rows + 63) & ~63 if states else rows, states     # the states 256-byte aligned
 
 
-def _make_bwd_plan(lib, dtype, B, H, H_kv, n_q, n_kv, D) -> Tuple[int, int, int]:
-    parts = int(lib.gki_cross_bwd_parts(dtype, B, H, H_kv, n_q, n_kv, D))
+def _make_bwd_plan(lib, dtype, B, H, H_kv, n_q, n_kv, D) -> Tuple[int, ...]:
+    slices = ctypes.c_int32()
+    parts = int(lib.gki_cross_bwd_parts(dtype, B, H, H_kv, n_q, n_kv, D, ctypes.byref(slices)))
     tile = _lib.tile_sizes()["tile_n"]
     sums = B * H_kv * -(-n_kv // tile) * parts * 2 * tile * D if parts > 1 else 0
-    return parts, (2 * B * H * n_q + 63) & ~63, sums
+    dq_sums = B * H * n_q * D * slices.value if slices.value > 1 else 0
+    return parts, slices.value, (2 * B * H * n_q + 63) & ~63, sums, dq_sums
 
 
 def _check(q, k, v, kv_lengths, enable_gqa) -> None:
@@ -77,9 +80,9 @@ def _check(q, k, v, kv_lengths, enable_gqa) -> None:
             raise ValueError(f"kv_lengths must live on {q.device}")
 
 
-def _forward(q, k, v, kv_lengths, scale):
-    """(o, lse rows and behind them the slices' states, key) of aligned inputs; key None:
-    nothing to compute."""
+def _forward(q, k, v, kv_lengths, scale, keep_lse=False):
+    """(o, lse rows, key) of aligned inputs; key None: nothing to compute. The slices'
+    states lie behind the rows, unless these are kept (``keep_lse``)."""
     B, H, n_q, D = q.shape
     n_kv = k.shape[2]
     o = torch.empty_like(q)
@@ -87,13 +90,17 @@ def _forward(q, k, v, kv_lengths, scale):
         return o.zero_(), torch.zeros(B * H * n_q, dtype=torch.float32, device=q.device), None
     key = (_DTYPE_CODE[q.dtype], B, H, k.shape[1], n_q, n_kv, D)
     splits, rows, states = _planned(_FWD_PLANS, key, _make_fwd_plan)
-    scratch = torch.empty(rows + states, dtype=torch.float32, device=q.device)
+    scratch = torch.empty(rows if keep_lse else rows + states, dtype=torch.float32, device=q.device)
     lse = scratch.data_ptr()
+    ws = lse + 4 * rows if states else 0
+    if keep_lse and states:
+        work = torch.empty(states, dtype=torch.float32, device=q.device)
+        ws = work.data_ptr()
     lib = _lib.load()
     with _on_device(q.device):
         rc = lib.gki_cross_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse, *key,
-            0 if kv_lengths is None else kv_lengths.data_ptr(), scale, lse + 4 * rows if states else 0, splits,
+            0 if kv_lengths is None else kv_lengths.data_ptr(), scale, ws, splits,
             _current_stream(q.device))
     if rc:
         _lib.check(rc, "gki_cross_fwd")
@@ -105,9 +112,7 @@ class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, kv_lengths, scale):  # type: ignore[override]
-        o, lse, key = _forward(q, k, v, kv_lengths, scale)
-        if key is not None and lse.numel() > o.numel() // o.shape[3]:
-            lse = lse[:o.numel() // o.shape[3]].clone()     # the states need not outlive the forward
+        o, lse, key = _forward(q, k, v, kv_lengths, scale, keep_lse=True)
         ctx.save_for_backward(q, k, v, o, lse, kv_lengths)
         ctx.call = key, scale
         return o
@@ -121,8 +126,8 @@ class _CrossAttention(torch.autograd.Function):
         if key is None:
             return dq.zero_(), dk.zero_(), dv.zero_(), None, None
         do = _aligned(do if do.dtype == q.dtype else do.to(q.dtype))
-        parts, terms, sums = _planned(_BWD_PLANS, key, _make_bwd_plan)
-        scratch = torch.empty(terms + sums, dtype=torch.float32, device=q.device)
+        parts, slices, terms, sums, dq_sums = _planned(_BWD_PLANS, key, _make_bwd_plan)
+        scratch = torch.empty(terms + sums + dq_sums, dtype=torch.float32, device=q.device)
         delta = scratch.data_ptr()
         lib = _lib.load()
         with _on_device(q.device):
@@ -130,7 +135,8 @@ class _CrossAttention(torch.autograd.Function):
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, *key,
                 0 if kv_lengths is None else kv_lengths.data_ptr(), scale, parts,
-                delta + 4 * terms if sums else 0, _current_stream(q.device))
+                delta + 4 * terms if sums else 0, slices, delta + 4 * (terms + sums) if dq_sums else 0,
+                _current_stream(q.device))
         if rc:
             _lib.check(rc, "gki_cross_bwd")
         return dq, dk, dv, None, None

@@ -355,19 +355,20 @@ int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* l
                   const int32_t* kv_len, float softmax_scale, float* workspace, int32_t n_splits,
                   void* stream);
 
-/* Parts per kv tile that gki_cross_bwd cuts dK/dV into for a full card (any
- * parts >= 1 is right). */
+/* Parts per kv tile that gki_cross_bwd cuts dK/dV into for a full card, and (dq_slices,
+ * may be NULL) slices of the keys for dQ; any >= 1 is right. */
 int gki_cross_bwd_parts(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
-                        int32_t n_kv, int32_t head_dim);
+                        int32_t n_kv, int32_t head_dim, int32_t* dq_slices);
 
 /* dQ, dK, dV (fully written) from the forward's O and LSE. delta: fp32
  * [2, B, H, n_q] workspace as in gki_bsa_bwd; kv_partials: 16-byte aligned fp32
- * workspace [B * H_kv][ceil(n_kv / 64) * parts][2][64][head_dim] when parts > 1. */
+ * workspace [B * H_kv][ceil(n_kv / 64) * parts][2][64][head_dim] when parts > 1;
+ * dq_sums: the same, [dq_slices][B * H * n_q][head_dim] when dq_slices > 1. */
 int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
                   const float* lse, void* dq, void* dk, void* dv, float* delta, int32_t dtype,
                   int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t n_kv, int32_t head_dim,
                   const int32_t* kv_len, float softmax_scale, int32_t parts, float* kv_partials,
-                  void* stream);
+                  int32_t dq_slices, float* dq_sums, void* stream);
 
 /* Measurement helper, no counterpart in the reference: reads exactly the K and V
  * bytes a single-position StreamingLLM decode step reads from a full cache --

@@ -37,9 +37,9 @@ def test_c_entries_refuse_before_launch():
     def fwd(q=16, o=16, dtype=2, H=4, H_kv=2, n_q=3, n_kv=9, D=64, scale=0.1, ws=0, splits=0):
         return lib.gki_cross_fwd(q, 16, 16, o, 16, dtype, 1, H, H_kv, n_q, n_kv, D, None, scale, ws, splits, null)
 
-    def bwd(dq=16, dtype=2, H_kv=2, n_kv=9, D=64, scale=0.1, parts=1, partials=0):
+    def bwd(dq=16, dtype=2, H_kv=2, n_kv=9, D=64, scale=0.1, parts=1, partials=0, slices=1, sums=0):
         return lib.gki_cross_bwd(16, 16, 16, 16, 16, 16, dq, 16, 16, 16, dtype, 1, 4, H_kv, 3, n_kv, D, None, scale,
-                                 parts, partials, null)
+                                 parts, partials, slices, sums, null)
 
     assert fwd(dtype=9) == 2 and fwd(D=48) == 2 and fwd(H_kv=3) == 1 and fwd(n_q=0) == 1 and fwd(n_kv=0) == 1
     assert fwd(q=0) == 1 and fwd(q=20) == 1 and fwd(scale=math.nan) == 1 and fwd(splits=-1) == 1
@@ -47,6 +47,7 @@ def test_c_entries_refuse_before_launch():
     assert fwd(splits=2, dtype=0) == 1 and fwd(splits=1, D=16) == 2 and fwd(ws=20, splits=2) == 1
     assert fwd(n_kv=2**30) == 1
     assert bwd(dtype=9) == 2 and bwd(D=8) == 2 and bwd(H_kv=3) == 1 and bwd(dq=0) == 1 and bwd(dq=8) == 1
+    assert bwd(slices=0) == 1 and bwd(slices=2) == 1 and bwd(sums=8) == 1 and bwd(slices=2**22, sums=16) == 1
     assert bwd(parts=0) == 1 and bwd(parts=2) == 1 and bwd(partials=8) == 1 and bwd(scale=math.inf) == 1
 
 
@@ -63,7 +64,10 @@ def test_launch_rules():
     assert lib.gki_cross_splits(2, 16, 16, 16, 500, 2000, 64) == 0
     for dtype in (0, 2):
         for n_q, n_kv, H, H_kv, D in ((1, 1, 1, 1, 16), (2048, 64, 32, 4, 128), (70000, 50, 8, 1, 64), (64, 8192, 4, 4, 32)):
-            parts = lib.gki_cross_bwd_parts(dtype, 1, H, H_kv, n_q, n_kv, D)
+            slices = ctypes.c_int32()
+            parts = lib.gki_cross_bwd_parts(dtype, 1, H, H_kv, n_q, n_kv, D, ctypes.byref(slices))
+            assert parts == lib.gki_cross_bwd_parts(dtype, 1, H, H_kv, n_q, n_kv, D, None)
+            assert 1 <= slices.value <= max(1, n_kv // 256)
             assert 1 <= parts <= max(1, -(-n_q // 64) * H // H_kv)
 
 
@@ -193,6 +197,26 @@ def test_single_tokens_at_any_number_of_slices(dtype, D, splits, monkeypatch):
         bound = _bounds(vals[:1], mags[:1], size, n_kv, dtype)[0]
         assert ((out.double() - vals[0]).abs() <= bound).all(), (H, H_kv, n_q, n_kv)
         assert not out[2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("parts,slices", [(1, 1), (2, 2), (3, 5), (7, 40)])
+def test_gradients_at_any_number_of_parts(dtype, D, parts, slices, monkeypatch):
+    from gki import cross
+
+    monkeypatch.setattr(cross, "_BWD_PLANS", {})
+
+    def cut(*a):
+        a[-1]._obj.value = slices
+        return parts
+
+    monkeypatch.setattr(_lib.load(), "gki_cross_bwd_parts", cut)
+    for H, H_kv, n_q, n_kv in ((2, 1, 3, 500), (3, 3, 130, 333), (2, 2, 20, 64)):
+        q, k, v, do = _inputs(3, H, H_kv, n_q, n_kv, D, dtype, seed=slices)
+        n = torch.tensor([n_kv, n_kv // 3, 0], dtype=torch.int32, device=DEV)
+        _compare(_run(q, k, v, do, n), q, k, v, do, n)
 
 
 @pytest.mark.gpu
