@@ -1488,6 +1488,7 @@ void launch_bwd16_as(const Geom& g, const void* q, const void* k, const void* v,
     hipLaunchKernelGGL((dq_kernel_q64<T, PRE, DENSE>), dim3(n_qt * BH * slices.n), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o,
                        (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order, slices);
+    if (DENSE && dk == nullptr) return;          // keys that need no gradient
     hipLaunchKernelGGL((dkdv_kernel_q64<T, PRE, DENSE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout,
                        (uint16_t*)dk, (uint16_t*)dv, lse2, delta, col_ptr, col_idx, w);
@@ -1495,6 +1496,7 @@ void launch_bwd16_as(const Geom& g, const void* q, const void* k, const void* v,
     hipLaunchKernelGGL((dq_kernel_16<T, D, FORM, DENSE>), dim3(n_qt * BH * slices.n), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)o,
                        (const uint16_t*)dout, (uint16_t*)dq, lse, delta, row_ptr, row_idx, n_qt, dq_order, slices);
+    if (DENSE && dk == nullptr) return;
     hipLaunchKernelGGL((dkdv_kernel_16<T, D, FORM, DENSE>), dim3(w.n_items * BHkv), dim3(256), 0, stream, g,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)dout,
                        (uint16_t*)dk, (uint16_t*)dv, lse2, delta, col_ptr, col_idx, w);
@@ -1543,9 +1545,11 @@ int launch_bwd(int dtype, const Geom& g, const void* q, const void* k, const voi
     else if (qblocks == 2) GKI_DQ32(2);
     else GKI_DQ32(4);
     const int kblocks = f32_kv_blocks(D, kgrid);
-    if (D <= 64 && kblocks == 1) GKI_DKDV32((D <= 64 ? 1 : 2));
-    else if (kblocks <= 2) GKI_DKDV32(2);
-    else GKI_DKDV32(4);
+    if (!DENSE || dk != nullptr) {
+      if (D <= 64 && kblocks == 1) GKI_DKDV32((D <= 64 ? 1 : 2));
+      else if (kblocks <= 2) GKI_DKDV32(2);
+      else GKI_DKDV32(4);
+    }
 #undef GKI_DQ32
 #undef GKI_DKDV32
     if (w.n_split > 0)
@@ -1602,7 +1606,7 @@ int cross_bwd_dispatch(int dtype, int head_dim, const Geom& g, const void* q, co
   KvWork w{};
   w.parts = parts;
   w.n_items = n_kt * parts;
-  if (parts > 1) w.n_split = n_kt, w.n_pslots = w.n_items;
+  if (parts > 1 && dk) w.n_split = n_kt, w.n_pslots = w.n_items;
   w.partials = partials;
 #define GKI_CROSS_CASE(DD)                                                                                 \
   case DD:                                                                                                 \

@@ -738,10 +738,10 @@ int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, co
                   int32_t parts, float* kv_partials, int32_t dq_slices, float* dq_sums, void* stream) {
   Geom g;
   if (int rc = cross_geom(g, dtype, B, H, H_kv, n_q, n_kv, head_dim, kv_len, softmax_scale)) return rc;
-  GKI_REQUIRE(q && k && v && o && dout && lse && dq && dk && dv && delta, 1, "gki_cross_bwd: null tensor");
+  GKI_REQUIRE(q && k && v && o && dout && lse && dq && delta && !dk == !dv, 1, "gki_cross_bwd: null tensor");
   GKI_REQUIRE(all_aligned16(q, k, v, o, dout, dq, dk, dv, kv_partials, dq_sums), 1,
               "gki_cross_bwd: q, k, v, o, dout, dq, dk, dv, kv_partials and dq_sums must be 16-byte aligned");
-  GKI_REQUIRE(parts >= 1 && (parts == 1 || kv_partials), 1,
+  GKI_REQUIRE(parts >= 1 && (parts == 1 || kv_partials || !dk), 1,
               "gki_cross_bwd: parts must be positive, and several need kv_partials");
   GKI_REQUIRE(dq_slices >= 1 && (dq_slices == 1 || dq_sums), 1,
               "gki_cross_bwd: dq_slices must be positive, and several need dq_sums");

@@ -3,8 +3,9 @@
 The second attention of an encoder-decoder layer. Every query row of batch entry ``b``
 sees the first ``kv_lengths[b]`` keys (all of them without lengths); nothing is causal
 and no mask is built: the kernels walk the tiles an entry has, forward (``gki_cross_fwd``)
-and backward (``gki_cross_bwd``). A decoder's step -- up to 32 query rows per K/V head
--- reads each key once for a whole group of heads, cut into slices that fill the card.
+and backward (``gki_cross_bwd``). Few query rows over long keys, a decoder's step among
+them, run against slices of the keys that fill the card; in 16 bits a whole group of
+heads shares each read of a key.
 
 There is no CPU or eager fallback: a missing library raises ``RuntimeError``.
 """
@@ -122,18 +123,21 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, do):  # type: ignore[override]
         q, k, v, o, lse, kv_lengths = ctx.saved_tensors
         key, scale = ctx.call
-        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        dq = torch.empty_like(q)
+        keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]     # a frozen encoder needs neither
+        dk, dv = (torch.empty_like(k), torch.empty_like(v)) if keys else (None, None)
         if key is None:
-            return dq.zero_(), dk.zero_(), dv.zero_(), None, None
+            return dq.zero_(), *((dk.zero_(), dv.zero_()) if keys else (None, None)), None, None
         do = _aligned(do if do.dtype == q.dtype else do.to(q.dtype))
         parts, slices, terms, sums, dq_sums = _planned(_BWD_PLANS, key, _make_bwd_plan)
+        sums = sums if keys else 0
         scratch = torch.empty(terms + sums + dq_sums, dtype=torch.float32, device=q.device)
         delta = scratch.data_ptr()
         lib = _lib.load()
         with _on_device(q.device):
             rc = lib.gki_cross_bwd(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, *key,
+                dq.data_ptr(), dk.data_ptr() if keys else 0, dv.data_ptr() if keys else 0, delta, *key,
                 0 if kv_lengths is None else kv_lengths.data_ptr(), scale, parts,
                 delta + 4 * terms if sums else 0, slices, delta + 4 * (terms + sums) if dq_sums else 0,
                 _current_stream(q.device))

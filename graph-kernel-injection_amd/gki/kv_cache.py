@@ -76,7 +76,8 @@ class StreamingKVCache:
     ``torch.float8_e4m3fn``. In 8 bits ``k_cache`` / ``v_cache`` are the codes and
     ``k_scale`` / ``v_scale`` (``float8_e8m0fnu``, ``[B, H, sink_size + ring_size]``)
     the rows' powers of two; infinities and NaN are stored as NaN, and tokens, queries
-    and outputs keep ``dtype``. No gradient flows through the cache.
+    and outputs keep ``dtype``. No gradient flows through the cache. A NaN or infinity among
+    the values reaches every query of the call that reads it, as in the sparse op.
     """
 
     def __init__(self, batch: int, heads: int, head_dim: int, spec: StreamingMaskSpec,

@@ -360,7 +360,7 @@ int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* l
 int gki_cross_bwd_parts(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q,
                         int32_t n_kv, int32_t head_dim, int32_t* dq_slices);
 
-/* dQ, dK, dV (fully written) from the forward's O and LSE. delta: fp32
+/* dQ, dK, dV (fully written) from the forward's O and LSE; dk and dv NULL: dQ alone. delta: fp32
  * [2, B, H, n_q] workspace as in gki_bsa_bwd; kv_partials: 16-byte aligned fp32
  * workspace [B * H_kv][ceil(n_kv / 64) * parts][2][64][head_dim] when parts > 1;
  * dq_sums: the same, [dq_slices][B * H * n_q][head_dim] when dq_slices > 1. */

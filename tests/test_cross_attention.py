@@ -48,6 +48,7 @@ def test_c_entries_refuse_before_launch():
     assert fwd(n_kv=2**30) == 1
     assert bwd(dtype=9) == 2 and bwd(D=8) == 2 and bwd(H_kv=3) == 1 and bwd(dq=0) == 1 and bwd(dq=8) == 1
     assert bwd(slices=0) == 1 and bwd(slices=2) == 1 and bwd(sums=8) == 1 and bwd(slices=2**22, sums=16) == 1
+    assert lib.gki_cross_bwd(16, 16, 16, 16, 16, 16, 16, 0, 16, 16, 2, 1, 4, 2, 3, 9, 64, None, 0.1, 1, 0, 1, 0, null) == 1
     assert bwd(parts=0) == 1 and bwd(parts=2) == 1 and bwd(partials=8) == 1 and bwd(scale=math.inf) == 1
 
 
@@ -351,6 +352,19 @@ def test_no_gradient_needed_once_differentiable_and_same_bits():
     (g,) = torch.autograd.grad(out, leaf, do, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 50, 200), (128, 300, 130), (32, 5, 3000), (64, 5, 0)])
+def test_gradients_of_some_inputs_only(dtype, D, n_q, n_kv):
+    q, k, v, do = _inputs(2, 4, 2, n_q, n_kv, D, dtype, seed=19)
+    full = _run(q, k, v, do, None)
+    for wanted in ((0,), (1,), (2,), (0, 2)):
+        leaves = [t.detach().clone().requires_grad_(i in wanted) for i, t in enumerate((q, k, v))]
+        out = cross_attention(*leaves, enable_gqa=True)
+        got = torch.autograd.grad(out, [leaves[i] for i in wanted], do)
+        assert all(torch.equal(g, full[1 + i]) for g, i in zip(got, wanted)), wanted
 
 
 @pytest.mark.gpu
