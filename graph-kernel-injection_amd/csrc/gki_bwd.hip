@@ -27,6 +27,9 @@
 // group) are cut into items of bounded length whose fp32 partials a reduce
 // pass sums in a fixed order; items are XCD-remapped so neighbouring tiles of
 // one head share L2.
+// Cross attention runs the same kernels without lists (DENSE): every kv tile of a batch
+// entry's own keys and every q tile, the dK/dV walks cut into equal parts, the dQ walks
+// of few rows into slices.
 #include "gki_common.cuh"
 
 namespace gki {

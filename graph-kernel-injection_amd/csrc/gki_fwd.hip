@@ -28,6 +28,8 @@
 //    skipped, exactly, when no row max of a block moved.
 //  * head_dim 128 runs the loop skewed by one kv tile (fwd_kernel_16's PIPE),
 //    so that one wave's MFMAs of the next tile overlap its own softmax.
+// Cross attention runs the same kernels without a list (DENSE): a q tile visits every
+// tile of its batch entry's own keys; fp32 rows too few for the card, slices of them.
 //  * The running max is kept on unscaled scores, so Q is read through the
 //    Geom::q_and / q_xor transform that makes the effective scale positive.
 // What bounds it: on long rows the matrix cores are 70% busy in cycles and the
