@@ -13,7 +13,6 @@
 e4m3 codes and one power of two: 2^e with the smallest e for which the row's largest magnitude is at most 448 * 2^e.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -246,9 +245,7 @@ def _plain_cross(x, train):
 # ---- the calls -----------------------------------------------------------------------------------------------------
 
 
-@functools.cache
 def _gki():
-    """The package, imported once, as a program's own import would."""
     root = str(Path(__file__).resolve().parents[1] / "graph-kernel-injection_amd")
     if root not in sys.path:
         sys.path.insert(0, root)
