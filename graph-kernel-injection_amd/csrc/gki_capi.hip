@@ -698,7 +698,8 @@ int gki_cross_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t 
     return n > 1 ? n : 0;
   }
   if (!cross_as_streams(dtype, head_dim, B, H, H_kv, n_q, n_kv)) return 0;
-  return gki_stream_splits(dtype, B, H, H_kv, n_q, head_dim, n_kv);
+  const int64_t rows = (int64_t)(H / H_kv) * n_q, tile = stream_rows_tile(false, rows);     // 16-bit rows
+  return stream_splits(head_dim, (int64_t)B * H_kv * ((rows + tile - 1) / tile), n_kv);
 }
 
 int gki_cross_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int32_t dtype, int32_t B, int32_t H,
