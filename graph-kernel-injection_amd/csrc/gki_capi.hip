@@ -654,13 +654,13 @@ int gki_rolling8_decode(const void* q, const void* k_codes, const void* v_codes,
                       n_splits, stream);
 }
 
-int gki_prefix_splits(int32_t dtype, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
+int gki_prefix_splits(int32_t /*dtype*/, int32_t B, int32_t H, int32_t H_kv, int32_t n_q, int32_t head_dim,
                       int32_t n_prefix, int64_t n_tokens, int32_t* own_splits) {
   if (own_splits) *own_splits = 1;
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv || n_q <= 0 || n_prefix <= 0 || n_tokens < 0) return 1;
   const int64_t own = (int64_t)(H / H_kv) * n_q, rows = B * own;
-  const int64_t tile = prefix_as_streams(rows) ? 32 : kTileMF, own_tile = stream_rows_tile(dtype != kBF16, own);
-  if (own_splits) *own_splits = stream_splits_beside(head_dim, (int64_t)B * H_kv * ((own + own_tile - 1) / own_tile), n_tokens);
+  const int64_t tile = prefix_as_streams(rows) ? 32 : kTileMF;
+  if (own_splits) *own_splits = stream_splits_beside(head_dim, (int64_t)B * H_kv * ((own + 15) / 16), n_tokens);
   return prefix_splits(H_kv * ((rows + tile - 1) / tile), n_prefix);
 }
 

@@ -917,10 +917,14 @@ inline int stream_splits(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
 // The same behind a shared prefix, where the states are joined in any case: long streams
 // in up to about 1024 pieces of 512 tokens or more, which even out the CUs that the
 // prefix loads. us with 1 / 2 / 4, the prefix in 8 slices: 256 streams of 2052 (16-bit)
-// 58.7 / 59.3 / 56.4, 512 of 2052 (8-bit) 87.4 / 86.2 / 86.6.
-inline int stream_splits_beside(int head_dim, int64_t n_workgroups, int64_t n_tokens) {
-  const int64_t even = std::min((1024 + n_workgroups - 1) / n_workgroups, n_tokens / 512);
-  return (int)std::max<int64_t>(stream_splits(head_dim, n_workgroups, n_tokens), even);
+// 58.7 / 59.3 / 56.4, 512 of 2052 (8-bit) 87.4 / 86.2 / 86.6. Every type counts `blocks` of
+// 16 rows, also where a workgroup takes two (and does the work of two). us
+// counted by 32 / by 16 rows, bf16 in 16 bits, in 8 bits: B2 H64/2 n_q 4, own parts of 3000,
+// D128 22.7 / 19.1, 22.3 / 18.0; B16 H64/2 n_q 2, 8192 54.0 / 46.4, 49.4 / 41.7; B32 H40/2
+// n_q 2, 2048 (the same slices) 44.3 / 44.5, 41.0 / 40.9.
+inline int stream_splits_beside(int head_dim, int64_t blocks, int64_t n_tokens) {
+  const int64_t even = std::min((1024 + blocks - 1) / blocks, n_tokens / 512);
+  return (int)std::max<int64_t>(stream_splits(head_dim, blocks, n_tokens), even);
 }
 
 // Slices of a shared prefix (their states are joined with the sequences' own in any
