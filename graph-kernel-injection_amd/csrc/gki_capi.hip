@@ -293,6 +293,8 @@ int rolling_wide(const void* q, const void* k_new, const void* v_new, const void
                                    softmax_scale, q, k_cache, v_cache, o, lse, n_splits))
     return rc;
   GKI_REQUIRE(!k_scale == !v_scale, 1, "rolling cache: one scale without the other");
+  GKI_REQUIRE((int64_t)sink_size + ring_size < (1ll << kPartialBit), 1,
+              "rolling cache: sink_size + ring_size must be below 2^30");
   GKI_REQUIRE(all_aligned16(o, workspace), 1, "rolling cache: o and the workspace must be 16-byte aligned");
   const int64_t rows = (int64_t)(H / H_kv) * n_q;
   GKI_REQUIRE((rows + 15) / 16 * n_splits * B * H_kv < (1ll << 23), 1, "rolling cache: the grid must fit");
