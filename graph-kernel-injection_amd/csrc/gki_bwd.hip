@@ -153,9 +153,11 @@ __global__ __launch_bounds__(256) void dkdv_reduce_kernel(Geom g, KvWork w,
   const int bh = rest / w.n_split, s = rest - bh * w.n_split;
   const int kt = DENSE ? s : w.split[3 * s], p0 = DENSE ? s * w.parts : w.split[3 * s + 1];
   int np = DENSE ? w.parts : w.split[3 * s + 2];
-  if constexpr (DENSE)       // past the entry's keys there are no partials, and the sums are zeros
-    if (kt * kTileN >= own_keys(g, bh / g.H_kv)) np = 0;
   const int idx = (part * 256 + threadIdx.x) * 4;      // first float of this thread
+  const int which = idx / TILE, rem = idx - which * TILE;   // 4 floats of one row (D % 4 == 0)
+  const int row = kt * kTileN + rem / D;
+  if constexpr (DENSE)       // a row past the entry's keys: zeros, whatever its partials (a tile past them has none)
+    if (row >= own_keys(g, bh / g.H_kv)) np = 0;
   const float4* src = (const float4*)(w.partials + ((size_t)bh * w.n_pslots + p0) * 2 * TILE + idx);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   int c = 0;
@@ -181,8 +183,6 @@ __global__ __launch_bounds__(256) void dkdv_reduce_kernel(Geom g, KvWork w,
     const float4 a = src[(size_t)c * STRIDE];
     acc.x += a.x, acc.y += a.y, acc.z += a.z, acc.w += a.w;
   }
-  const int which = idx / TILE, rem = idx - which * TILE;   // 4 floats of one row (D % 4 == 0)
-  const int row = kt * kTileN + rem / D;
   if (row >= g.n_kv) return;
   typename T::storage* dst = (which ? dV : dK) + (size_t)bh * g.n_kv * D + (size_t)row * D + rem % D;
   dst[0] = T::from_float(acc.x);
@@ -427,6 +427,8 @@ __global__ __launch_bounds__(256, D <= 32 ? 4 : FORM != kBwdPlain ? 2 : 1) void 
         a[i] = dk[dt][4 * q + i] + rk[i];
         b[i] = dv[dt][4 * q + i] + rv[i];
       }
+      if constexpr (DENSE)       // past the entry's keys: zeros, where 0 times an infinity or NaN of Q or dO is not
+        if (kt * kTileN + row >= g.n_kv) a = b = floatx4{0.f, 0.f, 0.f, 0.f};
       const int d0 = 32 * dt + 8 * q + 4 * hi_e;
       if (split) {
         *(floatx4*)(part + d0) = a;
@@ -663,11 +665,12 @@ __global__ __launch_bounds__(256, 3) void dkdv_kernel_q64(
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = k_w + 16 * b + 4 * grp + i;
+      const bool gone = DENSE && row >= g.n_kv;    // past the entry's keys: zeros, also beside an infinity or NaN of Q or dO
       if (row < n_rows) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          dK[kb + (size_t)row * D + 16 * dt + col] = T::from_float(dk[b][dt][i]);
-          dV[kb + (size_t)row * D + 16 * dt + col] = T::from_float(dv[b][dt][i]);
+          dK[kb + (size_t)row * D + 16 * dt + col] = T::from_float(gone ? 0.f : dk[b][dt][i]);
+          dV[kb + (size_t)row * D + 16 * dt + col] = T::from_float(gone ? 0.f : dv[b][dt][i]);
         }
       }
     }
@@ -893,6 +896,13 @@ __global__ __launch_bounds__(256, D >= 128 || (D == 64 && KB == 1) ? 1 : 2) void
   for (int i = 0; i < 4; ++i) {
     const int row = 4 * grp + i;
     if (!split && k_w + row >= n_rows) continue;
+    if constexpr (DENSE)       // past the entry's keys: zeros, also beside an infinity or NaN of Q or dO
+      if (k_w + row >= g.n_kv) {
+#pragma unroll
+        for (int v = 0; v < DV; ++v)
+#pragma unroll
+          for (int e = 0; e < DE; ++e) dk[v][e][i] = dv[v][e][i] = 0.f;
+      }
 #pragma unroll
     for (int v = 0; v < DV; ++v) {
       const int c = row * D + 64 * v + DE * col;
