@@ -20,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPE_CODE, _HEAD_DIMS, _aligned, _current_stream, _on_device
+from .ops import _DTYPE_CODE, _HEAD_DIMS, _aligned, _current_stream, _on_device, _refuse_tangents
 
 # launch plans: (dtype, B, H, H_kv, n_q, n_kv, D) -> (slices, floats of the LSE rows, of
 # the slices' states) of a forward, (parts of dK/dV, slices of dQ, floats of the row terms,
@@ -164,7 +164,7 @@ def cross_attention(
     gradients, an entry without keys gives zeros (and zero gradients).
     ``softmax_scale`` defaults to ``1/sqrt(D)``, any finite value is taken.
     ``enable_gqa``: K and V may have ``H_kv`` heads dividing Q's ``H``, as in
-    ``block_sparse_attention``. Differentiable once.
+    ``block_sparse_attention``. Differentiable once, in reverse mode.
     """
     _check(q, k, v, kv_lengths, enable_gqa)
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
@@ -174,6 +174,7 @@ def cross_attention(
         if kv_lengths.dtype != torch.int32:
             kv_lengths = kv_lengths.clamp(0, k.shape[2]).to(torch.int32)
         kv_lengths = kv_lengths.contiguous()
+    _refuse_tangents(q, k, v)
     # copies of strided inputs are made here, where autograd sees them
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -22,6 +22,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .lists import _CACHE, bwd_schedule, decode_schedule, fwd_plan
@@ -42,6 +43,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     copied)."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _refuse_tangents(*tensors: torch.Tensor) -> None:
+    """Raise, as an autograd function without a jvp does, where a tensor carries a
+    forward-mode tangent: the kernels read the primal alone."""
+    if getattr(forward_ad, "_current_level", 0) < 0 or not torch._C._is_fwd_grad_enabled():
+        return                       # no dual level: a test of an integer per call
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode derivatives are not implemented (no jvp)")
 
 
 def _device_mask(block_mask: torch.Tensor, device: torch.device) -> torch.Tensor:
