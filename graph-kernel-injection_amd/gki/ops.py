@@ -342,6 +342,7 @@ def block_sparse_attention(
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         # nothing to differentiate (inference, a decode step): the same forward
         # without the autograd node and its saved tensors
+        _refuse_tangents(q, k, v)
         return _attention_forward(q, k, v, block_mask, softmax_scale, block_m, block_n, is_causal, sink_size,
                                   window_size, enable_gqa, need_lse=False)[0]
     args = (q.contiguous(), k.contiguous(), v.contiguous(), block_mask, float(softmax_scale),

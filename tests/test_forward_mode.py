@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from gki import cross_attention
+from gki import StreamingMaskSpec, block_sparse_attention, cross_attention, make_streaming_mask
 from gki.ops import _refuse_tangents
 
 
@@ -45,3 +45,18 @@ def test_cross_attention(which, n_q):
         qkv[0].requires_grad_(True)
         with pytest.raises(NotImplementedError):
             cross_attention(*qkv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("n_q", [1, 128])
+def test_block_sparse_attention(which, n_q):
+    qkv = _inputs(n_q)
+    mask = make_streaming_mask(n_q, 128, StreamingMaskSpec(4, 64), 64, 64, device="cuda")
+    call = dict(is_causal=True, sink_size=4, window_size=64)
+    want = block_sparse_attention(*qkv, mask, **call)
+    with forward_ad.dual_level():
+        assert torch.equal(block_sparse_attention(*qkv, mask, **call), want)
+        qkv[which] = forward_ad.make_dual(qkv[which], torch.ones_like(qkv[which]))
+        with pytest.raises(NotImplementedError):
+            block_sparse_attention(*qkv, mask, **call)
