@@ -170,11 +170,12 @@ class StreamingKVCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Append ``[B, H, n, D]`` keys / values at positions length .. length+n-1."""
-        self._check_tokens("k", k)
-        self._check_tokens("v", v)
-        if k.shape != v.shape:
+        n = self._check_tokens("k", k)
+        if n != self._check_tokens("v", v):
             raise ValueError("k and v must share shape")
-        n = int(k.shape[2])
+        self._append(k, v, n)
+
+    def _append(self, k: torch.Tensor, v: torch.Tensor, n: int) -> None:
         if n == 0:
             return
         k, v = _aligned(k), _aligned(v)
@@ -222,12 +223,18 @@ class StreamingKVCache:
         of the cache; Hq a multiple of the cache's heads) over the shared prefix,
         if there is one, and the visible tokens: ``O`` (and the natural-log LSE ``[B, Hq, n_q]`` fp32 when
         ``return_lse``)."""
-        self._check_tokens("q", q, grouped=True)
-        n_q = int(q.shape[2])
+        return self._attend(q, self._check_queries(q, self.length), softmax_scale, return_lse)
+
+    def _check_queries(self, q: torch.Tensor, length: int) -> int:
+        """The rows of ``q``, which must be those of the last of ``length`` positions."""
+        n_q = self._check_tokens("q", q, grouped=True)
         if not 1 <= n_q <= self.max_query:
             raise ValueError(f"q must hold 1..{self.max_query} rows, got {n_q}")
-        if n_q > self.length:
-            raise ValueError(f"q has {n_q} rows but the cache holds {self.length} positions")
+        if n_q > length:
+            raise ValueError(f"q has {n_q} rows but the cache holds {length} positions")
+        return n_q
+
+    def _attend(self, q: torch.Tensor, n_q: int, softmax_scale: Optional[float], return_lse: bool):
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(self.head_dim)
         q = _aligned(q)
@@ -315,16 +322,19 @@ class StreamingKVCache:
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
              softmax_scale: Optional[float] = None) -> torch.Tensor:
-        """One decode step: append the new tokens' K / V, then attend with q."""
-        if self.k_scale is not None or self._prefix is not None:
-            n = self._check_tokens("q", q, grouped=True)
-            n_k = self._check_tokens("k", k)
-            if n_k != self._check_tokens("v", v):
-                raise ValueError("k and v must share shape")
-            if 1 <= n == n_k <= self.max_query:      # the tokens are written by the launch that attends them
-                scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
-                o = self._attend_streams(_aligned(q), n, scale, False, (_aligned(k), _aligned(v)))
-                self.length += n
-                return o
-        self.append(k, v)
-        return self.attend(q, softmax_scale)
+        """One decode step: append the new tokens' K / V, then attend with q. Arguments
+        are checked before anything is written."""
+        n_k = self._check_tokens("k", k)
+        if n_k != self._check_tokens("v", v):
+            raise ValueError("k and v must share shape")
+        n = self._check_queries(q, self.length + n_k)
+        if softmax_scale is not None and not math.isfinite(softmax_scale):
+            raise ValueError(f"softmax_scale must be finite, got {softmax_scale}")
+        if n == n_k and (self.k_scale is not None or self._prefix is not None):
+            # the tokens are written by the launch that attends them
+            scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
+            o = self._attend_streams(_aligned(q), n, scale, False, (_aligned(k), _aligned(v)))
+            self.length += n
+            return o
+        self._append(k, v, n_k)
+        return self._attend(q, n, softmax_scale, False)

@@ -104,3 +104,26 @@ def test_steps_of_a_long_window_while_its_ring_turns(dtype, storage, prefix, n_q
     _same_steps(caches, normal, 4, 4 + ring - 20, 60 // n_q, n_q)
     plan = list(caches[0]._plans.values())
     assert all(p[0] > 1 for p in plan)                            # several slices, unforced
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("storage,prefix", [(None, 0), (F8, 0), (None, 70), (F8, 70)])
+def test_a_refused_step_writes_nothing(storage, prefix):
+    (cache, _), normal = _twins(torch.bfloat16, storage, prefix, 64, 4, 30, 2, 2, seed=1)
+    k, v = normal(2, 2, 3, 64), normal(2, 2, 3, 64)
+    cache.append(k, v)
+    held = [t.view(torch.uint8).clone() for t in (cache.k_cache, cache.v_cache)]
+    q = normal(2, 4, 3, 64)
+    for args, match in (((q, k, v), "rows"),                              # more queries than max_query
+                        ((q[:, :, :0], k, v), "rows"), ((q[:, :3, :1], k, v), "multiple of 2"),
+                        ((q[..., :32], k, v), "must be"), ((q.half()[:, :, :1], k[:, :, :1], v[:, :, :1]), "bfloat16"),
+                        ((q[:, :, :1], k, v[:, :, :1]), "share shape"), ((q[:, :, :1].cpu(), k, v), "live on"),
+                        ((q[:, :, :1], k, v, float("inf")), "finite"), ((q[:, :, :1], k[:, :, :1], v[:, :, :1], float("nan")), "finite")):
+        with pytest.raises(ValueError, match=match):
+            cache.step(*args)
+        assert cache.length == 3
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(held, (cache.k_cache, cache.v_cache)))
+    cache.reset()
+    with pytest.raises(ValueError, match="positions"):
+        cache.step(q[:, :, :2], k[:, :, :1], v[:, :, :1])
+    assert cache.length == 0
