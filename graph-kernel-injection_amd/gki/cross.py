@@ -162,7 +162,8 @@ def cross_attention(
     each batch entry (the first ones; a value outside ``0 .. N_KV`` counts as the nearest
     of them, as the device is not asked); keys past them are not read and get zero
     gradients, an entry without keys gives zeros (and zero gradients).
-    ``softmax_scale`` defaults to ``1/sqrt(D)``, any finite value is taken.
+    ``softmax_scale`` defaults to ``1/sqrt(D)``, any finite value is taken. Tensors that are
+    not contiguous or not 16-byte aligned are copied by each call.
     ``enable_gqa``: K and V may have ``H_kv`` heads dividing Q's ``H``, as in
     ``block_sparse_attention``. Differentiable once, in reverse mode.
     """
