@@ -11,6 +11,7 @@
 
 #include "gki_bsa.h"
 #include "gki_common.cuh"
+#include "gki_paged.cuh"
 
 namespace gki {
 
@@ -69,6 +70,18 @@ int prefix_decode_dispatch(int dtype, int head_dim, const Geom& g, const void* q
                            const uint8_t* ks, const uint8_t* vs, const void* k_new, const void* v_new,
                            const void* prefix_k, const void* prefix_v, int n_prefix, void* o, float* lse, int ring,
                            float* ws, int n_prefix_splits, int n_splits, hipStream_t stream);
+int page_extend_dispatch(const PageTables& t, const PageStep& s, hipStream_t stream);
+int page_release_dispatch(const PageTables& t, const uint8_t* done, hipStream_t stream);
+int page_accept_dispatch(int32_t* lengths, const int32_t* base, const int32_t* row_starts, const int32_t* accepted,
+                         int R, hipStream_t stream);
+int paged_append_dispatch(int head_dim, const PageRows& p, hipStream_t stream);
+int paged_append_rotated_dispatch(int dtype, int head_dim, const PageRows& p, const RotaryArgs& a, const HeadRows& q,
+                                  hipStream_t stream);
+int paged_move_dispatch(int head_dim, const PageRows& p, const int32_t* row_starts, const int32_t* paths,
+                        const int32_t* accepted, int R, int path_len, hipStream_t stream);
+int paged_attend_dispatch(int dtype, int head_dim, const PagedArgs& a, hipStream_t stream);
+int rotary_dispatch(int dtype, int head_dim, const RotaryArgs& a, const HeadRows& q, const HeadRows& k,
+                    hipStream_t stream);
 int64_t read_probe_words(int BH);
 int read_probe_dispatch(const void* k, const void* v, int BH, int64_t n_kv, int row_bytes, int n_sink,
                         int64_t w_lo, uint32_t* out, hipStream_t stream);
@@ -313,6 +326,48 @@ int rolling_wide(const void* q, const void* k_new, const void* v_new, const void
   return prefix_decode_dispatch(dtype, head_dim, g, q, k_cache, v_cache, (const uint8_t*)k_scale,
                                 (const uint8_t*)v_scale, k_new, v_new, prefix_k, prefix_v, n_prefix, o, lse, ring_size,
                                 workspace, n_prefix_splits, n_splits, (hipStream_t)stream);
+}
+
+// Pool and heads of a paged cache.
+int paged_pool(const char* what, int dtype, int head_dim, int H_kv, int num_pages, int page_size) {
+  GKI_REQUIRE(dtype == kF16 || dtype == kBF16, 2, std::string(what) + ": pages hold fp16 (1) or bf16 (2)");
+  GKI_REQUIRE(head_dim == 64 || head_dim == 128, 2, std::string(what) + ": head_dim must be 64 or 128");
+  GKI_REQUIRE(H_kv > 0 && H_kv <= 65535, 1, std::string(what) + ": H_kv must be in 1 .. 65535");
+  GKI_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0, 1,
+              std::string(what) + ": page_size must be a power of two in 16 .. 1024");
+  GKI_REQUIRE(num_pages > 0 && (int64_t)num_pages * page_size < (1ll << 31), 1, std::string(what) + ": num_pages * page_size must be in 1 .. 2^31 - 1");
+  return 0;
+}
+inline int log2_of(int x) { return __builtin_ctz((unsigned)x); }
+
+// Rows of heads D apart, `stride` elements from row to row.
+inline bool row_stride_ok(int64_t stride, int64_t width) { return stride % 8 == 0 && stride >= width; }
+
+int page_tables(const char* what, PageTables& t, int32_t* lengths, int32_t* pages, int32_t* kept, int32_t* table,
+                int32_t* ring, int32_t* queue, int32_t* status, int R, int max_pages, int page_size, int num_pages,
+                int sink, int window) {
+  GKI_REQUIRE(R > 0 && max_pages > 0 && num_pages > 0, 1, std::string(what) + ": R, max_pages and num_pages must be positive");
+  GKI_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0, 1,
+              std::string(what) + ": page_size must be a power of two in 16 .. 1024");
+  GKI_REQUIRE((int64_t)max_pages * page_size <= (1ll << kPartialBit), 1, std::string(what) + ": max_pages * page_size must not pass 2^30");
+  GKI_REQUIRE((int64_t)num_pages * page_size < (1ll << 31), 1, std::string(what) + ": num_pages * page_size must be below 2^31");
+  GKI_REQUIRE(R <= (1 << 20), 1, std::string(what) + ": at most 2^20 requests");
+  GKI_REQUIRE(sink >= 0 && sink < (1 << kPartialBit) && window >= 0, 1, std::string(what) + ": sink_size must be in 0 .. 2^30 - 1 and window_size not negative");
+  GKI_REQUIRE(lengths && pages && kept && table && ring && queue && status, 1, std::string(what) + ": null pointer");
+  t = PageTables{lengths, pages, kept, table, ring, queue, status, R, max_pages, log2_of(page_size), num_pages, sink, window};
+  return 0;
+}
+
+int rotary_args(const char* what, RotaryArgs& a, int head_dim, const double* turns, const int32_t* axis, int pairs,
+                int interleaved, int inverse, const void* positions, int wide, int64_t pa, int64_t pb, int64_t pn,
+                int64_t batch, int64_t n) {
+  GKI_REQUIRE(turns && axis && positions, 1, std::string(what) + ": null pointer");
+  GKI_REQUIRE(pairs > 0 && pairs % 8 == 0 && 2 * pairs <= head_dim, 1,
+              std::string(what) + ": pairs must be a multiple of 8 and at most head_dim / 2");
+  GKI_REQUIRE(n < (1ll << 31) && batch * n < (1ll << 24), 1, std::string(what) + ": at most 2^24 - 1 tokens");
+  a = RotaryArgs{turns, axis, positions, pa, pb, pn, wide ? 1 : 0, pairs, interleaved ? 1 : 0, inverse ? -1.f : 1.f,
+                 batch * n, (int)n};
+  return 0;
 }
 
 }  // namespace
@@ -754,6 +809,165 @@ int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, co
                   (parts == 1 || n_kt * B * H_kv * (head_dim / 8) < (1ll << 24)), 1, "gki_cross_bwd: grid too large");
   return cross_bwd_dispatch(dtype, head_dim, g, q, k, v, o, dout, lse, dq, dk, dv, delta, parts, kv_partials,
                             dq_slices, dq_sums, (hipStream_t)stream);
+}
+
+int gki_rotary(const void* q, void* q_out, int32_t q_heads, const int64_t* q_strides, const void* k, void* k_out,
+               int32_t k_heads, const int64_t* k_strides, int32_t dtype, int64_t batch, int64_t n, int32_t head_dim,
+               const double* turns, const int32_t* axis, int32_t pairs, int32_t interleaved, int32_t inverse,
+               const void* positions, int32_t wide, const int64_t* position_strides, void* stream) {
+  GKI_REQUIRE(dtype == kF32 || dtype == kF16 || dtype == kBF16, 2, "gki_rotary: unsupported dtype code " + std::to_string(dtype));
+  GKI_REQUIRE(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128, 2,
+              "gki_rotary: head_dim must be 16, 32, 64 or 128");
+  GKI_REQUIRE(batch >= 0 && n >= 0 && q_heads > 0 && k_heads >= 0 && (k_heads > 0) == (k != nullptr), 1,
+              "gki_rotary: batch and n must not be negative, the heads positive");
+  if (batch == 0 || n == 0) return 0;
+  GKI_REQUIRE(q && q_out && q_strides && position_strides && !k == !k_out && (!k || k_strides), 1, "gki_rotary: null pointer");
+  GKI_REQUIRE(all_aligned16(q, q_out, k, k_out), 1, "gki_rotary: tensors must be 16-byte aligned");
+  GKI_REQUIRE((int64_t)(q_heads + k_heads) * head_dim < (1 << 26), 1, "gki_rotary: too many heads");
+  const int per16 = dtype == kF32 ? 4 : 8;
+  for (int i = 0; i < 6; ++i)
+    GKI_REQUIRE(q_strides[i] % per16 == 0 && (!k || k_strides[i] % per16 == 0), 1,
+                "gki_rotary: rows must start on 16-byte boundaries");
+  RotaryArgs a;
+  if (int rc = rotary_args("gki_rotary", a, head_dim, turns, axis, pairs, interleaved, inverse, positions, wide,
+                           position_strides[0], position_strides[1], position_strides[2], batch, n))
+    return rc;
+  auto rows = [](const void* src, void* dst, int heads, const int64_t* s) {
+    return HeadRows{src, dst, heads, s[0], s[1], s[2], s[3], s[4], s[5]};
+  };
+  return rotary_dispatch(dtype, head_dim, a, rows(q, q_out, q_heads, q_strides),
+                         k ? rows(k, k_out, k_heads, k_strides) : HeadRows{}, (hipStream_t)stream);
+}
+
+int gki_page_extend(const int32_t* counts, const int32_t* parents, int32_t rows, int32_t max_count, int32_t words,
+                    int32_t* lengths, int32_t* pages, int32_t* kept, int32_t* table, int32_t* ring, int32_t* queue,
+                    int32_t* status, int32_t R, int32_t max_pages, int32_t page_size, int32_t num_pages,
+                    int32_t sink_size, int32_t window_size, int32_t* row_starts, int32_t* base, int32_t* positions,
+                    int64_t* slots, uint64_t* ancestors, void* stream) {
+  const char* what = "gki_page_extend";
+  PageTables t;
+  if (int rc = page_tables(what, t, lengths, pages, kept, table, ring, queue, status, R, max_pages, page_size, num_pages,
+                           sink_size, window_size))
+    return rc;
+  GKI_REQUIRE(rows >= 0 && rows < (1 << kPartialBit) && max_count >= 0, 1, "gki_page_extend: rows must be in 0 .. 2^30 - 1 and max_count not negative");
+  GKI_REQUIRE(counts && row_starts && base && (rows == 0 || (positions && slots)), 1, "gki_page_extend: null pointer");
+  if (parents) {
+    GKI_REQUIRE(max_count <= 256 && words >= 1 && words <= 4 && max_count <= 64 * words, 1,
+                "gki_page_extend: trees hold up to 256 nodes, 64 to a word");
+    GKI_REQUIRE(rows == 0 || ancestors, 1, "gki_page_extend: null pointer");
+  }
+  const PageStep s{counts, parents, rows, max_count, words, row_starts, base, positions, slots, ancestors};
+  return page_extend_dispatch(t, s, (hipStream_t)stream);
+}
+
+int gki_page_release(const uint8_t* done, int32_t* lengths, int32_t* pages, int32_t* kept, int32_t* table,
+                     int32_t* ring, int32_t* queue, int32_t* status, int32_t R, int32_t max_pages, int32_t page_size,
+                     int32_t num_pages, int32_t sink_size, int32_t window_size, void* stream) {
+  PageTables t;
+  if (int rc = page_tables("gki_page_release", t, lengths, pages, kept, table, ring, queue, status, R, max_pages,
+                           page_size, num_pages, sink_size, window_size))
+    return rc;
+  GKI_REQUIRE(done, 1, "gki_page_release: null pointer");
+  return page_release_dispatch(t, done, (hipStream_t)stream);
+}
+
+int gki_page_accept(int32_t* lengths, const int32_t* base, const int32_t* row_starts, const int32_t* accepted, int32_t R,
+                    void* stream) {
+  GKI_REQUIRE(R > 0 && R <= (1 << 20) && lengths && base && row_starts && accepted, 1,
+              "gki_page_accept: R must be in 1 .. 2^20, no pointer null");
+  return page_accept_dispatch(lengths, base, row_starts, accepted, R, (hipStream_t)stream);
+}
+
+int gki_paged_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, void* k_pages, void* v_pages,
+                     const int64_t* slots, int32_t dtype, int32_t rows, int32_t H_kv, int32_t head_dim, int32_t num_pages,
+                     int32_t page_size, void* stream) {
+  const char* what = "gki_paged_append";
+  if (int rc = paged_pool(what, dtype, head_dim, H_kv, num_pages, page_size)) return rc;
+  GKI_REQUIRE(rows >= 0 && rows < (1 << kPartialBit), 1, "gki_paged_append: rows must be in 0 .. 2^30 - 1");
+  if (rows == 0) return 0;
+  GKI_REQUIRE(k && v && k_pages && v_pages && slots, 1, "gki_paged_append: null pointer");
+  GKI_REQUIRE(all_aligned16(k, v, k_pages, v_pages), 1, "gki_paged_append: tensors must be 16-byte aligned");
+  const int64_t width = (int64_t)H_kv * head_dim;
+  GKI_REQUIRE(row_stride_ok(k_stride, width) && row_stride_ok(v_stride, width), 1,
+              "gki_paged_append: row strides must be multiples of 8 elements that hold a row");
+  return paged_append_dispatch(head_dim, PageRows{k, v, k_stride, v_stride, k_pages, v_pages, slots,
+                                                  (int64_t)num_pages * page_size, rows, H_kv, log2_of(page_size)},
+                               (hipStream_t)stream);
+}
+
+int gki_paged_append_rotated(const void* q, void* q_out, int64_t q_stride, int32_t H, const void* k, const void* v,
+                             int64_t k_stride, int64_t v_stride, void* k_pages, void* v_pages, const int64_t* slots,
+                             int32_t dtype, int32_t rows, int32_t H_kv, int32_t head_dim, int32_t num_pages,
+                             int32_t page_size, const double* turns, const int32_t* axis, int32_t pairs,
+                             int32_t interleaved, const void* positions, int32_t wide, int64_t axis_stride,
+                             int64_t row_stride, void* stream) {
+  const char* what = "gki_paged_append_rotated";
+  if (int rc = paged_pool(what, dtype, head_dim, H_kv, num_pages, page_size)) return rc;
+  GKI_REQUIRE(rows >= 0 && rows < (1 << 24), 1, "gki_paged_append_rotated: rows must be in 0 .. 2^24 - 1");
+  GKI_REQUIRE(H > 0 && ((int64_t)H + H_kv) * head_dim < (1 << 26), 1, "gki_paged_append_rotated: H must be positive and not too large");
+  if (rows == 0) return 0;
+  GKI_REQUIRE(q && q_out && k && v && k_pages && v_pages && slots, 1, "gki_paged_append_rotated: null pointer");
+  GKI_REQUIRE(all_aligned16(q, q_out, k, v, k_pages, v_pages), 1, "gki_paged_append_rotated: tensors must be 16-byte aligned");
+  const int64_t width = (int64_t)H_kv * head_dim;
+  GKI_REQUIRE(row_stride_ok(q_stride, (int64_t)H * head_dim) && row_stride_ok(k_stride, width) && row_stride_ok(v_stride, width), 1,
+              "gki_paged_append_rotated: row strides must be multiples of 8 elements that hold a row");
+  RotaryArgs a;
+  if (int rc = rotary_args(what, a, head_dim, turns, axis, pairs, interleaved, 0, positions, wide, axis_stride, 0,
+                           row_stride, 1, rows))
+    return rc;
+  const HeadRows qr{q, q_out, H, 0, q_stride, head_dim, 0, (int64_t)H * head_dim, head_dim};
+  return paged_append_rotated_dispatch(dtype, head_dim,
+                                       PageRows{k, v, k_stride, v_stride, k_pages, v_pages, slots,
+                                                (int64_t)num_pages * page_size, rows, H_kv, log2_of(page_size)},
+                                       a, qr, (hipStream_t)stream);
+}
+
+int gki_paged_accept(void* k_pages, void* v_pages, const int64_t* slots, const int32_t* row_starts, const int32_t* paths,
+                     const int32_t* accepted, int32_t dtype, int32_t R, int32_t path_len, int32_t H_kv, int32_t head_dim,
+                     int32_t num_pages, int32_t page_size, void* stream) {
+  if (int rc = paged_pool("gki_paged_accept", dtype, head_dim, H_kv, num_pages, page_size)) return rc;
+  GKI_REQUIRE(R > 0 && R <= (1 << 20) && path_len >= 0, 1, "gki_paged_accept: R must be in 1 .. 2^20, path_len not negative");
+  GKI_REQUIRE((int64_t)R * H_kv < (1ll << 26), 1, "gki_paged_accept: R * H_kv too large");
+  if (path_len == 0) return 0;
+  GKI_REQUIRE(k_pages && v_pages && slots && row_starts && paths && accepted, 1, "gki_paged_accept: null pointer");
+  GKI_REQUIRE(all_aligned16(k_pages, v_pages), 1, "gki_paged_accept: pages must be 16-byte aligned");
+  return paged_move_dispatch(head_dim,
+                             PageRows{nullptr, nullptr, 0, 0, k_pages, v_pages, slots, (int64_t)num_pages * page_size, 0,
+                                      H_kv, log2_of(page_size)},
+                             row_starts, paths, accepted, R, path_len, (hipStream_t)stream);
+}
+
+int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o, float* lse,
+                     const int32_t* row_starts, const int32_t* base, const int32_t* positions, const int32_t* table,
+                     const uint64_t* ancestors, int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R,
+                     int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t num_pages, int32_t page_size,
+                     int32_t sink_size, int32_t window_size, float softmax_scale, float* workspace, int32_t n_slices,
+                     void* stream) {
+  if (int rc = paged_pool("gki_paged_attend", dtype, head_dim, H_kv, num_pages, page_size)) return rc;
+  GKI_REQUIRE(rows >= 0 && max_count >= 0 && R > 0 && R <= (1 << 20) && H > 0 && H % H_kv == 0 && max_pages > 0, 1,
+              "gki_paged_attend: R, H and max_pages must be positive, H_kv must divide H");
+  GKI_REQUIRE(sink_size >= 0 && sink_size < (1 << kPartialBit) && window_size >= 0, 1,
+              "gki_paged_attend: sink_size must be in 0 .. 2^30 - 1 and window_size not negative");
+  GKI_REQUIRE(std::isfinite(softmax_scale), 1, "gki_paged_attend: softmax_scale must be finite");
+  if (rows == 0) return 0;
+  GKI_REQUIRE((int64_t)rows * (H / H_kv) < (1ll << kPartialBit), 1, "gki_paged_attend: too many rows");
+  GKI_REQUIRE(q && k_pages && v_pages && o && row_starts && base && positions && table, 1, "gki_paged_attend: null pointer");
+  GKI_REQUIRE(!ancestors || (words >= 1 && words <= 4 && max_count <= 64 * words), 1, "gki_paged_attend: trees hold up to 256 nodes, 64 to a word");
+  GKI_REQUIRE(all_aligned16(q, k_pages, v_pages, o, workspace), 1, "gki_paged_attend: tensors must be 16-byte aligned");
+  GKI_REQUIRE(row_stride_ok(q_stride, (int64_t)H * head_dim), 1,
+              "gki_paged_attend: the row stride must be a multiple of 8 elements that holds a row");
+  Geom g;
+  set_scale(g, softmax_scale);
+  PagedArgs a{};
+  a.q = (const uint16_t*)q, a.k_pages = (const uint16_t*)k_pages, a.v_pages = (const uint16_t*)v_pages;
+  a.o = (uint16_t*)o, a.lse = lse;
+  a.row_starts = row_starts, a.base = base, a.positions = positions, a.table = table, a.ancestors = ancestors;
+  a.q_stride = q_stride;
+  a.R = R, a.rows = rows, a.max_count = max_count, a.H = H, a.H_kv = H_kv, a.group = H / H_kv;
+  a.max_pages = max_pages, a.shift = log2_of(page_size), a.num_pages = num_pages;
+  a.sink = sink_size, a.window = std::min(window_size, 1 << kPartialBit), a.words = words;
+  a.scale_log2 = g.qk_scale_log2, a.q_and = g.q_and, a.q_xor = g.q_xor;
+  return paged_attend_dispatch(dtype, head_dim, a, (hipStream_t)stream);
 }
 
 int64_t gki_read_probe_words(int32_t bh) { return bh > 0 ? read_probe_words(bh) : 0; }

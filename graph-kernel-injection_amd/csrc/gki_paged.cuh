@@ -1,0 +1,76 @@
+// What the paged cache's entry points and kernels share.
+#pragma once
+
+#include "gki_common.cuh"
+
+namespace gki {
+
+// Rotary positions with several axes: pair j of a row's P pairs of elements turns by
+//   angle = position[axis_j] * frequency_j,  (a, b) -> (a cos - b sin, a sin + b cos),
+// pairs (j, j + P) or, interleaved, (2 j, 2 j + 1); elements from 2 P on stay as they are.
+struct RotaryArgs {
+  const double* turns;         // [P] frequency / (2 pi): turns per position
+  const int32_t* axis;         // [P]
+  const void* positions;       // int32 or int64, axis a of token (b, i) at a * pa + b * pb + i * pn
+  int64_t pa, pb, pn;
+  int wide;                    // positions are int64
+  int pairs, interleaved;
+  float sign;                  // -1: the gradient's turn
+  int64_t tokens;              // B * n
+  int n;
+};
+
+// Rows of heads, D elements each: token (b, i), head h at b * sb + i * sn + h * sh of the
+// source, with the d strides of the destination.
+struct HeadRows {
+  const void* src;
+  void* dst;
+  int heads;
+  int64_t sb, sn, sh, db, dn, dh;
+};
+
+// Tables of requests: position p of request r lies in page table[r][p >> shift].
+struct PageTables {
+  int32_t *lengths, *pages, *kept;     // [R] positions held, pages taken so far, first page behind the sinks not given back
+  int32_t *table;                      // [R][max_pages], -1: none
+  int32_t *ring, *queue;               // free pages: [num_pages]; {head, count}
+  int32_t* status;
+  int R, max_pages, shift, num_pages, sink, window;
+};
+
+// A step's tokens: counts[r] of each request, one request's rows after the other's.
+struct PageStep {
+  const int32_t *counts, *parents;
+  int rows, max_count, words;
+  int32_t *row_starts, *base, *positions;
+  int64_t* slots;
+  uint64_t* ancestors;
+};
+
+// Rows of keys and values and the pool that they go to: [num_pages][H_kv][page_size][D].
+struct PageRows {
+  const void *k, *v;
+  int64_t k_stride, v_stride;          // elements between rows; heads lie D apart
+  void *k_pages, *v_pages;
+  const int64_t* slots;
+  int64_t n_slots;                     // of the pool
+  int rows, H_kv, shift;
+  // element of the pool where head h of a row at `slot` starts
+  __device__ inline size_t at(int64_t slot, int h, int D) const {
+    return ((((size_t)(slot >> shift) * H_kv + h) << shift) + (slot & ((1 << shift) - 1))) * D;
+  }
+};
+
+struct PagedArgs {
+  const uint16_t *q, *k_pages, *v_pages;
+  uint16_t* o;
+  float* lse;                          // [rows][H] or null
+  const int32_t *row_starts, *base, *positions, *table;
+  const uint64_t* ancestors;           // [rows][words], null: no trees
+  int64_t q_stride;                    // elements between rows of q; heads lie D apart
+  int R, rows, max_count, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;
+  float scale_log2;
+  uint32_t q_and, q_xor;               // as Geom's: the sign of the scale, or zero, in Q
+};
+
+}  // namespace gki

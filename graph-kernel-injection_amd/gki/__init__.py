@@ -18,16 +18,22 @@ from .kv_cache import StreamingKVCache
 from .lists import BlockLists, build_block_lists, clear_schedule_cache
 from .masks import StreamingMaskSpec, make_dense_mask, make_streaming_mask, streaming_token_mask
 from .ops import _BlockSparseFlashAttention, block_sparse_attention
+from .paged import PagedKVCache, PageTable, TokenBatch
 from .reference import reference_block_sparse_attention
+from .rotary import MultiAxisRotary
 
 __all__ = [
     "BlockLists",
     "BlockSparseAttentionInjector",
     "InjectionConfig",
+    "MultiAxisRotary",
+    "PageTable",
+    "PagedKVCache",
     "SingleLayerTransformer",
     "StandardAttention",
     "StreamingKVCache",
     "StreamingMaskSpec",
+    "TokenBatch",
     "block_sparse_attention",
     "build_block_lists",
     "clear_schedule_cache",

@@ -370,6 +370,95 @@ int gki_cross_bwd(const void* q, const void* k, const void* v, const void* o, co
                   const int32_t* kv_len, float softmax_scale, int32_t parts, float* kv_partials,
                   int32_t dq_slices, float* dq_sums, void* stream);
 
+/* ---- Rotary positions with several axes ----------------------------------------
+ * No reference counterpart. Pair j of a row's `pairs` pairs of elements turns by
+ * position[axis[j]] * turns[j] (in turns: frequency / 2 pi; device arrays, fp64 and int32),
+ * (a, b) -> (a cos - b sin, a sin + b cos), back with inverse != 0 (the gradient). Pairs
+ * are elements (j, j + pairs) or, interleaved != 0, (2 j, 2 j + 1); pairs a multiple of 8,
+ * at most head_dim / 2; elements behind them are copied. q and k (may be NULL, with
+ * k_heads 0) take one launch. *_strides (host): {batch, token, head} strides in elements
+ * of the source, then of the destination, each a multiple of 16 bytes. positions: int32 or
+ * (wide) int64, position_strides (host): {axis, batch, token}. batch * n < 2^24. */
+int gki_rotary(const void* q, void* q_out, int32_t q_heads, const int64_t* q_strides, const void* k,
+               void* k_out, int32_t k_heads, const int64_t* k_strides, int32_t dtype, int64_t batch,
+               int64_t n, int32_t head_dim, const double* turns, const int32_t* axis, int32_t pairs,
+               int32_t interleaved, int32_t inverse, const void* positions, int32_t wide,
+               const int64_t* position_strides, void* stream);
+
+/* ---- Page tables of requests ----------------------------------------------------
+ * No reference counterpart. The tables are the caller's device arrays: lengths, pages
+ * (taken so far) and kept (first page behind the sinks that is still held; at first
+ * ceil(sink_size / page_size)), int32 [R]; table, int32 [R, max_pages], -1 where there is
+ * no page; ring, int32 [num_pages], and queue {head, count}: the free pages in the order
+ * in which they are taken (at first all of them, {0, num_pages}); status, one int32.
+ * page_size is a power of two in 16 .. 1024, max_pages * page_size at most 2^30,
+ * num_pages * page_size below 2^31. */
+
+/* Places counts[r] new tokens of each request behind its lengths[r]: row_starts [R + 1],
+ * base [R] (the lengths before), and of each of `rows` packed rows its position and slot,
+ * page * page_size + place in the page (-1 behind the last request). Pages that the next
+ * token of an extended request does not see (StreamingLLM rule) go back first, in the
+ * order of requests and positions, as do pages taken. With parents (int32 [rows]): trees
+ * of up to 256 nodes; a node stands at base + depth, ancestors (uint64 [rows, words], words
+ * >= ceil(max_count / 64)) are the nodes that it sees. A step that does not fit changes
+ * nothing, leaves no rows and sets bits of status: 1 no free pages, 2 more tokens than
+ * rows, 4 a count below 0, above max_count or past max_pages * page_size. */
+int gki_page_extend(const int32_t* counts, const int32_t* parents, int32_t rows, int32_t max_count,
+                    int32_t words, int32_t* lengths, int32_t* pages, int32_t* kept, int32_t* table,
+                    int32_t* ring, int32_t* queue, int32_t* status, int32_t R, int32_t max_pages,
+                    int32_t page_size, int32_t num_pages, int32_t sink_size, int32_t window_size,
+                    int32_t* row_starts, int32_t* base, int32_t* positions, int64_t* slots,
+                    uint64_t* ancestors, void* stream);
+
+/* Requests with done[r] != 0 give all their pages back and hold nothing. */
+int gki_page_release(const uint8_t* done, int32_t* lengths, int32_t* pages, int32_t* kept,
+                     int32_t* table, int32_t* ring, int32_t* queue, int32_t* status, int32_t R,
+                     int32_t max_pages, int32_t page_size, int32_t num_pages, int32_t sink_size,
+                     int32_t window_size, void* stream);
+
+/* lengths[r] = base[r] + accepted[r], clamped to the tokens that the step gave r. */
+int gki_page_accept(int32_t* lengths, const int32_t* base, const int32_t* row_starts,
+                    const int32_t* accepted, int32_t R, void* stream);
+
+/* ---- Paged keys and values --------------------------------------------------------
+ * k_pages / v_pages: [num_pages, H_kv, page_size, head_dim], fp16 or bf16, head_dim 64 or
+ * 128. Packed rows of q, k, v: heads lie head_dim apart, rows *_stride elements (a multiple
+ * of 8). q_out and o are contiguous [rows, H, head_dim]. */
+
+/* Rows to their slots; rows whose slot is not one of the pool's are left out. */
+int gki_paged_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, void* k_pages,
+                     void* v_pages, const int64_t* slots, int32_t dtype, int32_t rows, int32_t H_kv,
+                     int32_t head_dim, int32_t num_pages, int32_t page_size, void* stream);
+
+/* The same with the keys turned as by gki_rotary, and the queries turned into q_out. */
+int gki_paged_append_rotated(const void* q, void* q_out, int64_t q_stride, int32_t H, const void* k,
+                             const void* v, int64_t k_stride, int64_t v_stride, void* k_pages,
+                             void* v_pages, const int64_t* slots, int32_t dtype, int32_t rows,
+                             int32_t H_kv, int32_t head_dim, int32_t num_pages, int32_t page_size,
+                             const double* turns, const int32_t* axis, int32_t pairs,
+                             int32_t interleaved, const void* positions, int32_t wide,
+                             int64_t axis_stride, int64_t row_stride, void* stream);
+
+/* Rows of each request's accepted path (node paths[r, i] >= i of its rows, i <
+ * accepted[r]) to the slots of its rows 0, 1, ...; any other node moves nothing. */
+int gki_paged_accept(void* k_pages, void* v_pages, const int64_t* slots, const int32_t* row_starts,
+                     const int32_t* paths, const int32_t* accepted, int32_t dtype, int32_t R,
+                     int32_t path_len, int32_t H_kv, int32_t head_dim, int32_t num_pages,
+                     int32_t page_size, void* stream);
+
+/* O (and, lse not NULL, the natural LSE [rows, H]) of a step's rows: a row at position p sees
+ * the keys x <= p of its request with x < sink_size or x > p - window_size; with ancestors,
+ * from base[r] on those that its words name. row_starts, base, positions, ancestors and
+ * table as gki_page_extend leaves them. Rows that see no key, and rows behind the last
+ * request: zeros. */
+int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o,
+                     float* lse, const int32_t* row_starts, const int32_t* base,
+                     const int32_t* positions, const int32_t* table, const uint64_t* ancestors,
+                     int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R, int32_t H,
+                     int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t num_pages,
+                     int32_t page_size, int32_t sink_size, int32_t window_size, float softmax_scale,
+                     float* workspace, int32_t n_slices, void* stream);
+
 /* Measurement helper, no counterpart in the reference: reads exactly the K and V
  * bytes a single-position StreamingLLM decode step reads from a full cache --
  * per (b, kv head) slice of bh slices of n_kv rows of row_bytes (a multiple of
