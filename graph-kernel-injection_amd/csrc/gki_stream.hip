@@ -25,30 +25,16 @@
 
 #include "gki_join.cuh"
 #include "gki_rows16.cuh"
+#include "gki_stream_wave.cuh"
 
 namespace gki {
 namespace {
 
 constexpr int kMinExponent = -117;           // 2^-9 (the smallest code) * 2^-117 is a normal float
-constexpr float kStreamSlack = 8.f;          // log2 units the lazy reference max may lag (p <= 2^8)
 
 // ---------------------------------------------------------------------------
 // Writing and reading back.
 // ---------------------------------------------------------------------------
-// Eight consecutive elements as floats, and back.
-template <typename T>
-__device__ inline void load8(const typename T::storage* p, float (&f)[8]) {
-  if constexpr (T::is_f32) {
-    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    const uint4 w = *(const uint4*)p;
-    const uint16_t* h = (const uint16_t*)&w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = T::to_float(h[i]);
-  }
-}
-
 // Rows that a launch writes into a rolling cache: of n_new from position start on, the
 // first n_a and n_b from the i_b-th on (surviving_rows).
 struct AppendRows {
@@ -138,7 +124,6 @@ __device__ inline f32x2 codes2(uint32_t w, bool high, float scale) {
   const auto x = high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
   return f32x2{x[0] * scale, x[1] * scale};
 }
-__device__ inline float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
 
 // The held rows in ascending order of position, as values of the cache's type, and
 // the positions. Row r < n_sink is position r, any other lo + r - n_sink. Eight
@@ -258,23 +243,6 @@ struct StreamArgs {
   int n_new, start;            // no such tokens: start past every position
 };
 
-// Queries as 1, 2 or 3 bfloat16 pieces whose sum they are (8, 11 and 24 significant
-// bits), so that products with the stored values are those of the queries themselves.
-template <typename T> constexpr int kPieces = std::is_same<T, BF16>::value ? 1 : std::is_same<T, F16>::value ? 2 : 3;
-
-template <typename C, int NPC>
-__device__ inline void split8(float (&f)[8], uint4 (&piece)[NPC]) {
-#pragma unroll
-  for (int n = 0; n < NPC; ++n) {
-    piece[n] = make_uint4(pack2<C>(f[0], f[1]), pack2<C>(f[2], f[3]), pack2<C>(f[4], f[5]), pack2<C>(f[6], f[7]));
-    if (n + 1 < NPC) {
-      const uint16_t* h = (const uint16_t*)&piece[n];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] -= C::to_float(h[i]);
-    }
-  }
-}
-
 // Where a workgroup works: 16 NB query rows (from row0 on) of stream s against the
 // slice [g0, g1) of its tokens. Row tiles of a slice are neighbours on one XCD.
 struct StreamPlace {
@@ -300,28 +268,6 @@ struct StreamPlace {
   __device__ inline int steps(int tokens) const { return (g1 - g0 + tokens - 1) / tokens; }
 };
 
-// A step's 128 rows of D codes in LDS: row-major, 16-byte chunks XOR-swizzled so that both
-// kinds of reads are free of conflicts: 16 bytes of rows {0-3, 8-11, 16-19, 24-27} (+ 4)
-// at one chunk, and transposed reads of 16 consecutive rows at one chunk.
-constexpr int kStep8 = 128;
-template <int D>
-__device__ inline int code_swz(int row) {
-  const int b3 = (row >> 3) & 1, b24 = ((row >> 2) ^ (row >> 4)) & 1;
-  return D >= 128 ? ((row >> 1) & 1) | b3 << 1 | b24 << 2 : b3 | b24 << 1;
-}
-template <int D>
-__device__ inline int code_off(int row, int byte) {
-  return row * D + (((byte >> 4) ^ code_swz<D>(row)) << 4) + (byte & 15);
-}
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-// Eight codes times a power of two, as bfloat16 (exact).
-__device__ inline uint4 bf16x8_of(uint32_t lo, uint32_t hi, float scale) {
-  return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false)),
-                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true)));
-}
 // One byte per lane to LDS dwords, lane i at lds + 4 i.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -330,239 +276,29 @@ __device__ inline void dma_load1(const void* src, uint32_t lds) {
 }
 #pragma clang diagnostic pop
 
-// One transposed read as lds_tr4's, of the rows rho(t, 4 g + e) that lane group g's
-// scores of subtile t belong to.
-template <int D>
-__device__ inline uint2 lds_tr4_rho(const uint16_t* tile, int t, int n0, int lane) {
-  const int g = lane >> 4, l = lane & 15;
-  const uint16_t* p = tile + lds_off<D>(rho(t, 4 * g + (l >> 2)), n0 + 4 * (l & 3));
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)p));
-}
-
-// A wave's share of a workgroup of four: 16 NB query rows, as columns of S^T = K Q^T on
-// v_mfma_f32_16x16x32, against 16 of the 64 tokens of each step (tiles of element
-// type C in LDS; the wave's tokens are those of subtile rho(wave, .), whose rows the
-// swizzle serves without conflicts), with a softmax state of its own. NPC: pieces of the queries and of
-// the probabilities. The reference max is lazy: it moves when a score exceeds it by
-// the slack, so that the rescale almost never runs.
+// The wave of a workgroup at its place, and what is left of its rows.
 template <typename T, typename C, int D, int NB, int NPC, bool RULE, bool EIGHT>
-struct StreamWave {
-  static constexpr int KS = D / 32, DT = D / 16;
-  uint4 qf[NB][KS][NPC];
-  floatx4 o[NB][DT];
-  float lsum[NB], m[NB];
-  int my_q[NB], wave, lane, grp, col;
-
-  __device__ inline StreamWave(const StreamArgs& a, const StreamPlace& at) {
-    lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    grp = lane >> 4, col = lane & 15;
-    // Q^T operand of column block h: lane (grp, col) holds elements 32 ks + 8 grp .. +7
-    // (EIGHT: 64 (ks / 2) + 16 grp + 8 (ks % 2) .. +7) of row row0 + 16 h + col
-#pragma unroll
-    for (int h = 0; h < NB; ++h) {
-      const int r = at.row0 + 16 * h + col;
-      my_q[h] = r % a.n_q;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        float f[8];
-        load8<T>((const typename T::storage*)a.q + at.q_row(a, r < a.n_rows ? r : 0) * D +
-                     (EIGHT ? 64 * (ks >> 1) + 16 * grp + 8 * (ks & 1) : 32 * ks + 8 * grp), f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = r < a.n_rows && a.q_sign != 0.f ? f[i] * a.q_sign : 0.f;
-        split8<C>(f, qf[h][ks]);
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[h][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
-      lsum[h] = 0.f;
-      m[h] = kNegInf;
+__device__ inline StreamWave<T, C, D, NB, NPC, RULE, EIGHT> stream_wave(const StreamArgs& a, const StreamPlace& at) {
+  return StreamWave<T, C, D, NB, NPC, RULE, EIGHT>(
+      at.row0, a.n_rows, a.q_sign, [&](int r) { return (const typename T::storage*)a.q + at.q_row(a, r) * D; },
+      [&](int r) { return r % a.n_q; });
+}
+template <typename T, int D, class Wave>
+__device__ inline void stream_finish(Wave& w, const StreamArgs& a, const StreamPlace& at, float* wacc, float* wml) {
+  w.finish(a.n_rows - at.row0, wacc, wml, [&](int r, int d, floatx4 x, float M, float L) {
+    const size_t row = at.q_row(a, at.row0 + r);
+    if (a.n_parts == 1) {
+      x = x / (L == 0.f ? 1.f : L);        // no visible token: 0; NaN stays NaN
+      typename T::storage* dst = (typename T::storage*)a.o + row * D + d;
+      if constexpr (T::is_f32) *(floatx4*)dst = x;
+      else *(uint2*)dst = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+      if (d == 0) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
+    } else {
+      *(floatx4*)(a.acc + (row * a.n_parts + a.part0 + at.split) * D + d) = x;
+      if (d == 0) *(float2*)(a.ml + (row * a.n_parts + a.part0 + at.split) * 2) = make_float2(M, L);
     }
-  }
-
-  // The reference max follows the rows' largest score (scaled, the lane's mx) where some
-  // row's exceeds it by the slack.
-  __device__ inline void move_max(int h, float mx) {
-    if (__any(mx > m[h] + kStreamSlack)) {
-      mx = wave_max16x4(mx);
-      const bool grow = mx > m[h] + kStreamSlack;
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m[h] - mx) : 1.f;
-      m[h] = grow ? mx : m[h];
-      lsum[h] *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[h][dt] *= alpha;
-    }
-  }
-
-  // The wave's 16 tokens of the step of 64 that starts at token t; g1 ends the slice.
-  template <class Src>
-  __device__ inline void step(const StreamArgs& a, const Src& src, const uint16_t* ck, const uint16_t* cv, int t, int g1) {
-    floatx4 s[NB];
-#pragma unroll
-    for (int h = 0; h < NB; ++h) s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const uint4 x = lds_row8<D>(ck, rho(wave, col), 32 * ks + 8 * grp);
-#pragma unroll
-      for (int h = 0; h < NB; ++h) s[h] = C::mfma(x, qf[h][ks][0], s[h]);
-    }
-    // lane (grp, col): s[h][i] = score of token t + rho(wave, 4 grp + i) for row row0 + 16 h + col
-    if (t + kTileN > g1 || (RULE && src.partly_hidden(t, kTileN))) {
-      const int t0 = t + rho(wave, 4 * grp);
-#pragma unroll
-      for (int h = 0; h < NB; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bool ok = t0 + i < g1;
-          if constexpr (RULE) ok = ok && src.visible(my_q[h], t0 + i);
-          s[h][i] = ok ? s[h][i] : kNegInf;
-        }
-    }
-    uint2 pb[NB];
-#pragma unroll
-    for (int h = 0; h < NB; ++h) {
-      move_max(h, fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3])) * a.scale_log2);
-      const float m_use = m[h] == kNegInf ? 0.f : m[h];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], a.scale_log2, -m_use));
-      lsum[h] += (s[h][0] + s[h][1]) + (s[h][2] + s[h][3]);
-      pb[h] = make_uint2(pack2<C>(s[h][0], s[h][1]), pack2<C>(s[h][2], s[h][3]));
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const uint2 x = lds_tr4_rho<D>(cv, wave, 16 * dt, lane);
-#pragma unroll
-      for (int h = 0; h < NB; ++h) o[h][dt] = mfma16k<C>(x, pb[h], o[h][dt]);
-    }
-  }
-
-  // The wave's 32 tokens (tile rows 32 wave ..) of the step of 128 over 8-bit rows that
-  // starts at token t. A lane's 16 codes of a K row feed two products (the queries list
-  // their elements in the same order), its scores belong to tokens 8 grp + 4 u + i: with
-  // their V row's power of two they are the operand of V^T, eight tokens of a column by
-  // one transposed read.
-  template <class Src>
-  __device__ inline void step8(const StreamArgs& a, const Src& src, const uint8_t* ck, const uint8_t* cv,
-                               const uint32_t* ks, const uint32_t* vs, int t, int g1) {
-    floatx4 s[NB][2];
-#pragma unroll
-    for (int h = 0; h < NB; ++h) s[h][0] = s[h][1] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = 32 * wave + rho(u, col);
-      const float scale = scale_of(ks[row]);
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        const uint4 w = *(const uint4*)(ck + code_off<D>(row, 64 * j + 16 * grp));
-        const uint4 x = bf16x8_of(w.x, w.y, scale), y = bf16x8_of(w.z, w.w, scale);
-#pragma unroll
-        for (int h = 0; h < NB; ++h)
-#pragma unroll
-          for (int n = 0; n < NPC; ++n) {
-            s[h][u] = C::mfma(x, qf[h][2 * j][n], s[h][u]);
-            s[h][u] = C::mfma(y, qf[h][2 * j + 1][n], s[h][u]);
-          }
-      }
-    }
-    const int t0 = t + 32 * wave + 8 * grp;
-    if (t + kStep8 > g1 || (RULE && src.partly_hidden(t, kStep8))) {
-#pragma unroll
-      for (int h = 0; h < NB; ++h)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            bool ok = t0 + 4 * u + i < g1;
-            if constexpr (RULE) ok = ok && src.visible(my_q[h], t0 + 4 * u + i);
-            s[h][u][i] = ok ? s[h][u][i] : kNegInf;
-          }
-    }
-    floatx4 sv[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint4 e = *(const uint4*)(vs + 32 * wave + 8 * grp + 4 * u);
-      sv[u] = floatx4{scale_of(e.x), scale_of(e.y), scale_of(e.z), scale_of(e.w)};
-    }
-    uint4 pb[NB][NPC];
-#pragma unroll
-    for (int h = 0; h < NB; ++h) {
-      float mx = kNegInf;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[h][u][i]);
-      move_max(h, mx * a.scale_log2);
-      const float m_use = m[h] == kNegInf ? 0.f : m[h];
-      float f[8];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[h][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][u][i], a.scale_log2, -m_use));
-          f[4 * u + i] = s[h][u][i] * sv[u][i];
-        }
-        lsum[h] += (s[h][u][0] + s[h][u][1]) + (s[h][u][2] + s[h][u][3]);
-      }
-      split8<C>(f, pb[h]);
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int l = lane & 15;
-      const uint8_t* v = cv + code_off<D>(32 * wave + 8 * grp + (l >> 1), 16 * dt + 8 * (l & 1));
-      const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)v);
-      const uint4 x = bf16x8_of((uint32_t)w.x, (uint32_t)w.y, 1.f);
-#pragma unroll
-      for (int h = 0; h < NB; ++h)
-#pragma unroll
-        for (int n = 0; n < NPC; ++n) o[h][dt] = C::mfma(x, pb[h][n], o[h][dt]);
-    }
-  }
-
-  // The four waves' states meet in LDS (wacc: 64 D floats, wml: 128), one column block
-  // at a time: lane (grp, col) holds O^T rows 16 dt + 4 grp + i of row row0 + 16 h + col.
-  __device__ inline void finish(const StreamArgs& a, const StreamPlace& at, float* wacc, float* wml) {
-#pragma unroll
-    for (int h = 0; h < NB; ++h) {
-      const float lw = wave_sum16x4(lsum[h]);
-      __syncthreads();                         // the tiles' (or the previous block's) readers are done
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        *(floatx4*)(wacc + (wave * 16 + col) * D + 16 * dt + 4 * grp) = o[h][dt];
-      if (grp == 0) {
-        wml[(wave * 16 + col) * 2] = m[h];
-        wml[(wave * 16 + col) * 2 + 1] = lw;
-      }
-      __syncthreads();
-      const int rows_h = min(16, a.n_rows - at.row0 - 16 * h);
-      for (int idx = threadIdx.x; idx < rows_h * (D / 4); idx += 256) {
-        const int rl = idx / (D / 4), d = 4 * (idx % (D / 4));
-        const size_t row = at.q_row(a, at.row0 + 16 * h + rl);
-        float M = kNegInf;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, wml[(w * 16 + rl) * 2]);
-        const float Mu = M == kNegInf ? 0.f : M;
-        float L = 0.f;
-        floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float f = __builtin_amdgcn_exp2f(wml[(w * 16 + rl) * 2] - Mu);
-          L += wml[(w * 16 + rl) * 2 + 1] * f;
-          x += *(const floatx4*)(wacc + (w * 16 + rl) * D + d) * f;
-        }
-        if (a.n_parts == 1) {
-          x = x / (L == 0.f ? 1.f : L);        // no visible token: 0; NaN stays NaN
-          typename T::storage* dst = (typename T::storage*)a.o + row * D + d;
-          if constexpr (T::is_f32) *(floatx4*)dst = x;
-          else *(uint2*)dst = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-          if (d == 0) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
-        } else {
-          *(floatx4*)(a.acc + (row * a.n_parts + a.part0 + at.split) * D + d) = x;
-          if (d == 0) *(float2*)(a.ml + (row * a.n_parts + a.part0 + at.split) * 2) = make_float2(M, L);
-        }
-      }
-    }
-  }
-};
+  });
+}
 
 // Over 8-bit rows: codes and exponents gathered into LDS by LDS-DMA as they are, two
 // steps of 128 tokens in flight (non-temporal: 6.6 against 5.9 TB/s on 1.08 GB; staged
@@ -585,7 +321,7 @@ __device__ inline void stream8_rows(const StreamArgs& a, const Src& src, int blo
   const uint8_t *K = (const uint8_t*)a.k + at.kb * D, *V = (const uint8_t*)a.v + at.kb * D;
   const uint8_t* E = (wave < 2 ? a.ks : a.vs) + at.kb;     // exponents: waves 0, 1 K's, 2, 3 V's, 64 rows each
   uint8_t *rk = (uint8_t*)sk, *rv = (uint8_t*)sv;
-  StreamWave<T, BF16, D, NB, kPieces<T>, RULE, true> w(a, at);
+  auto w = stream_wave<T, BF16, D, NB, kPieces<T>, RULE, true>(a, at);
   dma_wait();   // the Q loads are complete before any LDS-DMA is in flight
 
   int drow[NP], doff[NP];                      // the lane's row of its LDS blocks, and where its codes are in a tile
@@ -667,7 +403,7 @@ __device__ inline void stream8_rows(const StreamArgs& a, const Src& src, int blo
     __syncthreads();                           // every wave is done with buffer b
     if (c + 2 < n_steps) issue(c + 2, b);
   }
-  w.finish(a, at, (float*)sk, (float*)sv);
+  stream_finish<T, D>(w, a, at, (float*)sk, (float*)sv);
 }
 
 // Over 16-bit rows: gathered into LDS by LDS-DMA, two steps in flight, so that no
@@ -682,7 +418,7 @@ __device__ inline void stream16_rows(const StreamArgs& a, const Src& src, int bl
   const bool once = a.row_tiles == 1;
   const int n_chunks = at.steps(kTileN);
   const uint16_t *K = (const uint16_t*)a.k + at.kb * D, *V = (const uint16_t*)a.v + at.kb * D;
-  StreamWave<T, T, D, NB, 1, RULE, false> w(a, at);
+  auto w = stream_wave<T, T, D, NB, 1, RULE, false>(a, at);
   dma_wait();   // the Q loads are complete before any LDS-DMA is in flight
 
   // the lane's chunk of LDS block 4 p + wave of a tile: row, swizzled column
@@ -735,7 +471,7 @@ __device__ inline void stream16_rows(const StreamArgs& a, const Src& src, int bl
     __syncthreads();                           // every wave is done with buffer b
     if (c + 2 < n_chunks) issue(c + 2, b);
   }
-  w.finish(a, at, (float*)sk, (float*)sv);
+  stream_finish<T, D>(w, a, at, (float*)sk, (float*)sv);
 }
 
 template <typename T, int D, int NB, bool RULE, bool EIGHT, class Src>
