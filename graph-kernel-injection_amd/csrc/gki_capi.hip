@@ -937,6 +937,16 @@ int gki_paged_accept(void* k_pages, void* v_pages, const int64_t* slots, const i
                              row_starts, paths, accepted, R, path_len, (hipStream_t)stream);
 }
 
+int gki_paged_slices(int32_t rows, int32_t max_count, int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages,
+                     int32_t page_size, int32_t sink_size, int32_t window_size) {
+  if (rows <= 0 || max_count < 0 || H <= 0 || H_kv <= 0 || H % H_kv || max_pages <= 0 || page_size <= 0) return 1;
+  return paged_max_slices(head_dim, rows, max_count, H_kv, H / H_kv, sink_size, window_size, (int64_t)max_pages * page_size);
+}
+
+int64_t gki_paged_workspace_floats(int32_t rows, int32_t H, int32_t head_dim, int32_t n_slices) {
+  return n_slices > 1 ? (int64_t)rows * ((int64_t)H * n_slices * (head_dim + 2) + 1) : 0;
+}
+
 int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o, float* lse,
                      const int32_t* row_starts, const int32_t* base, const int32_t* positions, const int32_t* table,
                      const uint64_t* ancestors, int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R,
@@ -956,6 +966,8 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   GKI_REQUIRE(all_aligned16(q, k_pages, v_pages, o, workspace), 1, "gki_paged_attend: tensors must be 16-byte aligned");
   GKI_REQUIRE(row_stride_ok(q_stride, (int64_t)H * head_dim), 1,
               "gki_paged_attend: the row stride must be a multiple of 8 elements that holds a row");
+  GKI_REQUIRE(n_slices >= 1 && n_slices <= 64 && (n_slices == 1 || workspace), 1,
+              "gki_paged_attend: n_slices must be in 1 .. 64, and several need a workspace");
   Geom g;
   set_scale(g, softmax_scale);
   PagedArgs a{};
@@ -963,10 +975,16 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   a.o = (uint16_t*)o, a.lse = lse;
   a.row_starts = row_starts, a.base = base, a.positions = positions, a.table = table, a.ancestors = ancestors;
   a.q_stride = q_stride;
-  a.R = R, a.rows = rows, a.max_count = max_count, a.H = H, a.H_kv = H_kv, a.group = H / H_kv;
+  a.R = R, a.rows = rows, a.H = H, a.H_kv = H_kv, a.group = H / H_kv;
   a.max_pages = max_pages, a.shift = log2_of(page_size), a.num_pages = num_pages;
   a.sink = sink_size, a.window = std::min(window_size, 1 << kPartialBit), a.words = words;
   a.scale_log2 = g.qk_scale_log2, a.q_and = g.q_and, a.q_xor = g.q_xor;
+  a.q_sign = softmax_scale == 0.f ? 0.f : softmax_scale < 0.f ? -1.f : 1.f;
+  a.target = paged_target(head_dim), a.min_slice = kPagedMinSlice, a.max_slices = n_slices, a.whole = kPagedWhole;
+  a.acc = workspace;
+  a.ml = workspace + (int64_t)rows * H * n_slices * head_dim;
+  a.parts = (int32_t*)(a.ml + (int64_t)rows * H * n_slices * 2);
+  GKI_REQUIRE(paged_units(a) < (1ll << 24) && (int64_t)rows * H < (1ll << 26), 1, "gki_paged_attend: the grid must fit");
   return paged_attend_dispatch(dtype, head_dim, a, (hipStream_t)stream);
 }
 

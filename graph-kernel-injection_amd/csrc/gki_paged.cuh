@@ -61,6 +61,10 @@ struct PageRows {
   }
 };
 
+constexpr int kPagedWhole = 12;        // key tiles
+constexpr int kPagedMinSlice = 4;
+inline int paged_target(int head_dim) { return head_dim >= 128 ? 512 : 1024; }
+
 struct PagedArgs {
   const uint16_t *q, *k_pages, *v_pages;
   uint16_t* o;
@@ -68,9 +72,31 @@ struct PagedArgs {
   const int32_t *row_starts, *base, *positions, *table;
   const uint64_t* ancestors;           // [rows][words], null: no trees
   int64_t q_stride;                    // elements between rows of q; heads lie D apart
-  int R, rows, max_count, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;
-  float scale_log2;
-  uint32_t q_and, q_xor;               // as Geom's: the sign of the scale, or zero, in Q
+  int R, rows, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;
+  float scale_log2, q_sign;            // as StreamArgs': the sign of the scale, or zero, goes to q
+  uint32_t q_and, q_xor;               // the same as words of Q
+  // slices of the keys: about `target` units in all, of at least min_slice key tiles, up
+  // to max_slices of a row tile, none of fewer than `whole` key tiles
+  int target, min_slice, max_slices, whole;
+  float *acc, *ml;                     // their states
+  int32_t* parts;                      // [rows] slices that a token has
 };
+
+// An upper bound of a launch's units: the target, and one for each row tile and head where
+// a slice ends short (few rows are one tile; 128 a tile fill fewer than all of them).
+inline int64_t paged_units(const PagedArgs& a) {
+  return a.target + a.H_kv * ((int64_t)a.rows * a.group / 128 + std::min(a.R, a.rows));
+}
+
+// Slices that the keys of a row tile can be cut into, from what the host knows: rows of the
+// step, the largest count, and what a row can see.
+inline int paged_max_slices(int head_dim, int64_t rows, int64_t max_count, int H_kv, int group, int64_t sink,
+                            int64_t window, int64_t max_length) {
+  const int64_t seen = std::min(max_length, sink + window + max_count + 64);
+  const int64_t keys = (seen + 63) / 64 + 2, tiles = (rows * group + 127) / 128;
+  if (keys < kPagedWhole) return 1;
+  const int64_t most = (3 * paged_target(head_dim) / 2 + H_kv * tiles - 1) / (H_kv * tiles);
+  return (int)std::max<int64_t>(1, std::min({most, (keys + kPagedMinSlice - 1) / kPagedMinSlice, (int64_t)64}));
+}
 
 }  // namespace gki

@@ -7,53 +7,23 @@
 // Drafted trees: row i stands at p = base + depth_i; of the keys from base on it sees those
 // that its word of ancestors names (which has the rule in it already).
 //
-// The rows of a request that read one kv head, (token, q head of the group) token by
-// token, are cut into tiles; a tile walks the 64-key tiles of the sinks and of its rows'
-// windows once, whatever lies between. Pages are addressed a 1 KB LDS block at a time, each
-// of which lies in one page; keys past the request's last, and pages that it does not have,
-// are zeros without being read: what another request left in a page is never seen. (A NaN or
+// The rows of a request that read one kv head, (token, q head of the group) token by token,
+// are its rows here. Up to 32 of them run as a stream (four waves share out the keys of a
+// step), more as tiles of 128 (four waves of 32 rows). Either walks the 64-key tiles of the
+// sinks and of its rows' windows once, whatever lies between, or a slice of them; slices'
+// states are joined. Pages are addressed a 1 KB LDS block at a time, each of which lies in
+// one page; keys past the request's last, and pages that it does not have, are zeros
+// without being read: what another request left in a page is never seen. (A NaN or
 // infinity among the request's own values reaches every row of a tile that reads it.)
 #include "gki_paged.cuh"
+#include "gki_stream_wave.cuh"
 
 namespace gki {
 namespace {
 
-constexpr float kSlack = 8.f;          // log2 units that the reference max may lag
-constexpr int kTile = 128;             // rows of a tile: four waves of 32
-
-// What a workgroup works on: rows row0 .. row0 + n_rows - 1 of those that request r has of
-// a kv head.
-struct PagedPlace {
-  int r, tile, first, n, base;         // first row of the request in the step, its rows, its keys before them
-};
-
-// The place of tile number t over all requests: a wave counts 64 requests at a time.
-__device__ inline bool find_place(const PagedArgs& a, int t, PagedPlace& at) {
-  const int lane = threadIdx.x & 63;
-  for (int r0 = 0; r0 < a.R; r0 += 64) {
-    const int r = min(r0 + lane, a.R - 1);
-    const int s = a.row_starts[r], n = r0 + lane < a.R ? a.row_starts[r + 1] - s : 0;
-    const int tiles = (n * a.group + kTile - 1) / kTile;
-    int sum = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(sum, o);
-      if (lane >= o) sum += y;
-    }
-    const uint64_t past = __ballot(sum > t);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      at.r = r0 + l;
-      at.tile = t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l));
-      at.first = __builtin_amdgcn_readlane(s, l);
-      at.n = __builtin_amdgcn_readlane(n, l);
-      at.base = __builtin_amdgcn_readfirstlane(a.base[at.r]);
-      return true;
-    }
-    t -= __builtin_amdgcn_readlane(sum, 63);
-  }
-  return false;
-}
+constexpr int kRowTile = 128;          // rows of a tile: four waves of 32
+constexpr int kFewRows = 32;           // up to as many run as a stream
+constexpr int kIds = 1024;             // page ids held in LDS at a time
 
 // The 64-key tiles that rows at positions lo_pos .. see of keys 0 .. end - 1: the sinks',
 // then the window's.
@@ -67,6 +37,93 @@ struct KeyTiles {
   }
   __device__ inline int first_key(int i) const { return (i < n_sink ? i : w0 + (i - n_sink)) << 6; }
 };
+
+// ---------------------------------------------------------------------------
+// Which unit of work a workgroup takes. A unit is a slice of the keys of a row tile of one
+// request and kv head. Lengths are known on the device only, so every workgroup counts
+// for itself, a wave 64 requests at a time: the key tiles of all row tiles, from them the
+// length of a slice that fills the card, from it the units. The units of a (request, head)
+// are neighbours on one XCD, a slice's row tiles side by side.
+// ---------------------------------------------------------------------------
+struct Request {
+  int first, n, base, tiles, keys;     // first row of the step's, rows, keys before them; row tiles, key tiles
+  __device__ inline Request(const PagedArgs& a, int r) {
+    const bool ok = r < a.R;
+    r = ok ? r : a.R - 1;
+    first = a.row_starts[r];
+    n = ok ? a.row_starts[r + 1] - first : 0;
+    base = a.base[r];
+    const int rows = n * a.group;
+    tiles = rows <= kFewRows ? (rows + kFewRows - 1) / kFewRows : (rows + kRowTile - 1) / kRowTile;
+    keys = n ? KeyTiles(a, base, base + n).n : 0;
+  }
+  // Slices of about `length` key tiles.
+  __device__ inline int slices(const PagedArgs& a, int length) const {
+    return keys < a.whole ? 1 : min(a.max_slices, (keys + length - 1) / length);
+  }
+};
+
+__device__ inline int64_t wave_sum64(int64_t x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);       // the same everywhere: scalar
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | lo);
+}
+// Sum of lanes 0 .. l.
+__device__ inline int wave_prefix(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+__device__ inline int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+struct Unit {
+  int r, first, n, base;               // the request
+  int h, tile, slice, n_slices;
+};
+
+__device__ inline bool find_unit(const PagedArgs& a, int block, Unit& u) {
+  const int lane = threadIdx.x & 63;
+  int64_t all = 0;
+  for (int r0 = 0; r0 < a.R; r0 += 64) {
+    const Request q(a, r0 + lane);
+    all += (int64_t)q.tiles * q.keys;
+  }
+  all = wave_sum64(all) * a.H_kv;
+  const int length = (int)max((int64_t)a.min_slice, (all + a.target - 1) / a.target);
+  int units = 0;
+  for (int r0 = 0; r0 < a.R; r0 += 64) {
+    const Request q(a, r0 + lane);
+    units += q.tiles * q.slices(a, length);
+  }
+  units = (int)wave_sum64(units) * a.H_kv;
+  if (block >= units) return false;
+  int t = xcd_remap(block, units);
+  for (int r0 = 0; r0 < a.R; r0 += 64) {
+    const Request q(a, r0 + lane);
+    const int mine = q.tiles * q.slices(a, length) * a.H_kv, sum = wave_prefix(mine);
+    const uint64_t past = __ballot(sum > t);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      u.r = r0 + l;
+      u.first = lane_value(q.first, l), u.n = lane_value(q.n, l), u.base = lane_value(q.base, l);
+      u.n_slices = lane_value(q.slices(a, length), l);
+      const int tiles = lane_value(q.tiles, l);
+      t -= lane_value(sum - mine, l);
+      u.tile = t % tiles;
+      t /= tiles;
+      u.slice = t % u.n_slices;
+      u.h = t / u.n_slices;
+      return true;
+    }
+    t -= lane_value(sum, 63);
+  }
+  return false;
+}
 
 // Keys of the 64 from x0 on that a row sees.
 __device__ inline uint64_t seen_bits(const PagedArgs& a, int row, int pos, int base, int x0) {
@@ -87,53 +144,150 @@ __device__ inline uint64_t seen_bits(const PagedArgs& a, int row, int pos, int b
   return bits;
 }
 
-// A tile of 64 keys or values into LDS: the wave's 1 KB blocks, each from one page.
-template <int D>
-struct PageTile {
-  DmaTile<D, 4, true> dma;
+// The key tiles of a unit, into LDS by LDS-DMA: a wave's 1 KB blocks, each from one page.
+// The page ids of up to 1024 / (pages per tile) tiles ahead are held in LDS.
+template <int D, bool ROW32>
+struct PageTiles {
+  DmaTile<D, 4, ROW32> dma;
+  KeyTiles keys;
   const int32_t* table;                // the request's pages
-  int end, h;                          // its keys, the kv head
-  __device__ inline void load(const PagedArgs& a, const uint16_t* pool, int x0, const uint16_t* lds) const {
+  int* ids;
+  int end, h, c0, c1, filled;          // its keys, the kv head; the unit's tiles; those from `filled` - span on are held
+  int per, span;                       // pages per tile (at least one), tiles that `ids` holds
+  bool once;                           // no other workgroup reads these rows
+
+  __device__ inline PageTiles(const PagedArgs& a, const Unit& u, const KeyTiles& k, int* lds_ids, bool read_once)
+      : keys(k), ids(lds_ids), once(read_once) {
+    dma.init(threadIdx.x);
+    table = a.table + (int64_t)u.r * a.max_pages;
+    end = u.base + u.n;
+    h = u.h;
+    c0 = __builtin_amdgcn_readfirstlane((int)((int64_t)k.n * u.slice / u.n_slices));
+    c1 = __builtin_amdgcn_readfirstlane((int)((int64_t)k.n * (u.slice + 1) / u.n_slices));
+    per = max(1, kTileN >> a.shift);
+    span = kIds / per;
+    filled = c0;
+  }
+  // The ids of tiles c .. c + span - 1; every wave comes here at the same tile.
+  __device__ inline void fill(const PagedArgs& a, int c) {
+    __syncthreads();                   // the ids before have been read
+    for (int i = threadIdx.x; i < min(span, c1 - c) * per; i += 256) {
+      const int x = keys.first_key(c + i / per) + (i % per << a.shift);
+      const int id = table[min(x, end - 1) >> a.shift];
+      ids[i] = x < end && (unsigned)id < (unsigned)a.num_pages ? id : -1;
+    }
+    __syncthreads();
+    filled = c + span;
+  }
+  __device__ inline void before(const PagedArgs& a, int c) {
+    if (c >= filled) fill(a, c);
+  }
+  __device__ inline void load(const PagedArgs& a, const uint16_t* pool, int c, const uint16_t* lds) const {
     const uint32_t l0 = lds_addr(lds);
+    const int x0 = keys.first_key(c), i0 = (c - (filled - span)) * per;
 #pragma unroll
     for (int p = 0; p < dma.NP; ++p) {
       const int blk = 4 * p + dma.wave;
-      if (dma.NB % 4 == 0 || blk < dma.NB) {
-        const int row = blk * (512 / D), x = x0 + row;               // the block's first row; its page
-        const int id = x < end ? __builtin_amdgcn_readfirstlane(table[x >> a.shift]) : -1;
-        const bool there = (unsigned)id < (unsigned)a.num_pages;
-        const int in_page = x & ((1 << a.shift) - 1);
-        // as if the tile's row 0 lay in this page too: the lane's offsets are those of whole tiles
-        const int64_t row0 = ((((int64_t)(there ? id : 0) * a.H_kv + h) << a.shift) + in_page) - row;
-        const int rows = there ? row + min((1 << a.shift) - in_page, end - x) : 0;
-        dma_buf16(buffer_rsrc(pool + row0 * D, rows * D * 2), 2 * dma.off[p], l0 + blk * 1024);
-      }
+      const int row = blk * (512 / D), x = x0 + row;             // the block's first row
+      const int id = __builtin_amdgcn_readfirstlane(ids[i0 + (a.shift < 6 ? row >> a.shift : 0)]);
+      const int in_page = x & ((1 << a.shift) - 1);
+      // as if the tile's row 0 lay in this page too: the lane's offsets are those of whole tiles
+      const int64_t row0 = ((((int64_t)max(id, 0) * a.H_kv + h) << a.shift) + in_page) - row;
+      const int rows = id < 0 ? 0 : row + max(0, min((1 << a.shift) - in_page, end - x));
+      dma_buf16(buffer_rsrc(pool + row0 * D, rows * D * 2), 2 * dma.off[p], l0 + blk * 1024, once);
     }
   }
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_tiles_kernel(PagedArgs a) {
-  constexpr int KS = D / 16, DT = D / 32;
-  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
-  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = blockIdx.y;
-
-  // rows behind the last request have no output: zeros
-  for (int64_t x = (int64_t)a.row_starts[a.R] * a.H * (D / 8) + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid;
-       x < (int64_t)a.rows * a.H * (D / 8); x += (int64_t)gridDim.x * gridDim.y * 256) {
-    *(uint4*)(a.o + 8 * x) = make_uint4(0, 0, 0, 0);
-    if (a.lse && x % (D / 8) == 0) a.lse[x / (D / 8)] = 0.f;
+// ---------------------------------------------------------------------------
+// Up to 32 rows.
+// ---------------------------------------------------------------------------
+struct StreamRow {
+  int pos;
+  uint64_t word;                       // ancestors
+};
+// The token rule for StreamWave: token t is key t of the request.
+struct PagedRule {
+  int base, last, sink, window;        // last: of the rows' positions, or above it
+  bool tree;
+  __device__ inline bool partly_hidden(int t, int n) const {
+    return t + n > base || (t + n > sink && max(t, sink) <= last - window);
   }
-  PagedPlace at;
-  if (!find_place(a, blockIdx.x, at)) return;
-  const int rows = at.n * a.group, row0 = at.tile * kTile;
+  __device__ inline bool visible(const StreamRow& r, int t) const {
+    const bool rule = (t < sink) | (t > r.pos - window);
+    if (!tree) return (t <= r.pos) & rule;
+    return t < base ? rule : (r.word >> ((t - base) & 63)) & 1;
+  }
+};
+
+// The states that slices leave: acc [rows][max_slices][D], ml [rows][max_slices][2] for
+// rows = (token, q head), and how many a token has.
+__device__ inline float* slice_acc(const PagedArgs& a, int64_t row, int slice, int D) {
+  return a.acc + (row * a.max_slices + slice) * D;
+}
+__device__ inline float2* slice_ml(const PagedArgs& a, int64_t row, int slice) {
+  return (float2*)a.ml + row * a.max_slices + slice;
+}
+
+// As the streams of the other caches: two key tiles in flight, so that no registers hold
+// loads. Bound by HBM.
+template <typename T, int D, int NB>
+__device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int* ids) {
+  constexpr int TILE = kTileN * D;
+  const int rows = u.n * a.group;
+  auto token = [&](int r) { return u.first + min(r, rows - 1) / a.group; };
+  StreamWave<T, T, D, NB, 1, true, false, StreamRow> w(
+      0, rows, a.q_sign,
+      [&](int r) { return a.q + (int64_t)token(r) * a.q_stride + (u.h * a.group + r % a.group) * D; },
+      [&](int r) {
+        const int t = token(r);
+        return StreamRow{a.positions[t], a.ancestors ? a.ancestors[(int64_t)t * a.words] : 0};
+      });
+  const PagedRule rule{u.base, u.base + u.n - 1, a.sink, a.window, a.ancestors != nullptr};
+  PageTiles<D, false> page(a, u, KeyTiles(a, u.base, u.base + u.n), ids, true);
+  dma_wait();   // the loads above are complete before any LDS-DMA is in flight
+  auto issue = [&](int c) {
+    const int b = (c - page.c0) & 1;
+    page.before(a, c);
+    page.load(a, a.k_pages, c, sk + b * TILE);
+    page.load(a, a.v_pages, c, sv + b * TILE);
+  };
+  if (page.c0 < page.c1) issue(page.c0);
+  if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
+  for (int c = page.c0; c < page.c1; ++c) {
+    const int b = (c - page.c0) & 1;
+    wait_chunks<page.dma.NP, 2>(min(1, page.c1 - 1 - c));     // tile c has landed
+    __syncthreads();
+    w.step(a, rule, sk + b * TILE, sv + b * TILE, page.keys.first_key(c), page.end);
+    __syncthreads();                             // every wave is done with buffer b
+    if (c + 2 < page.c1) issue(c + 2);
+  }
+  w.finish(rows, (float*)sk, (float*)sv, [&](int r, int d, floatx4 x, float M, float L) {
+    const int64_t row = (int64_t)token(r) * a.H + u.h * a.group + r % a.group;
+    if (u.n_slices == 1) {
+      x = x / (L == 0.f ? 1.f : L);              // no visible key: 0; NaN stays NaN
+      *(uint2*)(a.o + row * D + d) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+      if (d == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
+    } else {
+      *(floatx4*)(slice_acc(a, row, u.slice, D) + d) = x;
+      if (d == 0) *slice_ml(a, row, u.slice) = make_float2(M, L);
+    }
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of 128 rows.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int* ids) {
+  constexpr int KS = D / 16, DT = D / 32, TILE = kTileN * D;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = u.n * a.group, row0 = u.tile * kRowTile;
   const int hi = lane >> 5, col = lane & 31;
   const Lane32<D> lanes(lane);
   const int my = row0 + wave * 32 + col;                   // the lane's row of the request's
   const bool mine = my < rows;
-  const int token = at.first + (mine ? my / a.group : 0), head = h * a.group + (mine ? my % a.group : 0);
+  const int token = u.first + (mine ? my / a.group : 0), head = u.h * a.group + (mine ? my % a.group : 0);
   const int pos = a.positions[token];
   uint4 qf[KS];
 #pragma unroll
@@ -145,14 +299,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_tiles_kernel(Paged
   dma_wait();   // these loads are complete before any LDS-DMA is in flight
 
   const bool tree = a.ancestors != nullptr;
-  const int last_token = min(row0 + kTile - 1, rows - 1) / a.group;
-  const int end = at.base + last_token + 1;                // an ancestor has a lower number
-  const KeyTiles keys(a, at.base + (tree ? 0 : row0 / a.group), end);
-  PageTile<D> page;
-  page.dma.init(tid);
-  page.table = a.table + (int64_t)at.r * a.max_pages;
-  page.end = at.base + at.n;
-  page.h = h;
+  const int last_token = min(row0 + kRowTile - 1, rows - 1) / a.group;
+  // an ancestor has a lower number, a node's position is at least base
+  const KeyTiles keys(a, u.base + (tree ? 0 : row0 / a.group), u.base + last_token + 1);
+  PageTiles<D, true> page(a, u, keys, ids, rows <= kRowTile);
 
   floatx16 o[DT];
 #pragma unroll
@@ -160,99 +310,169 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_tiles_kernel(Paged
   floatx4 lsum = floatx4{0.f, 0.f, 0.f, 0.f};
   // row sums on the matrix pipe: lane l gets that of row l & 31 of the operand of 32 rows
   const uint4 ones = ((lane >> 2) & 1) == ((lane >> 4) & 1) ? T::ones8() : make_uint4(0, 0, 0, 0);
-  const float slack = kSlack / a.scale_log2;
+  const float slack = kStreamSlack / a.scale_log2;
   float nm = 0.f, thr = kNegInf;
 
-  if (keys.n > 0) {
-    page.load(a, a.k_pages, keys.first_key(0), sk[0]);
-    page.load(a, a.v_pages, keys.first_key(0), sv[0]);
+  if (page.c0 < page.c1) {
+    page.before(a, page.c0);
+    page.load(a, a.k_pages, page.c0, sk);
+    page.load(a, a.v_pages, page.c0, sv);
   }
   dma_wait();
   __syncthreads();
-  auto step = [&](int i, int buf) {
-    const int x0 = keys.first_key(i);
-    if (i + 1 < keys.n) {
-      page.load(a, a.k_pages, keys.first_key(i + 1), sk[buf ^ 1]);
-      page.load(a, a.v_pages, keys.first_key(i + 1), sv[buf ^ 1]);
+  auto step = [&](int c, int buf) {
+    const int x0 = keys.first_key(c);
+    if (c + 1 < page.c1) {
+      page.before(a, c + 1);
+      page.load(a, a.k_pages, c + 1, sk + (buf ^ 1) * TILE);
+      page.load(a, a.v_pages, c + 1, sv + (buf ^ 1) * TILE);
     }
-    floatx16 s[2];
+    if (row0 + wave * 32 < rows) {
+      floatx16 s[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[t] = T::mfma32(lanes.rows(sk[buf], t, ks), qf[ks], ks == 0 ? splat16(0.f) : s[t]);
-    const uint64_t bits = mine ? seen_bits(a, token, pos, at.base, x0) : 0;
-    float mx = kNegInf;
+        for (int ks = 0; ks < KS; ++ks)
+          s[t] = T::mfma32(lanes.rows(sk + buf * TILE, t, ks), qf[ks], ks == 0 ? splat16(0.f) : s[t]);
+      const uint64_t bits = mine ? seen_bits(a, token, pos, u.base, x0) : 0;
+      float mx = kNegInf;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const LaneBits32 vis((uint32_t)(bits >> (32 * t)), hi);
+      for (int t = 0; t < 2; ++t) {
+        const LaneBits32 vis((uint32_t)(bits >> (32 * t)), hi);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[t][r] = vis.pick(r, s[t][r], kNegInf);
-        mx = fmaxf(mx, s[t][r]);
+        for (int r = 0; r < 16; ++r) {
+          s[t][r] = vis.pick(r, s[t][r], kNegInf);
+          mx = fmaxf(mx, s[t][r]);
+        }
       }
-    }
-    if (__any(mx > thr)) {
-      const float mr = half_max(mx);
-      const bool grow = mr > thr;
-      const float nm1 = grow ? -mr * a.scale_log2 : nm;
-      // a first reference below zero scales nothing yet (o = lsum = 0)
-      const float alpha = __builtin_amdgcn_exp2f(fminf(nm1 - nm, 0.f));
-      nm = nm1;
-      thr = grow ? mr + slack : thr;
-      lsum[0] *= alpha;
+      if (__any(mx > thr)) {
+        const float mr = half_max(mx);
+        const bool grow = mr > thr;
+        const float nm1 = grow ? -mr * a.scale_log2 : nm;
+        // a first reference below zero scales nothing yet (o = lsum = 0)
+        const float alpha = __builtin_amdgcn_exp2f(fminf(nm1 - nm, 0.f));
+        nm = nm1;
+        thr = grow ? mr + slack : thr;
+        lsum[0] *= alpha;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-    }
-    uint4 p[4];
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      }
+      uint4 p[4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2, nm));
-      p[2 * t] = pack8<T>(s[t], 0);
-      p[2 * t + 1] = pack8<T>(s[t], 1);
-    }
+        for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2, nm));
+        p[2 * t] = pack8<T>(s[t], 0);
+        p[2 * t + 1] = pack8<T>(s[t], 1);
+      }
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
+      for (int st = 0; st < 4; ++st) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma32(lanes.cols(sv[buf], st, dt), p[st], o[dt]);
-      lsum = T::mfma(ones, p[st], lsum);
+        for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma32(lanes.cols(sv + buf * TILE, st, dt), p[st], o[dt]);
+        lsum = T::mfma(ones, p[st], lsum);
+      }
     }
     dma_wait();
     __syncthreads();
   };
-  int i = 0;
-  for (; i + 1 < keys.n; i += 2) {
-    step(i, 0);
-    step(i + 1, 1);
+  int c = page.c0;
+  for (; c + 1 < page.c1; c += 2) {
+    step(c, 0);
+    step(c + 1, 1);
   }
-  if (i < keys.n) step(i, 0);
+  if (c < page.c1) step(c, 0);
 
   if (!mine) return;
-  const float l = lsum[0], inv = l > 0.f ? 1.f / l : 1.f;
-  uint16_t* dst = a.o + ((int64_t)token * a.H + head) * D;
+  const float l = lsum[0];
+  const int64_t row = (int64_t)token * a.H + head;
+  if (u.n_slices > 1) {
+    float* dst = slice_acc(a, row, u.slice, D);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *(floatx4*)(dst + 32 * dt + 8 * r + 4 * hi) =
+            floatx4{o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]};
+    if (hi == 0) *slice_ml(a, row, u.slice) = make_float2(l == 0.f ? kNegInf : -nm, l);
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : 1.f;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      *(uint2*)(dst + 32 * dt + 8 * r + 4 * hi) =
+      *(uint2*)(a.o + row * D + 32 * dt + 8 * r + 4 * hi) =
           make_uint2(pack2<T>(o[dt][4 * r] * inv, o[dt][4 * r + 1] * inv), pack2<T>(o[dt][4 * r + 2] * inv, o[dt][4 * r + 3] * inv));
-  if (hi == 0 && a.lse) a.lse[(int64_t)token * a.H + head] = l > 0.f ? lse_natural(-nm, l) : 0.f;
+  if (hi == 0 && a.lse) a.lse[row] = l > 0.f ? lse_natural(-nm, l) : 0.f;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_kernel(PagedArgs a) {
+  __shared__ __align__(16) uint16_t sk[2][kTileN * D];
+  __shared__ __align__(16) uint16_t sv[2][kTileN * D];
+  __shared__ int ids[kIds];
+  // rows behind the last request have no output: zeros
+  for (int64_t x = (int64_t)a.row_starts[a.R] * a.H * (D / 8) + (int64_t)blockIdx.x * 256 + threadIdx.x;
+       x < (int64_t)a.rows * a.H * (D / 8); x += (int64_t)gridDim.x * 256) {
+    *(uint4*)(a.o + 8 * x) = make_uint4(0, 0, 0, 0);
+    if (a.lse && x % (D / 8) == 0) a.lse[x / (D / 8)] = 0.f;
+  }
+  Unit u;
+  if (!find_unit(a, blockIdx.x, u)) return;
+  const int rows = u.n * a.group;
+  if (a.max_slices > 1 && u.h == 0 && u.slice == 0) {       // for the join
+    const int t0 = rows <= kFewRows ? 0 : u.tile * kRowTile / a.group;
+    for (int t = t0 + threadIdx.x; t < u.n && t * a.group < (u.tile + 1) * kRowTile; t += 256) a.parts[u.first + t] = u.n_slices;
+  }
+  if (rows <= 16) paged_stream<T, D, 1>(a, u, sk[0], sv[0], ids);
+  else if (rows <= kFewRows) paged_stream<T, D, 2>(a, u, sk[0], sv[0], ids);
+  else paged_tile<T, D>(a, u, sk[0], sv[0], ids);
+}
+
+// The slices of a row joined, a wave per (token, q head): as join_kernel, with the slices
+// that the token has. Rows of one slice are done.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+  constexpr int E = D / 64;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= (int64_t)a.row_starts[a.R] * a.H) return;
+  const int n = a.parts[row / a.H];
+  if (n == 1) return;
+  const float2* st = slice_ml(a, row, 0);
+  const float* x = slice_acc(a, row, 0, D) + E * lane;
+  float M = kNegInf;
+#pragma unroll 4
+  for (int p = 0; p < n; ++p) M = fmaxf(M, st[p].x);
+  const float Mu = M == kNegInf ? 0.f : M;
+  float L = 0.f, s[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) s[e] = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < n; ++p) {
+    const float f = __builtin_amdgcn_exp2f(st[p].x - Mu);
+    L += st[p].y * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] += x[(size_t)p * D + e] * f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) a.o[row * D + E * lane + e] = T::from_float(s[e] / (L == 0.f ? 1.f : L));
+  if (lane == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
+}
+
+template <typename T, int D>
+int paged_attend(const PagedArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_kernel<T, D>), dim3((unsigned)paged_units(a)), dim3(256), 0, stream, a);
+  if (a.max_slices > 1)
+    hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.rows * a.H + 3) / 4)), dim3(256), 0, stream, a);
+  return check_launch("gki_paged_attend");
 }
 
 }  // namespace
 
-// `tiles`: an upper bound of the requests' row tiles.
 int paged_attend_dispatch(int dtype, int head_dim, const PagedArgs& a, hipStream_t stream) {
-  const int64_t tiles = (int64_t)a.rows * a.group / kTile + std::min(a.R, a.rows);
-  const dim3 grid((unsigned)tiles, (unsigned)a.H_kv);
-#define GKI_PAGED(T, D) hipLaunchKernelGGL((paged_tiles_kernel<T, D>), grid, dim3(256), 0, stream, a)
-  if (dtype == kF16) {
-    if (head_dim == 64) GKI_PAGED(F16, 64);
-    else GKI_PAGED(F16, 128);
-  } else if (head_dim == 64) GKI_PAGED(BF16, 64);
-  else GKI_PAGED(BF16, 128);
-#undef GKI_PAGED
-  return check_launch("gki_paged_attend");
+  if (dtype == kF16) return head_dim == 64 ? paged_attend<F16, 64>(a, stream) : paged_attend<F16, 128>(a, stream);
+  return head_dim == 64 ? paged_attend<BF16, 64>(a, stream) : paged_attend<BF16, 128>(a, stream);
 }
 
 }  // namespace gki

@@ -446,6 +446,13 @@ int gki_paged_accept(void* k_pages, void* v_pages, const int64_t* slots, const i
                      int32_t path_len, int32_t H_kv, int32_t head_dim, int32_t num_pages,
                      int32_t page_size, void* stream);
 
+/* Slices that gki_paged_attend may cut a row tile's keys into, for a full card (any number
+ * from 1 to 64 is right; how many a request gets is decided on the device, by the lengths
+ * there), and the floats of 16-byte aligned workspace for as many (0 for one). */
+int gki_paged_slices(int32_t rows, int32_t max_count, int32_t H, int32_t H_kv, int32_t head_dim,
+                     int32_t max_pages, int32_t page_size, int32_t sink_size, int32_t window_size);
+int64_t gki_paged_workspace_floats(int32_t rows, int32_t H, int32_t head_dim, int32_t n_slices);
+
 /* O (and, lse not NULL, the natural LSE [rows, H]) of a step's rows: a row at position p sees
  * the keys x <= p of its request with x < sink_size or x > p - window_size; with ancestors,
  * from base[r] on those that its words name. row_starts, base, positions, ancestors and

@@ -64,6 +64,9 @@ def test_c_entries_refuse_before_launch():
     assert attend(dtype=0) == 2 and attend(D=16) == 2 and attend(H=3) == 1 and attend(R=0) == 1 and attend(q=0) == 1
     assert attend(o=8) == 1 and attend(stride=128) == 1 and attend(scale=math.inf) == 1 and attend(scale=math.nan) == 1
     assert attend(ancestors=16, words=0) == 1 and attend(ancestors=16, words=1, most=65, rows=65) == 1
+    assert attend(n=0) == 1 and attend(n=65, ws=16) == 1 and attend(n=2) == 1 and attend(n=2, ws=8) == 1
+    assert lib.gki_paged_slices(0, 1, 4, 2, 64, 8, 64, 4, 8) == 1 and lib.gki_paged_slices(9, 1, 3, 2, 64, 8, 64, 4, 8) == 1
+    assert lib.gki_paged_workspace_floats(5, 4, 64, 1) == 0 and lib.gki_paged_workspace_floats(5, 4, 64, 3) == 5 * (4 * 3 * 66 + 1)
     assert attend(sink=2**30) == 1 and attend(window=-1) == 1 and attend(rows=0) == 0
     assert lib.gki_paged_accept(16, 16, 16, 16, 0, 16, 2, 2, 5, 2, 64, 9, 64, NULL) == 1
     assert lib.gki_paged_accept(16, 16, 16, 16, 16, 16, 0, 2, 5, 2, 64, 9, 64, NULL) == 2
@@ -325,6 +328,54 @@ def test_trees_against_64_bits(dtype, D, page, heads, kv, sink, window, past, co
     o, lse = run.cache.attend(q, batch, return_lse=True)
     run.check_tables(batch)
     run.check_attend(batch, q, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slices", [1, 2, 7, 64])
+@pytest.mark.parametrize("counts,tree", [([1, 1, 1, 1], False), ([6, 1, 0, 20], False), ([40, 1, 300, 7], False), ([12, 30, 8, 1], True)])
+def test_any_number_of_slices(slices, counts, tree, monkeypatch):
+    monkeypatch.setattr(_lib.load(), "gki_paged_slices", lambda *a: slices)
+    rng = random.Random(17)
+    run = Run(4, 600, 4, 1500, 32, 2, 128, torch.bfloat16, seed=17)
+    run.grow([5000, 900, 0, 1600])
+    trees = [_tree(rng, n) for n in counts] if tree else None
+    batch = run.extend(counts, max_count=max(counts), parents=trees)
+    run.append(batch)
+    q = run.normal(batch.rows, 8)
+    o, lse = run.cache.attend(q, batch, return_lse=True)
+    run.check_attend(batch, q, o, lse)
+    assert torch.equal(o, run.cache.attend(q, batch))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slices", [1, None])
+@pytest.mark.parametrize("counts", [[1, 1], [2, 50]])
+def test_more_pages_than_are_held_at_once(slices, counts, monkeypatch):
+    """Walks of more than 1024 pages of 16 keys."""
+    if slices:
+        monkeypatch.setattr(_lib.load(), "gki_paged_slices", lambda *a: slices)
+    run = Run(2, 4200, 4, 30000, 16, 1, 64, torch.float16, seed=18)
+    run.grow([35000, 17000], 9000)
+    batch = run.extend(counts)
+    run.append(batch)
+    q = run.normal(batch.rows, 2)
+    o, lse = run.cache.attend(q, batch, return_lse=True)
+    run.check_attend(batch, q, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [63, 64, 65, 200])
+def test_many_requests(R):
+    """More requests than a wave counts at once, some without tokens."""
+    rng = random.Random(R)
+    run = Run(R, 40 * R, 4, 700, 32, 2, 64, torch.bfloat16, seed=R)
+    run.grow([rng.choice([0, 3, 100, 1100]) for _ in range(R)])
+    for counts in ([rng.choice([0, 1, 1, 2]) for _ in range(R)], [rng.choice([0, 1, 20, 70]) for _ in range(R)], [0] * (R - 1) + [3]):
+        batch = run.extend(counts, sum(counts) + 2, max_count=max(counts))
+        run.append(batch)
+        q = run.normal(batch.rows, 8)
+        o, lse = run.cache.attend(q, batch, return_lse=True)
+        run.check_attend(batch, q, o, lse)
 
 
 @pytest.mark.gpu
