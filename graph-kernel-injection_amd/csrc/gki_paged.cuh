@@ -82,10 +82,12 @@ struct PagedArgs {
   int32_t* parts;                      // [rows] slices that a token has
 };
 
-// An upper bound of a launch's units: the target, and one for each row tile and head where
-// a slice ends short (few rows are one tile; 128 a tile fill fewer than all of them).
+// An upper bound of a launch's units: all slices of all row tiles (few rows are one tile;
+// 128 a tile fill fewer than all of them), or the target and one for each row tile and
+// head where a slice ends short.
 inline int64_t paged_units(const PagedArgs& a) {
-  return a.target + a.H_kv * ((int64_t)a.rows * a.group / 128 + std::min(a.R, a.rows));
+  const int64_t tiles = a.H_kv * ((int64_t)a.rows * a.group / 128 + std::min(a.R, a.rows));
+  return std::min(a.target + tiles, tiles * a.max_slices);
 }
 
 // Slices that the keys of a row tile can be cut into, from what the host knows: rows of the

@@ -125,21 +125,18 @@ __device__ inline bool find_unit(const PagedArgs& a, int block, Unit& u) {
   return false;
 }
 
-// Keys of the 64 from x0 on that a row sees.
-__device__ inline uint64_t seen_bits(const PagedArgs& a, int row, int pos, int base, int x0) {
+// Keys of the 64 from x0 on that the i-th of a request's tokens sees.
+__device__ inline uint64_t seen_bits(const PagedArgs& a, const Unit& u, uint32_t i, int x0) {
+  const bool tree = a.ancestors != nullptr;
+  const int pos = tree ? (a.positions + u.first)[i] : u.base + (int)i;
   const uint64_t rule = bit_range(pos - a.window + 1 - x0, 63) | bit_range(0, a.sink - 1 - x0);
-  if (a.ancestors == nullptr) return bit_range(0, pos - x0) & rule;
-  uint64_t bits = bit_range(0, base - 1 - x0) & rule;
-  const uint64_t* word = a.ancestors + (int64_t)row * a.words;
-  const int from = x0 - base;          // number of the node at x0
-  if (from > -64) {
-    if (from < 0) {
-      bits |= word[0] << -from;
-    } else if ((from >> 6) < a.words) {
-      const int w = from >> 6, sh = from & 63;
-      bits |= word[w] >> sh;
-      if (sh && w + 1 < a.words) bits |= word[w + 1] << (64 - sh);
-    }
+  uint64_t bits = bit_range(0, (tree ? u.base - 1 : pos) - x0) & rule;
+  const int from = x0 - u.base;        // number of the node at x0
+  if (tree && from > -64) {
+    const uint64_t* word = a.ancestors + (int64_t)u.first * a.words;
+    const int w = from >> 6, sh = from & 63;                 // from < 0: w = -1
+    if (w >= 0 && w < a.words) bits |= word[i * a.words + w] >> sh;
+    if (sh && w + 1 < a.words) bits |= word[i * a.words + w + 1] << (64 - sh);
   }
   return bits;
 }
@@ -148,7 +145,10 @@ __device__ inline uint64_t seen_bits(const PagedArgs& a, int row, int pos, int b
 // The page ids of up to 1024 / (pages per tile) tiles ahead are held in LDS.
 template <int D, bool ROW32>
 struct PageTiles {
-  DmaTile<D, 4, ROW32> dma;
+  static constexpr int NB = D / 8, NP = NB / 4;          // 1 KB blocks of a tile, of a wave
+  // byte offset of the lane's 16 bytes in a block of a page; where 32 consecutive rows are read
+  // (ROW32) the swizzle is that of the wave for each of its blocks
+  int voff[ROW32 ? 1 : NP], wave;
   KeyTiles keys;
   const int32_t* table;                // the request's pages
   int* ids;
@@ -158,7 +158,13 @@ struct PageTiles {
 
   __device__ inline PageTiles(const PagedArgs& a, const Unit& u, const KeyTiles& k, int* lds_ids, bool read_once)
       : keys(k), ids(lds_ids), once(read_once) {
-    dma.init(threadIdx.x);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int p = 0; p < (ROW32 ? 1 : NP); ++p) {
+      const int e = (4 * p + wave) * 512 + 8 * lane, row = e / D;
+      voff[p] = 2 * (row * D + ((((e % D) >> 3) ^ lds_swz<D, ROW32>(row)) << 3) - (4 * p + wave) * 512);
+    }
     table = a.table + (int64_t)u.r * a.max_pages;
     end = u.base + u.n;
     h = u.h;
@@ -186,15 +192,13 @@ struct PageTiles {
     const uint32_t l0 = lds_addr(lds);
     const int x0 = keys.first_key(c), i0 = (c - (filled - span)) * per;
 #pragma unroll
-    for (int p = 0; p < dma.NP; ++p) {
-      const int blk = 4 * p + dma.wave;
-      const int row = blk * (512 / D), x = x0 + row;             // the block's first row
+    for (int p = 0; p < NP; ++p) {
+      const int blk = 4 * p + wave, row = blk * (512 / D), x = x0 + row;      // the block's first row
       const int id = __builtin_amdgcn_readfirstlane(ids[i0 + (a.shift < 6 ? row >> a.shift : 0)]);
       const int in_page = x & ((1 << a.shift) - 1);
-      // as if the tile's row 0 lay in this page too: the lane's offsets are those of whole tiles
-      const int64_t row0 = ((((int64_t)max(id, 0) * a.H_kv + h) << a.shift) + in_page) - row;
-      const int rows = id < 0 ? 0 : row + max(0, min((1 << a.shift) - in_page, end - x));
-      dma_buf16(buffer_rsrc(pool + row0 * D, rows * D * 2), 2 * dma.off[p], l0 + blk * 1024, once);
+      const int64_t first = (((int64_t)max(id, 0) * a.H_kv + h) << a.shift) + in_page;
+      const int rows = id < 0 ? 0 : max(0, min(512 / D, end - x));
+      dma_buf16(buffer_rsrc(pool + first * D, rows * D * 2), voff[ROW32 ? 0 : p], l0 + blk * 1024, once);
     }
   }
 };
@@ -256,7 +260,7 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
   if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
   for (int c = page.c0; c < page.c1; ++c) {
     const int b = (c - page.c0) & 1;
-    wait_chunks<page.dma.NP, 2>(min(1, page.c1 - 1 - c));     // tile c has landed
+    wait_chunks<page.NP, 2>(min(1, page.c1 - 1 - c));     // tile c has landed
     __syncthreads();
     w.step(a, rule, sk + b * TILE, sv + b * TILE, page.keys.first_key(c), page.end);
     __syncthreads();                             // every wave is done with buffer b
@@ -278,21 +282,28 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
 // ---------------------------------------------------------------------------
 // Tiles of 128 rows.
 // ---------------------------------------------------------------------------
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16, a wave's 32 rows as columns, the
+// row sums on the matrix pipe too. At head_dim 128 the loop is skewed by one key tile, as
+// in the prefill forward: S of tile c + 1 (matrix cores) while tile c's probabilities are
+// formed (VALU), then O of tile c while the maxima of S are taken, the two interleaved by
+// sched_group_barrier. K is read one tile ahead of V.
+template <int D> constexpr bool kPagedSkew = D >= 128;
+constexpr int kAheadS = 4, kAheadO = 8, kValuS = 3, kValuO = 1;
+
 template <typename T, int D>
 __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int* ids) {
   constexpr int KS = D / 16, DT = D / 32, TILE = kTileN * D;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rows = u.n * a.group, row0 = u.tile * kRowTile;
+  const int rows = u.n * a.group, row0 = u.tile * kRowTile, roww = row0 + wave * 32;
   const int hi = lane >> 5, col = lane & 31;
   const Lane32<D> lanes(lane);
-  const int my = row0 + wave * 32 + col;                   // the lane's row of the request's
-  const bool mine = my < rows;
-  const int token = u.first + (mine ? my / a.group : 0), head = u.h * a.group + (mine ? my % a.group : 0);
-  const int pos = a.positions[token];
+  const bool mine = roww + col < rows;                     // the lane's row of the request's
+  const uint32_t token = mine ? (roww + col) / a.group : 0;      // the request's
+  const int head = u.h * a.group + (mine ? (roww + col) % a.group : 0);
   uint4 qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    uint4 w = *(const uint4*)(a.q + (int64_t)token * a.q_stride + head * D + 16 * ks + 8 * hi);
+    uint4 w = *(const uint4*)(a.q + (int64_t)(u.first + token) * a.q_stride + head * D + 16 * ks + 8 * hi);
     w = make_uint4((w.x & a.q_and) ^ a.q_xor, (w.y & a.q_and) ^ a.q_xor, (w.z & a.q_and) ^ a.q_xor, (w.w & a.q_and) ^ a.q_xor);
     qf[ks] = mine ? w : make_uint4(0, 0, 0, 0);
   }
@@ -303,97 +314,207 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   // an ancestor has a lower number, a node's position is at least base
   const KeyTiles keys(a, u.base + (tree ? 0 : row0 / a.group), u.base + last_token + 1);
   PageTiles<D, true> page(a, u, keys, ids, rows <= kRowTile);
+  // the wave's rows see all keys up to all_to that no window hides: it reaches from above last_pos - W
+  const bool active = roww < rows;
+  const int all_to = tree ? u.base - 1 : u.base + min(roww, rows - 1) / a.group;
+  const int hidden_to = u.base + min(roww + 31, rows - 1) / a.group - a.window;
 
   floatx16 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = splat16(0.f);
   floatx4 lsum = floatx4{0.f, 0.f, 0.f, 0.f};
   // row sums on the matrix pipe: lane l gets that of row l & 31 of the operand of 32 rows
-  const uint4 ones = ((lane >> 2) & 1) == ((lane >> 4) & 1) ? T::ones8() : make_uint4(0, 0, 0, 0);
+  const uint32_t one = ((lane >> 2) & 1) == ((lane >> 4) & 1) ? T::ones8().x : 0u;
   const float slack = kStreamSlack / a.scale_log2;
   float nm = 0.f, thr = kNegInf;
 
-  if (page.c0 < page.c1) {
-    page.before(a, page.c0);
-    page.load(a, a.k_pages, page.c0, sk);
-    page.load(a, a.v_pages, page.c0, sv);
-  }
-  dma_wait();
-  __syncthreads();
-  auto step = [&](int c, int buf) {
+  auto scores = [&](const uint16_t* ck, floatx16 (&s)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[t] = T::mfma32(lanes.rows(ck, t, ks), qf[ks], ks == 0 ? splat16(0.f) : s[t]);
+  };
+  auto mask = [&](int c, floatx16 (&s)[2]) {
     const int x0 = keys.first_key(c);
-    if (c + 1 < page.c1) {
-      page.before(a, c + 1);
-      page.load(a, a.k_pages, c + 1, sk + (buf ^ 1) * TILE);
-      page.load(a, a.v_pages, c + 1, sv + (buf ^ 1) * TILE);
+    if (x0 + kTileN - 1 <= all_to && (x0 > hidden_to || x0 + kTileN <= a.sink)) return;
+    const uint64_t bits = seen_bits(a, u, token, x0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const LaneBits32 vis((uint32_t)(bits >> (32 * t)), hi);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = vis.pick(r, s[t][r], kNegInf);
     }
-    if (row0 + wave * 32 < rows) {
-      floatx16 s[2];
+  };
+  auto lane_max = [&](const floatx16 (&s)[2]) {
+    float mx = kNegInf;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          s[t] = T::mfma32(lanes.rows(sk + buf * TILE, t, ks), qf[ks], ks == 0 ? splat16(0.f) : s[t]);
-      const uint64_t bits = mine ? seen_bits(a, token, pos, u.base, x0) : 0;
-      float mx = kNegInf;
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+    return mx;
+  };
+  // the reference follows the row's largest score where this exceeds it by the slack
+  auto move_max = [&](float mx) {
+    if (__any(mx > thr)) {
+      const float mr = half_max(mx);
+      const bool grow = mr > thr;
+      const float nm1 = grow ? -mr * a.scale_log2 : nm;
+      // a first reference below zero scales nothing yet (o = lsum = 0)
+      const float alpha = __builtin_amdgcn_exp2f(fminf(nm1 - nm, 0.f));
+      nm = nm1;
+      thr = grow ? mr + slack : thr;
+      lsum[0] *= alpha;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const LaneBits32 vis((uint32_t)(bits >> (32 * t)), hi);
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
+  };
+  auto probs = [&](floatx16 (&s)[2], uint4 (&p)[4]) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[t][r] = vis.pick(r, s[t][r], kNegInf);
-          mx = fmaxf(mx, s[t][r]);
-        }
-      }
-      if (__any(mx > thr)) {
-        const float mr = half_max(mx);
-        const bool grow = mr > thr;
-        const float nm1 = grow ? -mr * a.scale_log2 : nm;
-        // a first reference below zero scales nothing yet (o = lsum = 0)
-        const float alpha = __builtin_amdgcn_exp2f(fminf(nm1 - nm, 0.f));
-        nm = nm1;
-        thr = grow ? mr + slack : thr;
-        lsum[0] *= alpha;
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-      }
-      uint4 p[4];
+      for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2, nm));
+      p[2 * t] = pack8<T>(s[t], 0);
+      p[2 * t + 1] = pack8<T>(s[t], 1);
+    }
+  };
+  auto pin = [&](uint4 (&p)[4]) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+    for (int st = 0; st < 4; ++st) {
+      u32x4 w = __builtin_bit_cast(u32x4, p[st]);
+      asm volatile("" : "+v"(w));
+      p[st] = __builtin_bit_cast(uint4, w);
+    }
+  };
+  auto accumulate = [&](const uint16_t* cv, const uint4 (&p)[4]) {
+    uint32_t w = one;                  // the operand is made here: four registers fewer while P is formed
+    asm volatile("" : "+v"(w));
+    const uint4 ones = make_uint4(w, w, w, w);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2, nm));
-        p[2 * t] = pack8<T>(s[t], 0);
-        p[2 * t + 1] = pack8<T>(s[t], 1);
-      }
+    for (int st = 0; st < 4; ++st) {
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma32(lanes.cols(sv + buf * TILE, st, dt), p[st], o[dt]);
-        lsum = T::mfma(ones, p[st], lsum);
-      }
+      for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma32(lanes.cols(cv, st, dt), p[st], o[dt]);
+      lsum = T::mfma(ones, p[st], lsum);
+    }
+  };
+  auto stage_k = [&](int c, int b) {
+    page.before(a, c);
+    page.load(a, a.k_pages, c, sk + b * TILE);
+  };
+  auto stage_v = [&](int c, int b) { page.load(a, a.v_pages, c, sv + b * TILE); };
+  const int c0 = page.c0, n = page.c1 - page.c0;
+  if constexpr (!kPagedSkew<D>) {
+    if (n > 0) {
+      stage_k(c0, 0);
+      stage_v(c0, 0);
     }
     dma_wait();
     __syncthreads();
-  };
-  int c = page.c0;
-  for (; c + 1 < page.c1; c += 2) {
-    step(c, 0);
-    step(c + 1, 1);
+    // unrolled by two so that the buffers are constants of the instructions
+    auto step = [&](int j, int buf) {
+      if (j + 1 < n) {
+        stage_k(c0 + j + 1, buf ^ 1);
+        stage_v(c0 + j + 1, buf ^ 1);
+      }
+      if (active) {
+        floatx16 s[2];
+        uint4 p[4];
+        mfma_priority_hi<true>();
+        scores(sk + buf * TILE, s);
+        mfma_priority_lo<true>();
+        mask(c0 + j, s);
+        move_max(lane_max(s));
+        probs(s, p);
+        mfma_priority_hi<true>();
+        accumulate(sv + buf * TILE, p);
+        mfma_priority_lo<true>();
+      }
+      dma_wait();
+      __syncthreads();
+    };
+    int j = 0;
+    for (; j + 1 < n; j += 2) {
+      step(j, 0);
+      step(j + 1, 1);
+    }
+    if (j < n) step(j, 0);
+  } else {
+    // prologue: K_0, V_0 and K_1 in LDS, S_0 with its maxima
+    floatx16 sa[2], sb[2];
+    if (n > 0) {
+      stage_k(c0, 0);
+      stage_v(c0, 0);
+      if (n > 1) stage_k(c0 + 1, 1);
+    }
+    dma_wait();
+    __syncthreads();
+    if (n > 0 && active) {
+      scores(sk, sa);
+      mask(c0, sa);
+      move_max(lane_max(sa));
+    }
+    __syncthreads();   // every wave is done with K_0 before iteration 0 refills its buffer
+    auto step = [&](int j, int par, floatx16 (&s)[2], floatx16 (&sn)[2]) {   // par = j & 1
+      stage_v(c0 + j + 1, par ^ 1);
+      if (j + 2 < n) stage_k(c0 + j + 2, par);
+      if (active) {
+        uint4 p[4];
+        scores(sk + (par ^ 1) * TILE, sn);
+        probs(s, p);
+        pin(p);                        // P is formed here, not sunk past the mask branch into the next block
+        __builtin_amdgcn_sched_group_barrier(0x100, kAheadS, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (i + kAheadS < 2 * KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, kValuS, 0);
+        }
+        mask(c0 + j + 1, sn);
+        accumulate(sv + par * TILE, p);
+        const float mx = lane_max(sn);
+        __builtin_amdgcn_sched_group_barrier(0x100, kAheadO, 1);
+#pragma unroll
+        for (int i = 0; i < 4 * DT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+          if (2 * i + kAheadO < 8 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+          __builtin_amdgcn_sched_group_barrier(0x002, kValuO, 1);
+        }
+        move_max(mx);
+      }
+      dma_wait();
+      __syncthreads();
+    };
+    // unrolled by two so that the score buffers swap roles without copies
+    int j = 0;
+    for (; j + 2 < n; j += 2) {
+      step(j, 0, sa, sb);
+      step(j + 1, 1, sb, sa);
+    }
+    if (j + 1 < n) {
+      step(j, 0, sa, sb);
+      sa[0] = sb[0], sa[1] = sb[1];
+    }
+    if (n > 0 && active) {
+      uint4 p[4];
+      probs(sa, p);
+      pin(p);
+      accumulate(sv + ((n - 1) & 1) * TILE, p);
+    }
   }
-  if (c < page.c1) step(c, 0);
 
-  if (!mine) return;
+  // the row afresh, not held through the loop
+  const int lane_e = lane_now(), hi_e = lane_e >> 5, my = roww + (lane_e & 31);
+  if (my >= rows) return;
   const float l = lsum[0];
-  const int64_t row = (int64_t)token * a.H + head;
+  const int64_t row = (int64_t)(u.first + my / a.group) * a.H + u.h * a.group + my % a.group;
   if (u.n_slices > 1) {
     float* dst = slice_acc(a, row, u.slice, D);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        *(floatx4*)(dst + 32 * dt + 8 * r + 4 * hi) =
+        *(floatx4*)(dst + 32 * dt + 8 * r + 4 * hi_e) =
             floatx4{o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]};
-    if (hi == 0) *slice_ml(a, row, u.slice) = make_float2(l == 0.f ? kNegInf : -nm, l);
+    if (hi_e == 0) *slice_ml(a, row, u.slice) = make_float2(l == 0.f ? kNegInf : -nm, l);
     return;
   }
   const float inv = l > 0.f ? 1.f / l : 1.f;
@@ -401,9 +522,9 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      *(uint2*)(a.o + row * D + 32 * dt + 8 * r + 4 * hi) =
+      *(uint2*)(a.o + row * D + 32 * dt + 8 * r + 4 * hi_e) =
           make_uint2(pack2<T>(o[dt][4 * r] * inv, o[dt][4 * r + 1] * inv), pack2<T>(o[dt][4 * r + 2] * inv, o[dt][4 * r + 3] * inv));
-  if (hi == 0 && a.lse) a.lse[row] = l > 0.f ? lse_natural(-nm, l) : 0.f;
+  if (hi_e == 0 && a.lse) a.lse[row] = l > 0.f ? lse_natural(-nm, l) : 0.f;
 }
 
 template <typename T, int D>

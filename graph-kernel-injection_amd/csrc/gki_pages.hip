@@ -319,14 +319,15 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(PageRows p, RotaryA
     }
 }
 
-// Rows of each request's accepted path to the slots of its first tokens. Node i of a path
-// is number path[i] >= i of the request's rows: a thread moves its 16 bytes of one row
-// after the other, so that each is read before its slot is written; a node that is not
-// such a number moves nothing.
+// Rows of each request's accepted path to the slots of its first tokens. Node i of a path is
+// number path[i] > i of the request's rows, or moves nothing. A thread has 16 bytes of every
+// row of a (request, head): it reads eight rows before it writes them, and what a later one
+// reads has a higher number than all that were written. Bound by latency (paths, slots,
+// rows, one after the other).
 template <int D>
 __global__ __launch_bounds__(256) void move_kernel(PageRows p, const int32_t* row_starts, const int32_t* paths,
                                                    const int32_t* accepted, int R, int path_len) {
-  constexpr int LPR = D / 8;
+  constexpr int LPR = D / 8, N = 8;
   const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
   const int ch = threadIdx.x % LPR;
   if (x >= 2ll * R * p.H_kv) return;
@@ -336,12 +337,26 @@ __global__ __launch_bounds__(256) void move_kernel(PageRows p, const int32_t* ro
   const int row0 = row_starts[r], n = row_starts[r + 1] - row0;
   const int last = min(min(accepted[r], n), path_len);
   uint16_t* pool = (uint16_t*)(is_v ? p.v_pages : p.k_pages) + 8 * ch;
-  for (int i = 0; i < last; ++i) {
-    const int j = paths[(int64_t)r * path_len + i];
-    if (j <= i || j >= n) continue;
-    const int64_t a = p.slots[row0 + j], b = p.slots[row0 + i];
-    if (a < 0 || a >= p.n_slots || b < 0 || b >= p.n_slots) continue;
-    *(uint4*)(pool + p.at(b, h, D)) = *(const uint4*)(pool + p.at(a, h, D));
+  for (int i0 = 0; i0 < last; i0 += N) {
+    int node[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      node[e] = paths[(int64_t)r * path_len + min(i0 + e, last - 1)];
+      if (i0 + e >= last || node[e] <= i0 + e || node[e] >= n) node[e] = -1;
+    }
+    int64_t from[N], to[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      from[e] = p.slots[row0 + max(node[e], 0)];
+      to[e] = p.slots[row0 + min(i0 + e, last - 1)];
+      if (from[e] < 0 || from[e] >= p.n_slots || to[e] < 0 || to[e] >= p.n_slots) node[e] = -1;
+    }
+    u32x4 w[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = *(const u32x4*)(pool + (node[e] < 0 ? 0 : p.at(from[e], h, D)));
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (node[e] >= 0) *(u32x4*)(pool + p.at(to[e], h, D)) = w[e];
   }
 }
 
