@@ -937,21 +937,22 @@ int gki_paged_accept(void* k_pages, void* v_pages, const int64_t* slots, const i
                              row_starts, paths, accepted, R, path_len, (hipStream_t)stream);
 }
 
-int gki_paged_slices(int32_t rows, int32_t max_count, int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages,
-                     int32_t page_size, int32_t sink_size, int32_t window_size) {
-  if (rows <= 0 || max_count < 0 || H <= 0 || H_kv <= 0 || H % H_kv || max_pages <= 0 || page_size <= 0) return 1;
-  return paged_max_slices(head_dim, rows, max_count, H_kv, H / H_kv, sink_size, window_size, (int64_t)max_pages * page_size);
-}
-
-int64_t gki_paged_workspace_floats(int32_t rows, int32_t H, int32_t head_dim, int32_t n_slices) {
-  return n_slices > 1 ? (int64_t)rows * ((int64_t)H * n_slices * (head_dim + 2) + 1) : 0;
+int gki_paged_groups(int32_t max_count, int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t page_size,
+                     int32_t sink_size, int32_t window_size, int64_t* workspace_floats) {
+  const int groups = paged_groups(head_dim);
+  if (workspace_floats) {
+    const bool ok = max_count > 0 && H > 0 && H_kv > 0 && H % H_kv == 0 && max_pages > 0 && page_size > 0;
+    *workspace_floats = ok ? paged_workspace(groups, head_dim, max_count, H / H_kv, sink_size, window_size,
+                                             (int64_t)max_pages * page_size) : 0;
+  }
+  return groups;
 }
 
 int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o, float* lse,
                      const int32_t* row_starts, const int32_t* base, const int32_t* positions, const int32_t* table,
                      const uint64_t* ancestors, int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R,
                      int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t num_pages, int32_t page_size,
-                     int32_t sink_size, int32_t window_size, float softmax_scale, float* workspace, int32_t n_slices,
+                     int32_t sink_size, int32_t window_size, float softmax_scale, float* workspace, int32_t groups,
                      void* stream) {
   if (int rc = paged_pool("gki_paged_attend", dtype, head_dim, H_kv, num_pages, page_size)) return rc;
   GKI_REQUIRE(rows >= 0 && max_count >= 0 && R > 0 && R <= (1 << 20) && H > 0 && H % H_kv == 0 && max_pages > 0, 1,
@@ -966,8 +967,7 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   GKI_REQUIRE(all_aligned16(q, k_pages, v_pages, o, workspace), 1, "gki_paged_attend: tensors must be 16-byte aligned");
   GKI_REQUIRE(row_stride_ok(q_stride, (int64_t)H * head_dim), 1,
               "gki_paged_attend: the row stride must be a multiple of 8 elements that holds a row");
-  GKI_REQUIRE(n_slices >= 1 && n_slices <= 64 && (n_slices == 1 || workspace), 1,
-              "gki_paged_attend: n_slices must be in 1 .. 64, and several need a workspace");
+  GKI_REQUIRE(groups >= 1 && groups <= 4096, 1, "gki_paged_attend: groups must be in 1 .. 4096");
   Geom g;
   set_scale(g, softmax_scale);
   PagedArgs a{};
@@ -980,11 +980,18 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   a.sink = sink_size, a.window = std::min(window_size, 1 << kPartialBit), a.words = words;
   a.scale_log2 = g.qk_scale_log2, a.q_and = g.q_and, a.q_xor = g.q_xor;
   a.q_sign = softmax_scale == 0.f ? 0.f : softmax_scale < 0.f ? -1.f : 1.f;
-  a.target = paged_target(head_dim), a.min_slice = kPagedMinSlice, a.max_slices = n_slices, a.whole = kPagedWhole;
+  a.groups = groups;
+  a.cap = paged_cap(std::max(max_count, 1), a.group);
   a.acc = workspace;
-  a.ml = workspace + (int64_t)rows * H * n_slices * head_dim;
-  a.parts = (int32_t*)(a.ml + (int64_t)rows * H * n_slices * 2);
-  GKI_REQUIRE(paged_units(a) < (1ll << 24) && (int64_t)rows * H < (1ll << 26), 1, "gki_paged_attend: the grid must fit");
+  if (workspace) {
+    a.ml = workspace + 2ll * groups * a.cap * head_dim;
+    a.cuts = (CutTile*)(a.ml + 4ll * groups * a.cap);
+  }
+  GKI_REQUIRE((int64_t)rows * H < (1ll << 26), 1, "gki_paged_attend: the grid must fit");
+  const int64_t tiles = ((int64_t)rows * a.group / 128 + std::min(R, rows)) * H_kv;
+  const int64_t keys = std::min<int64_t>((int64_t)max_pages * page_size, (int64_t)sink_size + a.window + max_count) / 64 + 4;
+  while (tiles * (std::max<int64_t>(kPagedMinShare, keys >> a.coarse) + 1) >= (1ll << 31) && a.coarse < 31) ++a.coarse;
+  GKI_REQUIRE(a.coarse < 31, 1, "gki_paged_attend: the grid must fit");
   return paged_attend_dispatch(dtype, head_dim, a, (hipStream_t)stream);
 }
 

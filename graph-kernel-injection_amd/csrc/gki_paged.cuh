@@ -61,9 +61,9 @@ struct PageRows {
   }
 };
 
-constexpr int kPagedWhole = 12;        // key tiles
-constexpr int kPagedMinSlice = 4;
-inline int paged_target(int head_dim) { return head_dim >= 128 ? 512 : 1024; }
+// Key tiles that a workgroup's share has at least, and workgroups that the card holds at once.
+constexpr int kPagedMinShare = 8;
+inline int paged_groups(int head_dim) { return head_dim >= 128 ? 512 : 768; }
 
 struct PagedArgs {
   const uint16_t *q, *k_pages, *v_pages;
@@ -75,30 +75,27 @@ struct PagedArgs {
   int R, rows, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;
   float scale_log2, q_sign;            // as StreamArgs': the sign of the scale, or zero, goes to q
   uint32_t q_and, q_xor;               // the same as words of Q
-  // slices of the keys: about `target` units in all, of at least min_slice key tiles, up
-  // to max_slices of a row tile, none of fewer than `whole` key tiles
-  int target, min_slice, max_slices, whole;
-  float *acc, *ml;                     // their states
-  int32_t* parts;                      // [rows] slices that a token has
+  int groups;                          // workgroups that share the work
+  int coarse;                          // a step of the work is 2^coarse key tiles, so that 31 bits count them all
+  // the states of row tiles that the shares' ends cut, of `cap` rows each; acc null: none is cut
+  int cap;
+  float *acc, *ml;
+  struct CutTile* cuts;                // [groups]
 };
 
-// An upper bound of a launch's units: all slices of all row tiles (few rows are one tile;
-// 128 a tile fill fewer than all of them), or the target and one for each row tile and
-// head where a slice ends short.
-inline int64_t paged_units(const PagedArgs& a) {
-  const int64_t tiles = a.H_kv * ((int64_t)a.rows * a.group / 128 + std::min(a.R, a.rows));
-  return std::min(a.target + tiles, tiles * a.max_slices);
-}
+// A row tile that ends a workgroup's share unfinished: its request's rows, its pieces (0: none).
+struct CutTile {
+  int first, n, h, tile, pieces;
+};
 
-// Slices that the keys of a row tile can be cut into, from what the host knows: rows of the
-// step, the largest count, and what a row can see.
-inline int paged_max_slices(int head_dim, int64_t rows, int64_t max_count, int H_kv, int group, int64_t sink,
-                            int64_t window, int64_t max_length) {
+// Rows of a piece's state, and the floats of all states and cuts (0 where no row tile's walk,
+// by what the host knows, is long enough to be cut).
+inline int paged_cap(int64_t max_count, int group) { return (int)std::min<int64_t>(128, max_count * group); }
+inline int64_t paged_workspace(int groups, int head_dim, int64_t max_count, int group, int64_t sink, int64_t window,
+                               int64_t max_length) {
   const int64_t seen = std::min(max_length, sink + window + max_count + 64);
-  const int64_t keys = (seen + 63) / 64 + 2, tiles = (rows * group + 127) / 128;
-  if (keys < kPagedWhole) return 1;
-  const int64_t most = (3 * paged_target(head_dim) / 2 + H_kv * tiles - 1) / (H_kv * tiles);
-  return (int)std::max<int64_t>(1, std::min({most, (keys + kPagedMinSlice - 1) / kPagedMinSlice, (int64_t)64}));
+  if ((seen + 63) / 64 + 2 < 2 * kPagedMinShare) return 0;
+  return (int64_t)groups * (2 * paged_cap(max_count, group) * (head_dim + 2) + 5);
 }
 
 }  // namespace gki

@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kRowTile = 128;          // rows of a tile: four waves of 32
 constexpr int kFewRows = 32;           // up to as many run as a stream
-constexpr int kIds = 1024;             // page ids held in LDS at a time
+constexpr int kPagePieces = 512;       // pieces of pages whose places are held in LDS at a time
 
 // The 64-key tiles that rows at positions lo_pos .. see of keys 0 .. end - 1: the sinks',
 // then the window's.
@@ -39,90 +39,144 @@ struct KeyTiles {
 };
 
 // ---------------------------------------------------------------------------
-// Which unit of work a workgroup takes. A unit is a slice of the keys of a row tile of one
-// request and kv head. Lengths are known on the device only, so every workgroup counts
-// for itself, a wave 64 requests at a time: the key tiles of all row tiles, from them the
-// length of a slice that fills the card, from it the units. The units of a (request, head)
-// are neighbours on one XCD, a slice's row tiles side by side.
+// Which work a workgroup takes. The key tiles of all row tiles of all requests and kv heads,
+// one after the other (request, head, row tile, key tile), are cut into equal shares, a
+// workgroup each: requests of any lengths load the card evenly. A row tile that a cut
+// divides leaves the states of its pieces, which are joined; a cut close to its ends
+// moves there. Lengths are known on the device only, so every workgroup counts for
+// itself, a wave 64 requests at a time. Neighbours work on one XCD: row tiles of a
+// (request, head) meet their keys in its L2.
 // ---------------------------------------------------------------------------
+// Sum of lanes 0 .. l, by DPP.
+template <int CTRL, int ROWS>
+__device__ inline uint32_t dpp_or_zero(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+__device__ inline uint32_t wave_prefix(uint32_t x) {
+  x += dpp_or_zero<0x111, 0xF>(x);     // row_shr 1, 2, 4, 8
+  x += dpp_or_zero<0x112, 0xF>(x);
+  x += dpp_or_zero<0x114, 0xF>(x);
+  x += dpp_or_zero<0x118, 0xF>(x);
+  x += dpp_or_zero<0x142, 0xA>(x);     // lane 15 of a row to the next, for rows 1 and 3
+  x += dpp_or_zero<0x143, 0xC>(x);     // lane 31 to rows 2 and 3
+  return x;
+}
+__device__ inline uint32_t lane_of(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
+__device__ inline uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
 struct Request {
-  int first, n, base, tiles, keys;     // first row of the step's, rows, keys before them; row tiles, key tiles
-  __device__ inline Request(const PagedArgs& a, int r) {
-    const bool ok = r < a.R;
-    r = ok ? r : a.R - 1;
+  uint32_t first, n, base, tiles, keys;  // first row of the step's, rows, keys before them; row tiles, the steps of each
+  __device__ inline Request(const PagedArgs& a, int r, int end) {
+    const bool ok = r < end;
+    r = ok ? r : 0;
     first = a.row_starts[r];
     n = ok ? a.row_starts[r + 1] - first : 0;
     base = a.base[r];
-    const int rows = n * a.group;
+    const uint32_t rows = n * a.group;
     tiles = rows <= kFewRows ? (rows + kFewRows - 1) / kFewRows : (rows + kRowTile - 1) / kRowTile;
-    keys = n ? KeyTiles(a, base, base + n).n : 0;
+    // a short walk counts for more than its key tiles: it has its prologue and epilogue too
+    const uint32_t k = KeyTiles(a, base, base + n).n;
+    keys = max((uint32_t)kPagedMinShare, (k + (1u << a.coarse) - 1) >> a.coarse);
   }
-  // Slices of about `length` key tiles.
-  __device__ inline int slices(const PagedArgs& a, int length) const {
-    return keys < a.whole ? 1 : min(a.max_slices, (keys + length - 1) / length);
+  __device__ inline uint32_t steps(const PagedArgs& a) const { return tiles * a.H_kv * keys; }
+};
+
+// The row tile that holds a step: its request, which of the request's it is (head by head),
+// its first step.
+struct Place {
+  uint32_t first, n, base, tiles, keys, number, start;
+  int r;
+  __device__ inline void set(const Request& q, int l, int request, uint32_t before, uint32_t step) {
+    r = request;
+    first = lane_of(q.first, l), n = lane_of(q.n, l), base = lane_of(q.base, l);
+    tiles = lane_of(q.tiles, l), keys = lane_of(q.keys, l);
+    number = scalar((step - before) / keys);
+    start = before + number * keys;
   }
 };
 
-__device__ inline int64_t wave_sum64(int64_t x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);       // the same everywhere: scalar
-  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | lo);
-}
-// Sum of lanes 0 .. l.
-__device__ inline int wave_prefix(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
+struct Shares {
+  Request q;                           // the lane's (its first of `run`)
+  int run;                             // requests per lane
+  uint32_t sum;                        // steps of lanes 0 .. this one
+  uint32_t all, share;                 // steps in all, of a workgroup
+  uint32_t edge;                       // cuts this close to a row tile's ends move there
+  int lane;
+  __device__ inline Shares(const PagedArgs& a, int tid)
+      : q(a, (tid & 63) * ((a.R + 63) >> 6), a.R), run((a.R + 63) >> 6), lane(tid & 63) {
+    uint32_t mine = q.steps(a);
+    for (int i = 1; i < run; ++i) mine += Request(a, lane * run + i, a.R).steps(a);
+    sum = wave_prefix(mine);
+    all = lane_of(sum, 63);
+    share = scalar(max((uint32_t)kPagedMinShare, (all + a.groups - 1) / a.groups));
+    edge = max((uint32_t)kPagedMinShare / 2, share / 4);
   }
-  return x;
-}
-__device__ inline int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+  __device__ inline Place place(const PagedArgs& a, uint32_t step) const {      // step < all
+    Place p;
+    const int l = __builtin_ctzll(__ballot(sum > step));
+    uint32_t before = l ? lane_of(sum, l - 1) : 0;
+    if (run == 1) {
+      p.set(q, l, l, before, step);
+      return p;
+    }
+    const int end = min((l + 1) * run, a.R);
+    for (int r0 = l * run;; r0 += 64) {
+      const Request x(a, r0 + lane, end);
+      const uint32_t upto = wave_prefix(x.steps(a));
+      const uint64_t past = __ballot(before + upto > step);
+      if (past || r0 + 64 >= end) {
+        const int m = past ? __builtin_ctzll(past) : 0;
+        p.set(x, m, r0 + m, before + (m ? lane_of(upto, m - 1) : 0), step);
+        return p;
+      }
+      before += lane_of(upto, 63);
+    }
+  }
+  // Where the cut at step c goes: it stays inside a row tile that is long enough.
+  __device__ inline uint32_t cut(const PagedArgs& a, uint32_t c) const {
+    if (c == 0 || c >= all) return min(c, all);
+    const Place p = place(a, c);
+    const uint32_t off = c - p.start;
+    if (off == 0 || (a.acc && p.keys >= 2 * kPagedMinShare && off >= edge && p.keys - off >= edge)) return c;
+    return 2 * off < p.keys ? p.start : p.start + p.keys;
+  }
+};
 
+// A piece of a row tile's walk: steps s0 .. s1 - 1 of `steps`. Of the pieces of a row tile that
+// is cut the first is the last of its workgroup's share, any other the first of its own: the
+// first of c workgroups from w on has state 2 w + 1, the others 2 (w + 1), 2 (w + 2), ...
 struct Unit {
   int r, first, n, base;               // the request
-  int h, tile, slice, n_slices;
+  int h, tile, state;                  // state -1: all of the walk
+  uint32_t s0, s1, steps;
+  __device__ inline Unit(const Place& p, uint32_t lo, uint32_t hi, int w) {
+    r = p.r, first = p.first, n = p.n, base = p.base;
+    h = scalar(p.number / p.tiles), tile = p.number - h * p.tiles;
+    steps = p.keys;
+    s0 = lo - p.start;
+    s1 = min(p.keys, hi - p.start);
+    state = s0 > 0 ? 2 * w : s1 < steps ? 2 * w + 1 : -1;
+  }
+  // The first of a walk's n key tiles that belongs to step s or a later one.
+  __device__ inline int tile_of(int n, uint32_t s) const {
+    if (s == 0 || s == steps || (uint32_t)n == steps) return s == steps ? n : s;
+    if ((n | s) < 65536) return scalar((uint32_t)n * s / steps);
+    return scalar((uint32_t)((uint64_t)n * s / steps));
+  }
 };
 
-__device__ inline bool find_unit(const PagedArgs& a, int block, Unit& u) {
-  const int lane = threadIdx.x & 63;
-  int64_t all = 0;
-  for (int r0 = 0; r0 < a.R; r0 += 64) {
-    const Request q(a, r0 + lane);
-    all += (int64_t)q.tiles * q.keys;
-  }
-  all = wave_sum64(all) * a.H_kv;
-  const int length = (int)max((int64_t)a.min_slice, (all + a.target - 1) / a.target);
-  int units = 0;
-  for (int r0 = 0; r0 < a.R; r0 += 64) {
-    const Request q(a, r0 + lane);
-    units += q.tiles * q.slices(a, length);
-  }
-  units = (int)wave_sum64(units) * a.H_kv;
-  if (block >= units) return false;
-  int t = xcd_remap(block, units);
-  for (int r0 = 0; r0 < a.R; r0 += 64) {
-    const Request q(a, r0 + lane);
-    const int mine = q.tiles * q.slices(a, length) * a.H_kv, sum = wave_prefix(mine);
-    const uint64_t past = __ballot(sum > t);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      u.r = r0 + l;
-      u.first = lane_value(q.first, l), u.n = lane_value(q.n, l), u.base = lane_value(q.base, l);
-      u.n_slices = lane_value(q.slices(a, length), l);
-      const int tiles = lane_value(q.tiles, l);
-      t -= lane_value(sum - mine, l);
-      u.tile = t % tiles;
-      t /= tiles;
-      u.slice = t % u.n_slices;
-      u.h = t / u.n_slices;
-      return true;
-    }
-    t -= lane_value(sum, 63);
-  }
-  return false;
+// The arguments of the running kernel, whose first they are, read anew where they are needed
+// once or seldom: they are not held in registers through the loops (scalar ones that do
+// not fit would take vector ones).
+__device__ inline PagedArgs fresh_args() {
+#ifdef __HIP_DEVICE_COMPILE__          // the host's pass does not know the builtin
+  const __attribute__((address_space(4))) PagedArgs* p =
+      (const __attribute__((address_space(4))) PagedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+#else
+  return PagedArgs{};
+#endif
 }
 
 // Keys of the 64 from x0 on that the i-th of a request's tokens sees.
@@ -142,64 +196,78 @@ __device__ inline uint64_t seen_bits(const PagedArgs& a, const Unit& u, uint32_t
 }
 
 // The key tiles of a unit, into LDS by LDS-DMA: a wave's 1 KB blocks, each from one page.
-// The page ids of up to 1024 / (pages per tile) tiles ahead are held in LDS.
-template <int D, bool ROW32>
+// Where the tiles' pieces (64 keys, or a page of 16 or 32) start in the pool is held in LDS
+// for up to kPieces of them at a time. ONCE: no other workgroup reads these keys.
+template <int D, bool ROW32, bool ONCE>
 struct PageTiles {
-  static constexpr int NB = D / 8, NP = NB / 4;          // 1 KB blocks of a tile, of a wave
+  static constexpr int NB = D / 8, NP = NB / 4, RB = 512 / D;      // 1 KB blocks of a tile, of a wave; rows of a block
   // byte offset of the lane's 16 bytes in a block of a page; where 32 consecutive rows are read
   // (ROW32) the swizzle is that of the wave for each of its blocks
   int voff[ROW32 ? 1 : NP], wave;
   KeyTiles keys;
-  const int32_t* table;                // the request's pages
-  int* ids;
-  int end, h, c0, c1, filled;          // its keys, the kv head; the unit's tiles; those from `filled` - span on are held
-  int per, span;                       // pages per tile (at least one), tiles that `ids` holds
-  bool once;                           // no other workgroup reads these rows
+  int64_t* pieces;                     // bytes from the pool's start, -1: no such page
+  int r, h, end, c0, c1, filled;       // its request, kv head, keys; the unit's tiles; those before `filled` are held
+  int piece, per, span;                // log2 of a piece's keys, pieces of a tile, tiles that `pieces` holds
 
-  __device__ inline PageTiles(const PagedArgs& a, const Unit& u, const KeyTiles& k, int* lds_ids, bool read_once)
-      : keys(k), ids(lds_ids), once(read_once) {
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+  __device__ inline PageTiles(const PagedArgs& a, const Unit& u, const KeyTiles& k, int64_t* lds, int tid)
+      : keys(k), pieces(lds), r(u.r), h(u.h), end(u.base + u.n) {
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63;
 #pragma unroll
     for (int p = 0; p < (ROW32 ? 1 : NP); ++p) {
       const int e = (4 * p + wave) * 512 + 8 * lane, row = e / D;
       voff[p] = 2 * (row * D + ((((e % D) >> 3) ^ lds_swz<D, ROW32>(row)) << 3) - (4 * p + wave) * 512);
     }
-    table = a.table + (int64_t)u.r * a.max_pages;
-    end = u.base + u.n;
-    h = u.h;
-    c0 = __builtin_amdgcn_readfirstlane((int)((int64_t)k.n * u.slice / u.n_slices));
-    c1 = __builtin_amdgcn_readfirstlane((int)((int64_t)k.n * (u.slice + 1) / u.n_slices));
-    per = max(1, kTileN >> a.shift);
-    span = kIds / per;
+    c0 = u.tile_of(k.n, u.s0);
+    c1 = u.tile_of(k.n, u.s1);
+    piece = min(a.shift, 6);
+    per = 64 >> piece;
+    span = kPagePieces / per;
     filled = c0;
   }
-  // The ids of tiles c .. c + span - 1; every wave comes here at the same tile.
-  __device__ inline void fill(const PagedArgs& a, int c) {
-    __syncthreads();                   // the ids before have been read
-    for (int i = threadIdx.x; i < min(span, c1 - c) * per; i += 256) {
-      const int x = keys.first_key(c + i / per) + (i % per << a.shift);
+  // The pieces of tiles c .. c + span - 1; every wave comes here at the same tile.
+  __device__ inline void fill(int c) {
+    const PagedArgs a = fresh_args();
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int32_t* table = a.table + (int64_t)r * a.max_pages;
+    __syncthreads();                   // the pieces before have been read
+    for (int i = tid; i < min(span, c1 - c) * per; i += 256) {
+      const int x = keys.first_key(c + i / per) + (i % per << piece);
       const int id = table[min(x, end - 1) >> a.shift];
-      ids[i] = x < end && (unsigned)id < (unsigned)a.num_pages ? id : -1;
+      const int64_t row = (((int64_t)id * a.H_kv + h) << a.shift) + (x & ((1 << a.shift) - 1));
+      pieces[i] = x < end && (unsigned)id < (unsigned)a.num_pages ? row * (2 * D) : -1;
     }
     __syncthreads();
     filled = c + span;
   }
-  __device__ inline void before(const PagedArgs& a, int c) {
-    if (c >= filled) fill(a, c);
-  }
-  __device__ inline void load(const PagedArgs& a, const uint16_t* pool, int c, const uint16_t* lds) const {
-    const uint32_t l0 = lds_addr(lds);
-    const int x0 = keys.first_key(c), i0 = (c - (filled - span)) * per;
+  __device__ inline void load(const uint16_t* pool, int c, const uint16_t* lds) {
+    if (c >= filled) fill(c);
+    int wave = this->wave;             // the wave's constants are made here, not held: scalars are short in the loops
+    asm volatile("" : "+s"(wave));
+    const uint32_t l0 = lds_addr(lds) + wave * 1024;
+    const int i0 = (c - (filled - span)) * per, x0 = keys.first_key(c);
+    if (per == 1) {
+      const int64_t at = scalar64(pieces[i0]);
+      const char* base = (const char*)pool + at + wave * 1024;
+      const int left = scalar(at < 0 ? 0 : end - x0);      // keys from the tile's first on
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int blk = 4 * p + wave, row = blk * (512 / D), x = x0 + row;      // the block's first row
-      const int id = __builtin_amdgcn_readfirstlane(ids[i0 + (a.shift < 6 ? row >> a.shift : 0)]);
-      const int in_page = x & ((1 << a.shift) - 1);
-      const int64_t first = (((int64_t)max(id, 0) * a.H_kv + h) << a.shift) + in_page;
-      const int rows = id < 0 ? 0 : max(0, min(512 / D, end - x));
-      dma_buf16(buffer_rsrc(pool + first * D, rows * D * 2), voff[ROW32 ? 0 : p], l0 + blk * 1024, once);
+      for (int p = 0; p < NP; ++p)
+        dma_buf16(buffer_rsrc(base + p * 4096, rows_left<RB>(left - (4 * p + wave) * RB) * D * 2), voff[ROW32 ? 0 : p],
+                  l0 + p * 4096, ONCE);
+    } else {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const int row = (4 * p + wave) * RB, y = row >> piece;             // the block's piece
+        const int64_t at = scalar64(pieces[i0 + y]);
+        const char* base = (const char*)pool + at + (row - (y << piece)) * (2 * D);
+        const int left = scalar(at < 0 ? 0 : end - x0 - row);
+        dma_buf16(buffer_rsrc(base, rows_left<RB>(left) * D * 2), voff[ROW32 ? 0 : p], l0 + p * 4096, ONCE);
+      }
     }
+  }
+  __device__ static inline int64_t scalar64(int64_t x) {
+    return (int64_t)((uint64_t)scalar((uint32_t)((uint64_t)x >> 32)) << 32 | scalar((uint32_t)x));
   }
 };
 
@@ -224,19 +292,14 @@ struct PagedRule {
   }
 };
 
-// The states that slices leave: acc [rows][max_slices][D], ml [rows][max_slices][2] for
-// rows = (token, q head), and how many a token has.
-__device__ inline float* slice_acc(const PagedArgs& a, int64_t row, int slice, int D) {
-  return a.acc + (row * a.max_slices + slice) * D;
-}
-__device__ inline float2* slice_ml(const PagedArgs& a, int64_t row, int slice) {
-  return (float2*)a.ml + row * a.max_slices + slice;
-}
+// Row r of a piece's state: acc [2 groups][cap][D], ml [2 groups][cap][2].
+__device__ inline float* piece_acc(const PagedArgs& a, int state, int r, int D) { return a.acc + ((int64_t)state * a.cap + r) * D; }
+__device__ inline float2* piece_ml(const PagedArgs& a, int state, int r) { return (float2*)a.ml + (int64_t)state * a.cap + r; }
 
 // As the streams of the other caches: two key tiles in flight, so that no registers hold
 // loads. Bound by HBM.
 template <typename T, int D, int NB>
-__device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int* ids) {
+__device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int64_t* pieces, int tid) {
   constexpr int TILE = kTileN * D;
   const int rows = u.n * a.group;
   auto token = [&](int r) { return u.first + min(r, rows - 1) / a.group; };
@@ -246,15 +309,14 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
       [&](int r) {
         const int t = token(r);
         return StreamRow{a.positions[t], a.ancestors ? a.ancestors[(int64_t)t * a.words] : 0};
-      });
+      }, tid);
   const PagedRule rule{u.base, u.base + u.n - 1, a.sink, a.window, a.ancestors != nullptr};
-  PageTiles<D, false> page(a, u, KeyTiles(a, u.base, u.base + u.n), ids, true);
+  PageTiles<D, false, true> page(a, u, KeyTiles(a, u.base, u.base + u.n), pieces, tid);
   dma_wait();   // the loads above are complete before any LDS-DMA is in flight
   auto issue = [&](int c) {
     const int b = (c - page.c0) & 1;
-    page.before(a, c);
-    page.load(a, a.k_pages, c, sk + b * TILE);
-    page.load(a, a.v_pages, c, sv + b * TILE);
+    page.load(a.k_pages, c, sk + b * TILE);
+    page.load(a.v_pages, c, sv + b * TILE);
   };
   if (page.c0 < page.c1) issue(page.c0);
   if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
@@ -266,17 +328,17 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
     __syncthreads();                             // every wave is done with buffer b
     if (c + 2 < page.c1) issue(c + 2);
   }
-  w.finish(rows, (float*)sk, (float*)sv, [&](int r, int d, floatx4 x, float M, float L) {
-    const int64_t row = (int64_t)token(r) * a.H + u.h * a.group + r % a.group;
-    if (u.n_slices == 1) {
+  w.finish(rows, (float*)sk, (float*)sv, [&, a = fresh_args()](int r, int d, floatx4 x, float M, float L) {
+    if (u.state < 0) {
+      const int64_t row = (int64_t)token(r) * a.H + u.h * a.group + r % a.group;
       x = x / (L == 0.f ? 1.f : L);              // no visible key: 0; NaN stays NaN
       *(uint2*)(a.o + row * D + d) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
       if (d == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
-    } else {
-      *(floatx4*)(slice_acc(a, row, u.slice, D) + d) = x;
-      if (d == 0) *slice_ml(a, row, u.slice) = make_float2(M, L);
+    } else if (r < a.cap) {
+      *(floatx4*)(piece_acc(a, u.state, r, D) + d) = x;
+      if (d == 0) *piece_ml(a, u.state, r) = make_float2(M, L);
     }
-  });
+  }, tid);
 }
 
 // ---------------------------------------------------------------------------
@@ -291,9 +353,9 @@ template <int D> constexpr bool kPagedSkew = D >= 128;
 constexpr int kAheadS = 4, kAheadO = 8, kValuS = 3, kValuO = 1;
 
 template <typename T, int D>
-__device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int* ids) {
+__device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int64_t* pieces, int tid) {
   constexpr int KS = D / 16, DT = D / 32, TILE = kTileN * D;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = u.n * a.group, row0 = u.tile * kRowTile, roww = row0 + wave * 32;
   const int hi = lane >> 5, col = lane & 31;
   const Lane32<D> lanes(lane);
@@ -310,21 +372,21 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   dma_wait();   // these loads are complete before any LDS-DMA is in flight
 
   const bool tree = a.ancestors != nullptr;
-  const int last_token = min(row0 + kRowTile - 1, rows - 1) / a.group;
+  // quotients as scalars, and with them the walk
+  const int last_token = scalar(min(row0 + kRowTile - 1, rows - 1) / a.group);
   // an ancestor has a lower number, a node's position is at least base
-  const KeyTiles keys(a, u.base + (tree ? 0 : row0 / a.group), u.base + last_token + 1);
-  PageTiles<D, true> page(a, u, keys, ids, rows <= kRowTile);
+  const KeyTiles keys(a, u.base + (tree ? 0 : (int)scalar(row0 / a.group)), u.base + last_token + 1);
+  PageTiles<D, true, false> page(a, u, keys, pieces, tid);
   // the wave's rows see all keys up to all_to that no window hides: it reaches from above last_pos - W
   const bool active = roww < rows;
-  const int all_to = tree ? u.base - 1 : u.base + min(roww, rows - 1) / a.group;
-  const int hidden_to = u.base + min(roww + 31, rows - 1) / a.group - a.window;
+  const int all_to = tree ? u.base - 1 : u.base + (int)scalar(min(roww, rows - 1) / a.group);
+  const int hidden_to = u.base + (int)scalar(min(roww + 31, rows - 1) / a.group) - a.window;
 
   floatx16 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = splat16(0.f);
   floatx4 lsum = floatx4{0.f, 0.f, 0.f, 0.f};
   // row sums on the matrix pipe: lane l gets that of row l & 31 of the operand of 32 rows
-  const uint32_t one = ((lane >> 2) & 1) == ((lane >> 4) & 1) ? T::ones8().x : 0u;
   const float slack = kStreamSlack / a.scale_log2;
   float nm = 0.f, thr = kNegInf;
 
@@ -337,7 +399,10 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   auto mask = [&](int c, floatx16 (&s)[2]) {
     const int x0 = keys.first_key(c);
     if (x0 + kTileN - 1 <= all_to && (x0 > hidden_to || x0 + kTileN <= a.sink)) return;
-    const uint64_t bits = seen_bits(a, u, token, x0);
+    int l = threadIdx.x & 31;
+    asm volatile("" : "+v"(l));
+    const PagedArgs e = fresh_args();
+    const uint64_t bits = seen_bits(e, u, min(roww + l, rows - 1) / e.group, x0);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const LaneBits32 vis((uint32_t)(bits >> (32 * t)), hi);
@@ -386,8 +451,9 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
     }
   };
   auto accumulate = [&](const uint16_t* cv, const uint4 (&p)[4]) {
-    uint32_t w = one;                  // the operand is made here: four registers fewer while P is formed
-    asm volatile("" : "+v"(w));
+    int l = threadIdx.x;               // the operand is made here: five registers fewer while P is formed
+    asm volatile("" : "+v"(l));
+    const uint32_t w = ((l >> 2) & 1) == ((l >> 4) & 1) ? T::ones8().x : 0u;
     const uint4 ones = make_uint4(w, w, w, w);
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -396,11 +462,8 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
       lsum = T::mfma(ones, p[st], lsum);
     }
   };
-  auto stage_k = [&](int c, int b) {
-    page.before(a, c);
-    page.load(a, a.k_pages, c, sk + b * TILE);
-  };
-  auto stage_v = [&](int c, int b) { page.load(a, a.v_pages, c, sv + b * TILE); };
+  auto stage_k = [&](int c, int b) { page.load(a.k_pages, c, sk + b * TILE); };
+  auto stage_v = [&](int c, int b) { page.load(a.v_pages, c, sv + b * TILE); };
   const int c0 = page.c0, n = page.c1 - page.c0;
   if constexpr (!kPagedSkew<D>) {
     if (n > 0) {
@@ -447,7 +510,17 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
     }
     dma_wait();
     __syncthreads();
-    if (n > 0 && active) {
+    if (!active) {     // a wave without rows brings its part of the tiles
+      __syncthreads();
+      for (int j = 0; j + 1 < n; ++j) {
+        stage_v(c0 + j + 1, (j & 1) ^ 1);
+        if (j + 2 < n) stage_k(c0 + j + 2, j & 1);
+        dma_wait();
+        __syncthreads();
+      }
+      return;
+    }
+    if (n > 0) {
       scores(sk, sa);
       mask(c0, sa);
       move_max(lane_max(sa));
@@ -456,7 +529,7 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
     auto step = [&](int j, int par, floatx16 (&s)[2], floatx16 (&sn)[2]) {   // par = j & 1
       stage_v(c0 + j + 1, par ^ 1);
       if (j + 2 < n) stage_k(c0 + j + 2, par);
-      if (active) {
+      {
         uint4 p[4];
         scores(sk + (par ^ 1) * TILE, sn);
         probs(s, p);
@@ -493,7 +566,7 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
       step(j, 0, sa, sb);
       sa[0] = sb[0], sa[1] = sb[1];
     }
-    if (n > 0 && active) {
+    if (n > 0) {
       uint4 p[4];
       probs(sa, p);
       pin(p);
@@ -502,90 +575,117 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   }
 
   // the row afresh, not held through the loop
-  const int lane_e = lane_now(), hi_e = lane_e >> 5, my = roww + (lane_e & 31);
+  int lane_e = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane_e));
+  const PagedArgs e = fresh_args();
+  const int hi_e = lane_e >> 5, my = roww + (lane_e & 31);
   if (my >= rows) return;
   const float l = lsum[0];
-  const int64_t row = (int64_t)(u.first + my / a.group) * a.H + u.h * a.group + my % a.group;
-  if (u.n_slices > 1) {
-    float* dst = slice_acc(a, row, u.slice, D);
+  if (u.state >= 0) {
+    if (my - row0 >= e.cap) return;
+    float* dst = piece_acc(e, u.state, my - row0, D);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         *(floatx4*)(dst + 32 * dt + 8 * r + 4 * hi_e) =
             floatx4{o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]};
-    if (hi_e == 0) *slice_ml(a, row, u.slice) = make_float2(l == 0.f ? kNegInf : -nm, l);
+    if (hi_e == 0) *piece_ml(e, u.state, my - row0) = make_float2(l == 0.f ? kNegInf : -nm, l);
     return;
   }
+  const int64_t row = (int64_t)(u.first + my / e.group) * e.H + u.h * e.group + my % e.group;
   const float inv = l > 0.f ? 1.f / l : 1.f;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      *(uint2*)(a.o + row * D + 32 * dt + 8 * r + 4 * hi_e) =
+      *(uint2*)(e.o + row * D + 32 * dt + 8 * r + 4 * hi_e) =
           make_uint2(pack2<T>(o[dt][4 * r] * inv, o[dt][4 * r + 1] * inv), pack2<T>(o[dt][4 * r + 2] * inv, o[dt][4 * r + 3] * inv));
-  if (hi_e == 0 && a.lse) a.lse[row] = l > 0.f ? lse_natural(-nm, l) : 0.f;
+  if (hi_e == 0 && e.lse) e.lse[row] = l > 0.f ? lse_natural(-nm, l) : 0.f;
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void paged_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs args) {
   __shared__ __align__(16) uint16_t sk[2][kTileN * D];
   __shared__ __align__(16) uint16_t sv[2][kTileN * D];
-  __shared__ int ids[kIds];
+  __shared__ int64_t pieces[kPagePieces];
+  __shared__ uint32_t todo[2][2];
   // rows behind the last request have no output: zeros
-  for (int64_t x = (int64_t)a.row_starts[a.R] * a.H * (D / 8) + (int64_t)blockIdx.x * 256 + threadIdx.x;
-       x < (int64_t)a.rows * a.H * (D / 8); x += (int64_t)gridDim.x * 256) {
-    *(uint4*)(a.o + 8 * x) = make_uint4(0, 0, 0, 0);
-    if (a.lse && x % (D / 8) == 0) a.lse[x / (D / 8)] = 0.f;
+  for (int64_t x = (int64_t)args.row_starts[args.R] * args.H * (D / 8) + (int64_t)blockIdx.x * 256 + threadIdx.x;
+       x < (int64_t)args.rows * args.H * (D / 8); x += (int64_t)gridDim.x * 256) {
+    *(uint4*)(args.o + 8 * x) = make_uint4(0, 0, 0, 0);
+    if (args.lse && x % (D / 8) == 0) args.lse[x / (D / 8)] = 0.f;
   }
-  Unit u;
-  if (!find_unit(a, blockIdx.x, u)) return;
-  const int rows = u.n * a.group;
-  if (a.max_slices > 1 && u.h == 0 && u.slice == 0) {       // for the join
-    const int t0 = rows <= kFewRows ? 0 : u.tile * kRowTile / a.group;
-    for (int t = t0 + threadIdx.x; t < u.n && t * a.group < (u.tile + 1) * kRowTile; t += 256) a.parts[u.first + t] = u.n_slices;
+  // One piece of the share after the other. Only the rest of the share is kept between two, in
+  // LDS (by turns, as a wave may read it late), so that the row tiles have their registers.
+  for (int turn = 0;; ++turn) {
+    const PagedArgs a = fresh_args();
+    int tid = threadIdx.x;             // not an invariant: nothing made from it is held either
+    asm volatile("" : "+v"(tid));
+    const Shares s(a, tid);
+    const int used = (int)((s.all + s.share - 1) / s.share);
+    const bool idle = (int)blockIdx.x >= used;
+    const int w = idle ? (int)blockIdx.x : xcd_remap(blockIdx.x, used);
+    uint32_t lo, hi;
+    if (turn == 0) {
+      if (a.acc && tid == 0) a.cuts[w].pieces = 0;
+      if (idle) return;
+      lo = s.cut(a, w * s.share), hi = s.cut(a, (w + 1) * s.share);
+    } else {
+      lo = scalar(todo[turn & 1][0]), hi = scalar(todo[turn & 1][1]);
+    }
+    if (lo >= hi) return;
+    const Place p = s.place(a, lo);
+    const Unit u(p, lo, hi, w);
+    if (tid == 0) {
+      todo[(turn + 1) & 1][0] = lo + (u.s1 - u.s0);
+      todo[(turn + 1) & 1][1] = hi;
+      if (u.state == 2 * w + 1)        // for the join: cuts at the shares' ends up to the edge
+        a.cuts[w] = CutTile{u.first, u.n, u.h, u.tile, 2 + (int)((p.start + p.keys - s.edge) / s.share - (w + 1))};
+    }
+    const int rows = u.n * a.group;
+    if (rows <= 16) paged_stream<T, D, 1>(a, u, sk[0], sv[0], pieces, tid);
+    else if (rows <= kFewRows) paged_stream<T, D, 2>(a, u, sk[0], sv[0], pieces, tid);
+    else paged_tile<T, D>(a, u, sk[0], sv[0], pieces, tid);
+    __syncthreads();                   // LDS is read no more
   }
-  if (rows <= 16) paged_stream<T, D, 1>(a, u, sk[0], sv[0], ids);
-  else if (rows <= kFewRows) paged_stream<T, D, 2>(a, u, sk[0], sv[0], ids);
-  else paged_tile<T, D>(a, u, sk[0], sv[0], ids);
 }
 
-// The slices of a row joined, a wave per (token, q head): as join_kernel, with the slices
-// that the token has. Rows of one slice are done.
+// The pieces of the row tile that workgroup blockIdx.x's share ends in, if it is cut, joined:
+// 32 rows for each blockIdx.y, D / 4 threads a row, pieces in order. As join_kernel: O = sum_p
+// f_p acc_p / sum_p f_p l_p, f_p = exp2(m_p - M).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-  constexpr int E = D / 64;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= (int64_t)a.row_starts[a.R] * a.H) return;
-  const int n = a.parts[row / a.H];
-  if (n == 1) return;
-  const float2* st = slice_ml(a, row, 0);
-  const float* x = slice_acc(a, row, 0, D) + E * lane;
-  float M = kNegInf;
+  const CutTile c = a.cuts[blockIdx.x];
+  if (c.pieces == 0) return;
+  const int rows = c.n * a.group, row0 = rows <= kFewRows ? 0 : c.tile * kRowTile;
+  const int here = min(min(rows - row0, kRowTile), a.cap), d = 4 * (threadIdx.x % (D / 4));
+  for (int r = 32 * blockIdx.y + threadIdx.x / (D / 4); r < min(here, 32 * (int)blockIdx.y + 32); r += 256 / (D / 4)) {
+    auto state = [&](int p) { return p == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + p); };
+    float M = kNegInf;
 #pragma unroll 4
-  for (int p = 0; p < n; ++p) M = fmaxf(M, st[p].x);
-  const float Mu = M == kNegInf ? 0.f : M;
-  float L = 0.f, s[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) s[e] = 0.f;
+    for (int p = 0; p < c.pieces; ++p) M = fmaxf(M, piece_ml(a, state(p), r)->x);
+    const float Mu = M == kNegInf ? 0.f : M;
+    float L = 0.f;
+    floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int p = 0; p < n; ++p) {
-    const float f = __builtin_amdgcn_exp2f(st[p].x - Mu);
-    L += st[p].y * f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[e] += x[(size_t)p * D + e] * f;
+    for (int p = 0; p < c.pieces; ++p) {
+      const float2 ml = *piece_ml(a, state(p), r);
+      const float f = __builtin_amdgcn_exp2f(ml.x - Mu);
+      L += ml.y * f;
+      x += *(const floatx4*)(piece_acc(a, state(p), r, D) + d) * f;
+    }
+    x = x / (L == 0.f ? 1.f : L);
+    const int64_t row = (int64_t)(c.first + (row0 + r) / a.group) * a.H + c.h * a.group + (row0 + r) % a.group;
+    *(uint2*)(a.o + row * D + d) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+    if (d == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) a.o[row * D + E * lane + e] = T::from_float(s[e] / (L == 0.f ? 1.f : L));
-  if (lane == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
 }
 
 template <typename T, int D>
 int paged_attend(const PagedArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_kernel<T, D>), dim3((unsigned)paged_units(a)), dim3(256), 0, stream, a);
-  if (a.max_slices > 1)
-    hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.rows * a.H + 3) / 4)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((paged_kernel<T, D>), dim3(a.groups), dim3(256), 0, stream, a);
+  if (a.acc) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.groups, (a.cap + 31) / 32), dim3(256), 0, stream, a);
   return check_launch("gki_paged_attend");
 }
 

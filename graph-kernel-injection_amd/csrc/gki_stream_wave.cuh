@@ -91,9 +91,9 @@ struct StreamWave {
 
   // Rows row0 .. n_rows - 1 of a stream: row_of(r) is where row r's elements are, rule_of(r) its Row.
   template <class Rows, class Rules>
-  __device__ inline StreamWave(int row0, int n_rows, float q_sign, Rows row_of, Rules rule_of) {
-    lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __device__ inline StreamWave(int row0, int n_rows, float q_sign, Rows row_of, Rules rule_of, int tid = threadIdx.x) {
+    lane = tid & 63;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     grp = lane >> 4, col = lane & 15;
     // Q^T operand of column block h: lane (grp, col) holds elements 32 ks + 8 grp .. +7
     // (EIGHT: 64 (ks / 2) + 16 grp + 8 (ks % 2) .. +7) of row row0 + 16 h + col
@@ -260,7 +260,7 @@ struct StreamWave {
   // write(r, d, x, M, L): elements d .. d + 3 of the r-th row's sum, its largest score, its row
   // sum; n_rows: the rows from row0 on.
   template <class Write>
-  __device__ inline void finish(int n_rows, float* wacc, float* wml, Write write) {
+  __device__ inline void finish(int n_rows, float* wacc, float* wml, Write write, int tid = threadIdx.x) {
 #pragma unroll
     for (int h = 0; h < NB; ++h) {
       const float lw = wave_sum16x4(lsum[h]);
@@ -274,7 +274,7 @@ struct StreamWave {
       }
       __syncthreads();
       const int rows_h = min(16, n_rows - 16 * h);
-      for (int idx = threadIdx.x; idx < rows_h * (D / 4); idx += 256) {
+      for (int idx = tid; idx < rows_h * (D / 4); idx += 256) {
         const int rl = idx / (D / 4), d = 4 * (idx % (D / 4));
         float M = kNegInf;
 #pragma unroll

@@ -84,8 +84,7 @@ SIGNATURES = {
                                  + [_c_ptr] * 3 + [_c_int] * 6 + [_c_ptr] * 2 + [_c_int] * 2 + [_c_ptr, _c_int]
                                  + [_c_i64] * 2 + [_c_ptr]),
     "gki_paged_accept": (ctypes.c_int, [_c_ptr] * 6 + [_c_int] * 7 + [_c_ptr]),
-    "gki_paged_slices": (ctypes.c_int, [_c_int] * 9),
-    "gki_paged_workspace_floats": (ctypes.c_int64, [_c_int] * 4),
+    "gki_paged_groups": (ctypes.c_int, [_c_int] * 8 + [_c_ptr]),
     "gki_paged_attend": (ctypes.c_int, [_c_ptr, _c_i64] + [_c_ptr] * 9 + [_c_int] * 13 + [_c_float, _c_ptr, _c_int,
                                                                                         _c_ptr]),
     "gki_read_probe_words": (ctypes.c_int64, [_c_int]),

@@ -32,6 +32,7 @@ There is no CPU or eager fallback: a missing library raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -239,7 +240,7 @@ class PagedKVCache:
         shape = (table.num_pages, self.heads, table.page_size, self.head_dim)
         self.k_pages, self.v_pages = (torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2))
         self._dtype = _DTYPE_CODE[dtype]
-        self._plans: dict = {}           # (rows, max_count, Hq) -> slices, floats of their workspace
+        self._plans: dict = {}           # (max_count, Hq) -> workgroups, floats of their workspace
 
     def _batch(self, batch: TokenBatch) -> None:
         if batch.table is not self.table:
@@ -317,17 +318,18 @@ class PagedKVCache:
         scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
         if not math.isfinite(scale):
             raise ValueError(f"softmax_scale must be finite, got {scale}")
-        t, H, rows = self.table, q.shape[1], batch.rows
+        t, H = self.table, q.shape[1]
         lib = _lib.load()
-        key = (rows, batch.max_count, H)
+        key = (batch.max_count, H)
         plan = self._plans.get(key)
         if plan is None:
             if len(self._plans) >= 4096:
                 self._plans.clear()
-            n = lib.gki_paged_slices(rows, batch.max_count, H, self.heads, self.head_dim, t.max_pages, t.page_size,
-                                     t.sink_size, t.window_size)
-            plan = self._plans[key] = n, int(lib.gki_paged_workspace_floats(rows, H, self.head_dim, n))
-        n_slices, floats = plan
+            n = ctypes.c_int64()
+            groups = lib.gki_paged_groups(batch.max_count, H, self.heads, self.head_dim, t.max_pages, t.page_size,
+                                          t.sink_size, t.window_size, ctypes.byref(n))
+            plan = self._plans[key] = groups, n.value
+        groups, floats = plan
         work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
@@ -337,7 +339,7 @@ class PagedKVCache:
                 0 if lse is None else lse.data_ptr(), *batch._pointers(), t.block_table.data_ptr(),
                 0 if batch.ancestors is None else batch.ancestors.data_ptr(), batch.words, self._dtype, batch.rows,
                 batch.max_count, t.max_requests, H, self.heads, self.head_dim, t.max_pages, t.num_pages, t.page_size,
-                t.sink_size, t.window_size, scale, work.data_ptr() if floats else 0, n_slices,
+                t.sink_size, t.window_size, scale, work.data_ptr() if floats else 0, groups,
                 _current_stream(self.device))
         if rc:
             _lib.check(rc, "gki_paged_attend")

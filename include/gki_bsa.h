@@ -446,17 +446,19 @@ int gki_paged_accept(void* k_pages, void* v_pages, const int64_t* slots, const i
                      int32_t path_len, int32_t H_kv, int32_t head_dim, int32_t num_pages,
                      int32_t page_size, void* stream);
 
-/* Slices that gki_paged_attend may cut a row tile's keys into, for a full card (any number
- * from 1 to 64 is right; how many a request gets is decided on the device, by the lengths
- * there), and the floats of 16-byte aligned workspace for as many (0 for one). */
-int gki_paged_slices(int32_t rows, int32_t max_count, int32_t H, int32_t H_kv, int32_t head_dim,
-                     int32_t max_pages, int32_t page_size, int32_t sink_size, int32_t window_size);
-int64_t gki_paged_workspace_floats(int32_t rows, int32_t H, int32_t head_dim, int32_t n_slices);
+/* Workgroups among which gki_paged_attend shares its work for a full card (any number from
+ * 1 to 4096 is right), and (workspace_floats, may be NULL) the floats of 16-byte aligned
+ * workspace that as many need: groups * (2 * min(128, max_count * H / H_kv) * (head_dim + 2)
+ * + 5), or 0 where no row can see enough keys for a walk to be cut. */
+int gki_paged_groups(int32_t max_count, int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages,
+                     int32_t page_size, int32_t sink_size, int32_t window_size,
+                     int64_t* workspace_floats);
 
 /* O (and, lse not NULL, the natural LSE [rows, H]) of a step's rows: a row at position p sees
  * the keys x <= p of its request with x < sink_size or x > p - window_size; with ancestors,
  * from base[r] on those that its words name. row_starts, base, positions, ancestors and
- * table as gki_page_extend leaves them. Rows that see no key, and rows behind the last
+ * table as gki_page_extend leaves them, max_count as it was given there. workspace NULL: no
+ * walk is cut. Rows that see no key, and rows behind the last
  * request: zeros. */
 int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o,
                      float* lse, const int32_t* row_starts, const int32_t* base,
@@ -464,7 +466,7 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
                      int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R, int32_t H,
                      int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t num_pages,
                      int32_t page_size, int32_t sink_size, int32_t window_size, float softmax_scale,
-                     float* workspace, int32_t n_slices, void* stream);
+                     float* workspace, int32_t groups, void* stream);
 
 /* Measurement helper, no counterpart in the reference: reads exactly the K and V
  * bytes a single-position StreamingLLM decode step reads from a full cache --

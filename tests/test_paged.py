@@ -64,9 +64,14 @@ def test_c_entries_refuse_before_launch():
     assert attend(dtype=0) == 2 and attend(D=16) == 2 and attend(H=3) == 1 and attend(R=0) == 1 and attend(q=0) == 1
     assert attend(o=8) == 1 and attend(stride=128) == 1 and attend(scale=math.inf) == 1 and attend(scale=math.nan) == 1
     assert attend(ancestors=16, words=0) == 1 and attend(ancestors=16, words=1, most=65, rows=65) == 1
-    assert attend(n=0) == 1 and attend(n=65, ws=16) == 1 and attend(n=2) == 1 and attend(n=2, ws=8) == 1
-    assert lib.gki_paged_slices(0, 1, 4, 2, 64, 8, 64, 4, 8) == 1 and lib.gki_paged_slices(9, 1, 3, 2, 64, 8, 64, 4, 8) == 1
-    assert lib.gki_paged_workspace_floats(5, 4, 64, 1) == 0 and lib.gki_paged_workspace_floats(5, 4, 64, 3) == 5 * (4 * 3 * 66 + 1)
+    assert attend(n=0) == 1 and attend(n=4097) == 1 and attend(ws=8) == 1
+    floats = ctypes.c_int64()
+    groups = lib.gki_paged_groups(30, 8, 2, 128, 100, 64, 4, 2048, ctypes.byref(floats))
+    assert groups >= 256 and floats.value == groups * (2 * 120 * 130 + 5)
+    assert lib.gki_paged_groups(200, 8, 2, 64, 100, 64, 4, 2048, ctypes.byref(floats)) * (2 * 128 * 66 + 5) == floats.value
+    for few in ((30, 8, 2, 128, 100, 64, 4, 100), (30, 8, 2, 128, 3, 64, 4, 2048), (0, 8, 2, 128, 100, 64, 4, 2048)):
+        assert lib.gki_paged_groups(*few, ctypes.byref(floats)) == groups and floats.value == 0
+    assert lib.gki_paged_groups(30, 8, 2, 128, 100, 64, 4, 2048, None) == groups
     assert attend(sink=2**30) == 1 and attend(window=-1) == 1 and attend(rows=0) == 0
     assert lib.gki_paged_accept(16, 16, 16, 16, 0, 16, 2, 2, 5, 2, 64, 9, 64, NULL) == 1
     assert lib.gki_paged_accept(16, 16, 16, 16, 16, 16, 0, 2, 5, 2, 64, 9, 64, NULL) == 2
@@ -179,6 +184,18 @@ class Run:
             at += n
         assert square <= 4 * allowed + 1e-30 * n_out, (tag, math.sqrt(square / max(allowed, 1e-300)))
         assert not got[at:].any() and (lse is None or not lse[at:].any()), tag
+
+
+def _share(monkeypatch, groups):
+    """Work shared among ``groups`` workgroups."""
+    real = _lib.load().gki_paged_groups
+
+    def fixed(*a):
+        n, floats = real(*a), a[-1]._obj
+        floats.value = floats.value // n * groups
+        return groups
+
+    monkeypatch.setattr(_lib.load(), "gki_paged_groups", fixed)
 
 
 def _tree(rng, n):
@@ -331,10 +348,10 @@ def test_trees_against_64_bits(dtype, D, page, heads, kv, sink, window, past, co
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("slices", [1, 2, 7, 64])
+@pytest.mark.parametrize("groups", [1, 2, 7, 64, 500, 4096])
 @pytest.mark.parametrize("counts,tree", [([1, 1, 1, 1], False), ([6, 1, 0, 20], False), ([40, 1, 300, 7], False), ([12, 30, 8, 1], True)])
-def test_any_number_of_slices(slices, counts, tree, monkeypatch):
-    monkeypatch.setattr(_lib.load(), "gki_paged_slices", lambda *a: slices)
+def test_any_number_of_workgroups(groups, counts, tree, monkeypatch):
+    _share(monkeypatch, groups)
     rng = random.Random(17)
     run = Run(4, 600, 4, 1500, 32, 2, 128, torch.bfloat16, seed=17)
     run.grow([5000, 900, 0, 1600])
@@ -348,12 +365,12 @@ def test_any_number_of_slices(slices, counts, tree, monkeypatch):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("slices", [1, None])
+@pytest.mark.parametrize("groups", [1, 3, None])
 @pytest.mark.parametrize("counts", [[1, 1], [2, 50]])
-def test_more_pages_than_are_held_at_once(slices, counts, monkeypatch):
+def test_more_pages_than_are_held_at_once(groups, counts, monkeypatch):
     """Walks of more than 1024 pages of 16 keys."""
-    if slices:
-        monkeypatch.setattr(_lib.load(), "gki_paged_slices", lambda *a: slices)
+    if groups:
+        _share(monkeypatch, groups)
     run = Run(2, 4200, 4, 30000, 16, 1, 64, torch.float16, seed=18)
     run.grow([35000, 17000], 9000)
     batch = run.extend(counts)
