@@ -109,7 +109,7 @@ struct Shares {
     sum = wave_prefix(mine);
     all = lane_of(sum, 63);
     share = scalar(max((uint32_t)kPagedMinShare, (all + a.groups - 1) / a.groups));
-    edge = max((uint32_t)kPagedMinShare / 2, share / 4);
+    edge = max((uint32_t)kPagedMinShare / 2, share / 16);
   }
   __device__ inline Place place(const PagedArgs& a, uint32_t step) const {      // step < all
     Place p;
@@ -245,7 +245,7 @@ struct PageTiles {
     if (c >= filled) fill(c);
     int wave = this->wave;             // the wave's constants are made here, not held: scalars are short in the loops
     asm volatile("" : "+s"(wave));
-    const uint32_t l0 = lds_addr(lds) + wave * 1024;
+    const uint32_t l0 = scalar(lds_addr(lds) + wave * 1024);
     const int i0 = (c - (filled - span)) * per, x0 = keys.first_key(c);
     if (per == 1) {
       const int64_t at = scalar64(pieces[i0]);
@@ -303,6 +303,15 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
   constexpr int TILE = kTileN * D;
   const int rows = u.n * a.group;
   auto token = [&](int r) { return u.first + min(r, rows - 1) / a.group; };
+  // the first keys are on their way while the queries are read
+  PageTiles<D, false, true> page(a, u, KeyTiles(a, u.base, u.base + u.n), pieces, tid);
+  auto issue = [&](int c) {
+    const int b = (c - page.c0) & 1;
+    page.load(a.k_pages, c, sk + b * TILE);
+    page.load(a.v_pages, c, sv + b * TILE);
+  };
+  if (page.c0 < page.c1) issue(page.c0);
+  if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
   StreamWave<T, T, D, NB, 1, true, false, StreamRow> w(
       0, rows, a.q_sign,
       [&](int r) { return a.q + (int64_t)token(r) * a.q_stride + (u.h * a.group + r % a.group) * D; },
@@ -311,15 +320,7 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
         return StreamRow{a.positions[t], a.ancestors ? a.ancestors[(int64_t)t * a.words] : 0};
       }, tid);
   const PagedRule rule{u.base, u.base + u.n - 1, a.sink, a.window, a.ancestors != nullptr};
-  PageTiles<D, false, true> page(a, u, KeyTiles(a, u.base, u.base + u.n), pieces, tid);
-  dma_wait();   // the loads above are complete before any LDS-DMA is in flight
-  auto issue = [&](int c) {
-    const int b = (c - page.c0) & 1;
-    page.load(a.k_pages, c, sk + b * TILE);
-    page.load(a.v_pages, c, sv + b * TILE);
-  };
-  if (page.c0 < page.c1) issue(page.c0);
-  if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
+  dma_wait();
   for (int c = page.c0; c < page.c1; ++c) {
     const int b = (c - page.c0) & 1;
     wait_chunks<page.NP, 2>(min(1, page.c1 - 1 - c));     // tile c has landed
@@ -361,16 +362,6 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   const Lane32<D> lanes(lane);
   const bool mine = roww + col < rows;                     // the lane's row of the request's
   const uint32_t token = mine ? (roww + col) / a.group : 0;      // the request's
-  const int head = u.h * a.group + (mine ? (roww + col) % a.group : 0);
-  uint4 qf[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    uint4 w = *(const uint4*)(a.q + (int64_t)(u.first + token) * a.q_stride + head * D + 16 * ks + 8 * hi);
-    w = make_uint4((w.x & a.q_and) ^ a.q_xor, (w.y & a.q_and) ^ a.q_xor, (w.z & a.q_and) ^ a.q_xor, (w.w & a.q_and) ^ a.q_xor);
-    qf[ks] = mine ? w : make_uint4(0, 0, 0, 0);
-  }
-  dma_wait();   // these loads are complete before any LDS-DMA is in flight
-
   const bool tree = a.ancestors != nullptr;
   // quotients as scalars, and with them the walk
   const int last_token = scalar(min(row0 + kRowTile - 1, rows - 1) / a.group);
@@ -382,6 +373,23 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   const int all_to = tree ? u.base - 1 : u.base + (int)scalar(min(roww, rows - 1) / a.group);
   const int hidden_to = u.base + (int)scalar(min(roww + 31, rows - 1) / a.group) - a.window;
 
+  auto stage_k = [&](int c, int b) { page.load(a.k_pages, c, sk + b * TILE); };
+  auto stage_v = [&](int c, int b) { page.load(a.v_pages, c, sv + b * TILE); };
+  // the first tiles are on their way while the queries are read
+  const int c0 = page.c0, n = page.c1 - page.c0;
+  if (n > 0) {
+    stage_k(c0, 0);
+    stage_v(c0, 0);
+    if (kPagedSkew<D> && n > 1) stage_k(c0 + 1, 1);
+  }
+  const int head = u.h * a.group + (mine ? (roww + col) % a.group : 0);
+  uint4 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    uint4 w = *(const uint4*)(a.q + (int64_t)(u.first + token) * a.q_stride + head * D + 16 * ks + 8 * hi);
+    w = make_uint4((w.x & a.q_and) ^ a.q_xor, (w.y & a.q_and) ^ a.q_xor, (w.z & a.q_and) ^ a.q_xor, (w.w & a.q_and) ^ a.q_xor);
+    qf[ks] = mine ? w : make_uint4(0, 0, 0, 0);
+  }
   floatx16 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = splat16(0.f);
@@ -462,14 +470,7 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
       lsum = T::mfma(ones, p[st], lsum);
     }
   };
-  auto stage_k = [&](int c, int b) { page.load(a.k_pages, c, sk + b * TILE); };
-  auto stage_v = [&](int c, int b) { page.load(a.v_pages, c, sv + b * TILE); };
-  const int c0 = page.c0, n = page.c1 - page.c0;
   if constexpr (!kPagedSkew<D>) {
-    if (n > 0) {
-      stage_k(c0, 0);
-      stage_v(c0, 0);
-    }
     dma_wait();
     __syncthreads();
     // unrolled by two so that the buffers are constants of the instructions
@@ -503,11 +504,6 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   } else {
     // prologue: K_0, V_0 and K_1 in LDS, S_0 with its maxima
     floatx16 sa[2], sb[2];
-    if (n > 0) {
-      stage_k(c0, 0);
-      stage_v(c0, 0);
-      if (n > 1) stage_k(c0 + 1, 1);
-    }
     dma_wait();
     __syncthreads();
     if (!active) {     // a wave without rows brings its part of the tiles
