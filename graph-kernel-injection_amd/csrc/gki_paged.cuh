@@ -94,7 +94,7 @@ inline int paged_cap(int64_t max_count, int group) { return (int)std::min<int64_
 inline int64_t paged_workspace(int groups, int head_dim, int64_t max_count, int group, int64_t sink, int64_t window,
                                int64_t max_length) {
   const int64_t seen = std::min(max_length, sink + window + max_count + 64);
-  if ((seen + 63) / 64 + 2 < 2 * kPagedMinShare) return 0;
+  if ((seen + 63) / 64 + 2 < 2 * kPagedMinShare) return 0;      // a join costs what eight steps do
   return (int64_t)groups * (2 * paged_cap(max_count, group) * (head_dim + 2) + 5);
 }
 

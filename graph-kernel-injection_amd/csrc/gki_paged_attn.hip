@@ -137,7 +137,7 @@ struct Shares {
     if (c == 0 || c >= all) return min(c, all);
     const Place p = place(a, c);
     const uint32_t off = c - p.start;
-    if (off == 0 || (a.acc && p.keys >= 2 * kPagedMinShare && off >= edge && p.keys - off >= edge)) return c;
+    if (off == 0 || (a.acc && off >= edge && p.keys - off >= edge)) return c;
     return 2 * off < p.keys ? p.start : p.start + p.keys;
   }
 };
