@@ -63,7 +63,7 @@ struct PageRows {
 
 // Key tiles that a workgroup's share has at least, and workgroups that the card holds at once.
 constexpr int kPagedMinShare = 8;
-inline int paged_groups(int head_dim) { return head_dim >= 128 ? 512 : 768; }
+inline int paged_groups(int head_dim) { return head_dim >= 128 ? 512 : 1024; }
 
 struct PagedArgs {
   const uint16_t *q, *k_pages, *v_pages;

@@ -32,6 +32,7 @@ _HEAD_DIMS = (16, 32, 64, 128)
 _DECODE_HEAD_DIMS = (64, 128)
 # decode workgroups to aim for: one 768-thread group on each of the 256 CUs
 _DECODE_TARGET_WGS = 256
+_HERE = contextlib.nullcontext()          # holds nothing: one for all calls
 # fp32 dK/dV work items wanted when the kv-tile columns are fewer: two per CU of the
 # 256 keep them all busy
 _FP32_DKDV_TARGET_ITEMS = 512
@@ -81,7 +82,7 @@ def _is_current(dev: torch.device) -> bool:
 def _on_device(dev: torch.device):
     """``dev`` as the current device for the launches (a no-op context when it
     already is)."""
-    return contextlib.nullcontext() if _is_current(dev) else torch.cuda.device(dev)
+    return _HERE if _is_current(dev) else torch.cuda.device(dev)
 
 
 def _decode_splits(n_tokens: int, bh: int) -> int:

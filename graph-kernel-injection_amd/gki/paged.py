@@ -50,6 +50,8 @@ _REFUSALS = ((1, "no free pages were left"), (2, "the counts sum to more than th
 
 
 def _int_vector(name: str, t: torch.Tensor, shape: Tuple[int, ...], device: torch.device) -> torch.Tensor:
+    if t.dtype == torch.int32 and t.shape == shape and t.device == device and t.is_contiguous():
+        return t                     # a step's host time counts
     if tuple(t.shape) != shape or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be an int32 or int64 tensor {list(shape)}, got {t.dtype} {tuple(t.shape)}")
     if t.device != device:
@@ -66,28 +68,35 @@ class TokenBatch:
     behind the last request. Drafts: ``ancestors``, 64 nodes to a word, which of a request's
     nodes a row sees."""
 
-    __slots__ = ("table", "rows", "max_count", "words", "slots", "ancestors", "_ints")
+    __slots__ = ("table", "rows", "max_count", "words", "ancestors", "_ints")
 
-    def __init__(self, table, rows, max_count, words, slots, ancestors, ints) -> None:
+    def __init__(self, table, rows, max_count, words, ancestors, ints) -> None:
         self.table, self.rows, self.max_count, self.words = table, rows, max_count, words
-        self.slots, self.ancestors, self._ints = slots, ancestors, ints
+        # slots (int64), then row_starts, base and positions, in one allocation of int32
+        self.ancestors, self._ints = ancestors, ints
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self._ints[:2 * self.rows].view(torch.int64)
 
     @property
     def row_starts(self) -> torch.Tensor:
-        return self._ints[:self.table.max_requests + 1]
+        return self._ints[2 * self.rows:2 * self.rows + self.table.max_requests + 1]
 
     @property
     def base(self) -> torch.Tensor:
-        n = self.table.max_requests
-        return self._ints[n + 1:2 * n + 1]
+        n, at = self.table.max_requests, 2 * self.rows
+        return self._ints[at + n + 1:at + 2 * n + 1]
 
     @property
     def positions(self) -> torch.Tensor:
-        return self._ints[2 * self.table.max_requests + 1:]
+        return self._ints[2 * (self.rows + self.table.max_requests) + 1:]
 
-    def _pointers(self) -> Tuple[int, int, int]:
+    def _pointers(self) -> Tuple[int, int, int, int]:
+        """Of slots, row_starts, base and positions."""
         at, n = self._ints.data_ptr(), self.table.max_requests
-        return at, at + 4 * (n + 1), at + 4 * (2 * n + 1)
+        starts = at + 8 * self.rows
+        return at, starts, starts + 4 * (n + 1), starts + 4 * (2 * n + 1)
 
 
 class PageTable:
@@ -126,6 +135,7 @@ class PageTable:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         n = self.max_requests
+        self._sizes = (n, self.max_pages, self.page_size, self.num_pages, self.sink_size, self.window_size)
         # lengths, pages taken, first page behind the sinks that is kept; the queue's head and count, the status
         self._state = torch.zeros(3 * n + 3, dtype=torch.int32, device=self.device)
         self._state[2 * n:3 * n] = -(-self.sink_size // self.page_size)
@@ -138,7 +148,7 @@ class PageTable:
     def _arguments(self) -> tuple:
         at, n = self._state.data_ptr(), self.max_requests
         return (at, at + 4 * n, at + 8 * n, self.block_table.data_ptr(), self._ring.data_ptr(), at + 12 * n,
-                at + 12 * n + 8, n, self.max_pages, self.page_size, self.num_pages, self.sink_size, self.window_size)
+                at + 12 * n + 8, *self._sizes)
 
     def extend(self, counts: torch.Tensor, rows: int, max_count: Optional[int] = None,
                parents: Optional[torch.Tensor] = None) -> TokenBatch:
@@ -169,15 +179,14 @@ class PageTable:
                 raise ValueError(f"trees hold up to {_MAX_DRAFT} nodes: max_count is {max_count}")
             words = max(1, -(-max_count // 64))
             ancestors = torch.empty((rows, words), dtype=torch.int64, device=self.device)
-        ints = torch.empty(2 * self.max_requests + 1 + rows, dtype=torch.int32, device=self.device)
-        slots = torch.empty(rows, dtype=torch.int64, device=self.device)
-        batch = TokenBatch(self, rows, max_count, words, slots, ancestors, ints)
-        row_starts, base, positions = batch._pointers()
+        ints = torch.empty(2 * self.max_requests + 1 + 3 * rows, dtype=torch.int32, device=self.device)
+        batch = TokenBatch(self, rows, max_count, words, ancestors, ints)
+        slots, row_starts, base, positions = batch._pointers()
         lib = _lib.load()
         with _on_device(self.device):
             rc = lib.gki_page_extend(
                 counts.data_ptr(), 0 if parents is None else parents.data_ptr(), rows, max_count, words,
-                *self._arguments(), row_starts, base, positions, slots.data_ptr(),
+                *self._arguments(), row_starts, base, positions, slots,
                 0 if ancestors is None else ancestors.data_ptr(), _current_stream(self.device))
         if rc:
             _lib.check(rc, "gki_page_extend")
@@ -189,10 +198,12 @@ class PageTable:
         if batch.table is not self:
             raise ValueError("the batch belongs to another table")
         accepted = _int_vector("accepted", accepted, (self.max_requests,), self.device)
-        row_starts, base, _ = batch._pointers()
+        _, row_starts, base, _ = batch._pointers()
         with _on_device(self.device):
-            _lib.check(_lib.load().gki_page_accept(self._state.data_ptr(), base, row_starts, accepted.data_ptr(),
-                                                   self.max_requests, _current_stream(self.device)), "gki_page_accept")
+            rc = _lib.load().gki_page_accept(self._state.data_ptr(), base, row_starts, accepted.data_ptr(),
+                                             self.max_requests, _current_stream(self.device))
+        if rc:
+            _lib.check(rc, "gki_page_accept")
 
     def release(self, done: torch.Tensor) -> None:
         """Requests marked in ``done`` (bool ``[max_requests]`` on the device) give their
@@ -240,6 +251,7 @@ class PagedKVCache:
         shape = (table.num_pages, self.heads, table.page_size, self.head_dim)
         self.k_pages, self.v_pages = (torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2))
         self._dtype = _DTYPE_CODE[dtype]
+        self._strides: dict = {}         # (shape, strides, ...) of rows -> their row stride, 0: to be copied
         self._plans: dict = {}           # (max_count, Hq) -> workgroups, floats of their workspace
 
     def _batch(self, batch: TokenBatch) -> None:
@@ -248,6 +260,19 @@ class PagedKVCache:
 
     def _rows(self, name: str, t: torch.Tensor, rows: int, grouped: bool = False) -> Tuple[torch.Tensor, int]:
         """``t`` as the kernels read it, and its row stride."""
+        key = (t.shape, t.stride(), t.dtype, t.device, rows, grouped)
+        stride = self._strides.get(key)          # checked before: a step's host time counts
+        if stride is None:
+            if len(self._strides) >= 4096:
+                self._strides.clear()
+            stride = self._strides[key] = self._row_stride(name, t, rows, grouped)
+        if stride and t.data_ptr() % 16 == 0:
+            return t, stride
+        t = t.contiguous()
+        return (t if t.data_ptr() % 16 == 0 else t.clone()), t.shape[1] * self.head_dim
+
+    def _row_stride(self, name: str, t: torch.Tensor, rows: int, grouped: bool) -> int:
+        """The row stride of ``t``, 0 if it has to be copied; raises where it does not fit."""
         shape = t.shape
         ok = len(shape) == 3 and shape[0] == rows and shape[2] == self.head_dim
         if not ok or not (shape[1] == self.heads or (grouped and shape[1] > 0 and shape[1] % self.heads == 0)):
@@ -260,10 +285,7 @@ class PagedKVCache:
         row, head, one = t.stride()
         width = shape[1] * self.head_dim
         # rows of a fused projection are read in place
-        if one == 1 and (head == self.head_dim or shape[1] == 1) and row >= width and row % 8 == 0 and t.data_ptr() % 16 == 0:
-            return t, row
-        t = t.contiguous()
-        return (t if t.data_ptr() % 16 == 0 else t.clone()), width
+        return row if one == 1 and (head == self.head_dim or shape[1] == 1) and row >= width and row % 8 == 0 else 0
 
     def append(self, k: torch.Tensor, v: torch.Tensor, batch: TokenBatch) -> None:
         """Writes the step's keys and values (``[rows, heads, D]``) to their slots; rows
@@ -274,7 +296,7 @@ class PagedKVCache:
         with _on_device(self.device):
             rc = _lib.load().gki_paged_append(
                 k.data_ptr(), v.data_ptr(), k_stride, v_stride, self.k_pages.data_ptr(), self.v_pages.data_ptr(),
-                batch.slots.data_ptr(), self._dtype, batch.rows, self.heads, self.head_dim, t.num_pages, t.page_size,
+                batch._pointers()[0], self._dtype, batch.rows, self.heads, self.head_dim, t.num_pages, t.page_size,
                 _current_stream(self.device))
         if rc:
             _lib.check(rc, "gki_paged_append")
@@ -290,7 +312,7 @@ class PagedKVCache:
         if rotary.head_dim != self.head_dim:
             raise ValueError(f"rotary must have head_dim {self.head_dim}, got {rotary.head_dim}")
         if positions is None:
-            at, wide, axis_stride, row_stride = batch._pointers()[2], 0, 0, 1
+            at, wide, axis_stride, row_stride = batch._pointers()[3], 0, 0, 1
         else:
             axis_stride, _, row_stride = rotary._position_strides(positions, q)
             at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
@@ -300,7 +322,7 @@ class PagedKVCache:
         with _on_device(self.device):
             rc = _lib.load().gki_paged_append_rotated(
                 q.data_ptr(), out.data_ptr(), q_stride, q.shape[1], k.data_ptr(), v.data_ptr(), k_stride, v_stride,
-                self.k_pages.data_ptr(), self.v_pages.data_ptr(), batch.slots.data_ptr(), self._dtype, batch.rows,
+                self.k_pages.data_ptr(), self.v_pages.data_ptr(), batch._pointers()[0], self._dtype, batch.rows,
                 self.heads, self.head_dim, t.num_pages, t.page_size, turns.data_ptr(), axis.data_ptr(), rotary.pairs,
                 int(rotary.interleaved), at, wide, axis_stride, row_stride, _current_stream(self.device))
         if rc:
@@ -336,7 +358,7 @@ class PagedKVCache:
         with _on_device(self.device):
             rc = lib.gki_paged_attend(
                 q.data_ptr(), q_stride, self.k_pages.data_ptr(), self.v_pages.data_ptr(), o.data_ptr(),
-                0 if lse is None else lse.data_ptr(), *batch._pointers(), t.block_table.data_ptr(),
+                0 if lse is None else lse.data_ptr(), *batch._pointers()[1:], t.block_table.data_ptr(),
                 0 if batch.ancestors is None else batch.ancestors.data_ptr(), batch.words, self._dtype, batch.rows,
                 batch.max_count, t.max_requests, H, self.heads, self.head_dim, t.max_pages, t.num_pages, t.page_size,
                 t.sink_size, t.window_size, scale, work.data_ptr() if floats else 0, groups,
@@ -358,7 +380,7 @@ class PagedKVCache:
         accepted = _int_vector("accepted", accepted, (t.max_requests,), self.device)
         with _on_device(self.device):
             rc = _lib.load().gki_paged_accept(
-                self.k_pages.data_ptr(), self.v_pages.data_ptr(), batch.slots.data_ptr(), batch._pointers()[0],
+                self.k_pages.data_ptr(), self.v_pages.data_ptr(), *batch._pointers()[:2],
                 paths.data_ptr(), accepted.data_ptr(), self._dtype, t.max_requests, paths.shape[1], self.heads,
                 self.head_dim, t.num_pages, t.page_size, _current_stream(self.device))
         if rc:

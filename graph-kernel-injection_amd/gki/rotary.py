@@ -25,12 +25,14 @@ from .ops import _DTYPE_CODE, _HEAD_DIMS, _current_stream, _on_device, _refuse_t
 _Strides3, _Strides6 = ctypes.c_int64 * 3, ctypes.c_int64 * 6
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with its rows in one piece on 16-byte boundaries: itself, or a copy."""
+def _in_place(t: torch.Tensor) -> bool:
+    """Whether rows lie in one piece on 16-byte boundaries."""
     per16 = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % per16 == 0 for s in t.stride()[:-1]):
-        return t
-    return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    return t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % per16 == 0 for s in t.stride()[:-1])
+
+
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(src: torch.Tensor, dst: torch.Tensor):
@@ -86,6 +88,8 @@ class MultiAxisRotary:
         self.head_dim, self.base = int(head_dim), float(base)
         self.interleaved, self.per_axis = bool(interleaved), bool(per_axis)
         self.pairs = pairs
+        self._known: dict = {}               # shapes, strides, ... of checked calls -> the positions' strides
+        self._launches: dict = {}            # of the tensors of a launch -> its sizes and strides
         self._tables: dict = {}              # device -> (turns per position, axis) of the pairs
 
     def _table(self, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -126,6 +130,18 @@ class MultiAxisRotary:
         of 1, or ``[N]`` (``[rows]``), gives every axis the same. Rows may lie anywhere (a
         projection's ``[B, N, H, D]`` transposed is read in place); the results are
         contiguous. Differentiable in reverse mode, any number of times."""
+        key = (q.shape, q.stride(), q.dtype, q.device, None if k is None else (k.shape, k.stride(), k.dtype, k.device),
+               positions.shape, positions.stride(), positions.dtype, positions.device)
+        strides = self._known.get(key)           # checked before: a step's host time counts
+        if strides is None:
+            if len(self._known) >= 4096:
+                self._known.clear()
+            strides = self._known[key] = self._check(q, k, positions)
+        _refuse_tangents(*((q,) if k is None else (q, k)))
+        return self._apply(q, k, positions, strides, False)
+
+    def _check(self, q, k, positions):
+        """The positions' strides; raises for tensors that do not fit."""
         if q.dim() not in (3, 4) or (k is not None and k.dim() != q.dim()):
             raise ValueError("q and k must both be [B, H, N, D] or both [rows, H, D]")
         for name, t in (("q", q), ("k", k)):
@@ -141,9 +157,7 @@ class MultiAxisRotary:
                 raise ValueError("q and k must live on one device")
         if k is not None and (k.shape[0] != q.shape[0] or (q.dim() == 4 and k.shape[2] != q.shape[2])):
             raise ValueError("q and k must hold the same tokens")
-        strides = self._position_strides(positions, q)
-        _refuse_tangents(*((q,) if k is None else (q, k)))
-        return self._apply(q, k, positions, strides, False)
+        return _Strides3(*self._position_strides(positions, q))
 
     def _apply(self, q, k, positions, strides, inverse):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
@@ -152,22 +166,51 @@ class MultiAxisRotary:
 
     def _rotate(self, q, k, positions, strides, inverse):
         """The launch; either tensor may be missing."""
-        outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
-        call = [(_readable(t), o) for t, o in zip((q, k), outs) if t is not None and t.numel()]
-        if not call:
-            return outs[0], outs[1]
-        src, dst = call[0]
-        packed = src.dim() == 3
-        heads = [(t.shape[1], _strides(t, o)) for t, o in call]
-        batch, n = (1, src.shape[0]) if packed else (src.shape[0], src.shape[2])
-        turns, axis = self._table(src.device)
-        second = (call[1][0].data_ptr(), call[1][1].data_ptr(), *heads[1]) if len(call) > 1 else (0, 0, 0, None)
-        lib = _lib.load()
-        with _on_device(src.device):
-            rc = lib.gki_rotary(src.data_ptr(), dst.data_ptr(), *heads[0], *second, _DTYPE_CODE[src.dtype], batch, n,
-                                self.head_dim, turns.data_ptr(), axis.data_ptr(), self.pairs, int(self.interleaved),
-                                int(inverse), positions.data_ptr(), int(positions.dtype == torch.int64), _Strides3(*strides),
-                                _current_stream(src.device))
+        if q is None or k is None or not (q.numel() and k.numel()):
+            outs = [None if t is None else self._launch(t, None, positions, strides, inverse)[0] for t in (q, k)]
+            return tuple(outs)
+        return self._launch(q, k, positions, strides, inverse)
+
+    def _launch(self, q, k, positions, strides, inverse):
+        """``q``, and ``k`` if there is one (neither then empty)."""
+        out, out_k = torch.empty(q.shape, dtype=q.dtype, device=q.device), None
+        if not q.numel():
+            return out, None
+        # the plan: (copy, heads, strides) of each, (batch, tokens, head_dim)
+        key = (q.shape, q.stride(), q.dtype, q.data_ptr() % 16,
+               None if k is None else (k.shape, k.stride(), k.data_ptr() % 16))
+        plan = self._launches.get(key)
+        if plan is None:
+            if len(self._launches) >= 4096:
+                self._launches.clear()
+            plan = self._launches[key] = self._plan(q, k)
+        copy, heads, at, copy_k, heads_k, at_k, sizes = plan
+        if copy:
+            q = _copied(q)
+        src_k = dst_k = 0
+        if k is not None:
+            out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            if copy_k:
+                k = _copied(k)
+            src_k, dst_k = k.data_ptr(), out_k.data_ptr()
+        device = q.device
+        turns, axis = self._table(device)
+        with _on_device(device):
+            rc = _lib.load().gki_rotary(
+                q.data_ptr(), out.data_ptr(), heads, at, src_k, dst_k, heads_k, at_k, _DTYPE_CODE[q.dtype], *sizes,
+                turns.data_ptr(), axis.data_ptr(), self.pairs, self.interleaved, inverse, positions.data_ptr(),
+                positions.dtype == torch.int64, strides, _current_stream(device))
         if rc:
             _lib.check(rc, "gki_rotary")
-        return outs[0], outs[1]
+        return out, out_k
+
+    def _plan(self, q, k):
+        plan = []
+        for t in (q, k):
+            if t is None:
+                plan += [False, 0, None]
+                continue
+            copy, dense = not _in_place(t), torch.empty(t.shape, dtype=t.dtype, device="meta")
+            plan += [copy, t.shape[1], _strides(dense if copy else t, dense)]
+        shape = q.shape
+        return (*plan, (1, shape[0], self.head_dim) if len(shape) == 3 else (shape[0], shape[2], self.head_dim))
