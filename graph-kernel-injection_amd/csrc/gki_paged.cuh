@@ -5,6 +5,21 @@
 
 namespace gki {
 
+// Sum of lanes 0 .. l, by DPP.
+template <int CTRL, int ROWS>
+__device__ inline uint32_t dpp_or_zero(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+__device__ inline uint32_t wave_prefix(uint32_t x) {
+  x += dpp_or_zero<0x111, 0xF>(x);     // row_shr 1, 2, 4, 8
+  x += dpp_or_zero<0x112, 0xF>(x);
+  x += dpp_or_zero<0x114, 0xF>(x);
+  x += dpp_or_zero<0x118, 0xF>(x);
+  x += dpp_or_zero<0x142, 0xA>(x);     // lane 15 of a row to the next, for rows 1 and 3
+  x += dpp_or_zero<0x143, 0xC>(x);     // lane 31 to rows 2 and 3
+  return x;
+}
+
 // Rotary positions with several axes: pair j of a row's P pairs of elements turns by
 //   angle = position[axis_j] * frequency_j,  (a, b) -> (a cos - b sin, a sin + b cos),
 // pairs (j, j + P) or, interleaved, (2 j, 2 j + 1); elements from 2 P on stay as they are.

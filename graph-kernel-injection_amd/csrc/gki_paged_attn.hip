@@ -47,20 +47,6 @@ struct KeyTiles {
 // itself, a wave 64 requests at a time. Neighbours work on one XCD: row tiles of a
 // (request, head) meet their keys in its L2.
 // ---------------------------------------------------------------------------
-// Sum of lanes 0 .. l, by DPP.
-template <int CTRL, int ROWS>
-__device__ inline uint32_t dpp_or_zero(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
-}
-__device__ inline uint32_t wave_prefix(uint32_t x) {
-  x += dpp_or_zero<0x111, 0xF>(x);     // row_shr 1, 2, 4, 8
-  x += dpp_or_zero<0x112, 0xF>(x);
-  x += dpp_or_zero<0x114, 0xF>(x);
-  x += dpp_or_zero<0x118, 0xF>(x);
-  x += dpp_or_zero<0x142, 0xA>(x);     // lane 15 of a row to the next, for rows 1 and 3
-  x += dpp_or_zero<0x143, 0xC>(x);     // lane 31 to rows 2 and 3
-  return x;
-}
 __device__ inline uint32_t lane_of(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
 __device__ inline uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
@@ -312,7 +298,7 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
   };
   if (page.c0 < page.c1) issue(page.c0);
   if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
-  StreamWave<T, T, D, NB, 1, true, false, StreamRow> w(
+  StreamWave<T, T, D, NB, 1, true, false, StreamRow, true> w(
       0, rows, a.q_sign,
       [&](int r) { return a.q + (int64_t)token(r) * a.q_stride + (u.h * a.group + r % a.group) * D; },
       [&](int r) {

@@ -20,12 +20,7 @@ enum Refusal : int { kOutOfPages = 1, kTooManyRows = 2, kBadCount = 4 };
 // Exclusive prefix of x over the workgroup, and the total; `part` holds one sum per wave.
 __device__ inline int block_scan(int x, int* part, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(s, o);
-    if (lane >= o) s += y;
-  }
+  const int s = (int)wave_prefix((uint32_t)x);
   __syncthreads();                     // `part` of the scan before has been read
   if (lane == 63) part[wave] = s;
   __syncthreads();
@@ -37,6 +32,12 @@ __device__ inline int block_scan(int x, int* part, int& total) {
     total += part[w];
   }
   return before + s - x;
+}
+
+// Adds the lanes' x to a sum in LDS: its low 15 bits and the rest apart, as 64 of these fit.
+__device__ inline void add_to(unsigned long long* sum, uint32_t x) {
+  const uint32_t lo = wave_prefix(x & 0x7FFF), hi = wave_prefix(x >> 15);
+  if ((threadIdx.x & 63) == 63 && (lo | hi)) atomicAdd(sum, ((unsigned long long)hi << 15) + lo);
 }
 
 // The last r of 0 .. n - 1 with start[r] <= i (start ascending, start[0] <= i): where
@@ -86,7 +87,7 @@ __device__ inline void no_row(const PageStep& s, int row) {
 template <bool PLACE>
 __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, PageStep s) {
   __shared__ int part[kBookThreads / 64];
-  __shared__ int first[kBookThreads + 1], from[kBookThreads];
+  __shared__ int first[kBookThreads + 1], from[kBookThreads], starts[kBookThreads];
   __shared__ unsigned long long sums[3];
   __shared__ int bad;
   const int tid = threadIdx.x;
@@ -94,16 +95,22 @@ __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, Page
   if (tid == 0) bad = 0;
   __syncthreads();
   const int head = t.queue[0], count = t.queue[1];
-  for (int r = tid; r < t.R; r += kBookThreads) {
-    const int c = s.counts[r];
-    if (c < 0 || c > s.max_count || (int64_t)t.lengths[r] + c > ((int64_t)t.max_pages << t.shift)) {
-      bad = 1;
-      continue;
+  for (int r0 = 0; r0 < t.R; r0 += kBookThreads) {
+    const int r = r0 + tid;
+    int c = 0, new_pages = 0, dead = 0;
+    if (r < t.R) {
+      c = s.counts[r];
+      if (c < 0 || c > s.max_count || (int64_t)t.lengths[r] + c > ((int64_t)t.max_pages << t.shift)) {
+        bad = 1;
+        c = 0;
+      }
+      const Need n(t, r, c);
+      new_pages = n.pages - t.pages[r];
+      dead = n.kept - t.kept[r];
     }
-    const Need n(t, r, c);
-    if (c) atomicAdd(&sums[0], (unsigned long long)c);
-    if (n.pages > t.pages[r]) atomicAdd(&sums[1], (unsigned long long)(n.pages - t.pages[r]));
-    if (n.kept > t.kept[r]) atomicAdd(&sums[2], (unsigned long long)(n.kept - t.kept[r]));
+    add_to(&sums[0], c);
+    add_to(&sums[1], new_pages);
+    add_to(&sums[2], dead);
   }
   __syncthreads();
   const int why = bad ? kBadCount : (sums[0] > (unsigned long long)s.rows ? kTooManyRows : 0) |
@@ -149,6 +156,7 @@ __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, Page
     const int start = rows + block_scan(c, part, total_rows);
     first[tid] = block_scan(pages - had, part, total);
     from[tid] = had;
+    starts[tid] = start;
     if (r < t.R) {
       s.row_starts[r] = start;
       s.base[r] = len;
@@ -176,8 +184,10 @@ __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, Page
         no_row(s, row);
         continue;
       }
-      const int r = locate(s.row_starts, t.R, row);
-      place_row(t, s, row, r, row - s.row_starts[r]);
+      // the starts of up to a workgroup's threads are in LDS
+      const bool held = t.R <= kBookThreads;
+      const int r = held ? locate(starts, t.R, row) : locate(s.row_starts, t.R, row);
+      place_row(t, s, row, r, row - (held ? starts[r] : s.row_starts[r]));
     }
   }
 }

@@ -79,8 +79,9 @@ __device__ inline uint2 lds_tr4_rho(const uint16_t* tile, int t, int n0, int lan
 // swizzle serves without conflicts), with a softmax state of its own. NPC: pieces of the queries and of
 // the probabilities. The reference max is lazy: it moves when a score exceeds it by
 // the slack, so that the rescale almost never runs.
-// Row: what the token rule wants to know of a row (RULE).
-template <typename T, typename C, int D, int NB, int NPC, bool RULE, bool EIGHT, typename Row = int>
+// Row: what the token rule wants to know of a row (RULE). ROUNDED: the row sums add the
+// probabilities as they are rounded for P V (16-bit rows), so that a part of their errors cancels.
+template <typename T, typename C, int D, int NB, int NPC, bool RULE, bool EIGHT, typename Row = int, bool ROUNDED = false>
 struct StreamWave {
   static constexpr int KS = D / 32, DT = D / 16;
   uint4 qf[NB][KS][NPC];
@@ -162,8 +163,13 @@ struct StreamWave {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         s[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], a.scale_log2, -m_use));
-      lsum[h] += (s[h][0] + s[h][1]) + (s[h][2] + s[h][3]);
       pb[h] = make_uint2(pack2<C>(s[h][0], s[h][1]), pack2<C>(s[h][2], s[h][3]));
+      if constexpr (ROUNDED) {
+        const uint16_t* r = (const uint16_t*)&pb[h];
+        lsum[h] += (C::to_float(r[0]) + C::to_float(r[1])) + (C::to_float(r[2]) + C::to_float(r[3]));
+      } else {
+        lsum[h] += (s[h][0] + s[h][1]) + (s[h][2] + s[h][3]);
+      }
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
