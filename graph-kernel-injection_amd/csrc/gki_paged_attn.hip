@@ -633,41 +633,43 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
   }
 }
 
-// The pieces of the row tile that workgroup blockIdx.x's share ends in, if it is cut, joined:
-// 32 rows for each blockIdx.y, D / 4 threads a row, pieces in order. As join_kernel: O = sum_p
-// f_p acc_p / sum_p f_p l_p, f_p = exp2(m_p - M).
+// The pieces of the row tile that workgroup blockIdx.x's share ends in, if it is cut, joined: a
+// thread for four elements of a row, pieces in order. As join_kernel: O = sum_p f_p acc_p / sum_p
+// f_p l_p, f_p = exp2(m_p - M). Bound by latency (the cut, the maxima, the sums): many small
+// workgroups, most of which leave at once.
+constexpr int kJoinThreads = 256;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a) {
+  constexpr int RPG = kJoinThreads / (D / 4);
   const CutTile c = a.cuts[blockIdx.x];
   if (c.pieces == 0) return;
   const int rows = c.n * a.group, row0 = rows <= kFewRows ? 0 : c.tile * kRowTile;
-  const int here = min(min(rows - row0, kRowTile), a.cap), d = 4 * (threadIdx.x % (D / 4));
-  for (int r = 32 * blockIdx.y + threadIdx.x / (D / 4); r < min(here, 32 * (int)blockIdx.y + 32); r += 256 / (D / 4)) {
-    auto state = [&](int p) { return p == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + p); };
-    float M = kNegInf;
+  const int r = blockIdx.y * RPG + threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
+  if (r >= min(min(rows - row0, kRowTile), a.cap)) return;
+  auto state = [&](int p) { return p == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + p); };
+  float M = kNegInf;
 #pragma unroll 4
-    for (int p = 0; p < c.pieces; ++p) M = fmaxf(M, piece_ml(a, state(p), r)->x);
-    const float Mu = M == kNegInf ? 0.f : M;
-    float L = 0.f;
-    floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < c.pieces; ++p) M = fmaxf(M, piece_ml(a, state(p), r)->x);
+  const float Mu = M == kNegInf ? 0.f : M;
+  float L = 0.f;
+  floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int p = 0; p < c.pieces; ++p) {
-      const float2 ml = *piece_ml(a, state(p), r);
-      const float f = __builtin_amdgcn_exp2f(ml.x - Mu);
-      L += ml.y * f;
-      x += *(const floatx4*)(piece_acc(a, state(p), r, D) + d) * f;
-    }
-    x = x / (L == 0.f ? 1.f : L);
-    const int64_t row = (int64_t)(c.first + (row0 + r) / a.group) * a.H + c.h * a.group + (row0 + r) % a.group;
-    *(uint2*)(a.o + row * D + d) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-    if (d == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
+  for (int p = 0; p < c.pieces; ++p) {
+    const float2 ml = *piece_ml(a, state(p), r);
+    const float f = __builtin_amdgcn_exp2f(ml.x - Mu);
+    L += ml.y * f;
+    x += *(const floatx4*)(piece_acc(a, state(p), r, D) + d) * f;
   }
+  x = x / (L == 0.f ? 1.f : L);
+  const int64_t row = (int64_t)(c.first + (row0 + r) / a.group) * a.H + c.h * a.group + (row0 + r) % a.group;
+  *(uint2*)(a.o + row * D + d) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+  if (d == 0 && a.lse) a.lse[row] = L == 0.f ? 0.f : lse_natural(M, L);
 }
 
 template <typename T, int D>
 int paged_attend(const PagedArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((paged_kernel<T, D>), dim3(a.groups), dim3(256), 0, stream, a);
-  if (a.acc) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.groups, (a.cap + 31) / 32), dim3(256), 0, stream, a);
+  if (a.acc) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.groups, (a.cap * (D / 4) + kJoinThreads - 1) / kJoinThreads), dim3(kJoinThreads), 0, stream, a);
   return check_launch("gki_paged_attend");
 }
 
