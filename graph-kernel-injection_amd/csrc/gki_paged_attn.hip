@@ -242,11 +242,14 @@ struct PageTiles {
         dma_buf16(buffer_rsrc(base + p * 4096, rows_left<RB>(left - (4 * p + wave) * RB) * D * 2), voff[ROW32 ? 0 : p],
                   l0 + p * 4096, ONCE);
     } else {
+      int64_t held[NP];                // all read before the first load is issued
+#pragma unroll
+      for (int p = 0; p < NP; ++p) held[p] = pieces[i0 + ((4 * p + wave) * RB >> piece)];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        const int row = (4 * p + wave) * RB, y = row >> piece;             // the block's piece
-        const int64_t at = scalar64(pieces[i0 + y]);
-        const char* base = (const char*)pool + at + (row - (y << piece)) * (2 * D);
+        const int row = (4 * p + wave) * RB;
+        const int64_t at = scalar64(held[p]);
+        const char* base = (const char*)pool + at + (row & ((1 << piece) - 1)) * (2 * D);
         const int left = scalar(at < 0 ? 0 : end - x0 - row);
         dma_buf16(buffer_rsrc(base, rows_left<RB>(left) * D * 2), voff[ROW32 ? 0 : p], l0 + p * 4096, ONCE);
       }
