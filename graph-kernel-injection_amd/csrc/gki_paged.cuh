@@ -78,6 +78,7 @@ struct PageRows {
 
 // Key tiles that a workgroup's share has at least, and workgroups that the card holds at once.
 constexpr int kPagedMinShare = 8;
+constexpr int kPagedPieceCost = 2;
 inline int paged_groups(int head_dim) { return head_dim >= 128 ? 512 : 1024; }
 
 struct PagedArgs {

@@ -60,8 +60,8 @@ struct Request {
     base = a.base[r];
     const uint32_t rows = n * a.group;
     tiles = rows <= kFewRows ? (rows + kFewRows - 1) / kFewRows : (rows + kRowTile - 1) / kRowTile;
-    // a short walk counts for more than its key tiles: it has its prologue and epilogue too
-    const uint32_t k = KeyTiles(a, base, base + n).n;
+    // a walk's prologue and epilogue cost about as much as kPagedPieceCost key tiles
+    const uint32_t k = KeyTiles(a, base, base + n).n + kPagedPieceCost;
     keys = max((uint32_t)kPagedMinShare, (k + (1u << a.coarse) - 1) >> a.coarse);
   }
   __device__ inline uint32_t steps(const PagedArgs& a) const { return tiles * a.H_kv * keys; }
