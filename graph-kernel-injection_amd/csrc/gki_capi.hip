@@ -843,20 +843,21 @@ int gki_page_extend(const int32_t* counts, const int32_t* parents, int32_t rows,
                     int32_t* lengths, int32_t* pages, int32_t* kept, int32_t* table, int32_t* ring, int32_t* queue,
                     int32_t* status, int32_t R, int32_t max_pages, int32_t page_size, int32_t num_pages,
                     int32_t sink_size, int32_t window_size, int32_t* row_starts, int32_t* base, int32_t* positions,
-                    int64_t* slots, uint64_t* ancestors, void* stream) {
+                    int64_t* slots, uint64_t* ancestors, int32_t* requests, void* stream) {
   const char* what = "gki_page_extend";
   PageTables t;
   if (int rc = page_tables(what, t, lengths, pages, kept, table, ring, queue, status, R, max_pages, page_size, num_pages,
                            sink_size, window_size))
     return rc;
   GKI_REQUIRE(rows >= 0 && rows < (1 << kPartialBit) && max_count >= 0, 1, "gki_page_extend: rows must be in 0 .. 2^30 - 1 and max_count not negative");
-  GKI_REQUIRE(counts && row_starts && base && (rows == 0 || (positions && slots)), 1, "gki_page_extend: null pointer");
+  GKI_REQUIRE(counts && row_starts && base && requests && (rows == 0 || (positions && slots)), 1, "gki_page_extend: null pointer");
+  GKI_REQUIRE(aligned16(requests), 1, "gki_page_extend: requests must be 16-byte aligned");
   if (parents) {
     GKI_REQUIRE(max_count <= 256 && words >= 1 && words <= 4 && max_count <= 64 * words, 1,
                 "gki_page_extend: trees hold up to 256 nodes, 64 to a word");
     GKI_REQUIRE(rows == 0 || ancestors, 1, "gki_page_extend: null pointer");
   }
-  const PageStep s{counts, parents, rows, max_count, words, row_starts, base, positions, slots, ancestors};
+  const PageStep s{counts, parents, rows, max_count, words, row_starts, base, positions, slots, ancestors, (int4*)requests};
   return page_extend_dispatch(t, s, (hipStream_t)stream);
 }
 
@@ -949,8 +950,8 @@ int gki_paged_groups(int32_t max_count, int32_t H, int32_t H_kv, int32_t head_di
 }
 
 int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o, float* lse,
-                     const int32_t* row_starts, const int32_t* base, const int32_t* positions, const int32_t* table,
-                     const uint64_t* ancestors, int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R,
+                     const int32_t* requests, const int32_t* positions, const int32_t* table, const uint64_t* ancestors,
+                     int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R,
                      int32_t H, int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t num_pages, int32_t page_size,
                      int32_t sink_size, int32_t window_size, float softmax_scale, float* workspace, int32_t groups,
                      void* stream) {
@@ -962,9 +963,9 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   GKI_REQUIRE(std::isfinite(softmax_scale), 1, "gki_paged_attend: softmax_scale must be finite");
   if (rows == 0) return 0;
   GKI_REQUIRE((int64_t)rows * (H / H_kv) < (1ll << kPartialBit), 1, "gki_paged_attend: too many rows");
-  GKI_REQUIRE(q && k_pages && v_pages && o && row_starts && base && positions && table, 1, "gki_paged_attend: null pointer");
+  GKI_REQUIRE(q && k_pages && v_pages && o && requests && positions && table, 1, "gki_paged_attend: null pointer");
   GKI_REQUIRE(!ancestors || (words >= 1 && words <= 4 && max_count <= 64 * words), 1, "gki_paged_attend: trees hold up to 256 nodes, 64 to a word");
-  GKI_REQUIRE(all_aligned16(q, k_pages, v_pages, o, workspace), 1, "gki_paged_attend: tensors must be 16-byte aligned");
+  GKI_REQUIRE(all_aligned16(q, k_pages, v_pages, o, workspace, requests), 1, "gki_paged_attend: tensors must be 16-byte aligned");
   GKI_REQUIRE(row_stride_ok(q_stride, (int64_t)H * head_dim), 1,
               "gki_paged_attend: the row stride must be a multiple of 8 elements that holds a row");
   GKI_REQUIRE(groups >= 1 && groups <= 4096, 1, "gki_paged_attend: groups must be in 1 .. 4096");
@@ -973,7 +974,7 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   PagedArgs a{};
   a.q = (const uint16_t*)q, a.k_pages = (const uint16_t*)k_pages, a.v_pages = (const uint16_t*)v_pages;
   a.o = (uint16_t*)o, a.lse = lse;
-  a.row_starts = row_starts, a.base = base, a.positions = positions, a.table = table, a.ancestors = ancestors;
+  a.requests = (const int4*)requests, a.positions = positions, a.table = table, a.ancestors = ancestors;
   a.q_stride = q_stride;
   a.R = R, a.rows = rows, a.H = H, a.H_kv = H_kv, a.group = H / H_kv;
   a.max_pages = max_pages, a.shift = log2_of(page_size), a.num_pages = num_pages;

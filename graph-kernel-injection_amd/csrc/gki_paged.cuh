@@ -60,6 +60,7 @@ struct PageStep {
   int32_t *row_starts, *base, *positions;
   int64_t* slots;
   uint64_t* ancestors;
+  int4* requests;                      // [R + 1] {requests with tokens, rows}, then of each {request, first row, rows, base}
 };
 
 // Rows of keys and values and the pool that they go to: [num_pages][H_kv][page_size][D].
@@ -85,7 +86,8 @@ struct PagedArgs {
   const uint16_t *q, *k_pages, *v_pages;
   uint16_t* o;
   float* lse;                          // [rows][H] or null
-  const int32_t *row_starts, *base, *positions, *table;
+  const int4* requests;                // PageStep's
+  const int32_t *positions, *table;
   const uint64_t* ancestors;           // [rows][words], null: no trees
   int64_t q_stride;                    // elements between rows of q; heads lie D apart
   int R, rows, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;

@@ -51,13 +51,13 @@ __device__ inline uint32_t lane_of(uint32_t x, int l) { return (uint32_t)__built
 __device__ inline uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
 struct Request {
-  uint32_t first, n, base, tiles, keys;  // first row of the step's, rows, keys before them; row tiles, the steps of each
-  __device__ inline Request(const PagedArgs& a, int r, int end) {
-    const bool ok = r < end;
-    r = ok ? r : 0;
-    first = a.row_starts[r];
-    n = ok ? a.row_starts[r + 1] - first : 0;
-    base = a.base[r];
+  uint32_t r, first, n, base;          // the request, first row of the step's, rows, keys before them
+  uint32_t tiles, keys;                // row tiles, the steps of each
+  // Number i of those that have tokens, `end` of them (a load of number 0, which may be none, is harmless).
+  __device__ inline Request(const PagedArgs& a, int i, int end) {
+    const int4 x = a.requests[1 + (i < end ? i : 0)];
+    r = x.x, first = x.y, base = x.w;
+    n = i < end ? x.z : 0;
     const uint32_t rows = n * a.group;
     tiles = rows <= kFewRows ? (rows + kFewRows - 1) / kFewRows : (rows + kRowTile - 1) / kRowTile;
     // a walk's prologue and epilogue cost about as much as kPagedPieceCost key tiles
@@ -72,8 +72,8 @@ struct Request {
 struct Place {
   uint32_t first, n, base, tiles, keys, number, start;
   int r;
-  __device__ inline void set(const Request& q, int l, int request, uint32_t before, uint32_t step) {
-    r = request;
+  __device__ inline void set(const Request& q, int l, uint32_t before, uint32_t step) {
+    r = lane_of(q.r, l);
     first = lane_of(q.first, l), n = lane_of(q.n, l), base = lane_of(q.base, l);
     tiles = lane_of(q.tiles, l), keys = lane_of(q.keys, l);
     number = scalar((step - before) / keys);
@@ -88,10 +88,11 @@ struct Shares {
   uint32_t all, share;                 // steps in all, of a workgroup
   uint32_t edge;                       // cuts this close to a row tile's ends move there
   int lane;
-  __device__ inline Shares(const PagedArgs& a, int tid)
-      : q(a, (tid & 63) * ((a.R + 63) >> 6), a.R), run((a.R + 63) >> 6), lane(tid & 63) {
+  int n;                               // requests that have tokens
+  __device__ inline Shares(const PagedArgs& a, int tid, int active)
+      : q(a, (tid & 63) * ((active + 63) >> 6), active), run((active + 63) >> 6), lane(tid & 63), n(active) {
     uint32_t mine = q.steps(a);
-    for (int i = 1; i < run; ++i) mine += Request(a, lane * run + i, a.R).steps(a);
+    for (int i = 1; i < run; ++i) mine += Request(a, lane * run + i, n).steps(a);
     sum = wave_prefix(mine);
     all = lane_of(sum, 63);
     share = scalar(max((uint32_t)kPagedMinShare, (all + a.groups - 1) / a.groups));
@@ -102,17 +103,17 @@ struct Shares {
     const int l = __builtin_ctzll(__ballot(sum > step));
     uint32_t before = l ? lane_of(sum, l - 1) : 0;
     if (run == 1) {
-      p.set(q, l, l, before, step);
+      p.set(q, l, before, step);
       return p;
     }
-    const int end = min((l + 1) * run, a.R);
+    const int end = min((l + 1) * run, n);
     for (int r0 = l * run;; r0 += 64) {
       const Request x(a, r0 + lane, end);
       const uint32_t upto = wave_prefix(x.steps(a));
       const uint64_t past = __ballot(before + upto > step);
       if (past || r0 + 64 >= end) {
         const int m = past ? __builtin_ctzll(past) : 0;
-        p.set(x, m, r0 + m, before + (m ? lane_of(upto, m - 1) : 0), step);
+        p.set(x, m, before + (m ? lane_of(upto, m - 1) : 0), step);
         return p;
       }
       before += lane_of(upto, 63);
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
   __shared__ int64_t pieces[kPagePieces];
   __shared__ uint32_t todo[2][2];
   // rows behind the last request have no output: zeros
-  for (int64_t x = (int64_t)args.row_starts[args.R] * args.H * (D / 8) + (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t x = (int64_t)args.requests[0].y * args.H * (D / 8) + (int64_t)blockIdx.x * 256 + threadIdx.x;
        x < (int64_t)args.rows * args.H * (D / 8); x += (int64_t)gridDim.x * 256) {
     *(uint4*)(args.o + 8 * x) = make_uint4(0, 0, 0, 0);
     if (args.lse && x % (D / 8) == 0) args.lse[x / (D / 8)] = 0.f;
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
     const PagedArgs a = fresh_args();
     int tid = threadIdx.x;             // not an invariant: nothing made from it is held either
     asm volatile("" : "+v"(tid));
-    const Shares s(a, tid);
+    const Shares s(a, tid, a.requests[0].x);
     const int used = (int)((s.all + s.share - 1) / s.share);
     const bool idle = (int)blockIdx.x >= used;
     const int w = idle ? (int)blockIdx.x : xcd_remap(blockIdx.x, used);

@@ -116,7 +116,10 @@ __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, Page
   const int why = bad ? kBadCount : (sums[0] > (unsigned long long)s.rows ? kTooManyRows : 0) |
                                         (sums[1] > (unsigned long long)count + sums[2] ? kOutOfPages : 0);
   if (why) {
-    if (tid == 0) *t.status |= why;
+    if (tid == 0) {
+      *t.status |= why;
+      s.requests[0] = make_int4(0, 0, 0, 0);
+    }
     for (int r = tid; r <= t.R; r += kBookThreads) {
       s.row_starts[r] = 0;
       if (r < t.R) s.base[r] = t.lengths[r];
@@ -147,13 +150,17 @@ __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, Page
     }
   }
   // pages that are taken, the rows' starts, lengths
-  int taken = 0, rows = 0;
+  int taken = 0, rows = 0, active = 0;
   for (int r0 = 0; r0 < t.R; r0 += kBookThreads) {
     const int r = r0 + tid, c = r < t.R ? s.counts[r] : 0;
     const int had = r < t.R ? t.pages[r] : 0, len = r < t.R ? t.lengths[r] : 0;
     const int pages = r < t.R && c > 0 ? max(had, (len + c + (1 << t.shift) - 1) >> t.shift) : had;
     int total_rows, total;
     const int start = rows + block_scan(c, part, total_rows);
+    int total_active;
+    const int place = active + block_scan(c > 0 ? 1 : 0, part, total_active);
+    if (c > 0) s.requests[1 + place] = make_int4(r, start, c, len);
+    active += total_active;
     first[tid] = block_scan(pages - had, part, total);
     from[tid] = had;
     starts[tid] = start;
@@ -174,6 +181,7 @@ __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, Page
   }
   if (tid == 0) {
     s.row_starts[t.R] = rows;
+    s.requests[0] = make_int4(active, rows, 0, 0);
     t.queue[0] = (int)(((int64_t)head + taken) % t.num_pages);
     t.queue[1] = count + given - taken;
   }

@@ -76,7 +76,7 @@ SIGNATURES = {
                                                                      _c_ptr]),
     "gki_rotary": (ctypes.c_int, [_c_ptr, _c_ptr, _c_int, _c_ptr] * 2 + [_c_int, _c_i64, _c_i64, _c_int] + [_c_ptr] * 2
                    + [_c_int] * 3 + [_c_ptr, _c_int, _c_ptr, _c_ptr]),
-    "gki_page_extend": (ctypes.c_int, [_c_ptr] * 2 + [_c_int] * 3 + [_c_ptr] * 7 + [_c_int] * 6 + [_c_ptr] * 6),
+    "gki_page_extend": (ctypes.c_int, [_c_ptr] * 2 + [_c_int] * 3 + [_c_ptr] * 7 + [_c_int] * 6 + [_c_ptr] * 7),
     "gki_page_release": (ctypes.c_int, [_c_ptr] * 8 + [_c_int] * 6 + [_c_ptr]),
     "gki_page_accept": (ctypes.c_int, [_c_ptr] * 4 + [_c_int, _c_ptr]),
     "gki_paged_append": (ctypes.c_int, [_c_ptr] * 2 + [_c_i64] * 2 + [_c_ptr] * 3 + [_c_int] * 6 + [_c_ptr]),
@@ -85,7 +85,7 @@ SIGNATURES = {
                                  + [_c_i64] * 2 + [_c_ptr]),
     "gki_paged_accept": (ctypes.c_int, [_c_ptr] * 6 + [_c_int] * 7 + [_c_ptr]),
     "gki_paged_groups": (ctypes.c_int, [_c_int] * 8 + [_c_ptr]),
-    "gki_paged_attend": (ctypes.c_int, [_c_ptr, _c_i64] + [_c_ptr] * 9 + [_c_int] * 13 + [_c_float, _c_ptr, _c_int,
+    "gki_paged_attend": (ctypes.c_int, [_c_ptr, _c_i64] + [_c_ptr] * 8 + [_c_int] * 13 + [_c_float, _c_ptr, _c_int,
                                                                                         _c_ptr]),
     "gki_read_probe_words": (ctypes.c_int64, [_c_int]),
     "gki_read_probe": (ctypes.c_int, [_c_ptr, _c_ptr, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_ptr,

@@ -72,31 +72,38 @@ class TokenBatch:
 
     def __init__(self, table, rows, max_count, words, ancestors, ints) -> None:
         self.table, self.rows, self.max_count, self.words = table, rows, max_count, words
-        # slots (int64), then row_starts, base and positions, in one allocation of int32
+        # requests (PageTable's for attend), slots (int64), row_starts, base and positions, in one
+        # allocation of int32
         self.ancestors, self._ints = ancestors, ints
 
     @property
     def slots(self) -> torch.Tensor:
-        return self._ints[:2 * self.rows].view(torch.int64)
+        at = 4 * (self.table.max_requests + 1)
+        return self._ints[at:at + 2 * self.rows].view(torch.int64)
+
+    def _after_slots(self, start: int, end: Optional[int]) -> torch.Tensor:
+        at = 4 * (self.table.max_requests + 1) + 2 * self.rows
+        return self._ints[at + start:None if end is None else at + end]
 
     @property
     def row_starts(self) -> torch.Tensor:
-        return self._ints[2 * self.rows:2 * self.rows + self.table.max_requests + 1]
+        return self._after_slots(0, self.table.max_requests + 1)
 
     @property
     def base(self) -> torch.Tensor:
-        n, at = self.table.max_requests, 2 * self.rows
-        return self._ints[at + n + 1:at + 2 * n + 1]
+        n = self.table.max_requests
+        return self._after_slots(n + 1, 2 * n + 1)
 
     @property
     def positions(self) -> torch.Tensor:
-        return self._ints[2 * (self.rows + self.table.max_requests) + 1:]
+        return self._after_slots(2 * self.table.max_requests + 1, None)
 
-    def _pointers(self) -> Tuple[int, int, int, int]:
-        """Of slots, row_starts, base and positions."""
+    def _pointers(self) -> Tuple[int, int, int, int, int]:
+        """Of requests, slots, row_starts, base and positions."""
         at, n = self._ints.data_ptr(), self.table.max_requests
-        starts = at + 8 * self.rows
-        return at, starts, starts + 4 * (n + 1), starts + 4 * (2 * n + 1)
+        slots = at + 16 * (n + 1)
+        starts = slots + 8 * self.rows
+        return at, slots, starts, starts + 4 * (n + 1), starts + 4 * (2 * n + 1)
 
 
 class PageTable:
@@ -179,15 +186,15 @@ class PageTable:
                 raise ValueError(f"trees hold up to {_MAX_DRAFT} nodes: max_count is {max_count}")
             words = max(1, -(-max_count // 64))
             ancestors = torch.empty((rows, words), dtype=torch.int64, device=self.device)
-        ints = torch.empty(2 * self.max_requests + 1 + 3 * rows, dtype=torch.int32, device=self.device)
+        ints = torch.empty(6 * self.max_requests + 5 + 3 * rows, dtype=torch.int32, device=self.device)
         batch = TokenBatch(self, rows, max_count, words, ancestors, ints)
-        slots, row_starts, base, positions = batch._pointers()
+        requests, slots, row_starts, base, positions = batch._pointers()
         lib = _lib.load()
         with _on_device(self.device):
             rc = lib.gki_page_extend(
                 counts.data_ptr(), 0 if parents is None else parents.data_ptr(), rows, max_count, words,
                 *self._arguments(), row_starts, base, positions, slots,
-                0 if ancestors is None else ancestors.data_ptr(), _current_stream(self.device))
+                0 if ancestors is None else ancestors.data_ptr(), requests, _current_stream(self.device))
         if rc:
             _lib.check(rc, "gki_page_extend")
         return batch
@@ -198,7 +205,7 @@ class PageTable:
         if batch.table is not self:
             raise ValueError("the batch belongs to another table")
         accepted = _int_vector("accepted", accepted, (self.max_requests,), self.device)
-        _, row_starts, base, _ = batch._pointers()
+        _, _, row_starts, base, _ = batch._pointers()
         with _on_device(self.device):
             rc = _lib.load().gki_page_accept(self._state.data_ptr(), base, row_starts, accepted.data_ptr(),
                                              self.max_requests, _current_stream(self.device))
@@ -296,7 +303,7 @@ class PagedKVCache:
         with _on_device(self.device):
             rc = _lib.load().gki_paged_append(
                 k.data_ptr(), v.data_ptr(), k_stride, v_stride, self.k_pages.data_ptr(), self.v_pages.data_ptr(),
-                batch._pointers()[0], self._dtype, batch.rows, self.heads, self.head_dim, t.num_pages, t.page_size,
+                batch._pointers()[1], self._dtype, batch.rows, self.heads, self.head_dim, t.num_pages, t.page_size,
                 _current_stream(self.device))
         if rc:
             _lib.check(rc, "gki_paged_append")
@@ -312,7 +319,7 @@ class PagedKVCache:
         if rotary.head_dim != self.head_dim:
             raise ValueError(f"rotary must have head_dim {self.head_dim}, got {rotary.head_dim}")
         if positions is None:
-            at, wide, axis_stride, row_stride = batch._pointers()[3], 0, 0, 1
+            at, wide, axis_stride, row_stride = batch._pointers()[4], 0, 0, 1
         else:
             axis_stride, _, row_stride = rotary._position_strides(positions, q)
             at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
@@ -322,7 +329,7 @@ class PagedKVCache:
         with _on_device(self.device):
             rc = _lib.load().gki_paged_append_rotated(
                 q.data_ptr(), out.data_ptr(), q_stride, q.shape[1], k.data_ptr(), v.data_ptr(), k_stride, v_stride,
-                self.k_pages.data_ptr(), self.v_pages.data_ptr(), batch._pointers()[0], self._dtype, batch.rows,
+                self.k_pages.data_ptr(), self.v_pages.data_ptr(), batch._pointers()[1], self._dtype, batch.rows,
                 self.heads, self.head_dim, t.num_pages, t.page_size, turns.data_ptr(), axis.data_ptr(), rotary.pairs,
                 int(rotary.interleaved), at, wide, axis_stride, row_stride, _current_stream(self.device))
         if rc:
@@ -355,10 +362,11 @@ class PagedKVCache:
         work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+        requests, _, _, _, positions = batch._pointers()
         with _on_device(self.device):
             rc = lib.gki_paged_attend(
                 q.data_ptr(), q_stride, self.k_pages.data_ptr(), self.v_pages.data_ptr(), o.data_ptr(),
-                0 if lse is None else lse.data_ptr(), *batch._pointers()[1:], t.block_table.data_ptr(),
+                0 if lse is None else lse.data_ptr(), requests, positions, t.block_table.data_ptr(),
                 0 if batch.ancestors is None else batch.ancestors.data_ptr(), batch.words, self._dtype, batch.rows,
                 batch.max_count, t.max_requests, H, self.heads, self.head_dim, t.max_pages, t.num_pages, t.page_size,
                 t.sink_size, t.window_size, scale, work.data_ptr() if floats else 0, groups,
@@ -380,7 +388,7 @@ class PagedKVCache:
         accepted = _int_vector("accepted", accepted, (t.max_requests,), self.device)
         with _on_device(self.device):
             rc = _lib.load().gki_paged_accept(
-                self.k_pages.data_ptr(), self.v_pages.data_ptr(), *batch._pointers()[:2],
+                self.k_pages.data_ptr(), self.v_pages.data_ptr(), *batch._pointers()[1:3],
                 paths.data_ptr(), accepted.data_ptr(), self._dtype, t.max_requests, paths.shape[1], self.heads,
                 self.head_dim, t.num_pages, t.page_size, _current_stream(self.device))
         if rc:

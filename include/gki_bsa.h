@@ -400,7 +400,9 @@ int gki_rotary(const void* q, void* q_out, int32_t q_heads, const int64_t* q_str
  * token of an extended request does not see (StreamingLLM rule) go back first, in the
  * order of requests and positions, as do pages taken. With parents (int32 [rows]): trees
  * of up to 256 nodes; a node stands at base + depth, ancestors (uint64 [rows, words], words
- * >= ceil(max_count / 64)) are the nodes that it sees. A step that does not fit changes
+ * >= ceil(max_count / 64)) are the nodes that it sees. requests (16-byte aligned int32
+ * [R + 1, 4], for gki_paged_attend): how many requests have tokens and their rows, then of each
+ * its number, first row, rows and base. A step that does not fit changes
  * nothing, leaves no rows and sets bits of status: 1 no free pages, 2 more tokens than
  * rows, 4 a count below 0, above max_count or past max_pages * page_size. */
 int gki_page_extend(const int32_t* counts, const int32_t* parents, int32_t rows, int32_t max_count,
@@ -408,7 +410,7 @@ int gki_page_extend(const int32_t* counts, const int32_t* parents, int32_t rows,
                     int32_t* ring, int32_t* queue, int32_t* status, int32_t R, int32_t max_pages,
                     int32_t page_size, int32_t num_pages, int32_t sink_size, int32_t window_size,
                     int32_t* row_starts, int32_t* base, int32_t* positions, int64_t* slots,
-                    uint64_t* ancestors, void* stream);
+                    uint64_t* ancestors, int32_t* requests, void* stream);
 
 /* Requests with done[r] != 0 give all their pages back and hold nothing. */
 int gki_page_release(const uint8_t* done, int32_t* lengths, int32_t* pages, int32_t* kept,
@@ -456,13 +458,13 @@ int gki_paged_groups(int32_t max_count, int32_t H, int32_t H_kv, int32_t head_di
 
 /* O (and, lse not NULL, the natural LSE [rows, H]) of a step's rows: a row at position p sees
  * the keys x <= p of its request with x < sink_size or x > p - window_size; with ancestors,
- * from base[r] on those that its words name. row_starts, base, positions, ancestors and
- * table as gki_page_extend leaves them, max_count as it was given there. workspace NULL: no
+ * from its base on those that its words name. requests, positions, ancestors and table as
+ * gki_page_extend leaves them, max_count as it was given there. workspace NULL: no
  * walk is cut. Rows that see no key, and rows behind the last
  * request: zeros. */
 int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* o,
-                     float* lse, const int32_t* row_starts, const int32_t* base,
-                     const int32_t* positions, const int32_t* table, const uint64_t* ancestors,
+                     float* lse, const int32_t* requests, const int32_t* positions,
+                     const int32_t* table, const uint64_t* ancestors,
                      int32_t words, int32_t dtype, int32_t rows, int32_t max_count, int32_t R, int32_t H,
                      int32_t H_kv, int32_t head_dim, int32_t max_pages, int32_t num_pages,
                      int32_t page_size, int32_t sink_size, int32_t window_size, float softmax_scale,

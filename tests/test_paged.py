@@ -28,16 +28,16 @@ def test_c_entries_refuse_before_launch():
     lib = _lib.load()
 
     def extend(counts=16, parents=0, rows=5, max_count=5, words=1, R=2, max_pages=8, page=64, pages=9, sink=4, window=8,
-               starts=16, slots=16, ancestors=16):
+               starts=16, slots=16, ancestors=16, requests=16):
         return lib.gki_page_extend(counts, parents, rows, max_count, words, *[16] * 7, R, max_pages, page, pages, sink,
-                                   window, starts, 16, 16, slots, ancestors, NULL)
+                                   window, starts, 16, 16, slots, ancestors, requests, NULL)
 
     assert extend(page=48) == 1 and extend(page=8) == 1 and extend(page=2048) == 1 and extend(R=0) == 1
     assert extend(pages=0) == 1 and extend(pages=2**25) == 1 and extend(max_pages=2**25) == 1 and extend(sink=-1) == 1
     assert extend(sink=2**30) == 1 and extend(window=-1) == 1 and extend(rows=-1) == 1 and extend(counts=0) == 1
     assert extend(starts=0) == 1 and extend(slots=0) == 1 and extend(R=2**21) == 1
     assert extend(parents=16, rows=300, max_count=257, words=5) == 1 and extend(parents=16, max_count=65, rows=65) == 1
-    assert extend(parents=16, ancestors=0) == 1
+    assert extend(parents=16, ancestors=0) == 1 and extend(requests=0) == 1 and extend(requests=8) == 1
     assert lib.gki_page_release(0, *[16] * 7, 2, 8, 64, 9, 4, 8, NULL) == 1
     assert lib.gki_page_accept(16, 16, 16, 16, 0, NULL) == 1 and lib.gki_page_accept(16, 0, 16, 16, 2, NULL) == 1
 
@@ -58,7 +58,7 @@ def test_c_entries_refuse_before_launch():
 
     def attend(q=16, stride=256, o=16, words=0, ancestors=0, dtype=2, rows=3, most=3, R=2, H=4, H_kv=2, D=64, scale=0.1,
                ws=0, n=1, sink=4, window=8):
-        return lib.gki_paged_attend(q, stride, 16, 16, o, 0, 16, 16, 16, 16, ancestors, words, dtype, rows, most, R, H, H_kv,
+        return lib.gki_paged_attend(q, stride, 16, 16, o, 0, 16, 16, 16, ancestors, words, dtype, rows, most, R, H, H_kv,
                                     D, 8, 9, 64, sink, window, scale, ws, n, NULL)
 
     assert attend(dtype=0) == 2 and attend(D=16) == 2 and attend(H=3) == 1 and attend(R=0) == 1 and attend(q=0) == 1
