@@ -988,7 +988,6 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
     a.ml = workspace + 2ll * groups * a.cap * head_dim;
     a.cuts = (CutTile*)(a.ml + 4ll * groups * a.cap);
   }
-  GKI_REQUIRE((int64_t)rows * H < (1ll << 26), 1, "gki_paged_attend: the grid must fit");
   const int64_t tiles = ((int64_t)rows * a.group / 128 + std::min(R, rows)) * H_kv;
   const int64_t keys = std::min<int64_t>((int64_t)max_pages * page_size, (int64_t)sink_size + a.window + max_count) / 64 + 4;
   while (tiles * (std::max<int64_t>(kPagedMinShare, keys >> a.coarse) + 1) >= (1ll << 31) && a.coarse < 31) ++a.coarse;

@@ -580,14 +580,14 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
     return;
   }
   const int64_t row = (int64_t)(u.first + my / e.group) * e.H + u.h * e.group + my % e.group;
-  const float inv = l > 0.f ? 1.f / l : 1.f;
+  const float inv = l == 0.f ? 1.f : 1.f / l;              // no visible key: 0; NaN stays NaN
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       *(uint2*)(e.o + row * D + 32 * dt + 8 * r + 4 * hi_e) =
           make_uint2(pack2<T>(o[dt][4 * r] * inv, o[dt][4 * r + 1] * inv), pack2<T>(o[dt][4 * r + 2] * inv, o[dt][4 * r + 3] * inv));
-  if (hi_e == 0 && e.lse) e.lse[row] = l > 0.f ? lse_natural(-nm, l) : 0.f;
+  if (hi_e == 0 && e.lse) e.lse[row] = l == 0.f ? 0.f : lse_natural(-nm, l);
 }
 
 template <typename T, int D>

@@ -66,7 +66,8 @@ class TokenBatch:
     ``r`` being ``row_starts[r] .. row_starts[r + 1] - 1``; ``base[r]`` positions came before
     them. ``slots`` (page * page_size + place in it) and ``positions`` of each row, -1 and 0
     behind the last request. Drafts: ``ancestors``, 64 nodes to a word, which of a request's
-    nodes a row sees."""
+    nodes a row sees. A batch serves its requests until their next ``extend`` or ``release``,
+    which may give pages back that its rows see."""
 
     __slots__ = ("table", "rows", "max_count", "words", "ancestors", "_ints")
 
@@ -200,8 +201,9 @@ class PageTable:
         return batch
 
     def accept(self, batch: TokenBatch, accepted: torch.Tensor) -> None:
-        """Of the tokens that the last ``extend`` placed, request ``r`` keeps the first
-        ``accepted[r]`` (clamped to ``0 .. count``); their pages stay the request's."""
+        """Of the tokens that ``batch`` placed, request ``r`` keeps the first ``accepted[r]``
+        (clamped to ``0 .. count``); their pages stay the request's. Requests without tokens
+        in the batch keep their length."""
         if batch.table is not self:
             raise ValueError("the batch belongs to another table")
         accepted = _int_vector("accepted", accepted, (self.max_requests,), self.device)
@@ -378,8 +380,8 @@ class PagedKVCache:
     def accept(self, batch: TokenBatch, paths: torch.Tensor, accepted: torch.Tensor) -> None:
         """Moves the rows of each request's accepted path, nodes ``paths[r, 0 .. accepted[r] -
         1]`` of the batch's drafts from the root down (int32 or int64 ``[max_requests, n]``),
-        to the slots of positions ``base[r], base[r] + 1, ...``; ``table.accept`` then sets the
-        lengths. A node that is not ``i .. count - 1`` at place ``i`` moves nothing."""
+        to the slots of positions ``base[r], base[r] + 1, ...``; ``table.accept`` with the same
+        ``accepted`` (at most ``n``) then sets the lengths. A node that is not ``i .. count - 1`` at place ``i`` moves nothing."""
         self._batch(batch)
         t = self.table
         if paths.dim() != 2:

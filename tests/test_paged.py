@@ -562,6 +562,53 @@ def test_an_accepted_path_moves_up(D, page):
 
 
 @pytest.mark.gpu
+def test_batches_of_different_requests_side_by_side():
+    """Two steps of one table, each with requests of its own, attended and accepted in any order."""
+    run = Run(3, 60, 4, 50, 16, seed=19)
+    run.grow([60, 5, 90])
+    one = run.extend([7, 0, 0])
+    k, v, q = run.normal(7, 2), run.normal(7, 2), run.normal(7, 4)
+    first = run.base, run.counts, k, v, q
+    two = run.extend([0, 2, 30])
+    run.append(two)
+    q2 = run.normal(32, 4)
+    run.cache.append(k, v, one)
+    run.check_attend(two, q2, run.cache.attend(q2, two))
+    run.table.accept(one, _ints([3, 9, 9]))
+    assert run.table.lengths.tolist() == [63, 7, 120]
+    run.table.accept(two, _ints([9, 1, 30]))
+    assert run.table.lengths.tolist() == [63, 6, 120]
+    run.base, run.counts, k, v, q = first
+    run.hold(k, v)
+    run.check_attend(one, q, run.cache.attend(q, one))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[1, 2], [70, 3]])
+def test_what_is_not_finite_stays_with_its_request(counts):
+    """NaN in one request's keys, values or queries reaches no other request; a NaN query its own row alone."""
+    run = Run(2, 60, 4, 100, 16, seed=20)
+    run.grow([30, 100])
+    batch = run.extend(counts)
+    k, v, q = run.normal(batch.rows, 2), run.normal(batch.rows, 2), run.normal(batch.rows, 4)
+    run.append(batch, k, v)
+    want, want_lse = run.cache.attend(q, batch, return_lse=True)
+    bad_q = q.clone()
+    bad_q[counts[0], 1] = math.nan
+    o, lse = run.cache.attend(bad_q, batch, return_lse=True)
+    assert o[counts[0], 1].isnan().all() and lse[counts[0], 1].isnan()
+    o[counts[0], 1], lse[counts[0], 1] = want[counts[0], 1], want_lse[counts[0], 1]
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+    for bad in (math.nan, math.inf, -math.inf):
+        bad_k, bad_v = k.clone(), v.clone()          # the first request's rows as before
+        bad_k[counts[0]:] = bad_v[counts[0]:] = bad
+        run.cache.append(bad_k, bad_v, batch)
+        o = run.cache.attend(q, batch)
+        assert torch.equal(o[:counts[0]], want[:counts[0]])
+        assert not o[counts[0]:].isfinite().all()
+
+
+@pytest.mark.gpu
 def test_paths_that_are_none_move_nothing():
     run = Run(2, 30, 4, 50, 16, seed=12)
     batch = run.extend([6, 3], parents=[[-1, 0, 0, 1, 1, 2], [-1, 0, 1]])
