@@ -280,13 +280,14 @@ __global__ __launch_bounds__(kBookThreads) void release_kernel(PageTables t, con
   if (tid == 0) t.queue[1] = count + given;
 }
 
-// lengths = base + what is accepted of the step's tokens; requests without any stay as they are.
+// lengths = base + what is accepted of the step's tokens, if less than they are: a request
+// that was released since holds no pages, and must not be long again.
 __global__ __launch_bounds__(256) void accept_kernel(int32_t* lengths, const int32_t* base, const int32_t* row_starts,
                                                      const int32_t* accepted, int R) {
   const int r = blockIdx.x * 256 + threadIdx.x;
   if (r >= R) return;
   const int n = row_starts[r + 1] - row_starts[r];
-  if (n > 0) lengths[r] = base[r] + max(0, min(accepted[r], n));
+  if (n > 0) lengths[r] = min(lengths[r], base[r] + max(0, min(accepted[r], n)));
 }
 
 // ---------------------------------------------------------------------------

@@ -203,7 +203,7 @@ class PageTable:
     def accept(self, batch: TokenBatch, accepted: torch.Tensor) -> None:
         """Of the tokens that ``batch`` placed, request ``r`` keeps the first ``accepted[r]``
         (clamped to ``0 .. count``); their pages stay the request's. Requests without tokens
-        in the batch keep their length."""
+        in the batch keep their length, and none grows: what a call gave up is gone."""
         if batch.table is not self:
             raise ValueError("the batch belongs to another table")
         accepted = _int_vector("accepted", accepted, (self.max_requests,), self.device)

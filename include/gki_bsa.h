@@ -418,8 +418,8 @@ int gki_page_release(const uint8_t* done, int32_t* lengths, int32_t* pages, int3
                      int32_t max_pages, int32_t page_size, int32_t num_pages, int32_t sink_size,
                      int32_t window_size, void* stream);
 
-/* lengths[r] = base[r] + accepted[r], clamped to the tokens that the step gave r, for each
- * request that got any. */
+/* lengths[r] = base[r] + accepted[r], clamped to the tokens that the step gave r, where that is
+ * less than lengths[r], for each request that got any. */
 int gki_page_accept(int32_t* lengths, const int32_t* base, const int32_t* row_starts,
                     const int32_t* accepted, int32_t R, void* stream);
 

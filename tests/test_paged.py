@@ -584,6 +584,30 @@ def test_batches_of_different_requests_side_by_side():
 
 
 @pytest.mark.gpu
+def test_accepting_never_lengthens():
+    """A second accept, or one after its request was released, gives no position without a page."""
+    run = Run(3, 60, 20, 50, 16, seed=21)
+    run.grow([60, 5, 90])
+    batch = run.extend([7, 2, 30])
+    run.append(batch)
+    run.table.accept(batch, _ints([3, 1, 20]))
+    run.table.accept(batch, _ints([7, 0, 25]))
+    assert run.table.lengths.tolist() == [63, 5, 110]
+    run.table.release(torch.tensor([True, False, True], device=DEV))
+    run.table.accept(batch, _ints([7, 2, 30]))
+    assert run.table.lengths.tolist() == [0, 5, 0]
+    run.book.release([True, False, True])
+    run.book.length[1] = 5
+    for r in (0, 2):
+        run.k[r], run.v[r] = run.k[r][:0], run.v[r][:0]
+    batch = run.extend([70, 3, 1])
+    run.append(batch)
+    run.check_tables(batch)
+    q = run.normal(74, 4)
+    run.check_attend(batch, q, run.cache.attend(q, batch))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("counts", [[1, 2], [70, 3]])
 def test_what_is_not_finite_stays_with_its_request(counts):
     """NaN in one request's keys, values or queries reaches no other request; a NaN query its own row alone."""
