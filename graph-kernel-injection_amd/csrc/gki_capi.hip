@@ -990,6 +990,7 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   }
   const int64_t tiles = ((int64_t)rows * a.group / 128 + std::min(R, rows)) * H_kv;
   const int64_t keys = std::min<int64_t>((int64_t)max_pages * page_size, (int64_t)sink_size + a.window + max_count) / 64 + 4;
+  a.least = (int)std::clamp<int64_t>(keys / kPagedPieces, kPagedMinShare, kPagedMostShare);
   while (tiles * (std::max<int64_t>(kPagedMinShare, keys >> a.coarse) + 1) >= (1ll << 31) && a.coarse < 31) ++a.coarse;
   GKI_REQUIRE(a.coarse < 31, 1, "gki_paged_attend: the grid must fit");
   return paged_attend_dispatch(dtype, head_dim, a, (hipStream_t)stream);

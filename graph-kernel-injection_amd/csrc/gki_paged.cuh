@@ -77,10 +77,24 @@ struct PageRows {
   }
 };
 
-// Key tiles that a workgroup's share has at least, and workgroups that the card holds at once.
-constexpr int kPagedMinShare = 8;
-constexpr int kPagedPieceCost = 2;
+// How attention over pages is shared out; us of kernel at bf16 D128, H32/8 (H64/8: trees of 60),
+// and fp16 D64 H16 ("mixed").
+//
+// Workgroups that take shares: as many as the card holds at once. 256 / 512 / 768 / 1024 at
+// D128: 32 decodes over up to 4096 keys 48 / 43 / 48 / 47, chunks of 512 137 / 109 / 124 / 112, trees of 60
+// 162 / 124 / 142 / 136; 512 / 768 / 1024 / 1536 at D64: mixed 57 / 51 / 48 / 50.
 inline int paged_groups(int head_dim) { return head_dim >= 128 ? 512 : 1024; }
+// What a walk's prologue and epilogue count, in 64-key steps: 0 / 2 / 4 / 6: chunks 108 / 102 / 101 /
+// 102, mixed 48.5 / 44.9 / 46.4 / 45.8, trees of 60 121 / 119 / 125 / 129.
+constexpr int kPagedPieceCost = 2;
+// Steps that a share has at least: a walk as long as the longest gets about kPagedPieces pieces,
+// whose join costs as much as they save from there on. One decode over 768 / 4096 / 16384 keys,
+// with the join: 2 steps at least 13.6 / 22.0 / 31.1, 4 15.8 / 18.5 / 30.4, 8 - / 20.9 / -, 16 - /
+// 27.4 / -; this rule 13.6 / 18.3 / 29.2.
+constexpr int kPagedMinShare = 2, kPagedMostShare = 8, kPagedPieces = 16;
+// Walks shorter than this are not cut: the join is another launch (9 key tiles of 8 heads, cut 14.1,
+// whole 11.0; 14 tiles cut 13.6, whole 17.5).
+constexpr int kPagedCutSteps = 16;
 
 struct PagedArgs {
   const uint16_t *q, *k_pages, *v_pages;
@@ -94,6 +108,7 @@ struct PagedArgs {
   float scale_log2, q_sign;            // as StreamArgs': the sign of the scale, or zero, goes to q
   uint32_t q_and, q_xor;               // the same as words of Q
   int groups;                          // workgroups that share the work
+  int least;                           // steps that a share has at least
   int coarse;                          // a step of the work is 2^coarse key tiles, so that 31 bits count them all
   // the states of row tiles that the shares' ends cut, of `cap` rows each; acc null: none is cut
   int cap;
@@ -106,13 +121,13 @@ struct CutTile {
   int first, n, h, tile, pieces;
 };
 
-// Rows of a piece's state, and the floats of all states and cuts (0 where no row tile's walk,
-// by what the host knows, is long enough to be cut).
+// Rows of a piece's state, and the floats of all states and cuts (0 where no row tile's walk, by what
+// the host knows, is long enough to be cut). States are in 32 bits.
 inline int paged_cap(int64_t max_count, int group) { return (int)std::min<int64_t>(128, max_count * group); }
 inline int64_t paged_workspace(int groups, int head_dim, int64_t max_count, int group, int64_t sink, int64_t window,
                                int64_t max_length) {
   const int64_t seen = std::min(max_length, sink + window + max_count + 64);
-  if ((seen + 63) / 64 + 2 < 2 * kPagedMinShare) return 0;      // a join costs what eight steps do
+  if ((seen + 63) / 64 + 2 < kPagedCutSteps) return 0;
   return (int64_t)groups * (2 * paged_cap(max_count, group) * (head_dim + 2) + 5);
 }
 

@@ -8,9 +8,9 @@
 // that its word of ancestors names (which has the rule in it already).
 //
 // The rows of a request that read one kv head, (token, q head of the group) token by token,
-// are its rows here. Up to 32 of them run as a stream (four waves share out the keys of a
+// are its rows here. Up to 16 of them run as a stream (four waves share out the keys of a
 // step), more as tiles of 128 (four waves of 32 rows). Either walks the 64-key tiles of the
-// sinks and of its rows' windows once, whatever lies between, or a slice of them; slices'
+// sinks and of its rows' windows once, whatever lies between, or a piece of them; pieces'
 // states are joined. Pages are addressed a 1 KB LDS block at a time, each of which lies in
 // one page; keys past the request's last, and pages that it does not have, are zeros
 // without being read: what another request left in a page is never seen. (A NaN or
@@ -22,7 +22,14 @@ namespace gki {
 namespace {
 
 constexpr int kRowTile = 128;          // rows of a tile: four waves of 32
-constexpr int kFewRows = 32;           // up to as many run as a stream
+// Up to as many run as a stream, us with the join, stream / tile: 32 requests' decodes of 4 rows over
+// 4096 keys (D128) 91 / 106, 64 of 16 rows over 2048 95 / 101, 16 of 16 rows over 4096 54 / 52, one
+// over 512 (D64) 11.1 / 12.9; with two blocks of 16 rows: 16 of 32 rows over 4096 63 / 55, 32 of 32
+// rows over 1024 (D64) 31 / 26.
+constexpr int kFewRows = 16;
+// A cut closer than this to a row tile's ends moves there, and closer than a 16th of a share (a 4th /
+// 8th / 16th: chunks of 512 112 / 110 / 107 us, trees of 60 131 / 126 / 122).
+constexpr uint32_t kCutEdge = 4;
 constexpr int kPagePieces = 512;       // pieces of pages whose places are held in LDS at a time
 
 // The 64-key tiles that rows at positions lo_pos .. see of keys 0 .. end - 1: the sinks',
@@ -44,7 +51,8 @@ struct KeyTiles {
 // workgroup each: requests of any lengths load the card evenly. A row tile that a cut
 // divides leaves the states of its pieces, which are joined; a cut close to its ends
 // moves there. Lengths are known on the device only, so every workgroup counts for
-// itself, a wave 64 requests at a time. Neighbours work on one XCD: row tiles of a
+// itself, a wave 64 requests at a time (`extend` lists those that have tokens: 32 of 4096
+// requests cost what 32 of 32 do, 47 us). Neighbours work on one XCD: row tiles of a
 // (request, head) meet their keys in its L2.
 // ---------------------------------------------------------------------------
 __device__ inline uint32_t lane_of(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
@@ -59,7 +67,7 @@ struct Request {
     r = x.x, first = x.y, base = x.w;
     n = i < end ? x.z : 0;
     const uint32_t rows = n * a.group;
-    tiles = rows <= kFewRows ? (rows + kFewRows - 1) / kFewRows : (rows + kRowTile - 1) / kRowTile;
+    tiles = (rows + kRowTile - 1) / kRowTile;
     // a walk's prologue and epilogue cost about as much as kPagedPieceCost key tiles
     const uint32_t k = KeyTiles(a, base, base + n).n + kPagedPieceCost;
     keys = max((uint32_t)kPagedMinShare, (k + (1u << a.coarse) - 1) >> a.coarse);
@@ -95,8 +103,8 @@ struct Shares {
     for (int i = 1; i < run; ++i) mine += Request(a, lane * run + i, n).steps(a);
     sum = wave_prefix(mine);
     all = lane_of(sum, 63);
-    share = scalar(max((uint32_t)kPagedMinShare, (all + a.groups - 1) / a.groups));
-    edge = max((uint32_t)kPagedMinShare / 2, share / 16);
+    share = scalar(max((uint32_t)a.least, (all + a.groups - 1) / a.groups));
+    edge = max(min(kCutEdge, share / 2), share / 16);
   }
   __device__ inline Place place(const PagedArgs& a, uint32_t step) const {      // step < all
     Place p;
@@ -262,7 +270,7 @@ struct PageTiles {
 };
 
 // ---------------------------------------------------------------------------
-// Up to 32 rows.
+// Up to 16 rows.
 // ---------------------------------------------------------------------------
 struct StreamRow {
   int pos;
@@ -286,9 +294,12 @@ struct PagedRule {
 __device__ inline float* piece_acc(const PagedArgs& a, int state, int r, int D) { return a.acc + ((int64_t)state * a.cap + r) * D; }
 __device__ inline float2* piece_ml(const PagedArgs& a, int state, int r) { return (float2*)a.ml + (int64_t)state * a.cap + r; }
 
-// As the streams of the other caches: two key tiles in flight, so that no registers hold
-// loads. Bound by HBM.
-template <typename T, int D, int NB>
+// As the streams of the other caches: two key tiles in flight by LDS-DMA, so that no registers
+// hold loads. P is rounded to T for the matrix pipe, and the sums are those of the rounded P, so
+// that what rounding adds to a row's weights it adds to their sum (fp16: 2.8e-4 of the result, 3.2e-4
+// with sums before rounding). Bound by HBM: 32 decodes over 4096 keys, D128 H32/8, 537 MB in
+// 91 us with the join, 5.9 TB/s.
+template <typename T, int D>
 __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int64_t* pieces, int tid) {
   constexpr int TILE = kTileN * D;
   const int rows = u.n * a.group;
@@ -302,7 +313,7 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
   };
   if (page.c0 < page.c1) issue(page.c0);
   if (page.c0 + 1 < page.c1) issue(page.c0 + 1);
-  StreamWave<T, T, D, NB, 1, true, false, StreamRow, true> w(
+  StreamWave<T, T, D, 1, 1, true, false, StreamRow, true> w(
       0, rows, a.q_sign,
       [&](int r) { return a.q + (int64_t)token(r) * a.q_stride + (u.h * a.group + r % a.group) * D; },
       [&](int r) {
@@ -339,7 +350,10 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
 // row sums on the matrix pipe too. At head_dim 128 the loop is skewed by one key tile, as
 // in the prefill forward: S of tile c + 1 (matrix cores) while tile c's probabilities are
 // formed (VALU), then O of tile c while the maxima of S are taken, the two interleaved by
-// sched_group_barrier. K is read one tile ahead of V.
+// sched_group_barrier. K is read one tile ahead of V. P is rounded to T, as are the outputs; S, the
+// maxima, the sums and O are in 32 bits. Two workgroups of a CU take 2.0 us for a 64-key step of
+// each (1.07 PFLOP/s on 256 CUs), one alone 1.25 to 1.43: bound by the matrix pipe and the VALU
+// together. Chunks of 512 (4 requests, H32/8, W4096) 99 us of kernel for 68 GFLOP.
 template <int D> constexpr bool kPagedSkew = D >= 128;
 constexpr int kAheadS = 4, kAheadO = 8, kValuS = 3, kValuO = 1;
 
@@ -383,8 +397,8 @@ __device__ inline void paged_tile(const PagedArgs& a, const Unit& u, uint16_t* s
   floatx16 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = splat16(0.f);
-  floatx4 lsum = floatx4{0.f, 0.f, 0.f, 0.f};
   // row sums on the matrix pipe: lane l gets that of row l & 31 of the operand of 32 rows
+  floatx4 lsum = floatx4{0.f, 0.f, 0.f, 0.f};
   const float slack = kStreamSlack / a.scale_log2;
   float nm = 0.f, thr = kNegInf;
 
@@ -630,8 +644,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
         a.cuts[w] = CutTile{u.first, u.n, u.h, u.tile, 2 + (int)((p.start + p.keys - s.edge) / s.share - (w + 1))};
     }
     const int rows = u.n * a.group;
-    if (rows <= 16) paged_stream<T, D, 1>(a, u, sk[0], sv[0], pieces, tid);
-    else if (rows <= kFewRows) paged_stream<T, D, 2>(a, u, sk[0], sv[0], pieces, tid);
+    if (rows <= kFewRows) paged_stream<T, D>(a, u, sk[0], sv[0], pieces, tid);
     else paged_tile<T, D>(a, u, sk[0], sv[0], pieces, tid);
     __syncthreads();                   // LDS is read no more
   }
@@ -640,14 +653,15 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
 // The pieces of the row tile that workgroup blockIdx.x's share ends in, if it is cut, joined: a
 // thread for four elements of a row, pieces in order. As join_kernel: O = sum_p f_p acc_p / sum_p
 // f_p l_p, f_p = exp2(m_p - M). Bound by latency (the cut, the maxima, the sums): many small
-// workgroups, most of which leave at once.
+// workgroups, most of which leave at once. 4.6 us for 32 decodes, 12 for trees of 60
+// (19 where a thread had more of a row), 13 where 128 rows of every share are cut (67 MB of states).
 constexpr int kJoinThreads = 256;
 template <typename T, int D>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a) {
   constexpr int RPG = kJoinThreads / (D / 4);
   const CutTile c = a.cuts[blockIdx.x];
   if (c.pieces == 0) return;
-  const int rows = c.n * a.group, row0 = rows <= kFewRows ? 0 : c.tile * kRowTile;
+  const int rows = c.n * a.group, row0 = c.tile * kRowTile;
   const int r = blockIdx.y * RPG + threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
   if (r >= min(min(rows - row0, kRowTile), a.cap)) return;
   auto state = [&](int p) { return p == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + p); };
@@ -673,7 +687,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a) {
 template <typename T, int D>
 int paged_attend(const PagedArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((paged_kernel<T, D>), dim3(a.groups), dim3(256), 0, stream, a);
-  if (a.acc) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.groups, (a.cap * (D / 4) + kJoinThreads - 1) / kJoinThreads), dim3(kJoinThreads), 0, stream, a);
+  const dim3 grid(a.groups, (a.cap * (D / 4) + kJoinThreads - 1) / kJoinThreads);
+  if (a.acc) hipLaunchKernelGGL((paged_join_kernel<T, D>), grid, dim3(kJoinThreads), 0, stream, a);
   return check_launch("gki_paged_attend");
 }
 

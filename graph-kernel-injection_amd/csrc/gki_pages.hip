@@ -12,7 +12,10 @@ namespace gki {
 namespace {
 
 constexpr int kBookThreads = 1024;
-constexpr int kBookRows = 8192;        // rows that the book-keeping workgroup places itself
+// Rows that the book-keeping workgroup places itself; more have a launch of their own. extend and
+// accept of 64 requests, us, placed by it / by a launch: 1024 rows 7.3 / 9.2, 4096 9.7 / 9.4, 8192
+// 12.7 / 9.3, 16384 19.2 / 9.4.
+constexpr int kBookRows = 4096;
 constexpr int kMaxDraft = 256;
 
 enum Refusal : int { kOutOfPages = 1, kTooManyRows = 2, kBadCount = 4 };
@@ -82,8 +85,9 @@ __device__ inline void no_row(const PageStep& s, int row) {
 }
 
 // One workgroup: checks the step, gives pages back, takes pages, and (PLACE) places the
-// rows. A step that does not fit changes nothing and leaves no rows. Bound by latency: three
-// passes over the requests, flat loops over pages and rows.
+// rows. A step that does not fit changes nothing and leaves no rows. Bound by latency (three
+// passes over the requests, flat loops over pages and rows): 5.3 us for 8 requests, 6.1 for 512.
+// One workgroup, since pages are given out in order; sums and prefixes by DPP (8.8 -> 5.6 us).
 template <bool PLACE>
 __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, PageStep s) {
   __shared__ int part[kBookThreads / 64];
@@ -293,7 +297,8 @@ __global__ __launch_bounds__(256) void accept_kernel(int32_t* lengths, const int
 // ---------------------------------------------------------------------------
 // Rows into pages.
 // ---------------------------------------------------------------------------
-// D / 8 lanes per head of a row; rows without a slot are left out. Bound by HBM.
+// D / 8 lanes per head of a row; rows without a slot are left out. Bound by HBM, small steps by
+// latency: 3.8 k rows of 16 heads (D64, 32 MB both ways) 6.8 us, 8 of 8 heads 1.8.
 template <int D>
 __global__ __launch_bounds__(256) void append_kernel(PageRows p) {
   constexpr int LPR = D / 8;
@@ -311,7 +316,10 @@ __global__ __launch_bounds__(256) void append_kernel(PageRows p) {
 }
 
 // The same with the keys turned by their positions, and the queries turned into q_out
-// ([rows][H][D]), also those of rows without a slot: a workgroup per row.
+// ([rows][H][D]), also those of rows without a slot: a workgroup per row, whose cosines and sines are
+// made once for all heads (rotary_turn). Turned rows are rounded once, to T. Bound by HBM, small
+// steps by latency: 1.7 k rows of 32 + 2 * 8 heads (D128, 43 MB both ways) 9.2 us, 32 rows 4.0;
+// apart, the turn and the append are two launches, and the keys are read twice.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void append_rotated_kernel(PageRows p, RotaryArgs a, HeadRows q) {
   __shared__ float2 cs[64];
@@ -343,8 +351,8 @@ __global__ __launch_bounds__(256) void append_rotated_kernel(PageRows p, RotaryA
 // Rows of each request's accepted path to the slots of its first tokens. Node i of a path is
 // number path[i] > i of the request's rows, or moves nothing. A thread has 16 bytes of every
 // row of a (request, head): it reads eight rows before it writes them, and what a later one
-// reads has a higher number than all that were written. Bound by latency (paths, slots,
-// rows, one after the other).
+// reads has a higher number than all that were written. Bound by latency (paths, slots, rows, one
+// after the other): 16 requests' paths of up to 26 nodes, 8 heads 5.4 us (a row at a time 9.6).
 template <int D>
 __global__ __launch_bounds__(256) void move_kernel(PageRows p, const int32_t* row_starts, const int32_t* paths,
                                                    const int32_t* accepted, int R, int path_len) {
