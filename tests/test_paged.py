@@ -232,7 +232,7 @@ def test_tables_step_by_step(R, page, sink, window, most):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [8192, 8193, 40000])
+@pytest.mark.parametrize("rows", [4096, 4097, 8192, 8193, 40000])
 def test_tables_of_many_rows(rows):
     """Rows placed by the book-keeping workgroup and by a grid of their own."""
     run = Run(3, 3000, 4, 100000, 64)
@@ -314,7 +314,8 @@ def test_counts_past_32_bits_are_refused():
     (12, 2, 1, 1, [40, 129], [60, 3]),
     (6, 3, 4, 0, [40, 0], [5, 70]),
     (4, 2, 20, 5000, [900, 0, 0, 30], [130, 257, 0, 1]),
-    (64, 1, 4, 90, [100, 2], [3, 1])])
+    (64, 1, 4, 90, [100, 2], [3, 1]),
+    (2, 2, 4, 200, [100, 90, 300, 0, 500], [16, 17, 33, 32, 128])])
 def test_attend_against_64_bits(dtype, D, page, heads, kv, sink, window, past, counts):
     run = Run(len(past), 4 * sum(past + counts) // page + 20, sink, window, page, kv, D, dtype, seed=sum(past) + heads)
     run.grow(past)
