@@ -41,7 +41,7 @@ import torch
 from . import _lib
 from .masks import StreamingMaskSpec
 from .ops import _DTYPE_CODE, _current_stream, _on_device
-from .rotary import MultiAxisRotary
+from .rotary import MultiAxisRotary, _dense_like
 
 _HEAD_DIMS = (64, 128)
 _MAX_DRAFT = 256
@@ -325,7 +325,7 @@ class PagedKVCache:
         else:
             axis_stride, _, row_stride = rotary._position_strides(positions, q)
             at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _dense_like(q)
         turns, axis = rotary._table(self.device)
         t = self.table
         with _on_device(self.device):
@@ -362,7 +362,7 @@ class PagedKVCache:
             plan = self._plans[key] = groups, n.value
         groups, floats = plan
         work = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o = _dense_like(q)
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
         requests, _, _, _, positions = batch._pointers()
         with _on_device(self.device):
