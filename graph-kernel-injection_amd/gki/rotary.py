@@ -57,7 +57,12 @@ class _Rotate(torch.autograd.Function):
         ctx.rope, ctx.strides, ctx.inverse = rope, strides, inverse
         ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
-        return rope._rotate(q, k, positions, strides, inverse)
+        outs = rope._rotate(q, k, positions, strides, inverse)
+        # a frozen tensor comes out frozen: what attends it computes no gradient for it
+        frozen = [o for o, needed in zip(outs, ctx.needs_input_grad[1:3]) if o is not None and not needed]
+        if frozen:
+            ctx.mark_non_differentiable(*frozen)
+        return outs
 
     @staticmethod
     def backward(ctx, dq, dk):  # type: ignore[override]
@@ -134,7 +139,8 @@ class MultiAxisRotary:
         int64, ``[axes, B, N]`` or ``[axes, N]`` (packed: ``[axes, rows]``); an axis dimension
         of 1, or ``[N]`` (``[rows]``), gives every axis the same. Rows may lie anywhere (a
         projection's ``[B, N, H, D]`` transposed is read in place); the results are
-        contiguous. Differentiable in reverse mode, any number of times."""
+        contiguous. Differentiable in reverse mode, any number of times; of a tensor that
+        needs no gradient, the result needs none."""
         key = (q.shape, q.stride(), q.dtype, q.device, None if k is None else (k.shape, k.stride(), k.dtype, k.device),
                positions.shape, positions.stride(), positions.dtype, positions.device)
         strides = self._known.get(key)           # checked before: a step's host time counts

@@ -16,7 +16,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from gki import MultiAxisRotary, StreamingMaskSpec, _lib, block_sparse_attention, make_streaming_mask
+from gki import MultiAxisRotary, StreamingMaskSpec, _lib, block_sparse_attention, cross_attention, make_streaming_mask
 
 DEV = "cuda"
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -195,6 +195,66 @@ def test_gradient_is_the_turn_back(dtype, interleaved):
     packed, _ = rope(packed_leaf, None, at.reshape(3, 90))
     back, = torch.autograd.grad(packed, packed_leaf, dq.transpose(1, 2).reshape(90, 6, 128))
     assert torch.equal(back.view(2, 45, 6, 128), got[0])
+
+
+def _turned_by_copies(monkeypatch):
+    """Launches replaced by copies, counted: what autograd asks for shows on the CPU."""
+    launched = []
+
+    def launch(self, q, k, positions, strides, inverse):
+        launched.append(sum(t is not None for t in (q, k)))
+        return q.clone(), None if k is None else k.clone()
+
+    monkeypatch.setattr(MultiAxisRotary, "_launch", launch)
+    return launched
+
+
+@pytest.mark.parametrize("trained", ["q", "k", "both", "none"])
+def test_a_frozen_tensor_is_returned_frozen(trained, monkeypatch):
+    launched = _turned_by_copies(monkeypatch)
+    q, k = torch.randn(5, 4, 64), torch.randn(5, 2, 64)
+    if trained in ("q", "both"):
+        q.requires_grad_(True)
+    if trained in ("k", "both"):
+        k.requires_grad_(True)
+    rope, at = MultiAxisRotary(64, (32,)), torch.arange(5)
+    turned = rope._apply(q, k, at, None, False)
+    assert [t.requires_grad for t in turned] == [q.requires_grad, k.requires_grad] and launched == [2]
+    if trained == "none":
+        return
+    leaves = [t for t in (q, k) if t.requires_grad]
+    sums = [t.square().sum() for t in turned if t.requires_grad]
+    grads = torch.autograd.grad(sum(sums), leaves, create_graph=True)
+    assert launched == [2, len(leaves)] and all(g.requires_grad for g in grads)
+    for leaf, second in zip(leaves, torch.autograd.grad(sum(g.sum() for g in grads), leaves)):
+        assert torch.equal(second, torch.full_like(leaf, 2.0))
+
+
+def test_a_gradient_that_is_not_asked_for_is_not_turned(monkeypatch):
+    launched = _turned_by_copies(monkeypatch)
+    q, k = torch.randn(5, 4, 64, requires_grad=True), torch.randn(5, 2, 64, requires_grad=True)
+    a, b = MultiAxisRotary(64, (32,))._apply(q, k, torch.arange(5), None, False)
+    dq, = torch.autograd.grad(a.sum() + b.sum(), q)
+    assert torch.equal(dq, torch.ones_like(q)) and launched[0] == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("trained", [0, 1])
+def test_frozen_beside_trained_costs_no_gradient_behind(trained):
+    """The other tensor needs no gradient after its turn either: attention behind it gives none."""
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    rope = MultiAxisRotary(64, (32,))
+    q, k, v = (torch.randn(1, 2, 130, 64, generator=gen, device=DEV) for _ in range(3))
+    leaf = (q, k)[trained].requires_grad_(True)
+    at = torch.arange(130, device=DEV)
+    turned = rope(q, k, at)
+    assert [t.requires_grad for t in turned] == [trained == 0, trained == 1]
+    apart = [t.detach().requires_grad_(i == trained) for i, t in enumerate(turned)]
+    do = torch.randn(1, 2, 130, 64, generator=gen, device=DEV)
+    got, = torch.autograd.grad(cross_attention(*turned, v), leaf, do)
+    behind, = torch.autograd.grad(cross_attention(*apart, v), apart[trained], do)
+    # -1 times each position turns back: the same angles, cosines and sines
+    assert torch.equal(got, rope(behind, None, -at)[0])
 
 
 @pytest.mark.gpu
