@@ -40,7 +40,7 @@ import torch
 
 from . import _lib
 from .masks import StreamingMaskSpec
-from .ops import _DTYPE_CODE, _current_stream, _on_device
+from .ops import _DTYPE_CODE, _current_stream, _on_device, _refuse_tangents
 from .rotary import MultiAxisRotary, _dense_like
 
 _HEAD_DIMS = (64, 128)
@@ -242,7 +242,8 @@ class PagedKVCache:
     ``[num_pages, heads, page_size, head_dim]`` in ``dtype`` (float16 or bfloat16), head_dim 64
     or 128. Queries may have any multiple of ``heads`` (grouped-query attention).
 
-    No gradient flows through the cache. A NaN or infinity among a request's own values
+    No gradient flows through the cache, and tensors with a forward-mode tangent are refused
+    (``NotImplementedError``). A NaN or infinity among a request's own values
     reaches the rows of the call that read it, as in the sparse op; what other requests
     left in a page is never seen. Calls on other streams than the table's last ``extend``
     have to be ordered behind it by the caller.
@@ -300,6 +301,7 @@ class PagedKVCache:
         """Writes the step's keys and values (``[rows, heads, D]``) to their slots; rows
         behind the last request are left out."""
         self._batch(batch)
+        _refuse_tangents(k, v)
         (k, k_stride), (v, v_stride) = self._rows("k", k, batch.rows), self._rows("v", v, batch.rows)
         t = self.table
         with _on_device(self.device):
@@ -316,6 +318,7 @@ class PagedKVCache:
         queries (``[rows, Hq, D]``) turned, contiguous. ``positions``: as ``rotary`` takes
         them for packed rows; default: the batch's, for every axis."""
         self._batch(batch)
+        _refuse_tangents(q, k, v)
         q, q_stride = self._rows("q", q, batch.rows, grouped=True)
         (k, k_stride), (v, v_stride) = self._rows("k", k, batch.rows), self._rows("v", v, batch.rows)
         if rotary.head_dim != self.head_dim:
@@ -345,6 +348,7 @@ class PagedKVCache:
         ``[rows, Hq]`` fp32 when ``return_lse``). A row that sees no key, and rows behind the
         last request, give zeros."""
         self._batch(batch)
+        _refuse_tangents(q)
         q, q_stride = self._rows("q", q, batch.rows, grouped=True)
         scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else float(softmax_scale)
         if not math.isfinite(scale):
