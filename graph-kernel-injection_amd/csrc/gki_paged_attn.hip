@@ -52,8 +52,10 @@ struct KeyTiles {
 // divides leaves the states of its pieces, which are joined; a cut close to its ends
 // moves there. Lengths are known on the device only, so every workgroup counts for
 // itself, a wave 64 requests at a time (`extend` lists those that have tokens: 32 of 4096
-// requests cost what 32 of 32 do, 47 us). Neighbours work on one XCD: row tiles of a
-// (request, head) meet their keys in its L2.
+// requests cost what 32 of 32 do, 47 us), once: it goes from one row tile of its share to the
+// next without counting again (single tokens of 8192 requests over 100 keys, 8 heads, D128: 4.46 ms
+// with a count for each, 1.00 so). Neighbours work on one XCD: row tiles of a (request, head) meet
+// their keys in its L2.
 // ---------------------------------------------------------------------------
 __device__ inline uint32_t lane_of(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
 __device__ inline uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
@@ -75,18 +77,28 @@ struct Request {
   __device__ inline uint32_t steps(const PagedArgs& a) const { return tiles * a.H_kv * keys; }
 };
 
-// The row tile that holds a step: its request, which of the request's it is (head by head),
-// its first step.
+// The row tile that holds a step: its request (`index` in the list), which of the request's it is
+// (head by head), its first step.
 struct Place {
   uint32_t first, n, base, tiles, keys, number, start;
-  int r;
-  __device__ inline void set(const Request& q, int l, uint32_t before, uint32_t step) {
+  int r, index;
+  __device__ inline void set(const Request& q, int l, int list_index, uint32_t before, uint32_t step) {
+    index = list_index;
     r = lane_of(q.r, l);
     first = lane_of(q.first, l), n = lane_of(q.n, l), base = lane_of(q.base, l);
     tiles = lane_of(q.tiles, l), keys = lane_of(q.keys, l);
     number = scalar((step - before) / keys);
     start = before + number * keys;
   }
+  // Row tile `number` of the request at `index`, whose first step is `start`.
+  __device__ inline Place(const PagedArgs& a, int index, uint32_t number, uint32_t start)
+      : number(number), start(start), index(index) {
+    const Request q(a, index, index + 1);
+    r = scalar(q.r);
+    first = scalar(q.first), n = scalar(q.n), base = scalar(q.base);
+    tiles = scalar(q.tiles), keys = scalar(q.keys);
+  }
+  __device__ inline Place() {}
 };
 
 struct Shares {
@@ -111,7 +123,7 @@ struct Shares {
     const int l = __builtin_ctzll(__ballot(sum > step));
     uint32_t before = l ? lane_of(sum, l - 1) : 0;
     if (run == 1) {
-      p.set(q, l, before, step);
+      p.set(q, l, l, before, step);
       return p;
     }
     const int end = min((l + 1) * run, n);
@@ -121,7 +133,7 @@ struct Shares {
       const uint64_t past = __ballot(before + upto > step);
       if (past || r0 + 64 >= end) {
         const int m = past ? __builtin_ctzll(past) : 0;
-        p.set(x, m, before + (m ? lane_of(upto, m - 1) : 0), step);
+        p.set(x, m, r0 + m, before + (m ? lane_of(upto, m - 1) : 0), step);
         return p;
       }
       before += lane_of(upto, 63);
@@ -609,39 +621,54 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
   __shared__ __align__(16) uint16_t sk[2][kTileN * D];
   __shared__ __align__(16) uint16_t sv[2][kTileN * D];
   __shared__ int64_t pieces[kPagePieces];
-  __shared__ uint32_t todo[2][2];
+  __shared__ uint32_t todo[2][4];
+  __shared__ uint32_t cut[3];
   // rows behind the last request have no output: zeros
   for (int64_t x = (int64_t)args.requests[0].y * args.H * (D / 8) + (int64_t)blockIdx.x * 256 + threadIdx.x;
        x < (int64_t)args.rows * args.H * (D / 8); x += (int64_t)gridDim.x * 256) {
     *(uint4*)(args.o + 8 * x) = make_uint4(0, 0, 0, 0);
     if (args.lse && x % (D / 8) == 0) args.lse[x / (D / 8)] = 0.f;
   }
-  // One piece of the share after the other. Only the rest of the share is kept between two, in
-  // LDS (by turns, as a wave may read it late), so that the row tiles have their registers.
+  // One piece of the share after the other. Only the rest of the share (steps lo .. hi - 1, the row
+  // tile at lo) and how shares are cut are kept between two, in LDS (the rest by turns, as a wave may
+  // read it late), so that the row tiles have their registers.
   for (int turn = 0;; ++turn) {
     const PagedArgs a = fresh_args();
     int tid = threadIdx.x;             // not an invariant: nothing made from it is held either
     asm volatile("" : "+v"(tid));
-    const Shares s(a, tid, a.requests[0].x);
-    const int used = (int)((s.all + s.share - 1) / s.share);
-    const bool idle = (int)blockIdx.x >= used;
-    const int w = idle ? (int)blockIdx.x : xcd_remap(blockIdx.x, used);
-    uint32_t lo, hi;
+    uint32_t lo, hi, share, edge;
+    int w;
+    Place p;
     if (turn == 0) {
+      const Shares s(a, tid, a.requests[0].x);
+      const int used = (int)((s.all + s.share - 1) / s.share);
+      const bool idle = (int)blockIdx.x >= used;
+      w = idle ? (int)blockIdx.x : xcd_remap(blockIdx.x, used);
       if (a.acc && tid == 0) a.cuts[w].pieces = 0;
       if (idle) return;
       lo = s.cut(a, w * s.share), hi = s.cut(a, (w + 1) * s.share);
+      if (lo >= hi) return;
+      p = s.place(a, lo);
+      share = s.share, edge = s.edge;
+      if (tid == 0) cut[0] = share, cut[1] = edge, cut[2] = w;
     } else {
-      lo = scalar(todo[turn & 1][0]), hi = scalar(todo[turn & 1][1]);
+      const uint32_t* rest = todo[turn & 1];
+      lo = scalar(rest[0]), hi = scalar(rest[1]);
+      if (lo >= hi) return;
+      p = Place(a, (int)scalar(rest[2]), scalar(rest[3]), lo);
+      share = scalar(cut[0]), edge = scalar(cut[1]), w = (int)scalar(cut[2]);
     }
-    if (lo >= hi) return;
-    const Place p = s.place(a, lo);
     const Unit u(p, lo, hi, w);
     if (tid == 0) {
-      todo[(turn + 1) & 1][0] = lo + (u.s1 - u.s0);
-      todo[(turn + 1) & 1][1] = hi;
+      // of the row tiles of all heads of all requests of the list the next
+      const bool more = p.number + 1 < p.tiles * a.H_kv;
+      uint32_t* rest = todo[(turn + 1) & 1];
+      rest[0] = lo + (u.s1 - u.s0);
+      rest[1] = hi;
+      rest[2] = more ? p.index : p.index + 1;
+      rest[3] = more ? p.number + 1 : 0;
       if (u.state == 2 * w + 1)        // for the join: cuts at the shares' ends up to the edge
-        a.cuts[w] = CutTile{u.first, u.n, u.h, u.tile, 2 + (int)((p.start + p.keys - s.edge) / s.share - (w + 1))};
+        a.cuts[w] = CutTile{u.first, u.n, u.h, u.tile, 2 + (int)((p.start + p.keys - edge) / share - (w + 1))};
     }
     const int rows = u.n * a.group;
     if (rows <= kFewRows) paged_stream<T, D>(a, u, sk[0], sv[0], pieces, tid);

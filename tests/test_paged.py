@@ -397,6 +397,52 @@ def test_many_requests(R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("most,kv,D", [(1, 2, 64), (20, 1, 128)])
+def test_thousands_that_attend_at_once(most, kv, D):
+    """More requests with tokens than 64 for each lane of a wave, some in between without."""
+    rng = random.Random(most)
+    R = 5000
+    run = Run(R, 12 * R, 4, 60, 16, kv, D, torch.bfloat16, seed=most)
+    run.grow([rng.choice([0, 3, 15, 64, 130]) for _ in range(R)])
+    counts = [0 if r % 9 == 4 else rng.randint(1, most) for r in range(R)]
+    assert sum(c > 0 for c in counts) > 4096
+    batch = run.extend(counts, sum(counts) + 5, max_count=most)
+    run.append(batch)
+    q = run.normal(batch.rows, 4 * kv)
+    o, lse = run.cache.attend(q, batch, return_lse=True)
+    run.check_attend(batch, q, o, lse)
+    assert torch.equal(o, run.cache.attend(q, batch))
+
+
+@pytest.mark.gpu
+def test_time_grows_with_the_requests_not_with_their_square():
+    """65536 requests' single tokens, 8 heads: 524288 short walks. Counting all requests again for each walk
+    takes 228 ms, the walks themselves less than 10."""
+    R, heads = 65536, 8
+    table = PageTable(R, 2 * R, StreamingMaskSpec(4, 100), page_size=16, max_length=32, device=DEV)
+    cache = PagedKVCache(table, heads, 64)
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    for n in (4, 1):
+        batch = table.extend(torch.full((R,), n, dtype=torch.int32, device=DEV), n * R, max_count=n)
+        k, v = (torch.randn((n * R, heads, 64), generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2))
+        cache.append(k, v, batch)
+    q = torch.zeros((R, heads, 64), dtype=torch.bfloat16, device=DEV)
+    took = []
+    for _ in range(4):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        o = cache.attend(q, batch)
+        end.record()
+        end.synchronize()
+        took.append(start.elapsed_time(end))
+    # equal scores: the mean of a request's five values
+    want = cache.v_pages[batch.slots // 16][:, :, :5].double().mean(2)
+    # half a unit of the result and of each of five equal weights' sum, fp32 below
+    assert (o.double() - want).abs().max() <= 2.0**-8 * want.abs().max() + 2.0**-20
+    assert min(took) < 60, took
+
+
+@pytest.mark.gpu
 def test_a_chain_is_plain_tokens():
     a, b = (Run(2, 60, 4, 50, 32, seed=3) for _ in range(2))
     for run in (a, b):
