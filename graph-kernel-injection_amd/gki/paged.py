@@ -114,7 +114,7 @@ class PageTable:
     ``page_size``: a power of two from 16 to 1024. ``spec``: what a query sees, the first
     ``sink_size`` and the last ``window_size`` positions; pages behind the window, sinks
     apart, return to the queue when their request is extended, so ``max_length`` bounds
-    positions, not memory. ``max_length`` defaults to all pages for one request.
+    positions, not memory. ``max_length``: up to 2^30; it defaults to all pages for one request.
 
     ``lengths`` (int32 ``[max_requests]``) and ``block_table`` (int32 ``[max_requests,
     pages]``, -1: none) are the table's own: read them, do not write.
@@ -130,7 +130,7 @@ class PageTable:
             raise ValueError(f"num_pages must be positive, num_pages * page_size below 2^31, got {num_pages}")
         if spec.sink_size >= 1 << 30:
             raise ValueError("sink_size must be below 2^30")
-        max_length = num_pages * page_size if max_length is None else int(max_length)
+        max_length = min(num_pages * page_size, 1 << 30) if max_length is None else int(max_length)
         if not 1 <= max_length <= 1 << 30:
             raise ValueError(f"max_length must be in [1, 2^30], got {max_length}")
         self.max_requests, self.num_pages, self.page_size = int(max_requests), int(num_pages), int(page_size)

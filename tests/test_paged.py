@@ -78,6 +78,16 @@ def test_c_entries_refuse_before_launch():
     assert lib.gki_paged_accept(16, 16, 16, 16, 16, 16, 2, 2, 0, 2, 64, 9, 64, NULL) == 0
 
 
+@pytest.mark.parametrize("pages,page", [(2**24, 64), (2**24 + 1, 64), (2**21 - 1, 1024), (2**27 - 1, 16)])
+def test_pools_past_the_longest_request_need_no_max_length(pages, page):
+    """Pools of 2^30 positions and more: all other arguments are right, so the device is what is refused."""
+    spec = StreamingMaskSpec(4, 100)
+    with pytest.raises(ValueError, match="CUDA"):
+        PageTable(1, pages, spec, page_size=page, device="cpu")
+    with pytest.raises(ValueError, match="max_length"):
+        PageTable(1, pages, spec, page_size=page, max_length=2**30 + 1, device="cpu")
+
+
 def test_oracle_sees_a_mistake():
     """The bounds are passed by neither zeros nor a shifted window."""
     gen = torch.Generator().manual_seed(0)
