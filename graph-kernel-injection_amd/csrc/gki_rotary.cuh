@@ -6,9 +6,11 @@
 namespace gki {
 namespace {
 
-// cos and sin of pair j at a token. The angle is reduced in 64 bits (turns, then the
+// cos and sin of pair j at a token. The angle is made and reduced in 64 bits (turns, then the
 // quarter it lies in: at most an eighth of a turn from it, which fp32 holds to 2^-28 of a
-// turn), so far positions lose nothing.
+// turn). The turns of a position and their product with it are rounded, by about 3.3 units of 2^-53
+// of the angle together: up to 2^-21.2 of a radian at position 2^30 and frequency 1, against exact
+// angles 2^-21.9 at most.
 __device__ inline float2 rotary_turn(const RotaryArgs& a, int64_t t, int j) {
   const int64_t at = a.axis[j] * a.pa + t / a.n * a.pb + t % a.n * a.pn;
   const double p = a.wide ? (double)((const int64_t*)a.positions)[at] : (double)((const int32_t*)a.positions)[at];

@@ -81,7 +81,8 @@ class MultiAxisRotary:
     Pair ``j`` of all ``P`` turns with frequency ``base ** (-j / P)``; with ``per_axis`` each
     axis has a ladder of its own, ``base ** (-i / size)`` for the ``i``-th pair of a section of
     that size. Pairs are elements ``(j, j + P)`` or, ``interleaved``, ``(2 j, 2 j + 1)``. Angles
-    are reduced in 64 bits, to an error below 2^-23 of a radian for positions below 2^30.
+    are made and reduced in 64 bits: off by less than 2^-21 of a radian for positions below 2^30
+    and frequencies up to 1 (a ``base`` of at least 1), in proportion more beyond either.
     """
 
     def __init__(self, head_dim: int, sections: Sequence[int], base: float = 10000.0, interleaved: bool = False,

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from decimal import Decimal, localcontext
 
 import pytest
 import torch
@@ -99,6 +100,54 @@ def test_against_64_bits(dtype, interleaved, per_axis, D, sections):
         packed = rope(rows[0], rows[1], at.reshape(len(sections), B * N))
         for x, y in zip(packed, got):
             assert torch.equal(x.view(B, N, -1, D).transpose(1, 2), y)
+
+
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+_FAR = [2**30 - 1, 2**30 - 77, 1054937413, 1073140401, 2**29 + 3, 777777777, 123456, 2**20 + 1, 3]
+
+
+def _exact_turns(rope, p):
+    """Of each pair at position p, reduced to half a turn on either side, from 50 digits."""
+    with localcontext() as c:
+        c.prec = 50
+        out = []
+        for j in range(rope.pairs):
+            t = p * Decimal(rope.base) ** (-Decimal(j) / rope.pairs) / (2 * _PI)
+            out.append(t - t.to_integral_value())
+        return out
+
+
+@pytest.mark.parametrize("base,pairs", [(1e6, 64), (100.0, 64), (10000.0, 24), (2.0, 64), (1.0, 8)])
+def test_far_angles_are_as_close_as_stated(base, pairs):
+    """The kernels' arithmetic on the host. In units of 2^-53 of the largest angle, 2^30: the frequency and its place in
+    the ladder 0.92, 2 pi 0.35, the division and the product 1 each; fp32 adds 2^-28 of a turn: below 2^-21 in all."""
+    rope, worst = MultiAxisRotary(128, (pairs,), base=base), 0.0
+    turns = rope._table(torch.device("cpu"))[0].tolist()
+    for p in _FAR:
+        for turn, exact in zip(turns, _exact_turns(rope, p)):
+            r = p * turn
+            r -= round(r)
+            quarter = round(4 * r)
+            x = torch.tensor(2 * (r - 0.25 * quarter), dtype=torch.float32).item()
+            off = Decimal(quarter) / 4 + Decimal(x) / 2 - exact
+            worst = max(worst, abs(float((off - off.to_integral_value()) * 2 * _PI)))
+    assert worst < 2.0**-21, worst * 2**23
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("base,pairs", [(1e6, 64), (100.0, 64), (10000.0, 24), (1.0, 8)])
+def test_far_positions_against_exact_angles(base, pairs):
+    """Rows of ones and zeros come out as cosines and sines: 2^-21 from the angle, 2^-22 from the functions and
+    their rounding."""
+    rope = MultiAxisRotary(128, (pairs,), base=base)
+    q = torch.zeros(len(_FAR), 1, 128, device=DEV)
+    q[..., :pairs] = 1
+    got, _ = rope(q, None, torch.tensor(_FAR, device=DEV))
+    for row, p in zip(got[:, 0].tolist(), _FAR):
+        for j, t in enumerate(_exact_turns(rope, p)):
+            phase = float(t * 2 * _PI)
+            assert abs(row[j] - math.cos(phase)) < 2.0**-21 + 2.0**-22, (p, j)
+            assert abs(row[pairs + j] - math.sin(phase)) < 2.0**-21 + 2.0**-22, (p, j)
 
 
 @pytest.mark.gpu
