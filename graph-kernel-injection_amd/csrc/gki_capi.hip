@@ -976,7 +976,7 @@ int gki_paged_attend(const void* q, int64_t q_stride, const void* k_pages, const
   a.o = (uint16_t*)o, a.lse = lse;
   a.requests = (const int4*)requests, a.positions = positions, a.table = table, a.ancestors = ancestors;
   a.q_stride = q_stride;
-  a.R = R, a.rows = rows, a.H = H, a.H_kv = H_kv, a.group = H / H_kv;
+  a.rows = rows, a.H = H, a.H_kv = H_kv, a.group = H / H_kv;
   a.max_pages = max_pages, a.shift = log2_of(page_size), a.num_pages = num_pages;
   a.sink = sink_size, a.window = std::min(window_size, 1 << kPartialBit), a.words = words;
   a.scale_log2 = g.qk_scale_log2, a.q_and = g.q_and, a.q_xor = g.q_xor;

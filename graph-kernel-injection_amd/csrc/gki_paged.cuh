@@ -104,7 +104,7 @@ struct PagedArgs {
   const int32_t *positions, *table;
   const uint64_t* ancestors;           // [rows][words], null: no trees
   int64_t q_stride;                    // elements between rows of q; heads lie D apart
-  int R, rows, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;
+  int rows, H, H_kv, group, max_pages, shift, num_pages, sink, window, words;
   float scale_log2, q_sign;            // as StreamArgs': the sign of the scale, or zero, goes to q
   uint32_t q_and, q_xor;               // the same as words of Q
   int groups;                          // workgroups that share the work

@@ -91,7 +91,7 @@ __device__ inline void no_row(const PageStep& s, int row) {
 template <bool PLACE>
 __global__ __launch_bounds__(kBookThreads) void extend_kernel(PageTables t, PageStep s) {
   __shared__ int part[kBookThreads / 64];
-  __shared__ int first[kBookThreads + 1], from[kBookThreads], starts[kBookThreads];
+  __shared__ int first[kBookThreads], from[kBookThreads], starts[kBookThreads];
   __shared__ unsigned long long sums[3];
   __shared__ int bad;
   const int tid = threadIdx.x;
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kMaxDraft) void tree_kernel(PageTables t, PageStep 
 // Requests marked in `done` give all their pages back and hold nothing.
 __global__ __launch_bounds__(kBookThreads) void release_kernel(PageTables t, const uint8_t* done) {
   __shared__ int part[kBookThreads / 64];
-  __shared__ int first[kBookThreads + 1], skip[kBookThreads];
+  __shared__ int first[kBookThreads], skip[kBookThreads];
   const int tid = threadIdx.x, head = t.queue[0], count = t.queue[1], n_sink = sink_pages(t);
   int given = 0;
   for (int r0 = 0; r0 < t.R; r0 += kBookThreads) {
