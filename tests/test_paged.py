@@ -453,6 +453,71 @@ def test_time_grows_with_the_requests_not_with_their_square():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [256, 512, 1024])
+@pytest.mark.parametrize("dtype,D,heads,kv,counts,tree", [
+    (torch.bfloat16, 128, 8, 2, [1, 3, 1, 0, 1], False), (torch.float16, 64, 4, 4, [1, 300, 40, 257, 5], False),
+    (torch.float16, 128, 8, 1, [26, 60, 1, 0, 17], True)])
+def test_attend_over_large_pages(page, dtype, D, heads, kv, counts, tree):
+    """Pages that several key tiles lie in, among them of requests that end in the first and the last."""
+    rng = random.Random(page)
+    run = Run(5, 40, 70, 900, page, kv, D, dtype, max_length=8000, seed=page)
+    run.grow([page - 1, 2 * page + 65, 3001, 0, 5])
+    trees = [_tree(rng, n) for n in counts] if tree else None
+    batch = run.extend(counts, max_count=max(counts), parents=trees)
+    run.append(batch)
+    q = run.normal(batch.rows, heads)
+    o, lse = run.cache.attend(q, batch, return_lse=True)
+    run.check_tables(batch)
+    run.check_attend(batch, q, o, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,tree", [([1] * 16, False), ([1] * 7 + [40, 300] + [2] * 7, False), ([1, 20, 7, 40] * 4, True)])
+def test_steps_of_several_key_tiles(counts, tree):
+    """A table whose longest requests could have more steps than 31 bits count: a step is two key tiles or more."""
+    rng = random.Random(len(counts))
+    run = Run(16, 130, 4, 2**30, 1024, 8, 64, torch.bfloat16, max_length=2**30, seed=22)
+    # as gki_paged_attend reckons: row tiles of the rows given, times the steps of the longest walk
+    tiles = (sum(counts) // 128 + 16) * 8
+    assert tiles * (2**30 // 64 + 4) >= 2**31
+    run.grow([rng.choice([0, 1, 63, 64, 500, 1025, 5000]) for _ in range(15)] + [9000], 3000)
+    trees = [_tree(rng, n) for n in counts] if tree else None
+    batch = run.extend(counts, max_count=max(counts), parents=trees)
+    run.append(batch)
+    q = run.normal(batch.rows, 8)
+    o, lse = run.cache.attend(q, batch, return_lse=True)
+    assert run.table.check() == len(run.book.queue)
+    run.check_attend(batch, q, o, lse)
+    assert torch.equal(o, run.cache.attend(q, batch))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40])
+def test_walks_of_more_than_65536_key_tiles(rows):
+    """Equal scores over 4.3 million keys: every key tile adds 64 to one element's sum, all of them whole numbers."""
+    past, page, D = 4300001, 1024, 64
+    table = PageTable(1, past // page + 2, StreamingMaskSpec(4, 2**30), page_size=page, device=DEV)
+    cache = PagedKVCache(table, 1, D, dtype=torch.float16)
+    gen = torch.Generator(device=DEV).manual_seed(23)
+    for n in (past, rows):
+        batch = table.extend(_ints([n]), n)
+        at = batch.positions[:, None] // 64 % D
+        v = (at == torch.arange(D, device=DEV)).to(torch.float16)[:, None]
+        cache.append(torch.zeros_like(v), v, batch)
+    assert table.check() >= 0
+    q = torch.randn((rows, 2, D), generator=gen, device=DEV).to(torch.float16)
+    o, lse = cache.attend(q, batch, return_lse=True)
+    n = past + 1 + torch.arange(rows, device=DEV).double()
+    at = torch.arange(past + rows, device=DEV) // 64 % D
+    held = torch.stack([torch.bincount(at[:past + 1 + i], minlength=D) for i in range(rows)]).double()
+    want = (held / n[:, None])[:, None]
+    # half a unit of fp16 (a tile of 64 more or less is two of them) and of the fp32 quotient
+    assert ((o.double() - want).abs() <= (2.0**-11 + 2.0**-22) * want).all()
+    # ln n is 15.3: fp32's logarithm and product, two units of 2^-23 of it each (a tile of 64 is 1.5e-5)
+    assert ((lse.double() - n.log()[:, None]).abs() <= 4 * 2.0**-23 * 16).all()
+
+
+@pytest.mark.gpu
 def test_a_chain_is_plain_tokens():
     a, b = (Run(2, 60, 4, 50, 32, seed=3) for _ in range(2))
     for run in (a, b):
