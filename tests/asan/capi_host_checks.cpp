@@ -200,6 +200,63 @@ static void check_rejections() {
   rejected(gki_read_probe(p, p, 0, 100, 256, 4, 16, up, need, nullptr), "read probe no slices");
 }
 
+// The entries of paged caches and rotary positions, refused after all that they read on the host.
+static void check_paged_rejections() {
+  alignas(16) static char buf[1024];
+  void* p = buf;
+  float* f = (float*)buf;
+  int32_t* ip = (int32_t*)buf;
+  int64_t* lp = (int64_t*)buf;
+  const double* dp = (const double*)buf;
+  uint64_t* up = (uint64_t*)buf;
+  auto rejected = [](int rc, const char* what) {
+    const std::string msg = gki_last_error();
+    CHECK(rc != 0 && !msg.empty(), "%s: rc %d, message '%s'", what, rc, msg.c_str());
+  };
+  auto extend = [&](const int32_t* parents, int rows, int max_count, int words, int R, int page, int32_t* requests) {
+    return gki_page_extend(ip, parents, rows, max_count, words, ip, ip, ip, ip, ip, ip, ip, R, 8, page, 9, 4, 16, ip, ip, ip,
+                           lp, up, requests, nullptr);
+  };
+  rejected(extend(nullptr, 5, 5, 0, 2, 48, ip), "extend page size 48");
+  rejected(extend(nullptr, 5, 5, 0, 0, 64, ip), "extend no requests");
+  rejected(extend(nullptr, -1, 5, 0, 2, 64, ip), "extend negative rows");
+  rejected(extend(ip, 300, 257, 5, 2, 64, ip), "extend trees of 257");
+  rejected(extend(nullptr, 5, 5, 0, 2, 64, ip + 1), "extend misaligned list");
+  rejected(gki_page_release(nullptr, ip, ip, ip, ip, ip, ip, ip, 2, 8, 64, 9, 4, 16, nullptr), "release null");
+  rejected(gki_page_accept(ip, ip, ip, nullptr, 2, nullptr), "table accept null");
+  rejected(gki_paged_append(p, p, 128, 120, p, p, lp, 2, 3, 2, 64, 9, 64, nullptr), "append short row stride");
+  rejected(gki_paged_append(p, p, 128, 128, p, p, lp, 0, 3, 2, 64, 9, 64, nullptr), "append fp32");
+  rejected(gki_paged_append_rotated(p, p, 256, 4, p, p, 128, 128, p, p, lp, 2, 3, 2, 64, 9, 64, dp, ip, 12, 0, ip, 0, 0, 1,
+                                    nullptr), "append_rotated 12 pairs");
+  rejected(gki_paged_accept(p, p, lp, ip, nullptr, ip, 2, 2, 5, 2, 64, 9, 64, nullptr), "accept null paths");
+  auto attend = [&](int64_t stride, int H, float scale, int groups, float* ws) {
+    return gki_paged_attend(p, stride, p, p, p, f, ip, ip, ip, nullptr, 0, 2, 3, 3, 2, H, 2, 64, 8, 9, 64, 4, 16, scale, ws,
+                            groups, nullptr);
+  };
+  rejected(attend(255, 4, 0.125f, 1, f), "attend odd row stride");
+  rejected(attend(256, 3, 0.125f, 1, f), "attend H_kv not dividing H");
+  rejected(attend(256, 4, __builtin_nanf(""), 1, f), "attend scale NaN");
+  rejected(attend(256, 4, 0.125f, 0, f), "attend no groups");
+  rejected(attend(256, 4, 0.125f, 1, f + 1), "attend misaligned workspace");
+  int64_t floats = -1;
+  const int groups = gki_paged_groups(30, 8, 2, 128, 100, 64, 4, 2048, &floats);
+  CHECK(groups >= 1 && floats == groups * (2ll * 120 * 130 + 5), "paged groups %d, floats %lld", groups, (long long)floats);
+  CHECK(gki_paged_groups(30, 8, 2, 128, 100, 64, 4, 2048, nullptr) == groups, "paged groups, null");
+  // strides exactly as long as the header says
+  const std::vector<int64_t> six = {0, 128, 64, 0, 128, 64}, odd = {0, 128, 64, 0, 128, 60}, three = {0, 0, 1};
+  auto rotary = [&](const void* k, const int64_t* k_strides, const int64_t* q_strides, int pairs, int64_t n) {
+    return gki_rotary(p, p, 2, q_strides, k, k ? p : nullptr, k ? 2 : 0, k_strides, 2, 1, n, 64, dp, ip, pairs, 0, 0, ip, 0,
+                      three.data(), nullptr);
+  };
+  rejected(rotary(p, six.data(), six.data(), 12, 3), "rotary 12 pairs");
+  rejected(rotary(nullptr, nullptr, six.data(), 40, 3), "rotary too many pairs, no k");
+  rejected(rotary(p, odd.data(), six.data(), 32, 3), "rotary odd strides of k");
+  rejected(rotary(nullptr, nullptr, odd.data(), 32, 3), "rotary odd strides");
+  rejected(rotary(p, nullptr, six.data(), 32, 3), "rotary null strides of k");
+  rejected(rotary(p, six.data(), six.data(), 32, 1ll << 24), "rotary too many tokens");
+  CHECK(rotary(p, six.data(), six.data(), 32, 0) == 0, "empty rotary rejected: %s", gki_last_error());
+}
+
 static void check_fwd_order(std::mt19937& rng) {
   for (int trial = 0; trial < 500; ++trial) {
     const int n_qt = 1 + (int)(rng() % 200);
@@ -237,6 +294,7 @@ int main() {
   check_fwd_order(rng);
   check_rolling_stream(rng);
   check_rejections();
+  check_paged_rejections();
   if (g_fail) {
     std::fprintf(stderr, "%d host check(s) failed\n", g_fail);
     return 1;
