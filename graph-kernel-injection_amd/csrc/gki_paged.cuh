@@ -77,23 +77,23 @@ struct PageRows {
   }
 };
 
-// How attention over pages is shared out; us of kernel at bf16 D128, H32/8 (H64/8: trees of 60),
+// How attention over pages is shared out; us with the join at bf16 D128, H32/8 (H64/8: trees of 60),
 // and fp16 D64 H16 ("mixed").
 //
 // Workgroups that take shares: as many as the card holds at once. 256 / 512 / 768 / 1024 at
-// D128: 32 decodes over up to 4096 keys 48 / 43 / 48 / 47, chunks of 512 137 / 109 / 124 / 112, trees of 60
-// 162 / 124 / 142 / 136; 512 / 768 / 1024 / 1536 at D64: mixed 57 / 51 / 48 / 50.
+// D128: 32 decodes over up to 4096 keys 52 / 44 / 49 / 48, chunks of 512 129 / 108 / 124 / 119, trees of 60
+// 145 / 121 / 137 / 133; 512 / 768 / 1024 / 1536 at D64: mixed 54 / 51 / 50 / 55.
 inline int paged_groups(int head_dim) { return head_dim >= 128 ? 512 : 1024; }
-// What a walk's prologue and epilogue count, in 64-key steps: 0 / 2 / 4 / 6: chunks 108 / 102 / 101 /
-// 102, mixed 48.5 / 44.9 / 46.4 / 45.8, trees of 60 121 / 119 / 125 / 129.
+// What a walk's prologue and epilogue count, in 64-key steps: 0 / 2 / 4 / 6: decodes 52.9 / 43.9 / 45.1 /
+// 45.1, chunks 111 / 108 / 110 / 109, mixed 53.3 / 49.8 / 51.6 / 50.7, trees of 60 120 / 121 / 122 / 123.
 constexpr int kPagedPieceCost = 2;
 // Steps that a share has at least: a walk as long as the longest gets about kPagedPieces pieces,
-// whose join costs as much as they save from there on. One decode over 768 / 4096 / 16384 keys,
-// with the join: 2 steps at least 13.6 / 22.0 / 31.1, 4 15.8 / 18.5 / 30.4, 8 - / 20.9 / -, 16 - /
-// 27.4 / -; this rule 13.6 / 18.3 / 29.2.
+// whose join costs as much as they save from there on. One decode over 768 / 4096 / 16384 keys:
+// 2 steps at least 13.1 / 20.5 / 29.5, 4 15.3 / 17.7 / 29.5, 8 18.8 / 20.1 / 28.1, 16 26.1 / 25.9 /
+// 28.5; this rule 13.2 / 17.7 / 28.0.
 constexpr int kPagedMinShare = 2, kPagedMostShare = 8, kPagedPieces = 16;
-// Walks shorter than this are not cut: the join is another launch (9 key tiles of 8 heads, cut 14.1,
-// whole 11.0; 14 tiles cut 13.6, whole 17.5).
+// Walks shorter than this are not cut: the join is another launch, and below there is little to win
+// (one decode of 8 heads, replayed: 9 key tiles cut 10.1, whole 10.6 to 10.9; 13 tiles cut 13.2, whole 17.4).
 constexpr int kPagedCutSteps = 16;
 
 struct PagedArgs {

@@ -23,12 +23,15 @@ namespace {
 
 constexpr int kRowTile = 128;          // rows of a tile: four waves of 32
 // Up to as many run as a stream, us with the join, stream / tile: 32 requests' decodes of 4 rows over
-// 4096 keys (D128) 91 / 106, 64 of 16 rows over 2048 95 / 101, 16 of 16 rows over 4096 54 / 52, one
-// over 512 (D64) 11.1 / 12.9; with two blocks of 16 rows: 16 of 32 rows over 4096 63 / 55, 32 of 32
+// 4096 keys (D128) 90 / 104, 64 of 16 rows over 2048 95 / 103, 16 of 16 rows over 4096 54 / 51, one
+// over 512 (D64) 10.8 / 12.7; with two blocks of 16 rows: 16 of 32 rows over 4096 63 / 55, 32 of 32
 // rows over 1024 (D64) 31 / 26.
 constexpr int kFewRows = 16;
-// A cut closer than this to a row tile's ends moves there, and closer than a 16th of a share (a 4th /
-// 8th / 16th: chunks of 512 112 / 110 / 107 us, trees of 60 131 / 126 / 122).
+// A cut closer than this many steps to a row tile's ends moves there (half a share at most), us with
+// the join for 1 / 2 / 3 / 4 / 6 / 8: 32 decodes 44.7 / 45.0 / 43.7 / 43.8 / 44.2 / 46.7, chunks of 512
+// 110 / 110 / 109 / 108 / 107 / 107, mixed 51.7 / 51.2 / 48.7 / 49.8 / 48.2 / 48.0, trees of 26 36.1 /
+// 36.1 / 34.3 / 34.4 / 34.4 / 34.4, of 60 121 for all. In shares above 64 steps, closer than a 16th: four
+// times 2048 rows behind 4000 keys (H32/8 D128) 587, with a 4th / an 8th / 4 steps 600 / 596 / 594.
 constexpr uint32_t kCutEdge = 4;
 constexpr int kPagePieces = 512;       // pieces of pages whose places are held in LDS at a time
 
@@ -48,7 +51,10 @@ struct KeyTiles {
 // ---------------------------------------------------------------------------
 // Which work a workgroup takes. The key tiles of all row tiles of all requests and kv heads,
 // one after the other (request, head, row tile, key tile), are cut into equal shares, a
-// workgroup each: requests of any lengths load the card evenly. A row tile that a cut
+// workgroup each. A row tile counts as many key tiles as its request's rows see together: requests of
+// any lengths load the card evenly, but the row tiles of a chunk longer than the keys before it do
+// not, as the first of them walk less than they count (four prompts of 2048 tokens, H32/8 D128: 0.52
+// PFLOP/s at the start, 0.93 behind 4000 keys). A row tile that a cut
 // divides leaves the states of its pieces, which are joined; a cut close to its ends
 // moves there. Lengths are known on the device only, so every workgroup counts for
 // itself, a wave 64 requests at a time (`extend` lists those that have tokens: 32 of 4096
@@ -310,7 +316,7 @@ __device__ inline float2* piece_ml(const PagedArgs& a, int state, int r) { retur
 // hold loads. P is rounded to T for the matrix pipe, and the sums are those of the rounded P, so
 // that what rounding adds to a row's weights it adds to their sum (fp16: 2.8e-4 of the result, 3.2e-4
 // with sums before rounding). Bound by HBM: 32 decodes over 4096 keys, D128 H32/8, 537 MB in
-// 91 us with the join, 5.9 TB/s.
+// 90 us with the join, 6.0 TB/s.
 template <typename T, int D>
 __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t* sk, uint16_t* sv, int64_t* pieces, int tid) {
   constexpr int TILE = kTileN * D;
@@ -364,8 +370,11 @@ __device__ inline void paged_stream(const PagedArgs& a, const Unit& u, uint16_t*
 // formed (VALU), then O of tile c while the maxima of S are taken, the two interleaved by
 // sched_group_barrier. K is read one tile ahead of V. P is rounded to T, as are the outputs; S, the
 // maxima, the sums and O are in 32 bits. Two workgroups of a CU take 2.0 us for a 64-key step of
-// each (1.07 PFLOP/s on 256 CUs), one alone 1.25 to 1.43: bound by the matrix pipe and the VALU
-// together. Chunks of 512 (4 requests, H32/8, W4096) 99 us of kernel for 68 GFLOP.
+// each (1.07 PFLOP/s on 256 CUs), one alone 1.25 to 1.43. Chunks of 512 (4 requests, H32/8, W4096) 101
+// us of kernel for 68 GFLOP: 1.4 of two waves a SIMD on average, as shares are uneven and pieces have
+// their ends, the matrix cores busy for 33% of it, the VALU for 26%. Trees of 60 (8 requests, H64/8,
+// W8192) 114 us: the row tiles of a (request, head) read its keys apart in time, 591 MB past L2 for 200
+// MB of keys and values, 5.2 TB/s.
 template <int D> constexpr bool kPagedSkew = D >= 128;
 constexpr int kAheadS = 4, kAheadO = 8, kValuS = 3, kValuO = 1;
 
@@ -680,7 +689,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : 2) void paged_kernel(PagedArgs a
 // The pieces of the row tile that workgroup blockIdx.x's share ends in, if it is cut, joined: a
 // thread for four elements of a row, pieces in order. As join_kernel: O = sum_p f_p acc_p / sum_p
 // f_p l_p, f_p = exp2(m_p - M). Bound by latency (the cut, the maxima, the sums): many small
-// workgroups, most of which leave at once. 4.6 us for 32 decodes, 12 for trees of 60
+// workgroups, most of which leave at once. 4.5 us for 32 decodes, 12 for trees of 60
 // (19 where a thread had more of a row), 13 where 128 rows of every share are cut (67 MB of states).
 constexpr int kJoinThreads = 256;
 template <typename T, int D>
